@@ -196,6 +196,207 @@ def decode_kv8(fmt: int, q, k8, v8, k_scale, v_scale, block_table, kv_len, gate=
     return out
 
 
+# ---------------------------------------------------------------- several rotary axes, spans of keys, shared pages
+NUM_SMS = 148
+ROW_TILE, KEY_TILE = 256, 128            # (token, head) rows and keys of a tile in attn_spans.cu
+
+
+def _need(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _index(t, shape, device, what: str) -> None:
+    _need(t.dtype == torch.int32 and t.device == device and tuple(t.shape) == shape and t.is_contiguous(),
+          f"{what}: contiguous int32 {list(shape)} on {device} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
+    """Checks what the calls over spans have in common; (rows, Hq, pages, Hkv, page size, sequences, scale, out)."""
+    _need(q.is_cuda and q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[2] == D and q.is_contiguous(), "q: contiguous bf16 [T, Hq, 128]")
+    t, hq, _ = q.shape
+    for c in (k_cache, v_cache):
+        _need(c.dim() == 4 and c.dtype == torch.bfloat16 and c.shape[3] == D and c.is_contiguous() and c.device == q.device and c.shape == k_cache.shape,
+              "caches: contiguous bf16 [pages, kv heads, page size, 128] on the device of q")
+    nb, hkv, bs, _ = k_cache.shape
+    _need(nb > 0 and hkv > 0 and hq > 0 and hq % hkv == 0, f"{hq} query heads over {hkv} key/value heads")
+    _need(bs in (16, 32, 64, 128, 256), f"page size {bs}: 16, 32, 64, 128 or 256 expected")
+    _need(block_table.dim() == 2 and block_table.shape[1] > 0, "block_table: int32 [sequences, pages]")
+    b = block_table.shape[0]
+    _index(block_table, (b, block_table.shape[1]), q.device, "block_table")
+    _index(kv_len, (b,), q.device, "kv_len")
+    for x, what in ((gate, "gate"), (out, "out")):
+        _need(x is None or (x.dtype == q.dtype and x.shape == q.shape and x.is_contiguous() and x.device == q.device), f"{what}: as q")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    _need(0.0 < scale < math.inf, f"scale {scale}: positive expected")
+    _need(0.0 <= cap < math.inf, f"cap {cap}: positive, or 0 for none")
+    return t, hq, nb, hkv, bs, b, scale, torch.empty_like(q) if out is None else out
+
+
+def rotary_axes(sections, interleaved: bool = False) -> tuple[int, ...]:
+    """Axis of every rotary pair from the number of pairs of each axis: one block per axis, or - ``interleaved`` - the axes in
+    turn (T H W T H W ..), where pairs that no other axis claims stay on the first."""
+    sections = [int(n) for n in sections]
+    _need(sections and min(sections) >= 0 and 0 < sum(sections) <= D // 2, f"sections {sections}: 1 to {D // 2} pairs in all expected")
+    if not interleaved:
+        return tuple(a for a, n in enumerate(sections) for _ in range(n))
+    axes = [0] * sum(sections)
+    for a, n in enumerate(sections[1:], 1):
+        _need(n == 0 or a + len(sections) * (n - 1) < len(axes), f"sections {sections}: axis {a} is too long to take turns")
+        axes[a:a + len(sections) * n:len(sections)] = [a] * n
+    return tuple(axes)
+
+
+def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_off, v_src, v_off, q_gamma, k_gamma,
+                             unit_offset, eps, inv_freq, axes, positions, slots, k_cache, v_cache, n_q_heads, n_kv_heads,
+                             mscale: float = 1.0):
+    """``qk_norm_rope_append`` with rotary positions of several axes: pair i turns by ``positions[axes[i], t] * inv_freq[i]``.
+
+    ``axes`` from ``rotary_axes`` (a multiple of 4 pairs); ``positions`` int32 [axes, T]; ``slots`` int32 [T], distinct; rows
+    with a negative slot are not cached.  Returns (q [T, Hq, 128], gate [T, Hq, 128] or None).
+    """
+    t, dev = q_src.shape[0], q_src.device
+    for x, last, what in ((q_src, q_off + (n_q_heads - 1) * q_head_stride + (2 * D if gate_in_q else D), "q_src"),
+                          (k_src, k_off + n_kv_heads * D, "k_src"), (v_src, v_off + n_kv_heads * D, "v_src")):
+        _need(x.is_cuda and x.dim() == 2 and x.dtype == torch.bfloat16 and x.shape[0] == t and x.stride(1) == 1 and x.device == dev and
+              x.data_ptr() % 8 == 0 and last <= x.shape[1], f"{what}: bf16 [{t}, >= {last}] with contiguous rows on {dev} expected")
+    _need(min(q_off, k_off, v_off) >= 0 and q_head_stride >= 0, "offsets of heads begin at 0")
+    _need(not any(x % 4 for x in (q_off, q_head_stride, k_off, v_off)) and not any(x.stride(0) % 4 for x in (q_src, k_src, v_src)),
+          "offsets and row strides: multiples of 4")
+    for c in (k_cache, v_cache):
+        _need(c.dim() == 4 and c.dtype == torch.bfloat16 and c.shape[1] == n_kv_heads and c.shape[3] == D and c.is_contiguous() and
+              c.device == dev and c.shape == k_cache.shape, "caches: contiguous bf16 [pages, kv heads, page size, 128]")
+    for g in (q_gamma, k_gamma):
+        _need(g is None or (g.dtype == torch.bfloat16 and g.numel() == D and g.is_contiguous() and g.device == dev), "gammas: bf16 [128]")
+    _need(n_q_heads > 0 and n_kv_heads > 0 and len(axes) % 4 == 0 and 0 < len(axes) <= D // 2 and min(axes) >= 0, "axes: 4, 8 .. 64 pairs")
+    _need(inv_freq.dtype == torch.float32 and inv_freq.numel() == len(axes) and inv_freq.is_contiguous() and inv_freq.device == dev,
+          "inv_freq: fp32, one per pair")
+    _need(positions.dim() == 2 and positions.shape[0] > max(axes), f"positions: a row for each of {max(axes) + 1} axes expected")
+    _index(positions, (positions.shape[0], t), dev, "positions")
+    _index(slots, (t,), dev, "slots")
+    q_out = torch.empty(t, n_q_heads, D, dtype=torch.bfloat16, device=dev)
+    gate_out = torch.empty_like(q_out) if gate_in_q else None
+    if t == 0:
+        return q_out, gate_out
+    with torch.cuda.device(dev):
+        _lib.check_indices(slots, 0, k_cache.shape[0] * k_cache.shape[2], 2, keep=-1)
+        rc = _lib.lib().b200_qk_norm_rope_axes_append(
+            _lib.ptr(q_src), q_src.stride(0), q_off, q_head_stride, int(gate_in_q),
+            _lib.ptr(k_src), k_src.stride(0), k_off, _lib.ptr(v_src), v_src.stride(0), v_off,
+            _lib.ptr(q_gamma), _lib.ptr(k_gamma), int(unit_offset), _f(eps), _lib.ptr(inv_freq), 2 * len(axes), _f(mscale), bytes(axes),
+            positions.shape[0], _lib.ptr(positions), t, _lib.ptr(slots), _lib.ptr(q_out), _lib.ptr(gate_out), _lib.ptr(k_cache),
+            _lib.ptr(v_cache), k_cache.shape[0], k_cache.shape[2], t, n_q_heads, n_kv_heads, _lib.stream())
+    _lib.check(rc, "qk_norm_rope_axes_append")
+    return q_out, gate_out
+
+
+def visible_spans(kv_len: int, documents=None, blocks=(), window: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """``lo``, ``hi`` int32 [kv_len] (host) of the positions of one sequence: causal within each of ``documents`` (lengths that add
+    up to ``kv_len``), not further back than ``window`` keys, and inside a block ``(first, end)`` - an image, a prefix - up to
+    the block's end."""
+    pos = torch.arange(kv_len)
+    lo, hi = torch.zeros_like(pos), pos + 1
+    if documents is not None:
+        lengths = torch.as_tensor(documents, dtype=torch.long).reshape(-1)
+        _need(int(lengths.sum()) == kv_len and bool((lengths >= 0).all()), f"documents of {int(lengths.sum())} tokens in a context of {kv_len}")
+        lo = torch.repeat_interleave(lengths.cumsum(0) - lengths, lengths)
+    if window > 0:
+        lo = torch.maximum(lo, pos + 1 - window)
+    for first, end in blocks:
+        _need(0 <= first <= end <= kv_len, f"block ({first}, {end}) in a context of {kv_len}")
+        hi[first:end] = end
+    return lo.to(torch.int32), hi.to(torch.int32)
+
+
+def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_q_len, lo=None, hi=None, gate=None, scale=None,
+                  cap: float = 0.0, max_kv_len: int | None = None, splits: int | None = None, out=None):
+    """Attention of new rows against the paged cache (which already holds their keys and values), every row over a span of keys
+    of its own: row t sees ``lo[t] <= j < min(hi[t], kv_len)`` of its sequence - documents in one context, blocks that see each
+    other, prefixes, windows (``visible_spans``).  Without ``lo`` the span begins at 0, without ``hi`` it is causal.
+    ``cap`` > 0: a score s becomes cap tanh(s / cap).  A row that sees nothing is 0; a key outside a row's span has no part in
+    it, whatever the cache holds there.
+
+    q: [T, Hq, 128]; block_table [B, max_blocks], q_start / q_len / kv_len [B], lo / hi [T]: int32 device tensors.  Rows of no
+    sequence are not written (``out``: where to write).  ``max_kv_len`` bounds the contexts, for the choice of ``splits``.
+    """
+    t, hq, nb, hkv, bs, b, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
+    _index(q_start, (b,), q.device, "q_start")
+    _index(q_len, (b,), q.device, "q_len")
+    for x, what in ((lo, "lo"), (hi, "hi")):
+        if x is not None:
+            _index(x, (t,), q.device, what)
+    max_q_len = min(int(max_q_len), t)
+    if t == 0 or b == 0 or max_q_len <= 0:
+        return out
+    if splits is None:
+        g = hq // hkv
+        tiles = hkv * min(b * -(-max_q_len * g // ROW_TILE), t * g // ROW_TILE + b)
+        keys = -(-(max_kv_len if max_kv_len is not None else block_table.shape[1] * bs) // KEY_TILE)
+        splits = max(1, min(NUM_SMS // tiles, keys // 2))
+    _need(1 <= splits <= 1024, f"{splits} splits")
+    with torch.cuda.device(q.device):
+        ws = torch.empty(splits * t * hq * (D + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+        _lib.check_indices(block_table, 0, nb, 3)
+        rc = _lib.lib().b200_attn_spans(
+            _lib.ptr(q), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(out), _lib.ptr(gate), _lib.ptr(block_table), _lib.ptr(q_start),
+            _lib.ptr(q_len), _lib.ptr(kv_len), _lib.ptr(lo), _lib.ptr(hi), b, max_q_len, t, block_table.shape[1], nb, bs, hq, hkv, _f(scale),
+            _f(cap), splits, _lib.ptr(ws), _lib.ptr(_lib.status_word(q.device)), _lib.stream())
+    _lib.check(rc, "prefill_spans", 2 if splits > 1 else 1)
+    return out
+
+
+def shared_groups(pages, block_size: int) -> tuple[list[int], list[int]]:
+    """``group_start``, ``shared_len`` for ``decode_shared`` from the page lists of the sequences, in batch order: neighbours with the
+    same first page form a group, which shares their common leading pages (a sequence alone shares nothing)."""
+    start, shared, b = [0], [], 0
+    pages = [[int(x) for x in row] for row in pages]
+    while b < len(pages):
+        e, n = b + 1, len(pages[b])
+        while e < len(pages) and n and pages[e][:1] == pages[b][:1]:
+            n = next((i for i, (x, y) in enumerate(zip(pages[b][:n], pages[e])) if x != y), min(n, len(pages[e])))
+            e += 1
+        start.append(e)
+        shared.append(n * block_size if e - b > 1 else 0)
+        b = e
+    return start, shared
+
+
+def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_len, gate=None, scale=None, cap: float = 0.0,
+                  max_shared: int | None = None, max_kv_len: int | None = None, splits: tuple[int, int] | None = None, out=None):
+    """``decode`` (one query row per sequence) where groups of sequences hold the same leading pages, as a prefix cache hands them
+    out: those keys are read and multiplied once for the whole group.
+
+    q: [B, Hq, 128]; group_start int32 [groups + 1], shared_len int32 [groups] (device; ``shared_groups``): the rows
+    group_start[g] .. group_start[g + 1] - 1 of ``block_table`` begin with the same pages, whose first shared_len[g] keys they have
+    in common (keys at ``kv_len`` and beyond stay unseen); rows of no group are on their own.  ``cap`` as in ``prefill_spans``;
+    ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys, of a sequence's own)."""
+    t, hq, nb, hkv, bs, b, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
+    _need(b == t, f"{t} rows for {b} sequences")
+    _need(shared_len.dim() == 1, "shared_len: int32 [groups]")
+    n = shared_len.shape[0]
+    _index(shared_len, (n,), q.device, "shared_len")
+    _index(group_start, (n + 1,), q.device, "group_start")
+    if b == 0:
+        return out
+    if splits is None:
+        longest = max_kv_len if max_kv_len is not None else block_table.shape[1] * bs
+        common = 0 if n == 0 else longest if max_shared is None else min(longest, max(0, int(max_shared)))
+        keys, own_keys = -(-common // KEY_TILE), -(-(longest - common) // KEY_TILE) + 1
+        tiles = (b * (hq // hkv) // ROW_TILE + n) * hkv
+        share = (tiles * keys + b * hkv * own_keys) / NUM_SMS             # key tiles of an SM
+        splits = (max(1, min(64, round(keys / max(2.0, share)))), max(1, min(64, round(own_keys / max(4.0, share)))))
+    _need(1 <= min(splits) and max(splits) <= 1024, f"splits {splits}")
+    with torch.cuda.device(q.device):
+        ws = torch.empty(sum(splits) * b * hq * (D + 2), dtype=torch.float32, device=q.device)
+        _lib.check_indices(block_table, 0, nb, 3)
+        rc = _lib.lib().b200_attn_shared(
+            _lib.ptr(q), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(out), _lib.ptr(gate), _lib.ptr(block_table), _lib.ptr(kv_len),
+            _lib.ptr(group_start), _lib.ptr(shared_len), n, b, block_table.shape[1], nb, bs, hq, hkv, _f(scale), _f(cap), splits[0], splits[1],
+            _lib.ptr(ws), _lib.ptr(_lib.status_word(q.device)), _lib.stream())
+    _lib.check(rc, "decode_shared", 2)
+    return out
+
+
 # ---------------------------------------------------------------- fp32 oracles
 def rope_ref(x, positions, inv_freq, rot):
     """Half-split rotation over the first ``rot`` dims. x: [T, H, D] fp32."""
