@@ -38,6 +38,11 @@ constexpr int BKV = 128;          // keys per tile
 constexpr int ATOM = 16384;       // bytes of one [128 x 64] bf16 swizzled slab
 constexpr int TILE = 2 * ATOM;
 constexpr int STAGES = 5;
+#ifndef EMU
+#define EMU 2
+#endif
+constexpr int EMULATED = EMU;       // of 8 pairs of exponentials: those on the arithmetic units
+constexpr int ITEMS = 4;          // items the producer may be ahead of the slowest role
 constexpr int NTHREADS = 384;
 constexpr int SMEM_BYTES = 1024 + (2 + STAGES) * TILE + 2048;
 static_assert(SMEM_BYTES <= 232448, "shared memory of a block");
@@ -85,6 +90,25 @@ constexpr uint32_t idesc_pv = umma_idesc_bf16(128, 128) | (1u << 16);   // B is 
 __device__ __forceinline__ void tmem_ld_32x1(uint32_t taddr, uint32_t& v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr) : "memory");
 }
+// mbar_wait for a whole warp, each lane on a barrier of its own if it likes: no lane leaves the loop before the others, so that the
+// warp stays converged (its addresses and ring places are in uniform registers).  false: not all phases have come in time.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  uint64_t t0 = 0;
+  for (uint32_t n = 1;; ++n) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((n & 255) == 0) {
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (__any_sync(0xffffffffu, now - t0 > B200_WAIT_BUDGET_NS)) return false;
+    }
+  }
+}
+__device__ __forceinline__ void l2_prefetch(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy16_async(void* smem, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(src) : "memory");
+}
 // Two fp32 operations per instruction.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;
@@ -108,9 +132,71 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of two numbers below 128 on the arithmetic units: 2^round(x) by the exponent bits, 2^f of the rest, |f| <= 1/2, by a cubic with
+// constant term 1 (fitted to the relative error, 1e-4: P is rounded to 2^-9).  From -127 down the result is exactly zero.  Not for NaN.
+__device__ __forceinline__ void exp2_fma(float& a, float& b) {
+  constexpr float BIG = 12582912.f;                          // 1.5 2^23: the sum's low bits are the rounded integer
+  constexpr float E1 = 0.693282961845398f, E2 = 0.24221111834049225f, E3 = 0.05500898137688637f;
+  const uint64_t x = pack2(fmaxf(a, -127.f), fmaxf(b, -127.f));
+  const uint64_t r = add2(x, pack2(BIG, BIG));
+  const uint64_t f = add2(x, fma2(r, pack2(-1.f, -1.f), pack2(BIG, BIG)));
+  uint64_t y = fma2(f, pack2(E3, E3), pack2(E2, E2));
+  y = fma2(y, f, pack2(E1, E1));
+  y = fma2(y, f, pack2(1.f, 1.f));
+  float r0, r1, y0, y1;
+  unpack2(r, r0, r1);
+  unpack2(y, y0, y1);
+  a = __int_as_float(__float_as_int(y0) + (__float_as_int(r0) << 23));
+  b = __int_as_float(__float_as_int(y1) + (__float_as_int(r1) << 23));
+}
+
+// Scores s to tanh(k s).  On [-1, 1], where scores hardly ever leave, tanh(z) = z P(z^2) with an interpolation of tanh(z) / z at
+// Chebyshev points, off by 5e-7 at most, on the arithmetic units: two exponential units' steps per score cost as much as both
+// products.  NaN stays.
+__device__ __forceinline__ void cap_scores(uint32_t (&sv)[2][32], float k) {
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < 64; i += 2) big = max3(big, fabsf(__uint_as_float(sv[i >> 5][i & 31])), fabsf(__uint_as_float(sv[i >> 5][(i & 31) + 1])));
+  if (__all_sync(0xffffffffu, big * k <= 1.f)) {
+    constexpr float C[6] = {0.9999994039535522f, -0.3332895040512085f, 0.1328072100877762f, -0.0515859872102737f, 0.0167208556085825f, -0.0030582291074097f};
+    const uint64_t k2 = pack2(k, k);
+#pragma unroll
+    for (int i = 0; i < 64; i += 8) {                        // four chains of two
+      uint64_t z[4], u[4], y[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        z[x] = mul2(pack2(__uint_as_float(sv[i >> 5][(i & 31) + 2 * x]), __uint_as_float(sv[i >> 5][(i & 31) + 2 * x + 1])), k2);
+        u[x] = mul2(z[x], z[x]);
+        y[x] = fma2(u[x], pack2(C[5], C[5]), pack2(C[4], C[4]));
+      }
+#pragma unroll
+      for (int d = 3; d >= 0; --d)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) y[x] = fma2(y[x], u[x], pack2(C[d], C[d]));
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float a, b;
+        unpack2(mul2(y[x], z[x]), a, b);
+        sv[i >> 5][(i & 31) + 2 * x] = __float_as_uint(a);
+        sv[i >> 5][(i & 31) + 2 * x + 1] = __float_as_uint(b);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 64; ++i)
+      sv[i >> 5][i & 31] = __float_as_uint(1.f - 2.f * __fdividef(1.f, 1.f + exp2f(__uint_as_float(sv[i >> 5][i & 31]) * k * 2.885390081777927f)));
+  }
+}
+
 // One piece of work; the same in every thread of a warp.
 struct Item {
-  int n_rows;            // rows of the tile that are there (0: no such item)
+  int n_rows;            // rows of the tile that are there (0: the list has ended)
   int r0;                // first of them among the packed rows of base_tok
   int base_tok;          // q row of packed row 0
   int kvh, trow, slot;   // kv head; row of the block table; slot of the partial sums
@@ -120,6 +206,7 @@ struct Item {
   int kv_end;            // keys of the sequence
   int own_lo, own_hi;    // span of rows that have no span of their own (one row per sequence)
   int delta;             // position of a token minus its q row (prompt rows)
+  int pad;
   __device__ __forceinline__ bool dual() const { return n_rows <= BQ; }
   __device__ __forceinline__ int steps() const { return dual() ? t1 - t0 : 2 * (t1 - t0); }
 };
@@ -147,20 +234,39 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
       split = idx % p.splits;
       splits = p.splits;
       it.kvh = idx / p.splits % p.Hkv;
-      int tile = idx / (p.splits * p.Hkv), g = 0, b0 = 0, rows = 0;
-      for (; g < p.n_groups; ++g) {
-        b0 = max(0, min(p.batch, p.group_start[g]));
-        rows = max(0, min(p.batch, p.group_start[g + 1]) - b0) * p.G;
-        const int tiles = (rows + 2 * BQ - 1) / (2 * BQ);
-        if (tile < tiles) break;
-        tile -= tiles;
+      int tile = idx / (p.splits * p.Hkv), b0 = 0, rows = -1, shared = 0;
+      for (int base = 0; base < p.n_groups && rows < 0; base += 32) {      // a group per lane
+        const int g = base + lane;
+        int first = 0, n = 0, sh = 0;
+        if (g < p.n_groups) {
+          first = max(0, min(p.batch, p.group_start[g]));
+          n = max(0, min(p.batch, p.group_start[g + 1]) - first) * p.G;
+          sh = p.shared_len[g];
+        }
+        const int tiles = (n + 2 * BQ - 1) / (2 * BQ);
+        int upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += x;
+        }
+        const uint32_t here = __ballot_sync(0xffffffffu, tile < upto);
+        if (here) {
+          const int src = __ffs(here) - 1;
+          b0 = __shfl_sync(0xffffffffu, first, src);
+          rows = __shfl_sync(0xffffffffu, n, src);
+          shared = __shfl_sync(0xffffffffu, sh, src);
+          tile -= __shfl_sync(0xffffffffu, upto - tiles, src);
+        } else {
+          tile -= __shfl_sync(0xffffffffu, upto, 31);
+        }
       }
-      if (g == p.n_groups) return false;
+      if (rows < 0) return false;
       it.base_tok = it.trow = b0;
       it.r0 = tile * 2 * BQ;
       rows_all = rows;
       it.own_lo = 0;
-      it.own_hi = p.shared_len[g];
+      it.own_hi = shared;
       it.slot = split;
       if (it.own_hi <= 0) return false;                    // (the join does not look at its slots either)
     } else {                                               // a sequence's own keys
@@ -172,9 +278,10 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
       it.base_tok = it.trow = b;
       it.r0 = 0;
       rows_all = p.G;
-      it.own_lo = 0;
-      for (int g = 0; g < p.n_groups; ++g)
-        if (b >= p.group_start[g] && b < p.group_start[g + 1]) it.own_lo = max(0, p.shared_len[g]);
+      int shared = 0;
+      for (int g = lane; g < p.n_groups; g += 32)
+        if (b >= p.group_start[g] && b < p.group_start[g + 1]) shared = max(shared, p.shared_len[g]);
+      it.own_lo = __reduce_max_sync(0xffffffffu, shared);
       it.own_hi = 0x7fffffff;
       it.slot = p.splits + split;
     }
@@ -225,6 +332,13 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
   return true;
 }
 
+static_assert(sizeof(Item) == 64, "copied as four 16-byte words");
+
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
 struct Ring {
   int st;
   uint32_t ph;
@@ -235,6 +349,10 @@ struct Ring {
     const int s = st + n, w = s / STAGES;
     st = s - w * STAGES;
     ph ^= w & 1;
+  }
+  __device__ __forceinline__ void two() {
+    st += 2;
+    if (st >= STAGES) { st -= STAGES; ph ^= 1; }
   }
 };
 
@@ -251,28 +369,39 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   uint64_t* v_ok = bars + 2 * STAGES;                       // values checked (tile by tile, not by place in the ring)
   uint64_t* q_full = bars + 3 * STAGES;                     // per stream: queries there, O zero
   uint64_t* s_full = q_full + 2;
-  uint64_t* p_full = q_full + 4;
-  uint64_t* o_full = q_full + 6;
-  uint64_t* j_full = q_full + 8;                            // stream 1's part lies in the scratch
-  uint64_t* j_empty = q_full + 9;                           // and has been read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 10);
+  uint64_t* p_half = q_full + 4;                            // P of the tile's first 64 keys
+  uint64_t* p_full = q_full + 6;
+  uint64_t* o_full = q_full + 8;
+  uint64_t* j_full = q_full + 10;                           // stream 1's part lies in the scratch
+  uint64_t* j_empty = q_full + 11;                          // and has been read
+  uint64_t* i_full = q_full + 12;                           // items
+  uint64_t* i_empty = i_full + ITEMS;
+  uint64_t* pv_half = i_empty + ITEMS;                      // per stream: the product with the values of a tile's first 64 keys
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_half + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* s_bad = reinterpret_cast<uint32_t*>(bars + 32); // [STAGES][4] keys with values that are not finite
-  float* s_ml = reinterpret_cast<float*>(bars + 48);        // [2][128] maximum and sum of stream 1
+  uint32_t* s_bad = reinterpret_cast<uint32_t*>(bars + 48); // [STAGES][4] keys with values that are not finite
+  float* s_ml = reinterpret_cast<float*>(bars + 58);        // [2][128] maximum and sum of stream 1
+  Item* s_item = reinterpret_cast<Item*>(bars + 58 + 128);  // [ITEMS]
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform: the issuer depends on it
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&r_full[i], 1);
       mbar_init(&r_empty[i], 1);
-      mbar_init(&v_ok[i], 2);
+      mbar_init(&v_ok[i], 1);
     }
     for (int m = 0; m < 2; ++m) {
       mbar_init(&q_full[m], 4);
       mbar_init(&s_full[m], 1);
+      mbar_init(&p_half[m], 4);
       mbar_init(&p_full[m], 4);
       mbar_init(&o_full[m], 1);
     }
+    for (int i = 0; i < ITEMS; ++i) {
+      mbar_init(&i_full[i], 1);
+      mbar_init(&i_empty[i], 10);
+    }
+    for (int m = 0; m < 2; ++m) mbar_init(&pv_half[m], 1);
     mbar_init(j_full, 4);
     mbar_init(j_empty, 4);
     *abort_flag = 0;
@@ -290,9 +419,24 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   pdl_wait();
 
   Item it;
-  // registers per thread at launch: 168 (3 x 168 = 2 x 216 + 72)
+  // The next item, in shared memory: every role but the producer, which has put it there.
+  int i_at = 0;
+  uint32_t i_ph = 0;
+  auto next_item = [&]() -> bool {
+    bool ok = warp_wait(&i_full[i_at], i_ph) && !*abort_flag;
+    if (!ok) return false;
+    const int4* src = reinterpret_cast<const int4*>(s_item + i_at);
+    int4* dst = reinterpret_cast<int4*>(&it);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = src[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[i_at]);
+    if (++i_at == ITEMS) { i_at = 0; i_ph ^= 1; }
+    return true;
+  };
+  // registers per thread at launch: 168 (3 x 168 = 2 x 224 + 56)
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     Ring r = {0, 0}, c = {0, 0};                           // places of tiles in the ring; of value tiles among their checks
     bool ok = true;
     if (warp == 8) {
@@ -303,8 +447,32 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         tma_prefetch_desc(&tmV);
       }
       r.ph = 1;
-      for (int idx = blockIdx.x; ok && idx < p.n_items; idx += gridDim.x) {
-        if (!get_item<SHARED>(p, idx, lane, it)) continue;
+      bool more = true;
+      for (int round = 0; ok && more; ++round) {
+        // items come longest first: every other round is dealt in the opposite order
+        const int idx = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        more = round * gridDim.x < p.n_items;
+        it.n_rows = 0;
+        if (more && (idx >= p.n_items || !get_item<SHARED>(p, idx, lane, it))) continue;
+        ok = warp_wait(&i_empty[i_at], i_ph ^ 1) && !*abort_flag;
+        if (!ok) break;
+        if (lane == 0) {
+          int4* dst = reinterpret_cast<int4*>(s_item + i_at);
+          const int4* src = reinterpret_cast<const int4*>(&it);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = src[i];
+          mbar_arrive(&i_full[i_at]);
+        }
+        if (++i_at == ITEMS) { i_at = 0; i_ph ^= 1; }
+        if (!more) break;
+        {                                                                  // queries and gate on their way to L2
+          const int tok0 = it.base_tok + it.r0 / p.G, tok1 = it.base_tok + (it.r0 + it.n_rows - 1) / p.G;
+          for (int t = tok0 + lane; t <= tok1; t += 32) {
+            const size_t at = ((size_t)t * p.Hq + it.kvh * p.G) * D;
+            l2_prefetch(p.q + at, p.G * D * 2);
+            if (p.gate && !p.part_o) l2_prefetch(p.gate + at, p.G * D * 2);
+          }
+        }
         const int* bt = p.block_table + (size_t)it.trow * p.max_blocks;
         const int last_page = (it.k_end - 1) / p.bs;
         auto page_row = [&](int tile) {                                    // cache row where this lane's part of a tile begins
@@ -318,7 +486,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           const int next_row = page_row(t + 1);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&r_empty[r.st], r.ph)) && !*abort_flag;
+            ok = warp_wait(&r_empty[r.st], r.ph) && !*abort_flag;
             if (!ok) break;
             if (lane == 0) mbar_expect_tx(&r_full[r.st], n * 2 * sub_bytes);
             __syncwarp();
@@ -334,82 +502,89 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       }
       if (!ok && lane == 0) { atomicExch(p.status, ERR_WAIT_STAGE); *abort_flag = 1; }
     } else if (warp == 9) {
-      // The whole warp walks the loop, so that addresses and descriptors stay warp-uniform, and one elected lane issues.
+      // The whole warp walks the loop, so that addresses and descriptors stay warp-uniform, and one elected lane issues.  What a step
+      // costs beside the products is as long as they are if it is not kept short: even lanes wait for one barrier while odd lanes
+      // wait for another, and what the streams share is waited for once.
       const uint32_t on = elect_one();
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar, parity)) && !*abort_flag;
+      auto wait2 = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+        ok = warp_wait(lane & 1 ? b : a, lane & 1 ? pb : pa);
         return ok;
       };
-      const uint64_t dq = umma_desc_sw128(sQ), dk = umma_desc_sw128(sR), dv = desc_mn_sw128(sR, ATOM, 1024);
+      const uint64_t dq0 = umma_desc_sw128(sQ), dk = umma_desc_sw128(sR), dv = desc_mn_sw128(sR, ATOM, 1024);
       uint32_t ph_q[2] = {0, 0}, ph_p[2] = {0, 0};
-      for (int idx = blockIdx.x; ok && idx < p.n_items; idx += gridDim.x) {
-        if (!get_item<SHARED>(p, idx, lane, it)) continue;
+      Ring k = {0, 0}, v = {1, 0};                         // places of the next key tile and the next value tile
+      for (;;) {
+        if (ok) ok = next_item();
+        if (!ok || it.n_rows == 0) break;
         const int steps = it.steps();
         if (steps == 0) continue;
         const bool dual = it.dual();
-        Ring k = r;                                        // keys of the tile whose scores come next
-        auto issue_s = [&](int u) {
-          const int m = u & 1;
-          if (!wait(&r_full[k.st], k.ph)) return;
-          tc_fence_after();
-          const uint64_t a = dq + (dual ? 0 : m * (TILE >> 4)), b = dk + k.st * (TILE >> 4);
+        auto scores = [&](const int m) {                   // of the tile at k, which is there
+          const uint64_t a = dq0 + (dual ? 0 : m * (TILE >> 4)), b = dk + k.st * (TILE >> 4);
 #pragma unroll
           for (int s = 0; s < 8; ++s)
             umma_bf16_ss_warp(on, tmem + m * 128, a + (s >> 2) * (ATOM >> 4) + 2 * (s & 3), b + (s >> 2) * (ATOM >> 4) + 2 * (s & 3), idesc_qk,
                               s ? 1u : 0u);
+          umma_commit_warp(on, &s_full[m]);
           if (dual || m) {
             umma_commit_warp(on, &r_empty[k.st]);
-            k.skip(2);
+            k.two();
           }
-          umma_commit_warp(on, &s_full[m]);
         };
 #pragma unroll
         for (int m = 0; m < 2; ++m)
-          if (ok && m < steps && wait(&q_full[m], ph_q[m])) {
+          if (ok && m < steps && wait2(&q_full[m], ph_q[m], &r_full[k.st], k.ph)) {
             ph_q[m] ^= 1;
-            issue_s(m);
+            tc_fence_after();
+            scores(m);
           }
-        for (int u = 0; ok && u < steps; ++u) {
-          const int m = u & 1;
-          if (dual || m == 0) {
-            if (u) r.next();
-            r.next();                                      // r: values of this step's tile
-          }
-          if (!wait(&p_full[m], ph_p[m]) || !wait(&v_ok[c.st], c.ph)) break;
-          ph_p[m] ^= 1;
-          tc_fence_after();
-          const uint64_t b = dv + r.st * (TILE >> 4);
+        for (int u0 = 0; ok && u0 < steps; u0 += 2) {
 #pragma unroll
-          for (int s = 0; s < 8; ++s) umma_bf16_ts_warp(on, tmem + 256 + m * 128, tmem + m * 128 + s * 8, b + s * 128, idesc_pv, 1u);
-          if (dual || m) {
-            umma_commit_warp(on, &r_empty[r.st]);
-            c.next();
+          for (int m = 0; m < 2; ++m) {
+            const int u = u0 + m;
+            if (!ok || u >= steps) break;
+            if (!wait2(&p_half[m], ph_p[m], &v_ok[c.st], c.ph)) break;
+            tc_fence_after();
+            const uint64_t b = dv + v.st * (TILE >> 4);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) umma_bf16_ts_warp(on, tmem + 256 + m * 128, tmem + m * 128 + s * 8, b + s * 128, idesc_pv, 1u);
+            umma_commit_warp(on, &pv_half[m]);
+            const bool more = u + 2 < steps;
+            if (!wait2(&p_full[m], ph_p[m], more ? &r_full[k.st] : &p_full[m], more ? k.ph : ph_p[m])) break;
+            ph_p[m] ^= 1;
+            tc_fence_after();
+#pragma unroll
+            for (int s = 4; s < 8; ++s) umma_bf16_ts_warp(on, tmem + 256 + m * 128, tmem + m * 128 + s * 8, b + s * 128, idesc_pv, 1u);
+            if (dual || m) {
+              umma_commit_warp(on, &r_empty[v.st]);
+              v.two();
+              c.next();
+            }
+            if (more) scores(m);
+            else umma_commit_warp(on, &o_full[m]);
           }
-          if (u + 2 < steps) issue_s(u + 2);
-          else umma_commit_warp(on, &o_full[m]);
         }
-        r.next();
       }
       if (!ok && lane == 0) { atomicExch(p.status, ERR_WAIT_TMA); *abort_flag = 1; }
-    } else {
-      const int w = warp - 10;                             // keys 64 w .. 64 w + 63 of a tile, lane: two of them
-      for (int idx = blockIdx.x; ok && idx < p.n_items; idx += gridDim.x) {
-        if (!get_item<SHARED>(p, idx, lane, it)) continue;
+    } else if (warp == 10) {
+      for (;;) {
+        if (ok) ok = next_item();
+        if (!ok || it.n_rows == 0) break;
         for (int t = it.t0; ok && t < it.t1; ++t) {
           r.next();
-          ok = __all_sync(0xffffffffu, mbar_wait(&r_full[r.st], r.ph)) && !*abort_flag;
+          ok = warp_wait(&r_full[r.st], r.ph) && !*abort_flag;
           if (!ok) break;
           const int key0 = t * BKV;
           if (key0 < it.lo_max || key0 + BKV > it.hi_min) {
             bool wrote = false;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int key = w * 64 + i * 32 + lane;
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+              const int key = i * 32 + lane;
               uint8_t* row = sR + r.st * TILE + key * 128;
               const bool there = key0 + key < it.k_end;
               uint32_t acc = 0;
               if (there) {
-#pragma unroll
+#pragma unroll 8
                 for (int d = 0; d < 16; ++d) {
                   const uint4 x = *reinterpret_cast<const uint4*>(row + (d >> 3) * ATOM + (((d & 7) ^ (key & 7)) << 4));
                   // bit 15 / 31 where an exponent is all ones
@@ -419,7 +594,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
               }
               const bool bad = (acc & 0x80008000u) != 0;
               const uint32_t mask = __ballot_sync(0xffffffffu, bad);
-              if (lane == 0) s_bad[c.st * 4 + w * 2 + i] = mask;
+              if (lane == 0) s_bad[c.st * 4 + i] = mask;
               if (bad || !there) {
                 wrote = true;
 #pragma unroll
@@ -437,24 +612,25 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       if (!ok && lane == 0) { atomicExch(p.status, ERR_WAIT_STAGE); *abort_flag = 1; }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int m = warp >> 2;                               // stream
     const int lr = threadIdx.x & 127;                      // row of the stream == TMEM lane
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + m * 128 + lane_off, tO = tmem + 256 + m * 128 + lane_off;
     uint32_t ph_s = 0, ph_o = 0, ph_j = 0;
-    Ring c = {0, 0};
+    Ring checks = {0, 0};
     bool alive = true;
-    for (int idx = blockIdx.x; alive && idx < p.n_items; idx += gridDim.x) {
-      if (!get_item<SHARED>(p, idx, lane, it)) continue;
+    for (;;) {
+      if (alive) alive = next_item();
+      if (!alive || it.n_rows == 0) break;
       const bool dual = it.dual();
       const int steps = it.steps();
       const int row = dual ? lr : threadIdx.x;             // of the item
       const bool row_ok = row < it.n_rows;
       const bool warp_on = __any_sync(0xffffffffu, row_ok);
       const int rr = it.r0 + min(row, it.n_rows - 1);
-      const int tok = it.base_tok + rr / p.G, head = it.kvh * p.G + rr % p.G;
-      const size_t at = (size_t)tok * p.Hq + head;         // row of q and out
+      const int tok = it.base_tok + rr / p.G;
+      const uint32_t at = (uint32_t)tok * p.Hq + it.kvh * p.G + rr % p.G;      // row of q and out
       int lo, hi;
       span_of<SHARED>(p, it, tok, lo, hi);
       float m_run = -INFINITY, l_run = 0.f;
@@ -462,13 +638,17 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       if (my_steps > 0) {
         if (warp_on) {
           if (!(dual && m)) {
-            uint8_t* dst = sQ + m * TILE + lr * 128;
-            const uint4* src = reinterpret_cast<const uint4*>(p.q + at * D);
+            // half a warp per row: whole lines on both sides
             uint4 x[16];
 #pragma unroll
-            for (int c = 0; c < 16; ++c) x[c] = src[c];
+            for (int i = 0; i < 16; ++i)
+              x[i] = reinterpret_cast<const uint4*>(p.q + (size_t)__shfl_sync(0xffffffffu, at, 2 * i + (lane >> 4)) * D)[lane & 15];
+            uint8_t* dst = sQ + m * TILE + ((lane >> 3) & 1) * ATOM + (warp & 3) * 4096;
 #pragma unroll
-            for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * ATOM + (((c & 7) ^ (lr & 7)) << 4)) = x[c];
+            for (int i = 0; i < 16; ++i) {
+              const int r = 2 * i + (lane >> 4);
+              *reinterpret_cast<uint4*>(dst + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = x[i];
+            }
             fence_proxy_async_smem();
           }
           uint32_t z[32];
@@ -484,87 +664,134 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       }
       for (int j = 0; j < my_steps; ++j) {
         const int t = dual ? 2 * j + m : j;                // tile of the item
-        bool ok = mbar_wait(&s_full[m], ph_s);
-        ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
-        if (!ok) { alive = false; break; }
+        if (!(alive = warp_wait(&s_full[m], ph_s) && !*abort_flag)) break;
         ph_s ^= 1;
+        const int key0 = (it.t0 + t) * BKV;
+        const bool edge = key0 < it.lo_max || key0 + BKV > it.hi_min;
         if (warp_on) {
           tc_fence_after();
-          uint32_t sv[4][32];                              // the row's 128 scores
+          // The tile's scores in halves of 64, each a step of the online softmax: the second half is loaded and its maximum found
+          // under the exponentials of the first, and the products with the first half's values begin before the
+          // second is done.  Cycles a tile of one warp alone / two warps of a scheduler, without the products: 1977 / 2853
+          // in one piece, 1396 / 2314 in halves, 1197 / 2098 with a quarter of the exponentials on the arithmetic units.
+          uint32_t sv[2][2][32];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32(tS + c * 32, sv[c]);
-          tmem_ld_wait();
-          const int key0 = (it.t0 + t) * BKV;
-          const bool edge = key0 < it.lo_max || key0 + BKV > it.hi_min;
-          const float scale = CAP ? 1.f : p.scale_log2;
-          if (CAP) {
-            const float k = p.cap_in, c = p.cap_out;
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 128; ++i) {
-              const float z = __uint_as_float(sv[i >> 5][i & 31]) * k;
-              const float e = exp2f(z * 2.885390081777927f);
-              sv[i >> 5][i & 31] = __float_as_uint(c - 2.f * c * __fdividef(1.f, 1.f + e));
+            for (int c = 0; c < 2; ++c) {
+              tmem_ld_32x32(tS + h * 64 + c * 32, sv[h][c]);
+              if (h == 0 && c == 1) tmem_ld_wait();
+            }
+          const float scale = CAP ? p.cap_out : p.scale_log2;
+          const uint64_t sc2 = pack2(scale, scale);
+          auto max_of = [&](const int h) {                 // independent chains
+            float mx[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(sv[h][0][i]);
+#pragma unroll
+            for (int i = 4; i < 60; i += 8)
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                mx[x] = max3(mx[x], __uint_as_float(sv[h][(i + 2 * x) >> 5][(i + 2 * x) & 31]), __uint_as_float(sv[h][(i + 2 * x + 1) >> 5][(i + 2 * x + 1) & 31]));
+            return scale * max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], __uint_as_float(sv[h][1][28]), __uint_as_float(sv[h][1][29])),
+                                max3(__uint_as_float(sv[h][1][29]), __uint_as_float(sv[h][1][30]), __uint_as_float(sv[h][1][31])));
+          };
+          float m_edge = -INFINITY;
+          if (edge) {                                      // both halves at once: their products wait for the check of the values
+            tmem_ld_wait();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (CAP) cap_scores(sv[h], p.cap_in);
+              const int a = lo - key0 - h * 64, b = hi - key0 - h * 64;          // bits [a, b) of these 64 stay
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const int x = min(32, max(0, a - c * 32)), y = min(32, max(0, b - c * 32));
+                const uint32_t seen = (uint32_t)((1ull << y) - 1) & ~(uint32_t)((1ull << x) - 1);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!(seen & (1u << i))) sv[h][c][i] = 0xff800000u;            // -inf
+              }
+              const float x = max_of(h);
+              m_edge = max3(m_edge, x, x);
             }
           }
-          if (edge) {
-            const int a = lo - key0, b = hi - key0;
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (i < a || i >= b) sv[i >> 5][i & 31] = 0xff800000u;      // -inf
-          }
-          float mx[8];                                     // independent chains
-#pragma unroll
-          for (int i = 0; i < 8; ++i) mx[i] = __uint_as_float(sv[0][i]);
-#pragma unroll
-          for (int i = 8; i < 128; ++i) mx[i & 7] = fmaxf(mx[i & 7], __uint_as_float(sv[i >> 5][i & 31]));
-          const float m_tile = scale * fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-          const float m_new = fmaxf(m_run, m_tile);
-          const bool grow = m_new > m_run + 8.f;           // (the first visible key: from -inf)
-          const float m_next = grow ? m_new : m_run;
-          if (__any_sync(0xffffffffu, grow && l_run != 0.f)) {
-            // the product that last added to O has finished: it was issued before the scores that arrived
-            const float alpha = grow ? exp2f(m_run - m_next) : 1.f;
-            l_run *= alpha;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t v[32];
-              tmem_ld_32x32(tO + c * 32, v);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-              tmem_st_32x32(tO + c * 32, v);
+          for (int h = 0; h < 2; ++h) {
+            float m_tile = h == 0 ? m_edge : -INFINITY;
+            if (!edge) {
+              if (h == 1) tmem_ld_wait();
+              if (CAP) cap_scores(sv[h], p.cap_in);
+              m_tile = max_of(h);
             }
-          }
-          m_run = m_next;
-          const float m_use = m_run == -INFINITY ? 0.f : m_run;          // (nothing visible yet: every exponential is zero)
-          const uint64_t sc2 = pack2(scale, scale), nm2 = pack2(-m_use, -m_use);
-          uint64_t sum2[2] = {0, 0};
+            // a score of NaN or +inf makes the whole row NaN, whatever the exponentials below give
+            if (!(m_tile < INFINITY)) l_run = __int_as_float(0x7fffffff);
+            const float m_new = fmaxf(m_run, m_tile);
+            const bool grow = m_new > m_run + 8.f;         // (the first visible key: from -inf)
+            const float m_next = grow ? m_new : m_run;
+            if (__any_sync(0xffffffffu, grow && l_run != 0.f)) {
+              // The product that last added to O has to have finished: the one of the tile before has, as it was issued before the scores
+              // that arrived; the first half's may be on its way.
+              if (h == 1 && !(alive = warp_wait(&pv_half[m], ph_s ^ 1))) break;
+              tc_fence_after();
+              const float alpha = !grow ? 1.f : exp2f(m_run - m_next);
+              l_run *= alpha;
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                uint32_t v[32];
+                tmem_ld_32x32(tO + c * 32, v);
+                tmem_ld_wait();
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                tmem_st_32x32(tO + c * 32, v);
+              }
+            }
+            m_run = m_next;
+            const float m_use = m_run == -INFINITY ? 0.f : m_run;        // (nothing visible yet: every exponential is zero)
+            const uint64_t nm2 = pack2(-m_use, -m_use);
+            uint64_t sum2[4] = {0, 0, 0, 0};
             uint32_t w[32];
+            float e[2][16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int kx = half * 64 + 2 * i;
-              float e0, e1;
-              unpack2(fma2(pack2(__uint_as_float(sv[kx >> 5][kx & 31]), __uint_as_float(sv[kx >> 5][(kx & 31) + 1])), sc2, nm2), e0, e1);
-              e0 = exp2f(e0);
-              e1 = exp2f(e1);
-              sum2[i & 1] = add2(sum2[i & 1], pack2(e0, e1));
-              __nv_bfloat162 x = __floats2bfloat162_rn(e0, e1);
-              w[i] = *reinterpret_cast<uint32_t*>(&x);
+            for (int b = 0; b < 5; ++b) {                  // 16 exponentials, then the sums and packing of the 16 before
+              if (b < 4) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  float &x = e[b & 1][2 * i], &y = e[b & 1][2 * i + 1];
+                  unpack2(fma2(pack2(__uint_as_float(sv[h][b >> 1][(b & 1) * 16 + 2 * i]), __uint_as_float(sv[h][b >> 1][(b & 1) * 16 + 2 * i + 1])), sc2, nm2), x, y);
+                  if (i >= 8 - EMULATED) {
+                    exp2_fma(x, y);
+                  } else {
+                    x = exp2f(x);
+                    y = exp2f(y);
+                  }
+                }
+              }
+              if (b > 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float x = e[(b - 1) & 1][2 * i], y = e[(b - 1) & 1][2 * i + 1];
+                  sum2[i & 3] = add2(sum2[i & 3], pack2(x, y));
+                  const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
+                  w[(b - 1) * 8 + i] = *reinterpret_cast<const uint32_t*>(&z);
+                }
+              }
             }
-            // 64 keys = 32 columns of packed pairs over this tile's own scores, which are all in registers by now
-            tmem_st_32x32(tS + half * 32, w);
+            tmem_st_32x32(tS + h * 32, w);                 // packed pairs over the first half's scores
+            tmem_st_wait();
+            if (h == 0 && !edge) {                         // (values that are not finite go to O before any product does)
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_half[m]);
+            }
+            float l0, l1;
+            unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), l0, l1);
+            l_run += l0 + l1;
           }
-          tmem_st_wait();
-          float l0, l1;
-          unpack2(add2(sum2[0], sum2[1]), l0, l1);
-          l_run += l0 + l1;
+          if (!alive) break;
           if (edge) {
-            Ring v = c;
+            Ring v = checks;
             v.skip(t);
-            bool ok2 = __all_sync(0xffffffffu, mbar_wait(&v_ok[v.st], v.ph));
-            if (!ok2) { alive = false; break; }
+            if (!(alive = warp_wait(&v_ok[v.st], v.ph))) break;
             for (int part = 0; part < 4; ++part)
               for (uint32_t bad = *(volatile uint32_t*)(s_bad + v.st * 4 + part); bad; bad &= bad - 1) {
                 // a key with values that are not finite: its row in shared memory is zero, the rows that see it add it here
@@ -573,6 +800,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 tmem_ld_32x1(tS + (kx >> 1), w);
                 tmem_ld_wait();
                 const float pv = __uint_as_float(kx & 1 ? w & 0xFFFF0000u : w << 16);
+                if (key >= it.k_end) continue;
                 const bool seen = key >= lo && key < hi && pv != 0.f;
                 const size_t vrow = ((size_t)p.block_table[(size_t)it.trow * p.max_blocks + key / p.bs] * p.Hkv + it.kvh) * p.bs + key % p.bs;
 #pragma unroll 1
@@ -591,137 +819,162 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[m]);
+        if (lane == 0) {
+          if (edge || !warp_on) mbar_arrive(&p_half[m]);
+          mbar_arrive(&p_full[m]);
+        }
       }
       if (!alive) break;
-      c.skip(it.t1 - it.t0);
+      checks.skip(it.t1 - it.t0);
+      const bool joined = dual && steps > 1;               // both streams have a part of every row
+      const bool writer = warp_on && !(dual && m);
+      const size_t row0 = (size_t)it.slot * p.T * p.Hq;    // of the partial sums
+      const int rows_here = min(32, it.n_rows - (row - lane));             // of this warp
+      uint8_t* own = sQ + m * TILE + (warp & 3) * 4096;    // this warp's 32 rows of the two slabs, which held its queries
+      auto load_gate = [&]() {                             // half a warp per row, as the queries lay
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const int r = 2 * i + (lane >> 4);
+          copy16_async(own + ((lane >> 3) & 1) * ATOM + r * 128 + (((lane & 7) ^ (r & 7)) << 4),
+                       p.gate + (size_t)__shfl_sync(0xffffffffu, at, r) * D + (lane & 15) * 8);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      const bool gated = p.gate && !p.part_o && writer;
+      // (this stream's score products have all finished: the scores of its last tile have arrived.  Stream 1's of a joined item
+      // read the same queries and may not have.)
+      if (gated && !joined) load_gate();
       if (my_steps > 0) {
-        const bool ok = mbar_wait(&o_full[m], ph_o);
-        if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+        if (!(alive = warp_wait(&o_full[m], ph_o))) break;
         ph_o ^= 1;
         tc_fence_after();
       }
-      // ---- results of the item: O / l, or O with (m, l) for the join of several items
-      const bool joined = dual && steps > 1;               // both streams have a part of every row
+      // ---- results of the item: O / l through the gate, or O with (m, l) for the join of several items.  A warp's rows go through
+      // the shared memory that held its queries, so that whole lines are stored: as bf16 over the gate, or in fp32
+      // 64 columns at a time, four columns of a row at place (column / 4, row ^ column / 4 mod 8).
+      if (!writer && !joined) continue;                    // (a stream without a part, or without rows: the others write)
       float w_own = 1.f, w_other = 0.f;
-      float4* s_o = reinterpret_cast<float4*>(sQ);         // [32][128 rows]
-      if (joined) {
-        if (m == 1) {
-          // (every score product of the item, which read the scratch as queries, was issued before the product this stream waited for)
+      auto staged = [&](int tile, int c4, int r) -> float4* {
+        return reinterpret_cast<float4*>(sQ + tile * TILE + (c4 >> 3) * ATOM + (warp & 3) * 4096 + (((c4 & 7) * 32 + (r ^ (c4 & 7))) << 4));
+      };
+#pragma unroll 1
+      for (int half = 0; half < 2 && alive; ++half) {
+        uint32_t v[2][32];
+        if (my_steps > 0) {
+          tmem_ld_32x32(tO + half * 64, v[0]);
+          tmem_ld_32x32(tO + half * 64 + 32, v[1]);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = 0;
+        }
+        auto four = [&](int i) {
+          return make_float4(__uint_as_float(v[i >> 3][4 * (i & 7)]), __uint_as_float(v[i >> 3][4 * (i & 7) + 1]), __uint_as_float(v[i >> 3][4 * (i & 7) + 2]),
+                             __uint_as_float(v[i >> 3][4 * (i & 7) + 3]));
+        };
+        if (joined && m == 1) {
           if (warp_on) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t u[32];
-              tmem_ld_32x32(tO + c * 32, u);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                s_o[(c * 8 + i) * 128 + lr] = make_float4(__uint_as_float(u[4 * i]), __uint_as_float(u[4 * i + 1]), __uint_as_float(u[4 * i + 2]), __uint_as_float(u[4 * i + 3]));
-            }
+            for (int i = 0; i < 16; ++i) *staged(1, i, lane) = four(i);
           }
           s_ml[lr] = m_run;
           s_ml[128 + lr] = l_run;
           __syncwarp();
           if (lane == 0) mbar_arrive(j_full);
-        } else {
-          const bool ok = mbar_wait(j_full, ph_j);
-          if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+          alive = warp_wait(j_empty, ph_j);                // it has been read
+          ph_j ^= 1;
+          continue;
         }
-        if (m == 0) {
-          const float m1 = s_ml[lr], l1 = s_ml[128 + lr];
-          const float mm = fmaxf(m_run, m1);
-          w_own = m_run == -INFINITY ? 0.f : exp2f(m_run - mm);
-          w_other = m1 == -INFINITY ? 0.f : exp2f(m1 - mm);
-          l_run = (l_run == 0.f ? 0.f : l_run * w_own) + (l1 == 0.f ? 0.f : l1 * w_other);
-          m_run = mm;
+        if (joined) {                                      // (then both streams' score products, which read the queries here, have finished)
+          alive = warp_wait(j_full, ph_j);
+          ph_j ^= 1;
+          if (!alive) break;
+          if (half == 0) {
+            const float m1 = s_ml[lr], l1 = s_ml[128 + lr], mm = fmaxf(m_run, m1);
+            w_own = m_run == -INFINITY ? 0.f : exp2f(m_run - mm);
+            w_other = m1 == -INFINITY ? 0.f : exp2f(m1 - mm);
+            l_run = (l_run == 0.f ? 0.f : l_run * w_own) + (l1 == 0.f ? 0.f : l1 * w_other);
+            m_run = mm;
+          }
         }
-      }
-      if (warp_on && !(dual && m)) {
-        if (p.part_o) {
-          const size_t prow = (size_t)it.slot * p.T * p.Hq + at;
-          if (row_ok) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m_run, l_run);
+        if (half == 0) {
+          if (p.part_o) {
+            if (row_ok) *reinterpret_cast<float2*>(p.part_ml + ((size_t)it.slot * p.T * p.Hq + at) * 2) = make_float2(m_run, l_run);
+          } else {
+            const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+            w_own *= inv;
+            w_other *= inv;
+          }
+        }
+        if (warp_on && p.part_o) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float4 o = four(i);
+            if (joined) {
+              const float4 x = *staged(1, i, lane);
+              o.x = o.x * w_own + x.x * w_other;
+              o.y = o.y * w_own + x.y * w_other;
+              o.z = o.z * w_own + x.z * w_other;
+              o.w = o.w * w_own + x.w * w_other;
+            }
+            *staged(m, i, lane) = o;
+          }
+          __syncwarp();
           if (steps) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + prow * D);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t u[32];
-              tmem_ld_32x32(tO + c * 32, u);
-              tmem_ld_wait();
-              if (row_ok) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  float4 o = make_float4(__uint_as_float(u[4 * i]), __uint_as_float(u[4 * i + 1]), __uint_as_float(u[4 * i + 2]), __uint_as_float(u[4 * i + 3]));
-                  if (joined) {
-                    const float4 x = s_o[(c * 8 + i) * 128 + lr];
-                    o.x = o.x * w_own + x.x * w_other;
-                    o.y = o.y * w_own + x.y * w_other;
-                    o.z = o.z * w_own + x.z * w_other;
-                    o.w = o.w * w_own + x.w * w_other;
-                  }
-                  dst[c * 8 + i] = o;
-                }
-              }
+#pragma unroll 4
+            for (int i = 0; i < (rows_here + 1) / 2; ++i) {                // half a warp per row
+              const int r = 2 * i + (lane >> 4);
+              const size_t prow = row0 + __shfl_sync(0xffffffffu, at, r);
+              if (r < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + half * 64)[lane & 15] = *staged(m, lane & 15, r);
             }
           }
-        } else {
-          const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-          w_own *= inv;
-          w_other *= inv;
-          __nv_bfloat16* dst = p.out + at * D;
+        } else if (warp_on) {
+          if (half == 0 && gated) {
+            if (joined) load_gate();
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+          }
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t u[32];
-            if (steps) {
-              tmem_ld_32x32(tO + c * 32, u);
-              tmem_ld_wait();
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) u[i] = 0;
+          for (int i = 0; i < 8; ++i) {
+            uint4* place = reinterpret_cast<uint4*>(own + half * ATOM + lane * 128 + ((i ^ (lane & 7)) << 4));
+            const float4 a = four(2 * i), b = four(2 * i + 1);
+            float o[8] = {a.x * w_own, a.y * w_own, a.z * w_own, a.w * w_own, b.x * w_own, b.y * w_own, b.z * w_own, b.w * w_own};
+            if (joined) {
+              const float4 x = *staged(1, 2 * i, lane), y = *staged(1, 2 * i + 1, lane);
+              o[0] += x.x * w_other; o[1] += x.y * w_other; o[2] += x.z * w_other; o[3] += x.w * w_other;
+              o[4] += y.x * w_other; o[5] += y.y * w_other; o[6] += y.z * w_other; o[7] += y.w * w_other;
             }
-            if (row_ok) {
+            if (p.gate) {
+              const uint4 g = *place;
+              const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&g);
 #pragma unroll
-              for (int i = 0; i < 32; i += 8) {
-                float o[8];
-#pragma unroll
-                for (int x = 0; x < 8; ++x) o[x] = __uint_as_float(u[i + x]) * w_own;
-                if (joined) {
-#pragma unroll
-                  for (int x = 0; x < 2; ++x) {
-                    const float4 y = s_o[(c * 8 + i / 4 + x) * 128 + lr];
-                    o[4 * x] += y.x * w_other;
-                    o[4 * x + 1] += y.y * w_other;
-                    o[4 * x + 2] += y.z * w_other;
-                    o[4 * x + 3] += y.w * w_other;
-                  }
-                }
-                if (p.gate) {
-                  const uint4 gu = *reinterpret_cast<const uint4*>(p.gate + at * D + c * 32 + i);
-                  const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&gu);
-#pragma unroll
-                  for (int x = 0; x < 4; ++x) {
-                    const float2 gf = __bfloat1622float2(gh[x]);
-                    o[2 * x] *= 1.f / (1.f + __expf(-gf.x));
-                    o[2 * x + 1] *= 1.f / (1.f + __expf(-gf.y));
-                  }
-                }
-                uint4 u4;
-                __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u4);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) h2[x] = __floats2bfloat162_rn(o[2 * x], o[2 * x + 1]);
-                *reinterpret_cast<uint4*>(dst + c * 32 + i) = u4;
+              for (int x = 0; x < 4; ++x) {
+                const float2 gf = __bfloat1622float2(gh[x]);
+                o[2 * x] = __fdividef(o[2 * x], 1.f + __expf(-gf.x));
+                o[2 * x + 1] = __fdividef(o[2 * x + 1], 1.f + __expf(-gf.y));
               }
+            }
+            uint4 u4;
+            __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u4);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) h2[x] = __floats2bfloat162_rn(o[2 * x], o[2 * x + 1]);
+            *place = u4;
+          }
+          if (half) {
+            __syncwarp();
+#pragma unroll 4
+            for (int i = 0; i < (rows_here + 1) / 2; ++i) {
+              const int r = 2 * i + (lane >> 4);
+              const uint4 u4 = *reinterpret_cast<const uint4*>(own + ((lane >> 3) & 1) * ATOM + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+              const size_t to = __shfl_sync(0xffffffffu, at, r);
+              if (r < rows_here) reinterpret_cast<uint4*>(p.out + to * D)[lane & 15] = u4;
             }
           }
         }
+        __syncwarp();
+        if (joined && lane == 0) mbar_arrive(j_empty);
       }
       tc_fence_before();
-      if (joined) {                                        // the scratch is read before the next rows overwrite it
-        __syncwarp();
-        if (m == 0 && lane == 0) mbar_arrive(j_empty);
-        const bool ok = mbar_wait(j_empty, ph_j);
-        if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
-        ph_j ^= 1;
-      }
     }
     if (!alive) {
       if (lane == 0) atomicExch(p.status, ERR_WAIT_ACC);

@@ -4,6 +4,7 @@ append, tcgen05 flash prefill, split-context decode.  Cache layout:
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -206,31 +207,71 @@ def _need(ok, what: str) -> None:
         raise ValueError(what)
 
 
-def _index(t, shape, device, what: str) -> None:
-    _need(t.dtype == torch.int32 and t.device == device and tuple(t.shape) == shape and t.is_contiguous(),
-          f"{what}: contiguous int32 {list(shape)} on {device} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+def _index(t, shape, dev: int, what: str) -> None:
+    if t.dtype != torch.int32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous int32 {list(shape)} on cuda:{dev} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _like(t, q, dev: int, what: str) -> None:
+    if t.dtype != torch.bfloat16 or t.shape != q.shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous bf16 {list(q.shape)} on cuda:{dev} expected, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
-    """Checks what the calls over spans have in common; (rows, Hq, pages, Hkv, page size, sequences, scale, out)."""
-    _need(q.is_cuda and q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[2] == D and q.is_contiguous(), "q: contiguous bf16 [T, Hq, 128]")
+    """Checks what the calls over spans have in common; (device, rows, Hq, pages, Hkv, page size, sequences, table width, scale, out)."""
+    dev = q.get_device()
+    if dev < 0 or q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != D or not q.is_contiguous():
+        raise ValueError(f"q: contiguous bf16 [T, Hq, 128] on a GPU expected, got {q.dtype} {list(q.shape)} on {q.device}")
     t, hq, _ = q.shape
-    for c in (k_cache, v_cache):
-        _need(c.dim() == 4 and c.dtype == torch.bfloat16 and c.shape[3] == D and c.is_contiguous() and c.device == q.device and c.shape == k_cache.shape,
-              "caches: contiguous bf16 [pages, kv heads, page size, 128] on the device of q")
+    if k_cache.dim() != 4 or k_cache.dtype != torch.bfloat16 or k_cache.shape[3] != D or k_cache.get_device() != dev or not k_cache.is_contiguous():
+        raise ValueError("caches: contiguous bf16 [pages, kv heads, page size, 128] on the device of q expected")
+    _like(v_cache, k_cache, dev, "v_cache")
     nb, hkv, bs, _ = k_cache.shape
-    _need(nb > 0 and hkv > 0 and hq > 0 and hq % hkv == 0, f"{hq} query heads over {hkv} key/value heads")
-    _need(bs in (16, 32, 64, 128, 256), f"page size {bs}: 16, 32, 64, 128 or 256 expected")
-    _need(block_table.dim() == 2 and block_table.shape[1] > 0, "block_table: int32 [sequences, pages]")
-    b = block_table.shape[0]
-    _index(block_table, (b, block_table.shape[1]), q.device, "block_table")
-    _index(kv_len, (b,), q.device, "kv_len")
-    for x, what in ((gate, "gate"), (out, "out")):
-        _need(x is None or (x.dtype == q.dtype and x.shape == q.shape and x.is_contiguous() and x.device == q.device), f"{what}: as q")
+    if nb < 1 or hkv < 1 or hq < 1 or hq % hkv:
+        raise ValueError(f"{hq} query heads over {hkv} key/value heads in {nb} pages")
+    if bs not in (16, 32, 64, 128, 256):
+        raise ValueError(f"page size {bs}: 16, 32, 64, 128 or 256 expected")
+    if block_table.dim() != 2 or block_table.shape[1] < 1:
+        raise ValueError("block_table: int32 [sequences, pages] expected")
+    b, width = block_table.shape
+    _index(block_table, (b, width), dev, "block_table")
+    _index(kv_len, (b,), dev, "kv_len")
+    if gate is not None:
+        _like(gate, q, dev, "gate")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _like(out, q, dev, "out")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    _need(0.0 < scale < math.inf, f"scale {scale}: positive expected")
-    _need(0.0 <= cap < math.inf, f"cap {cap}: positive, or 0 for none")
-    return t, hq, nb, hkv, bs, b, scale, torch.empty_like(q) if out is None else out
+    if not 0.0 < scale < math.inf or not 0.0 <= cap < math.inf:
+        raise ValueError(f"scale {scale}, cap {cap}: a positive scale and a cap that is positive, or 0 for none, expected")
+    return dev, t, hq, nb, hkv, bs, b, width, scale, out
+
+
+_P, _I = ctypes.c_void_p, ctypes.c_int
+_typed = False
+
+
+def _kernels() -> ctypes.CDLL:
+    """The kernel library with the parameter types of the calls below, which take plain addresses and numbers."""
+    global _typed
+    lib = _lib.lib()
+    if not _typed:
+        lib.b200_qk_norm_rope_axes_append.argtypes = [_P, _I, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _f, _P, _I, _f, ctypes.c_char_p, _I, _P,
+                                                      _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]
+        lib.b200_attn_spans.argtypes = [_P] * 11 + [_I] * 8 + [_f, _f, _I, _P, _P, _P]
+        lib.b200_attn_shared.argtypes = [_P] * 9 + [_I] * 7 + [_f, _f, _I, _I, _P, _P, _P]
+        _typed = True
+    return lib
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _on(dev: int):
+    """Makes ``dev`` the current device for a launch, where it is not."""
+    return contextlib.nullcontext() if torch._C._cuda_getDevice() == dev else torch.cuda.device(dev)
 
 
 def rotary_axes(sections, interleaved: bool = False) -> tuple[int, ...]:
@@ -255,37 +296,39 @@ def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_of
     ``axes`` from ``rotary_axes`` (a multiple of 4 pairs); ``positions`` int32 [axes, T]; ``slots`` int32 [T], distinct; rows
     with a negative slot are not cached.  Returns (q [T, Hq, 128], gate [T, Hq, 128] or None).
     """
-    t, dev = q_src.shape[0], q_src.device
-    for x, last, what in ((q_src, q_off + (n_q_heads - 1) * q_head_stride + (2 * D if gate_in_q else D), "q_src"),
-                          (k_src, k_off + n_kv_heads * D, "k_src"), (v_src, v_off + n_kv_heads * D, "v_src")):
-        _need(x.is_cuda and x.dim() == 2 and x.dtype == torch.bfloat16 and x.shape[0] == t and x.stride(1) == 1 and x.device == dev and
-              x.data_ptr() % 8 == 0 and last <= x.shape[1], f"{what}: bf16 [{t}, >= {last}] with contiguous rows on {dev} expected")
-    _need(min(q_off, k_off, v_off) >= 0 and q_head_stride >= 0, "offsets of heads begin at 0")
-    _need(not any(x % 4 for x in (q_off, q_head_stride, k_off, v_off)) and not any(x.stride(0) % 4 for x in (q_src, k_src, v_src)),
-          "offsets and row strides: multiples of 4")
-    for c in (k_cache, v_cache):
-        _need(c.dim() == 4 and c.dtype == torch.bfloat16 and c.shape[1] == n_kv_heads and c.shape[3] == D and c.is_contiguous() and
-              c.device == dev and c.shape == k_cache.shape, "caches: contiguous bf16 [pages, kv heads, page size, 128]")
+    dev, t = q_src.get_device(), q_src.shape[0]
+    for x, off, last, what in ((q_src, q_off, q_off + (n_q_heads - 1) * q_head_stride + (2 * D if gate_in_q else D), "q_src"),
+                               (k_src, k_off, k_off + n_kv_heads * D, "k_src"), (v_src, v_off, v_off + n_kv_heads * D, "v_src")):
+        if (dev < 0 or x.get_device() != dev or x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[0] != t or x.stride(1) != 1 or last > x.shape[1] or
+                off < 0 or off % 4 or x.stride(0) % 4 or x.data_ptr() % 8):
+            raise ValueError(f"{what}: bf16 rows [{t}, >= {last}] on a GPU, 8-byte aligned, expected; got {x.dtype} {list(x.shape)} on {x.device} from {off}")
+    if q_head_stride < 0 or q_head_stride % 4 or n_q_heads < 1 or n_kv_heads < 1:
+        raise ValueError(f"{n_q_heads} / {n_kv_heads} heads, {q_head_stride} columns apart")
+    if (k_cache.dim() != 4 or k_cache.dtype != torch.bfloat16 or k_cache.shape[1] != n_kv_heads or k_cache.shape[3] != D or
+            k_cache.get_device() != dev or not k_cache.is_contiguous()):
+        raise ValueError("caches: contiguous bf16 [pages, kv heads, page size, 128] on the device of the rows expected")
+    _like(v_cache, k_cache, dev, "v_cache")
     for g in (q_gamma, k_gamma):
-        _need(g is None or (g.dtype == torch.bfloat16 and g.numel() == D and g.is_contiguous() and g.device == dev), "gammas: bf16 [128]")
-    _need(n_q_heads > 0 and n_kv_heads > 0 and len(axes) % 4 == 0 and 0 < len(axes) <= D // 2 and min(axes) >= 0, "axes: 4, 8 .. 64 pairs")
-    _need(inv_freq.dtype == torch.float32 and inv_freq.numel() == len(axes) and inv_freq.is_contiguous() and inv_freq.device == dev,
-          "inv_freq: fp32, one per pair")
-    _need(positions.dim() == 2 and positions.shape[0] > max(axes), f"positions: a row for each of {max(axes) + 1} axes expected")
+        if g is not None and (g.dtype != torch.bfloat16 or g.numel() != D or not g.is_contiguous() or g.get_device() != dev):
+            raise ValueError("gammas: bf16 [128] on the device of the rows expected")
+    n = len(axes)
+    if n % 4 or not 0 < n <= D // 2 or min(axes) < 0 or positions.dim() != 2 or positions.shape[0] <= max(axes):
+        raise ValueError(f"axes: 4, 8 .. {D // 2} pairs, each with a row of positions, expected")
+    if inv_freq.dtype != torch.float32 or inv_freq.numel() != n or not inv_freq.is_contiguous() or inv_freq.get_device() != dev:
+        raise ValueError("inv_freq: fp32, one per pair, on the device of the rows expected")
     _index(positions, (positions.shape[0], t), dev, "positions")
     _index(slots, (t,), dev, "slots")
-    q_out = torch.empty(t, n_q_heads, D, dtype=torch.bfloat16, device=dev)
+    q_out = torch.empty((t, n_q_heads, D), dtype=torch.bfloat16, device=q_src.device)
     gate_out = torch.empty_like(q_out) if gate_in_q else None
     if t == 0:
         return q_out, gate_out
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.check_indices(slots, 0, k_cache.shape[0] * k_cache.shape[2], 2, keep=-1)
-        rc = _lib.lib().b200_qk_norm_rope_axes_append(
-            _lib.ptr(q_src), q_src.stride(0), q_off, q_head_stride, int(gate_in_q),
-            _lib.ptr(k_src), k_src.stride(0), k_off, _lib.ptr(v_src), v_src.stride(0), v_off,
-            _lib.ptr(q_gamma), _lib.ptr(k_gamma), int(unit_offset), _f(eps), _lib.ptr(inv_freq), 2 * len(axes), _f(mscale), bytes(axes),
-            positions.shape[0], _lib.ptr(positions), t, _lib.ptr(slots), _lib.ptr(q_out), _lib.ptr(gate_out), _lib.ptr(k_cache),
-            _lib.ptr(v_cache), k_cache.shape[0], k_cache.shape[2], t, n_q_heads, n_kv_heads, _lib.stream())
+        rc = _kernels().b200_qk_norm_rope_axes_append(
+            q_src.data_ptr(), q_src.stride(0), q_off, q_head_stride, gate_in_q, k_src.data_ptr(), k_src.stride(0), k_off, v_src.data_ptr(),
+            v_src.stride(0), v_off, _at(q_gamma), _at(k_gamma), unit_offset, eps, inv_freq.data_ptr(), 2 * n, mscale, bytes(axes),
+            positions.shape[0], positions.data_ptr(), t, slots.data_ptr(), q_out.data_ptr(), _at(gate_out), k_cache.data_ptr(),
+            v_cache.data_ptr(), k_cache.shape[0], k_cache.shape[2], t, n_q_heads, n_kv_heads, torch._C._cuda_getCurrentRawStream(dev))
     _lib.check(rc, "qk_norm_rope_axes_append")
     return q_out, gate_out
 
@@ -319,28 +362,30 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
     q: [T, Hq, 128]; block_table [B, max_blocks], q_start / q_len / kv_len [B], lo / hi [T]: int32 device tensors.  Rows of no
     sequence are not written (``out``: where to write).  ``max_kv_len`` bounds the contexts, for the choice of ``splits``.
     """
-    t, hq, nb, hkv, bs, b, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
-    _index(q_start, (b,), q.device, "q_start")
-    _index(q_len, (b,), q.device, "q_len")
-    for x, what in ((lo, "lo"), (hi, "hi")):
-        if x is not None:
-            _index(x, (t,), q.device, what)
+    dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
+    _index(q_start, (b,), dev, "q_start")
+    _index(q_len, (b,), dev, "q_len")
+    if lo is not None:
+        _index(lo, (t,), dev, "lo")
+    if hi is not None:
+        _index(hi, (t,), dev, "hi")
     max_q_len = min(int(max_q_len), t)
     if t == 0 or b == 0 or max_q_len <= 0:
         return out
     if splits is None:
         g = hq // hkv
         tiles = hkv * min(b * -(-max_q_len * g // ROW_TILE), t * g // ROW_TILE + b)
-        keys = -(-(max_kv_len if max_kv_len is not None else block_table.shape[1] * bs) // KEY_TILE)
+        keys = -(-(max_kv_len if max_kv_len is not None else width * bs) // KEY_TILE)
         splits = max(1, min(NUM_SMS // tiles, keys // 2))
-    _need(1 <= splits <= 1024, f"{splits} splits")
-    with torch.cuda.device(q.device):
+    if not 1 <= splits <= 1024:
+        raise ValueError(f"{splits} splits")
+    with _on(dev):
         ws = torch.empty(splits * t * hq * (D + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
         _lib.check_indices(block_table, 0, nb, 3)
-        rc = _lib.lib().b200_attn_spans(
-            _lib.ptr(q), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(out), _lib.ptr(gate), _lib.ptr(block_table), _lib.ptr(q_start),
-            _lib.ptr(q_len), _lib.ptr(kv_len), _lib.ptr(lo), _lib.ptr(hi), b, max_q_len, t, block_table.shape[1], nb, bs, hq, hkv, _f(scale),
-            _f(cap), splits, _lib.ptr(ws), _lib.ptr(_lib.status_word(q.device)), _lib.stream())
+        rc = _kernels().b200_attn_spans(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), q_start.data_ptr(),
+            q_len.data_ptr(), kv_len.data_ptr(), _at(lo), _at(hi), b, max_q_len, t, width, nb, bs, hq, hkv, scale, cap, splits, _at(ws),
+            _lib.status_word(q.device).data_ptr(), torch._C._cuda_getCurrentRawStream(dev))
     _lib.check(rc, "prefill_spans", 2 if splits > 1 else 1)
     return out
 
@@ -370,29 +415,30 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     group_start[g] .. group_start[g + 1] - 1 of ``block_table`` begin with the same pages, whose first shared_len[g] keys they have
     in common (keys at ``kv_len`` and beyond stay unseen); rows of no group are on their own.  ``cap`` as in ``prefill_spans``;
     ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys, of a sequence's own)."""
-    t, hq, nb, hkv, bs, b, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
-    _need(b == t, f"{t} rows for {b} sequences")
-    _need(shared_len.dim() == 1, "shared_len: int32 [groups]")
+    dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
+    if b != t or shared_len.dim() != 1:
+        raise ValueError(f"{t} rows for {b} sequences, shared lengths {list(shared_len.shape)}: a row per sequence and a length per group expected")
     n = shared_len.shape[0]
-    _index(shared_len, (n,), q.device, "shared_len")
-    _index(group_start, (n + 1,), q.device, "group_start")
+    _index(shared_len, (n,), dev, "shared_len")
+    _index(group_start, (n + 1,), dev, "group_start")
     if b == 0:
         return out
     if splits is None:
-        longest = max_kv_len if max_kv_len is not None else block_table.shape[1] * bs
+        longest = max_kv_len if max_kv_len is not None else width * bs
         common = 0 if n == 0 else longest if max_shared is None else min(longest, max(0, int(max_shared)))
         keys, own_keys = -(-common // KEY_TILE), -(-(longest - common) // KEY_TILE) + 1
         tiles = (b * (hq // hkv) // ROW_TILE + n) * hkv
         share = (tiles * keys + b * hkv * own_keys) / NUM_SMS             # key tiles of an SM
         splits = (max(1, min(64, round(keys / max(2.0, share)))), max(1, min(64, round(own_keys / max(4.0, share)))))
-    _need(1 <= min(splits) and max(splits) <= 1024, f"splits {splits}")
-    with torch.cuda.device(q.device):
+    if not (1 <= splits[0] <= 1024 and 1 <= splits[1] <= 1024):
+        raise ValueError(f"splits {splits}")
+    with _on(dev):
         ws = torch.empty(sum(splits) * b * hq * (D + 2), dtype=torch.float32, device=q.device)
         _lib.check_indices(block_table, 0, nb, 3)
-        rc = _lib.lib().b200_attn_shared(
-            _lib.ptr(q), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(out), _lib.ptr(gate), _lib.ptr(block_table), _lib.ptr(kv_len),
-            _lib.ptr(group_start), _lib.ptr(shared_len), n, b, block_table.shape[1], nb, bs, hq, hkv, _f(scale), _f(cap), splits[0], splits[1],
-            _lib.ptr(ws), _lib.ptr(_lib.status_word(q.device)), _lib.stream())
+        rc = _kernels().b200_attn_shared(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
+            group_start.data_ptr(), shared_len.data_ptr(), n, b, width, nb, bs, hq, hkv, scale, cap, splits[0], splits[1], ws.data_ptr(),
+            _lib.status_word(q.device).data_ptr(), torch._C._cuda_getCurrentRawStream(dev))
     _lib.check(rc, "decode_shared", 2)
     return out
 
