@@ -1,0 +1,335 @@
+// One query row per sequence over the keys that are the sequence's own, joined with what attn_spans.cu has summed over the keys it
+// shares with others (paged bf16 cache, head width 128), sm_100a.
+//
+//   s_j = scale q . k_j (cap c: c tanh(s / c)), shared <= j < kv_len; o = (sum_j 2^(s_j - m) v_j + partial sums) / sum, out = o sigmoid(gate)
+//
+// Bound by memory: a key and its value are read once for the (up to 8 or 16) query heads of their kv head, straight into
+// the fragments of the tensor core's warp-level products, 16 bytes a lane and whole lines a row:
+//   scores^T [16 keys x 8 heads] = K [keys x dims] Q^T: the order of the 128 dims is free, so that a lane's 16 bytes of a row are
+//     two of its fragments;
+//   O^T [16 dims x 8 heads] = V^T [dims x keys] P^T: a lane holds the same 8 dims of its four keys and pairs them up;
+//   P^T comes from the scores by an 8 x 8 transpose in registers.
+// Heads as the narrow side of the products keep O of a kv head in 32 registers.  A warp takes 16 keys at a time (of one page: their
+// page is looked up once), the warps of up to 8 blocks of a cluster share a sequence's keys, and the sums are joined in shared memory.
+// The first products do not wait for the kernel before (it writes only the partial sums).
+#include <cuda_bf16.h>
+#include <stdint.h>
+#include "launch.h"
+#include "ops.h"
+
+namespace {
+
+constexpr int D = 128;
+constexpr int WARPS = 4;
+constexpr int LD = 132;              // floats of a row of O in shared memory: the fragments' stores then meet no bank twice
+
+struct OwnParams {
+  const __nv_bfloat16* q;            // [B, Hq, 128]
+  const __nv_bfloat16* gate;         // optional
+  __nv_bfloat16* out;
+  const __nv_bfloat16* k_cache;      // [num_blocks, Hkv, bs, 128]
+  const __nv_bfloat16* v_cache;
+  const int* block_table;            // [B, max_blocks]
+  const int* kv_len;                 // [B]
+  const int* group_start;
+  const int* shared_len;
+  int n_groups;
+  const float* part_o;               // [slots, B, Hq, 128]
+  const float* part_ml;              // [slots, B, Hq, 2]
+  int slots;
+  int B, max_blocks, num_blocks, bs, bs_log2, Hq, Hkv, G, chunks, cluster;
+  float scale_log2, cap_in, cap_out;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2, const uint32_t a3, const uint32_t b0,
+                                         const uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+__device__ __forceinline__ uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+  uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+  return v;
+}
+
+// NB: groups of 8 heads a block works on.
+template <int NB>
+__global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
+own_rows_kernel(const __grid_constant__ OwnParams p) {
+  constexpr int H = 8 * NB;
+  __shared__ float s_m[WARPS][H], s_l[WARPS][H];
+  __shared__ float s_o[WARPS][H][LD];
+  b200::pdl_grid_trigger();
+  if (p.slots == 0) b200::pdl_grid_wait();               // (otherwise the kernel before has waited for what these products read)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int rank = blockIdx.x % p.cluster;
+  int x = blockIdx.x / p.cluster;
+  const int h0 = (x % p.chunks) * H;                     // first head of the kv head's G
+  x /= p.chunks;
+  const int kvh = x % p.Hkv, b = x / p.Hkv;
+  const int heads = min(H, p.G - h0);
+
+  int shared = 0;
+  for (int i = lane; i < p.n_groups; i += 32)
+    if (b >= p.group_start[i] && b < p.group_start[i + 1]) shared = max(shared, p.shared_len[i]);
+  shared = __reduce_max_sync(0xffffffffu, shared);
+  const int kv = max(0, min(p.kv_len[b], p.max_blocks * p.bs));
+  const int first = shared >> 4, n_blk = max(0, ((kv + 15) >> 4) - first);               // blocks of 16 keys
+  const int* bt = p.block_table + (size_t)b * p.max_blocks;
+
+  uint4 q[NB][4];                                        // head 8 i + g, dims 32 x + 8 c ..
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      q[i][d] = i * 8 + g < heads
+                    ? *reinterpret_cast<const uint4*>(p.q + ((size_t)b * p.Hq + kvh * p.G + h0 + i * 8 + g) * D + d * 32 + c * 8)
+                    : make_uint4(0, 0, 0, 0);
+  float o[NB][8][4];                                     // dims 8 g + i, 64 + 8 g + i of heads 2 c, 2 c + 1
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) o[i][d][y] = 0.f;
+  float m[NB][2], l[NB][2];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) m[i][0] = m[i][1] = -INFINITY, l[i][0] = l[i][1] = 0.f;
+
+  // keys of block n: rows g and g + 8; values: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9, dims 8 g and 64 + 8 g.  Rows that do not count are
+  // zero: a product of zero with what they may hold would not be.
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 k[2][4], v[4][2];
+  auto row_of = [&](int blk) {
+    const int key = (first + blk) << 4, page = bt[key >> p.bs_log2];
+    return (unsigned)page < (unsigned)p.num_blocks ? ((size_t)page * p.Hkv + kvh) * p.bs + (key & (p.bs - 1)) : ~(size_t)0;
+  };
+  auto counts = [&](int blk, int i, size_t row) {
+    const int key = ((first + blk) << 4) + i;
+    return blk < n_blk && row != ~(size_t)0 && key >= shared && key < kv;
+  };
+  auto load_k = [&](int blk, size_t row) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        k[i][d] = counts(blk, g + 8 * i, row) ? *reinterpret_cast<const uint4*>(p.k_cache + (row + g + 8 * i) * D + d * 32 + c * 8) : zero;
+  };
+  auto load_v = [&](int blk, size_t row) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = 2 * c + (i & 1) + (i >> 1) * 8;
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+        v[i][d] = counts(blk, key, row) ? *reinterpret_cast<const uint4*>(p.v_cache + (row + key) * D + d * 64 + g * 8) : zero;
+    }
+  };
+  const int step = WARPS * p.cluster;
+  int blk = rank * WARPS + warp;
+  size_t row = blk < n_blk ? row_of(blk) : ~(size_t)0;
+  load_k(blk, row);
+  load_v(blk, row);
+  for (; blk < n_blk; blk += step) {
+    const bool ok0 = counts(blk, g, row), ok1 = counts(blk, g + 8, row);
+    float s[NB][4];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        mma_bf16(s[i], k[0][d].x, k[1][d].x, k[0][d].y, k[1][d].y, q[i][d].x, q[i][d].y);
+        mma_bf16(s[i], k[0][d].z, k[1][d].z, k[0][d].w, k[1][d].w, q[i][d].z, q[i][d].w);
+      }
+    }
+    const int next = blk + step;
+    const size_t next_row = next < n_blk ? row_of(next) : ~(size_t)0;
+    load_k(next, next_row);
+    uint32_t pt[NB][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        if (p.cap_out > 0.f) s[i][y] = p.cap_out * (1.f - 2.f * __fdividef(1.f, 1.f + exp2f(s[i][y] * p.cap_in * 2.885390081777927f)));
+        else s[i][y] *= p.scale_log2;
+        if (!((y < 2) ? ok0 : ok1)) s[i][y] = -INFINITY;
+      }
+      float alpha[2];
+      bool grown = false;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {                      // heads 2 c, 2 c + 1: their keys lie in the 8 lanes of the same c
+        float mx = fmaxf(s[i][y], s[i][y + 2]);
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float mn = fmaxf(m[i][y], mx);
+        const bool grow = mn > m[i][y] + 8.f;            // (the first key: from -inf)
+        alpha[y] = grow ? exp2f(m[i][y] - mn) : 1.f;
+        grown |= grow && m[i][y] != -INFINITY;
+        if (grow) m[i][y] = mn;
+        l[i][y] *= alpha[y];
+        const float use = m[i][y] == -INFINITY ? 0.f : m[i][y];
+        s[i][y] = exp2f(s[i][y] - use);
+        s[i][y + 2] = exp2f(s[i][y + 2] - use);
+        l[i][y] += s[i][y] + s[i][y + 2];
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          o[i][d][0] *= alpha[0];
+          o[i][d][1] *= alpha[1];
+          o[i][d][2] *= alpha[0];
+          o[i][d][3] *= alpha[1];
+        }
+      }
+      pt[i][0] = transpose8(pack(s[i][0], s[i][1]));
+      pt[i][1] = transpose8(pack(s[i][2], s[i][3]));
+    }
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const uint32_t sel = d & 1 ? 0x7632 : 0x5410;      // the high or the low halves of two words
+      const uint32_t a0 = __byte_perm(word(v[0][0], d >> 1), word(v[1][0], d >> 1), sel), a1 = __byte_perm(word(v[0][1], d >> 1), word(v[1][1], d >> 1), sel);
+      const uint32_t a2 = __byte_perm(word(v[2][0], d >> 1), word(v[3][0], d >> 1), sel), a3 = __byte_perm(word(v[2][1], d >> 1), word(v[3][1], d >> 1), sel);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) mma_bf16(o[i][d], a0, a1, a2, a3, pt[i][0], pt[i][1]);
+    }
+    row = next_row;
+    load_v(next, row);
+  }
+
+  // ---- the warps' sums, then the blocks'
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) l[i][y] += __shfl_xor_sync(0xffffffffu, l[i][y], w);
+      const int h = i * 8 + 2 * c + y;
+      if (g == 0) {
+        s_m[warp][h] = m[i][y];
+        s_l[warp][h] = l[i][y];
+      }
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {                      // dim 64 y' + 8 g + d lies at 64 y' + 8 d + g
+        s_o[warp][h][d * 8 + g] = o[i][d][y];
+        s_o[warp][h][64 + d * 8 + g] = o[i][d][y + 2];
+      }
+    }
+  __syncthreads();
+  if (p.cluster > 1) cluster_sync();
+  if (p.slots) b200::pdl_grid_wait();
+  const size_t rows = (size_t)p.B * p.Hq;
+  // four dims of a head a thread: a warp per head
+  for (int h = rank * WARPS + warp; h < heads; h += WARPS * p.cluster) {
+    const size_t at = (size_t)b * p.Hq + kvh * p.G + h0 + h;
+    const int pos = (lane >> 4) * 64 + (lane & 1) * 32 + ((lane >> 1) & 7);              // of dims 4 lane ..: 64 y' + 8 d + g, d = 4 (lane & 1) ..
+    float M = -INFINITY;
+    for (int r = 0; r < p.cluster; ++r)
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, p.cluster > 1 ? ld_cluster(&s_m[w][h], r) : s_m[w][h]);
+    const int slots = shared > 0 ? p.slots : 0;
+    for (int s = 0; s < slots; ++s) M = fmaxf(M, p.part_ml[(s * rows + at) * 2]);
+    float L = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < p.cluster; ++r)
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float lw = p.cluster > 1 ? ld_cluster(&s_l[w][h], r) : s_l[w][h];
+        if (lw == 0.f) continue;
+        const float f = exp2f((p.cluster > 1 ? ld_cluster(&s_m[w][h], r) : s_m[w][h]) - M);
+        L += f * lw;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) a[y] += f * (p.cluster > 1 ? ld_cluster(&s_o[w][h][pos + 8 * y], r) : s_o[w][h][pos + 8 * y]);
+      }
+#pragma unroll 4
+    for (int s = 0; s < slots; ++s) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + at) * 2);
+      if (ml.y == 0.f) continue;                         // (nothing seen: the sums may not have been written)
+      const float4 y = *reinterpret_cast<const float4*>(p.part_o + (s * rows + at) * D + lane * 4);
+      const float f = exp2f(ml.x - M);
+      L += f * ml.y;
+      a[0] += f * y.x; a[1] += f * y.y; a[2] += f * y.z; a[3] += f * y.w;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) a[y] *= inv;
+    if (p.gate) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p.gate + at * D + lane * 4);
+      const __nv_bfloat162* hp = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const float2 f = __bfloat1622float2(hp[y]);
+        a[2 * y] *= 1.f / (1.f + __expf(-f.x));
+        a[2 * y + 1] *= 1.f / (1.f + __expf(-f.y));
+      }
+    }
+    *reinterpret_cast<uint2*>(p.out + at * D + lane * 4) = make_uint2(pack(a[0], a[1]), pack(a[2], a[3]));
+  }
+  if (p.cluster > 1) cluster_sync();                     // the others may still read this block's sums
+}
+
+template <int NB>
+cudaError_t launch(const OwnParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hkv * p.chunks * p.cluster));
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, own_rows_kernel<NB>, p);
+}
+
+}  // namespace
+
+// q / out / gate [B, Hq, 128]; sequence b: the keys shared .. kv_len[b] - 1 of table row b, shared = shared_len[g] of the group with
+// group_start[g] <= b < group_start[g + 1] (0 without one).  slots > 0: partial sums over the shared keys from b200_attn_shared,
+// launched before this one.  cluster: blocks (1, 2, 4 or 8) that share a sequence's keys.
+extern "C" int b200_attn_own_rows(const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate,
+                                  const int* block_table, const int* kv_len, const int* group_start, const int* shared_len, int n_groups,
+                                  int batch, int max_blocks, int num_blocks, int block_size, int n_q_heads, int n_kv_heads, float scale,
+                                  float cap, int slots, const float* workspace, int cluster, cudaStream_t stream) {
+  const bool pow2 = block_size >= 16 && block_size <= 256 && !(block_size & (block_size - 1));
+  if (!pow2 || n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads || batch < 1 || max_blocks < 1 || num_blocks < 1 || n_groups < 0 ||
+      !(scale > 0.f) || !(cap >= 0.f) || (long long)max_blocks * block_size > 0x7fffff00ll || slots < 0 || (slots > 0 && !workspace) ||
+      (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8))
+    return -6;
+  OwnParams p = {};
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  p.gate = reinterpret_cast<const __nv_bfloat16*>(gate);
+  p.out = reinterpret_cast<__nv_bfloat16*>(out);
+  p.k_cache = reinterpret_cast<const __nv_bfloat16*>(k_cache);
+  p.v_cache = reinterpret_cast<const __nv_bfloat16*>(v_cache);
+  p.block_table = block_table; p.kv_len = kv_len;
+  p.group_start = group_start; p.shared_len = shared_len; p.n_groups = n_groups;
+  p.part_o = workspace;
+  p.part_ml = workspace ? workspace + (size_t)slots * batch * n_q_heads * D : nullptr;
+  p.slots = slots;
+  p.B = batch; p.max_blocks = max_blocks; p.num_blocks = num_blocks; p.bs = block_size;
+  while ((1 << p.bs_log2) < block_size) ++p.bs_log2;
+  p.Hq = n_q_heads; p.Hkv = n_kv_heads; p.G = n_q_heads / n_kv_heads;
+  const int H = p.G <= 8 ? 8 : 16;
+  p.chunks = (p.G + H - 1) / H;
+  p.cluster = cluster;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.cap_in = cap > 0.f ? scale / cap : 0.f;
+  p.cap_out = cap * 1.4426950408889634f;
+  if ((long long)batch * n_kv_heads * p.chunks * cluster > 0x7fffffffll) return -6;
+  return (int)(H == 8 ? launch<1>(p, stream) : launch<2>(p, stream));
+}

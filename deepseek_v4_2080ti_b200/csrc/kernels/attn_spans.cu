@@ -67,7 +67,7 @@ struct Params {
   float* part_ml;                 // [slots, T, Hq, 2]
   int batch, T, max_blocks, bs, Hq, Hkv, G;
   int row_tiles;                  // row tiles per sequence (prompt rows), over all groups (shared keys)
-  int splits, own_splits;         // key ranges per row tile; of a sequence's own keys
+  int splits;                     // key ranges per row tile
   int n_items;
   float scale_log2;               // scale * log2(e)
   float cap_in, cap_out;          // scale / cap, cap * log2(e)
@@ -228,72 +228,51 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
   it.n_rows = 0;
   int split, splits;
   int rows_all;
+  split = idx % p.splits;
+  splits = p.splits;
+  int x = idx / p.splits;
+  it.kvh = x % p.Hkv;
+  x /= p.Hkv;
+  it.slot = split;
   if (SHARED) {
-    const int n_shared = p.row_tiles * p.Hkv * p.splits;
-    if (idx < n_shared) {                                  // keys of a group
-      split = idx % p.splits;
-      splits = p.splits;
-      it.kvh = idx / p.splits % p.Hkv;
-      int tile = idx / (p.splits * p.Hkv), b0 = 0, rows = -1, shared = 0;
-      for (int base = 0; base < p.n_groups && rows < 0; base += 32) {      // a group per lane
-        const int g = base + lane;
-        int first = 0, n = 0, sh = 0;
-        if (g < p.n_groups) {
-          first = max(0, min(p.batch, p.group_start[g]));
-          n = max(0, min(p.batch, p.group_start[g + 1]) - first) * p.G;
-          sh = p.shared_len[g];
-        }
-        const int tiles = (n + 2 * BQ - 1) / (2 * BQ);
-        int upto = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += x;
-        }
-        const uint32_t here = __ballot_sync(0xffffffffu, tile < upto);
-        if (here) {
-          const int src = __ffs(here) - 1;
-          b0 = __shfl_sync(0xffffffffu, first, src);
-          rows = __shfl_sync(0xffffffffu, n, src);
-          shared = __shfl_sync(0xffffffffu, sh, src);
-          tile -= __shfl_sync(0xffffffffu, upto - tiles, src);
-        } else {
-          tile -= __shfl_sync(0xffffffffu, upto, 31);
-        }
+    int tile = x, b0 = 0, rows = -1, shared = 0;
+    for (int base = 0; base < p.n_groups && rows < 0; base += 32) {      // a group per lane
+      const int g = base + lane;
+      int first = 0, n = 0, sh = 0;
+      if (g < p.n_groups) {
+        first = max(0, min(p.batch, p.group_start[g]));
+        n = max(0, min(p.batch, p.group_start[g + 1]) - first) * p.G;
+        sh = p.shared_len[g];
       }
-      if (rows < 0) return false;
-      it.base_tok = it.trow = b0;
-      it.r0 = tile * 2 * BQ;
-      rows_all = rows;
-      it.own_lo = 0;
-      it.own_hi = shared;
-      it.slot = split;
-      if (it.own_hi <= 0) return false;                    // (the join does not look at its slots either)
-    } else {                                               // a sequence's own keys
-      idx -= n_shared;
-      split = idx % p.own_splits;
-      splits = p.own_splits;
-      it.kvh = idx / p.own_splits % p.Hkv;
-      const int b = idx / (p.own_splits * p.Hkv);
-      it.base_tok = it.trow = b;
-      it.r0 = 0;
-      rows_all = p.G;
-      int shared = 0;
-      for (int g = lane; g < p.n_groups; g += 32)
-        if (b >= p.group_start[g] && b < p.group_start[g + 1]) shared = max(shared, p.shared_len[g]);
-      it.own_lo = __reduce_max_sync(0xffffffffu, shared);
-      it.own_hi = 0x7fffffff;
-      it.slot = p.splits + split;
+      const int tiles = (n + 2 * BQ - 1) / (2 * BQ);
+      int upto = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      const uint32_t here = __ballot_sync(0xffffffffu, tile < upto);
+      if (here) {
+        const int src = __ffs(here) - 1;
+        b0 = __shfl_sync(0xffffffffu, first, src);
+        rows = __shfl_sync(0xffffffffu, n, src);
+        shared = __shfl_sync(0xffffffffu, sh, src);
+        tile -= __shfl_sync(0xffffffffu, upto - tiles, src);
+      } else {
+        tile -= __shfl_sync(0xffffffffu, upto, 31);
+      }
     }
+    if (rows < 0) return false;
+    it.base_tok = it.trow = b0;
+    it.r0 = tile * 2 * BQ;
+    rows_all = rows;
+    it.own_lo = 0;
+    it.own_hi = shared;
+    if (shared <= 0) return false;                         // (nobody looks at its slots)
     it.kv_end = p.max_blocks * p.bs;
     it.delta = 0;
   } else {
-    split = idx % p.splits;
-    splits = p.splits;
-    int x = idx / p.splits;
-    it.kvh = x % p.Hkv;
-    x /= p.Hkv;
-    const int b = x % p.batch, tile = p.row_tiles - 1 - x / p.batch;      // long contexts first
+    const int b = x % p.batch, tile = p.row_tiles - 1 - x / p.batch;       // long contexts first
     const int q0 = p.q_start[b], n = p.q_len[b];
     const int len = q0 < 0 ? 0 : min(n, p.T - q0);
     rows_all = max(0, len) * p.G;
@@ -302,7 +281,6 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
     it.base_tok = q0;
     it.kv_end = max(0, min(p.kv_len[b], p.max_blocks * p.bs));
     it.delta = p.kv_len[b] - n - q0;
-    it.slot = split;
     it.own_lo = it.own_hi = 0;
   }
   it.n_rows = min(2 * BQ, rows_all - it.r0);
@@ -415,8 +393,8 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();                                  // (after the wait: the kernel that joins shared keys begins with what this one reads)
 
   Item it;
   // The next item, in shared memory: every role but the producer, which has put it there.
@@ -995,8 +973,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   }
 }
 
-// Joins a row's partial sums; one warp per row of one head, lane: four columns.
-template <bool SHARED>
+// Joins a prompt row's partial sums; one warp per row of one head, lane: four columns.
 __global__ void __launch_bounds__(256)
 spans_join_kernel(const __grid_constant__ Params p) {
   pdl_launch_dependents();
@@ -1005,24 +982,15 @@ spans_join_kernel(const __grid_constant__ Params p) {
   if (at >= rows) return;
   pdl_wait();
   const int tok = (int)(at / p.Hq);
-  int s0 = 0;
-  if (SHARED) {                                            // slots of the shared keys are there for rows of a group that shares some
-    s0 = p.splits;
-    for (int g = lane; g < p.n_groups; g += 32)
-      if (tok >= p.group_start[g] && tok < p.group_start[g + 1] && p.shared_len[g] > 0) s0 = 0;
-    s0 = __reduce_min_sync(0xffffffffu, s0);
-  } else {                                                 // rows of no sequence stay as they are
-    int mine = 0;
-    for (int b = lane; b < p.batch; b += 32) mine |= p.q_start[b] >= 0 && tok >= p.q_start[b] && tok - p.q_start[b] < p.q_len[b];
-    if (!__any_sync(0xffffffffu, mine)) return;
-  }
-  const int s1 = p.splits + p.own_splits;
+  int mine = 0;                                            // rows of no sequence stay as they are
+  for (int b = lane; b < p.batch; b += 32) mine |= p.q_start[b] >= 0 && tok >= p.q_start[b] && tok - p.q_start[b] < p.q_len[b];
+  if (!__any_sync(0xffffffffu, mine)) return;
   float M = -INFINITY;
-  for (int s = s0 + lane; s < s1; s += 32) M = fmaxf(M, p.part_ml[(s * rows + at) * 2]);
+  for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, p.part_ml[(s * rows + at) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = s0; s < s1; ++s) {
+  for (int s = 0; s < p.splits; ++s) {
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + at) * 2);
     if (ml.y == 0.f) continue;                             // (nothing seen: the item may not have written its sums)
     const float w = exp2f(ml.x - M);
@@ -1060,18 +1028,18 @@ int launch_as(const CUtensorMap& tmK, const CUtensorMap& tmV, const Params& p, c
     configured = true;
   }
   cudaError_t e = launch_pdl(spans_kernel<SHARED, CAP>, dim3(min(p.n_items, sm_count())), dim3(NTHREADS), SMEM_BYTES, stream, tmK, tmV, p);
-  if (e != cudaSuccess || !p.part_o) return (int)e;
-  return (int)launch_pdl(spans_join_kernel<SHARED>, dim3((unsigned)(((size_t)p.T * p.Hq + 7) / 8)), dim3(256), 0, stream, p);
+  if (e != cudaSuccess || SHARED || !p.part_o) return (int)e;
+  return (int)launch_pdl(spans_join_kernel, dim3((unsigned)(((size_t)p.T * p.Hq + 7) / 8)), dim3(256), 0, stream, p);
 }
 
 template <bool SHARED>
 int launch(Params& p, const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate, const int* block_table,
            const int* kv_len, int batch, int T, int max_blocks, int num_blocks, int block_size, int n_q_heads, int n_kv_heads, float scale,
-           float cap, float* workspace, int slots, int* status, cudaStream_t stream) {
+           float cap, float* workspace, int* status, cudaStream_t stream) {
   const bool pow2 = block_size >= 16 && block_size <= 256 && !(block_size & (block_size - 1));
   if (!pow2 || n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads || batch < 1 || T < 1 || max_blocks < 1 || num_blocks < 1 ||
       !(scale > 0.f) || !(cap >= 0.f) || (long long)max_blocks * block_size > 0x7fffff00ll ||
-      (long long)num_blocks * n_kv_heads * block_size > 0x7fffff00ll || (slots > 1 && !workspace))
+      (long long)num_blocks * n_kv_heads * block_size > 0x7fffff00ll || ((SHARED || p.splits > 1) && !workspace))
     return -ERR_BAD_ARG;
   p.q = reinterpret_cast<const __nv_bfloat16*>(q);
   p.gate = reinterpret_cast<const __nv_bfloat16*>(gate);
@@ -1082,8 +1050,9 @@ int launch(Params& p, const void* q, const void* k_cache, const void* v_cache, v
   p.batch = batch; p.T = T; p.max_blocks = max_blocks; p.bs = block_size;
   p.Hq = n_q_heads; p.Hkv = n_kv_heads; p.G = n_q_heads / n_kv_heads;
   const size_t rows = (size_t)T * n_q_heads;
-  p.part_o = slots > 1 ? workspace : nullptr;
-  p.part_ml = slots > 1 ? workspace + rows * slots * D : nullptr;
+  const bool parts = SHARED || p.splits > 1;
+  p.part_o = parts ? workspace : nullptr;
+  p.part_ml = parts ? workspace + rows * p.splits * D : nullptr;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.cap_in = cap > 0.f ? scale / cap : 0.f;
   p.cap_out = cap * 1.4426950408889634f;
@@ -1118,29 +1087,27 @@ extern "C" int b200_attn_spans(const void* q, const void* k_cache, const void* v
   if (tiles * batch * n_kv_heads * splits > 0x7fffffffll) return -ERR_BAD_ARG;
   p.row_tiles = (int)tiles;
   p.splits = splits;
-  p.own_splits = 0;
   p.n_items = (int)(tiles * batch * n_kv_heads * splits);
   return spans::launch<false>(p, q, k_cache, v_cache, out, gate, block_table, kv_len, batch, T, max_blocks, num_blocks, block_size, n_q_heads,
-                              n_kv_heads, scale, cap, workspace, splits, status, stream);
+                              n_kv_heads, scale, cap, workspace, status, stream);
 }
 
-// One row per sequence.  q / out / gate [B, Hq, 128]; sequence b: the first kv_len[b] keys of table row b.  The sequences
-// group_start[g] <= b < group_start[g + 1] hold the same first shared_len[g] keys in the same pages; sequences of no group
-// share nothing.  splits / own_splits: items the shared keys and a sequence's own keys are cut into; workspace: fp32
-// [(splits + own_splits) B Hq 130].
-extern "C" int b200_attn_shared(const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate,
-                                const int* block_table, const int* kv_len, const int* group_start, const int* shared_len, int n_groups,
-                                int batch, int max_blocks, int num_blocks, int block_size, int n_q_heads, int n_kv_heads, float scale,
-                                float cap, int splits, int own_splits, float* workspace, int* status, cudaStream_t stream) {
-  if (n_groups < 0 || splits < 1 || own_splits < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || batch < 1) return -ERR_BAD_ARG;
+// One row per sequence: partial sums over the keys that groups of sequences share, for b200_attn_own_rows.  q [B, Hq, 128];
+// the sequences group_start[g] <= b < group_start[g + 1] hold the same first shared_len[g] keys in the same pages (those of the
+// group's first row of the table); sequence b sees kv_len[b] of them.  splits: items the keys are cut into; workspace: fp32
+// [splits B Hq 130].
+extern "C" int b200_attn_shared(const void* q, const void* k_cache, const void* v_cache, const int* block_table, const int* kv_len,
+                                const int* group_start, const int* shared_len, int n_groups, int batch, int max_blocks, int num_blocks,
+                                int block_size, int n_q_heads, int n_kv_heads, float scale, float cap, int splits, float* workspace,
+                                int* status, cudaStream_t stream) {
+  if (n_groups < 1 || splits < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || batch < 1) return -ERR_BAD_ARG;
   spans::Params p = {};
   p.group_start = group_start; p.shared_len = shared_len; p.n_groups = n_groups;
-  const long long rows = (long long)batch * (n_q_heads / n_kv_heads), tiles = n_groups ? rows / (2 * spans::BQ) + n_groups : 0;
-  if ((tiles * splits + (long long)batch * own_splits) * n_kv_heads > 0x7fffffffll) return -ERR_BAD_ARG;
+  const long long rows = (long long)batch * (n_q_heads / n_kv_heads), tiles = rows / (2 * spans::BQ) + n_groups;
+  if (tiles * splits * n_kv_heads > 0x7fffffffll) return -ERR_BAD_ARG;
   p.row_tiles = (int)tiles;
   p.splits = splits;
-  p.own_splits = own_splits;
-  p.n_items = (int)((tiles * splits + (long long)batch * own_splits) * n_kv_heads);
-  return spans::launch<true>(p, q, k_cache, v_cache, out, gate, block_table, kv_len, batch, batch, max_blocks, num_blocks, block_size,
-                             n_q_heads, n_kv_heads, scale, cap, workspace, splits + own_splits, status, stream);
+  p.n_items = (int)(tiles * splits * n_kv_heads);
+  return spans::launch<true>(p, q, k_cache, v_cache, nullptr, nullptr, block_table, kv_len, batch, batch, max_blocks, num_blocks, block_size,
+                             n_q_heads, n_kv_heads, scale, cap, workspace, status, stream);
 }

@@ -179,8 +179,8 @@ int b200_gqa_decode_ex(const void* q, const void* k_cache, const void* v_cache, 
 int b200_gqa_decode(const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate,
                     const int* block_table, const int* kv_len, float* workspace, int batch, int max_blocks,
                     int block_size, int n_q_heads, int n_kv_heads, int splits, float softmax_scale, cudaStream_t stream);
-// rotary positions of several axes with the append (rope_axes_kv.cu); rows with spans of keys of their own, and one row per sequence
-// over pages that groups of sequences share (attn_spans.cu)
+// rotary positions of several axes with the append (rope_axes_kv.cu); rows with spans of keys of their own (attn_spans.cu); one row per
+// sequence over pages that groups of sequences share: partial sums over those (attn_spans.cu), own keys and join (attn_own_rows.cu)
 int b200_qk_norm_rope_axes_append(const void* q_src, int ldq, int q_off, int q_head_stride, int gate_in_q, const void* k_src,
                                   int ldk, int k_off, const void* v_src, int ldv, int v_off, const void* q_gamma,
                                   const void* k_gamma, int unit_offset, float eps, const float* inv_freq, int rot, float mscale,
@@ -191,10 +191,14 @@ int b200_attn_spans(const void* q, const void* k_cache, const void* v_cache, voi
                     const int* q_start, const int* q_len, const int* kv_len, const int* lo, const int* hi, int batch,
                     int max_q_len, int T, int max_blocks, int num_blocks, int block_size, int n_q_heads, int n_kv_heads,
                     float scale, float cap, int splits, float* workspace, int* status, cudaStream_t stream);
-int b200_attn_shared(const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate, const int* block_table,
-                     const int* kv_len, const int* group_start, const int* shared_len, int n_groups, int batch, int max_blocks,
-                     int num_blocks, int block_size, int n_q_heads, int n_kv_heads, float scale, float cap, int splits,
-                     int own_splits, float* workspace, int* status, cudaStream_t stream);
+int b200_attn_shared(const void* q, const void* k_cache, const void* v_cache, const int* block_table, const int* kv_len,
+                     const int* group_start, const int* shared_len, int n_groups, int batch, int max_blocks, int num_blocks,
+                     int block_size, int n_q_heads, int n_kv_heads, float scale, float cap, int splits, float* workspace,
+                     int* status, cudaStream_t stream);
+int b200_attn_own_rows(const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate, const int* block_table,
+                       const int* kv_len, const int* group_start, const int* shared_len, int n_groups, int batch, int max_blocks,
+                       int num_blocks, int block_size, int n_q_heads, int n_kv_heads, float scale, float cap, int slots,
+                       const float* workspace, int cluster, cudaStream_t stream);
 // FlashMemory retriever (flashmemory.cu): chunk scores of one scorer layer, layer ensemble, top-k, index offset
 int b200_fm_score_layer(const float* hidden, const void* wq_a, const void* wq_b, const float* q_norm, const void* weights_proj,
                         const float* inv_freqs, const void* keys8, const float* keysf, float* q_scratch, float* qlora_scratch,

@@ -260,7 +260,8 @@ def _kernels() -> ctypes.CDLL:
         lib.b200_qk_norm_rope_axes_append.argtypes = [_P, _I, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _f, _P, _I, _f, ctypes.c_char_p, _I, _P,
                                                       _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]
         lib.b200_attn_spans.argtypes = [_P] * 11 + [_I] * 8 + [_f, _f, _I, _P, _P, _P]
-        lib.b200_attn_shared.argtypes = [_P] * 9 + [_I] * 7 + [_f, _f, _I, _I, _P, _P, _P]
+        lib.b200_attn_shared.argtypes = [_P] * 7 + [_I] * 7 + [_f, _f, _I, _P, _P, _P]
+        lib.b200_attn_own_rows.argtypes = [_P] * 9 + [_I] * 7 + [_f, _f, _I, _P, _I, _P]
         _typed = True
     return lib
 
@@ -407,14 +408,14 @@ def shared_groups(pages, block_size: int) -> tuple[list[int], list[int]]:
 
 
 def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_len, gate=None, scale=None, cap: float = 0.0,
-                  max_shared: int | None = None, max_kv_len: int | None = None, splits: tuple[int, int] | None = None, out=None):
+                  max_shared: int | None = None, max_kv_len: int | None = None, splits: int | None = None, out=None):
     """``decode`` (one query row per sequence) where groups of sequences hold the same leading pages, as a prefix cache hands them
     out: those keys are read and multiplied once for the whole group.
 
     q: [B, Hq, 128]; group_start int32 [groups + 1], shared_len int32 [groups] (device; ``shared_groups``): the rows
     group_start[g] .. group_start[g + 1] - 1 of ``block_table`` begin with the same pages, whose first shared_len[g] keys they have
     in common (keys at ``kv_len`` and beyond stay unseen); rows of no group are on their own.  ``cap`` as in ``prefill_spans``;
-    ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys, of a sequence's own)."""
+    ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys)."""
     dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
     if b != t or shared_len.dim() != 1:
         raise ValueError(f"{t} rows for {b} sequences, shared lengths {list(shared_len.shape)}: a row per sequence and a length per group expected")
@@ -423,23 +424,31 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     _index(group_start, (n + 1,), dev, "group_start")
     if b == 0:
         return out
+    longest = max_kv_len if max_kv_len is not None else width * bs
+    common = 0 if n == 0 else longest if max_shared is None else min(longest, max(0, int(max_shared)))
+    g = hq // hkv
     if splits is None:
-        longest = max_kv_len if max_kv_len is not None else width * bs
-        common = 0 if n == 0 else longest if max_shared is None else min(longest, max(0, int(max_shared)))
-        keys, own_keys = -(-common // KEY_TILE), -(-(longest - common) // KEY_TILE) + 1
-        tiles = (b * (hq // hkv) // ROW_TILE + n) * hkv
-        share = (tiles * keys + b * hkv * own_keys) / NUM_SMS             # key tiles of an SM
-        splits = (max(1, min(64, round(keys / max(2.0, share)))), max(1, min(64, round(own_keys / max(4.0, share)))))
-    if not (1 <= splits[0] <= 1024 and 1 <= splits[1] <= 1024):
-        raise ValueError(f"splits {splits}")
+        tiles = (b * g // ROW_TILE + n) * hkv
+        splits = max(1, min(64, NUM_SMS // max(1, tiles), -(-common // (2 * KEY_TILE))))
+    if not 1 <= splits <= 1024:
+        raise ValueError(f"{splits} splits")
+    # blocks that share a sequence's own keys: while the GPU has room for more and a block has 128 keys
+    blocks, cluster = b * hkv * -(-g // 16), 1
+    while cluster < 8 and 2 * cluster * blocks <= 3 * NUM_SMS and (longest - common) > 128 * cluster:
+        cluster *= 2
     with _on(dev):
-        ws = torch.empty(sum(splits) * b * hq * (D + 2), dtype=torch.float32, device=q.device)
+        lib, stream = _kernels(), torch._C._cuda_getCurrentRawStream(dev)
         _lib.check_indices(block_table, 0, nb, 3)
-        rc = _kernels().b200_attn_shared(
+        ws = torch.empty(splits * b * hq * (D + 2), dtype=torch.float32, device=q.device) if n else None
+        if n:
+            rc = lib.b200_attn_shared(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(), group_start.data_ptr(),
+                shared_len.data_ptr(), n, b, width, nb, bs, hq, hkv, scale, cap, splits, ws.data_ptr(), _lib.status_word(q.device).data_ptr(), stream)
+            _lib.check(rc, "decode_shared")
+        rc = lib.b200_attn_own_rows(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
-            group_start.data_ptr(), shared_len.data_ptr(), n, b, width, nb, bs, hq, hkv, scale, cap, splits[0], splits[1], ws.data_ptr(),
-            _lib.status_word(q.device).data_ptr(), torch._C._cuda_getCurrentRawStream(dev))
-    _lib.check(rc, "decode_shared", 2)
+            group_start.data_ptr(), shared_len.data_ptr(), n, b, width, nb, bs, hq, hkv, scale, cap, splits if n else 0, _at(ws), cluster, stream)
+    _lib.check(rc, "decode_shared")
     return out
 
 

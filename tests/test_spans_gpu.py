@@ -246,7 +246,7 @@ def test_shared_pages(groups, hq, hkv, bs, gate, cap):
     run_shared(groups, hq, hkv, bs, cap=cap, gate=gate)
 
 
-@pytest.mark.parametrize("splits", [(1, 1), (2, 3), (7, 2), (64, 64)])
+@pytest.mark.parametrize("splits", [1, 2, 7, 64])
 def test_shared_pages_cut_into_items(splits):
     run_shared([(900 // 64 * 64, [10, 700, 64]), (192, [1] * 6)], 8, 2, 64, splits=splits, gate=True, alone=3)
 
@@ -261,3 +261,15 @@ def test_values_that_are_not_finite_in_one_sequence():
         rows[1][1][700, :, 5] = NAN
         rows[2][1][705, 0, 6] = math.inf
     run_shared([(640, [70, 70, 70])], 4, 2, 64, poke=poke)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (7, 1), (8, 1), (9, 1), (24, 2), (17, 1), (40, 1)])
+def test_head_counts(hq, hkv):
+    """One, a group of 8, two, and more heads of a kv head than a block takes."""
+    run_shared([(128, [1, 130, 64]), (64, [300])], hq, hkv, 32, alone=2, gate=True)
+    run_spans([(20, 150), (3, 3)], hq, hkv, 32, causal)
+
+
+@pytest.mark.parametrize("own", [15, 16, 17, 500, 2100, 9000])
+def test_long_own_contexts(own):
+    run_shared([(64, [own, 1]), (0, [own])], 6, 2, 16, cap=20.0)
