@@ -15,6 +15,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 #include "launch.h"
+#include "per_device.h"
 #include "ops.h"
 
 namespace {
@@ -57,6 +58,11 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&x);
 }
 __device__ __forceinline__ uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+__device__ __forceinline__ uint4 lds128(const uint4* p) {          // (not to be kept in registers over a loop)
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"((uint32_t)__cvta_generic_to_shared(p)));
+  return v;
+}
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
   uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
@@ -66,13 +72,22 @@ __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ float4 ld_cluster4(const float* p, uint32_t rank) {
+  uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(r) : "memory");
+  return v;
+}
+
 // NB: groups of 8 heads a block works on.
 template <int NB>
 __global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
 own_rows_kernel(const __grid_constant__ OwnParams p) {
   constexpr int H = 8 * NB;
   __shared__ float s_m[WARPS][H], s_l[WARPS][H];
-  __shared__ float s_o[WARPS][H][LD];
+  __shared__ __align__(16) float s_o[WARPS][H][LD];
+  __shared__ uint4 s_q[H][20];
   b200::pdl_grid_trigger();
   if (p.slots == 0) b200::pdl_grid_wait();               // (otherwise the kernel before has waited for what these products read)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -83,22 +98,26 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
   const int kvh = x % p.Hkv, b = x / p.Hkv;
   const int heads = min(H, p.G - h0);
 
-  int shared = 0;
-  for (int i = lane; i < p.n_groups; i += 32)
-    if (b >= p.group_start[i] && b < p.group_start[i + 1]) shared = max(shared, p.shared_len[i]);
-  shared = __reduce_max_sync(0xffffffffu, shared);
   const int kv = max(0, min(p.kv_len[b], p.max_blocks * p.bs));
+  int shared = 0, group_lo = -1, group_hi = -1;
+  for (int i = lane; i < p.n_groups; i += 32) {
+    const int lo = p.group_start[i], hi = p.group_start[i + 1], n = p.shared_len[i];     // (one trip to memory for the three)
+    if (b >= lo && b < hi && n > 0) {
+      shared = n;
+      group_lo = lo;
+      group_hi = hi;
+    }
+  }
+  shared = __reduce_max_sync(0xffffffffu, shared);
   const int first = shared >> 4, n_blk = max(0, ((kv + 15) >> 4) - first);               // blocks of 16 keys
   const int* bt = p.block_table + (size_t)b * p.max_blocks;
 
-  uint4 q[NB][4];                                        // head 8 i + g, dims 32 x + 8 c ..
-#pragma unroll
-  for (int i = 0; i < NB; ++i)
-#pragma unroll
-    for (int d = 0; d < 4; ++d)
-      q[i][d] = i * 8 + g < heads
-                    ? *reinterpret_cast<const uint4*>(p.q + ((size_t)b * p.Hq + kvh * p.G + h0 + i * 8 + g) * D + d * 32 + c * 8)
-                    : make_uint4(0, 0, 0, 0);
+  // The queries stay in shared memory (rows of 320 bytes: free of bank conflicts for the reads below), so that four blocks fit an SM.
+  for (int i = threadIdx.x; i < H * 16; i += WARPS * 32) {
+    const int h = i >> 4, d = i & 15;
+    s_q[h][d] = h < heads ? reinterpret_cast<const uint4*>(p.q + ((size_t)b * p.Hq + kvh * p.G + h0 + h) * D)[d] : make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
   float o[NB][8][4];                                     // dims 8 g + i, 64 + 8 g + i of heads 2 c, 2 c + 1
 #pragma unroll
   for (int i = 0; i < NB; ++i)
@@ -151,8 +170,9 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
       s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        mma_bf16(s[i], k[0][d].x, k[1][d].x, k[0][d].y, k[1][d].y, q[i][d].x, q[i][d].y);
-        mma_bf16(s[i], k[0][d].z, k[1][d].z, k[0][d].w, k[1][d].w, q[i][d].z, q[i][d].w);
+        const uint4 q = lds128(&s_q[i * 8 + g][d * 4 + c]);                // head 8 i + g, dims 32 d + 8 c ..
+        mma_bf16(s[i], k[0][d].x, k[1][d].x, k[0][d].y, k[1][d].y, q.x, q.y);
+        mma_bf16(s[i], k[0][d].z, k[1][d].z, k[0][d].w, k[1][d].w, q.z, q.w);
       }
     }
     const int next = blk + step;
@@ -228,50 +248,104 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
       }
     }
   __syncthreads();
-  if (p.cluster > 1) cluster_sync();
+  const bool many = p.cluster > 1;
+  if (many) cluster_sync();
   if (p.slots) b200::pdl_grid_wait();
-  const size_t rows = (size_t)p.B * p.Hq;
-  // four dims of a head a thread: a warp per head
-  for (int h = rank * WARPS + warp; h < heads; h += WARPS * p.cluster) {
-    const size_t at = (size_t)b * p.Hq + kvh * p.G + h0 + h;
-    const int pos = (lane >> 4) * 64 + (lane & 1) * 32 + ((lane >> 1) & 7);              // of dims 4 lane ..: 64 y' + 8 d + g, d = 4 (lane & 1) ..
-    float M = -INFINITY;
-    for (int r = 0; r < p.cluster; ++r)
+  const size_t rows = (size_t)p.B * p.Hq, at0 = (size_t)b * p.Hq + kvh * p.G + h0;
+  // how often the keys of a head's row tile were cut: half as often for a rest of at most 128 (row, head) pairs
+  group_lo = max(0, __reduce_max_sync(0xffffffffu, group_lo));
+  group_hi = min(p.B, __reduce_max_sync(0xffffffffu, group_hi));
+  auto slots_of = [&](int h) {
+    const int r = (b - group_lo) * p.G + h0 + h, rest = (group_hi - group_lo) * p.G - r / 256 * 256;
+    return shared <= 0 ? 0 : rest <= 128 ? (p.slots + 1) / 2 : p.slots;
+  };
+  const int slots = shared > 0 ? p.slots : 0, W = rank * WARPS + warp, n_warps = WARPS * p.cluster;
+  // Every warp finds the maximum and the sum of every head over all warps and slots (a lane per warp and two slots); it then weighs
+  // its own sums and every n_warps'th slot's, four dims a lane, into its rows of shared memory.
+  float inv = 0.f;                                       // of head `lane`
+#pragma unroll 1
+  for (int i = 0; i < heads; i += 4) {                   // (four heads at a time: their slots' sums fit the registers)
+    float2 ml[4][2];
+    float mw[4], lw[4];
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, p.cluster > 1 ? ld_cluster(&s_m[w][h], r) : s_m[w][h]);
-    const int slots = shared > 0 ? p.slots : 0;
-    for (int s = 0; s < slots; ++s) M = fmaxf(M, p.part_ml[(s * rows + at) * 2]);
-    float L = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < 4; ++h) {
+      const bool ok = i + h < heads;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int sl = lane + 32 * y;
+        ml[h][y] = ok && sl < slots_of(i + h) ? *reinterpret_cast<const float2*>(p.part_ml + (sl * rows + at0 + i + h) * 2) : make_float2(-INFINITY, 0.f);
+      }
+      mw[h] = -INFINITY;
+      lw[h] = 0.f;
+      if (lane < n_warps) {
+        const int r = lane / WARPS, w = lane % WARPS;
+        mw[h] = many ? ld_cluster(&s_m[w][i + h], r) : s_m[w][i + h];
+        lw[h] = many ? ld_cluster(&s_l[w][i + h], r) : s_l[w][i + h];
+      }
+    }
+    float f_own[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      float M = fmaxf(mw[h], fmaxf(ml[h][0].x, ml[h][1].x));
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+      // (a sum of zero weighs nothing: what lies beside it may not have been written)
+      const float fw = lw[h] == 0.f ? 0.f : exp2f(mw[h] - M);
+      ml[h][0].x = ml[h][0].y == 0.f ? 0.f : exp2f(ml[h][0].x - M);
+      ml[h][1].x = ml[h][1].y == 0.f ? 0.f : exp2f(ml[h][1].x - M);
+      float L = fw * lw[h] + ml[h][0].x * ml[h][0].y + ml[h][1].x * ml[h][1].y;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+      if (lane == i + h) inv = L == 0.f ? 0.f : 1.f / L;
+      f_own[h] = __shfl_sync(0xffffffffu, fw, W);
+    }
+    const int pos = (lane >> 4) * 64 + (lane & 1) * 32 + ((lane >> 1) & 7);            // of dims 4 lane ..: 64 y' + 8 d + g, d = 4 (lane & 1) ..
+    float a[4][4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) a[h][y] = f_own[h] == 0.f ? 0.f : f_own[h] * s_o[warp][i + h][pos + 8 * y];
+#pragma unroll 2
+    for (int sl = W; sl < slots; sl += n_warps) {
+      float4 x[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        x[h] = i + h < heads ? *reinterpret_cast<const float4*>(p.part_o + (sl * rows + at0 + i + h) * D + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const float f = __shfl_sync(0xffffffffu, sl < 32 ? ml[h][0].x : ml[h][1].x, sl & 31);
+        if (f == 0.f) continue;                          // (nothing seen, or no such slot: what lies there is not looked at)
+        a[h][0] += f * x[h].x; a[h][1] += f * x[h].y; a[h][2] += f * x[h].z; a[h][3] += f * x[h].w;
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 4; ++h) *reinterpret_cast<float4*>(&s_o[warp][i + h][lane * 4]) = make_float4(a[h][0], a[h][1], a[h][2], a[h][3]);
+  }
+  __syncthreads();
+  if (many) cluster_sync();
+#pragma unroll 1
+  for (int h = W; h < heads; h += n_warps) {             // a warp per head
+    const size_t at = at0 + h;
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    uint2 u = make_uint2(0, 0);
+    if (p.gate) u = *reinterpret_cast<const uint2*>(p.gate + at * D + lane * 4);
     for (int r = 0; r < p.cluster; ++r)
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float lw = p.cluster > 1 ? ld_cluster(&s_l[w][h], r) : s_l[w][h];
-        if (lw == 0.f) continue;
-        const float f = exp2f((p.cluster > 1 ? ld_cluster(&s_m[w][h], r) : s_m[w][h]) - M);
-        L += f * lw;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) a[y] += f * (p.cluster > 1 ? ld_cluster(&s_o[w][h][pos + 8 * y], r) : s_o[w][h][pos + 8 * y]);
+        const float4 x = many ? ld_cluster4(&s_o[w][h][lane * 4], r) : *reinterpret_cast<const float4*>(&s_o[w][h][lane * 4]);
+        a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w;
       }
-#pragma unroll 4
-    for (int s = 0; s < slots; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + at) * 2);
-      if (ml.y == 0.f) continue;                         // (nothing seen: the sums may not have been written)
-      const float4 y = *reinterpret_cast<const float4*>(p.part_o + (s * rows + at) * D + lane * 4);
-      const float f = exp2f(ml.x - M);
-      L += f * ml.y;
-      a[0] += f * y.x; a[1] += f * y.y; a[2] += f * y.z; a[3] += f * y.w;
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const float f = __shfl_sync(0xffffffffu, inv, h);
 #pragma unroll
-    for (int y = 0; y < 4; ++y) a[y] *= inv;
+    for (int y = 0; y < 4; ++y) a[y] *= f;
     if (p.gate) {
-      const uint2 u = *reinterpret_cast<const uint2*>(p.gate + at * D + lane * 4);
       const __nv_bfloat162* hp = reinterpret_cast<const __nv_bfloat162*>(&u);
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const float2 f = __bfloat1622float2(hp[y]);
-        a[2 * y] *= 1.f / (1.f + __expf(-f.x));
-        a[2 * y + 1] *= 1.f / (1.f + __expf(-f.y));
+        const float2 z = __bfloat1622float2(hp[y]);
+        a[2 * y] *= 1.f / (1.f + __expf(-z.x));
+        a[2 * y + 1] *= 1.f / (1.f + __expf(-z.y));
       }
     }
     *reinterpret_cast<uint2*>(p.out + at * D + lane * 4) = make_uint2(pack(a[0], a[1]), pack(a[2], a[3]));
@@ -281,6 +355,14 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
 
 template <int NB>
 cudaError_t launch(const OwnParams& p, cudaStream_t stream) {
+  static b200::PerDeviceOnce once_;
+  bool& configured = once_.slot();
+  if (!configured) {
+    // the split of the SMs' memory that the kernel over the shared keys has: another one would wait for every block of that kernel to leave
+    const cudaError_t e = cudaFuncSetAttribute(own_rows_kernel<NB>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+    configured = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hkv * p.chunks * p.cluster));
   cfg.blockDim = dim3(WARPS * 32);
@@ -307,7 +389,7 @@ extern "C" int b200_attn_own_rows(const void* q, const void* k_cache, const void
                                   float cap, int slots, const float* workspace, int cluster, cudaStream_t stream) {
   const bool pow2 = block_size >= 16 && block_size <= 256 && !(block_size & (block_size - 1));
   if (!pow2 || n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads || batch < 1 || max_blocks < 1 || num_blocks < 1 || n_groups < 0 ||
-      !(scale > 0.f) || !(cap >= 0.f) || (long long)max_blocks * block_size > 0x7fffff00ll || slots < 0 || (slots > 0 && !workspace) ||
+      !(scale > 0.f) || !(cap >= 0.f) || (long long)max_blocks * block_size > 0x7fffff00ll || slots < 0 || slots > 64 || (slots > 0 && !workspace) ||
       (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8))
     return -6;
   OwnParams p = {};

@@ -228,14 +228,11 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
   it.n_rows = 0;
   int split, splits;
   int rows_all;
-  split = idx % p.splits;
-  splits = p.splits;
-  int x = idx / p.splits;
-  it.kvh = x % p.Hkv;
-  x /= p.Hkv;
-  it.slot = split;
   if (SHARED) {
-    int tile = x, b0 = 0, rows = -1, shared = 0;
+    // A group's rows are whole tiles and a rest; a rest of at most 128 rows takes half the time per key (both streams work on it), so its
+    // keys are cut into half as many items.
+    const int few = (p.splits + 1) / 2;
+    int y = idx, b0 = 0, rows = -1, shared = 0;
     for (int base = 0; base < p.n_groups && rows < 0; base += 32) {      // a group per lane
       const int g = base + lane;
       int first = 0, n = 0, sh = 0;
@@ -244,34 +241,48 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
         n = max(0, min(p.batch, p.group_start[g + 1]) - first) * p.G;
         sh = p.shared_len[g];
       }
-      const int tiles = (n + 2 * BQ - 1) / (2 * BQ);
-      int upto = tiles;
+      const int rest = n % (2 * BQ), tiles = n / (2 * BQ) + (rest > BQ);
+      const int items = sh > 0 ? p.Hkv * (tiles * p.splits + (rest > 0 && rest <= BQ ? few : 0)) : 0;
+      int upto = items;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
+        const int before = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += before;
       }
-      const uint32_t here = __ballot_sync(0xffffffffu, tile < upto);
+      const uint32_t here = __ballot_sync(0xffffffffu, y < upto);
       if (here) {
         const int src = __ffs(here) - 1;
         b0 = __shfl_sync(0xffffffffu, first, src);
         rows = __shfl_sync(0xffffffffu, n, src);
         shared = __shfl_sync(0xffffffffu, sh, src);
-        tile -= __shfl_sync(0xffffffffu, upto - tiles, src);
+        y -= __shfl_sync(0xffffffffu, upto - items, src);
       } else {
-        tile -= __shfl_sync(0xffffffffu, upto, 31);
+        y -= __shfl_sync(0xffffffffu, upto, 31);
       }
     }
     if (rows < 0) return false;
+    const int tiles = rows / (2 * BQ) + (rows % (2 * BQ) > BQ), whole = p.Hkv * tiles * p.splits;
+    const bool last = y >= whole;                          // the rest
+    splits = last ? few : p.splits;
+    if (last) y -= whole;
+    split = y % splits;
+    it.kvh = y / splits % p.Hkv;
+    const int tile = last ? tiles : y / (splits * p.Hkv);
+    it.slot = split;
     it.base_tok = it.trow = b0;
     it.r0 = tile * 2 * BQ;
     rows_all = rows;
     it.own_lo = 0;
     it.own_hi = shared;
-    if (shared <= 0) return false;                         // (nobody looks at its slots)
     it.kv_end = p.max_blocks * p.bs;
     it.delta = 0;
   } else {
+    split = idx % p.splits;
+    splits = p.splits;
+    int x = idx / p.splits;
+    it.kvh = x % p.Hkv;
+    x /= p.Hkv;
+    it.slot = split;
     const int b = x % p.batch, tile = p.row_tiles - 1 - x / p.batch;       // long contexts first
     const int q0 = p.q_start[b], n = p.q_len[b];
     const int len = q0 < 0 ? 0 : min(n, p.T - q0);
@@ -342,10 +353,13 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   uint8_t* sQ = smem;                                       // [2 streams] tiles; scratch of the join of the streams
   uint8_t* sR = smem + 2 * TILE;                            // ring of key and value tiles
   uint64_t* bars = reinterpret_cast<uint64_t*>(sR + STAGES * TILE);
-  uint64_t* r_full = bars;
-  uint64_t* r_empty = bars + STAGES;
-  uint64_t* v_ok = bars + 2 * STAGES;                       // values checked (tile by tile, not by place in the ring)
-  uint64_t* q_full = bars + 3 * STAGES;                     // per stream: queries there, O zero
+  // Stages are given back by place in the ring, but filled by tile: a stage holds keys and values in turn, loads finish in any order, and
+  // a role that waits for the values alone would take the phase of two loads ago for the one it waits for.
+  uint64_t* r_empty = bars;
+  uint64_t* k_full = bars + STAGES;                         // by tile, modulo STAGES (never more than three tiles are on their way)
+  uint64_t* v_full = bars + 2 * STAGES;
+  uint64_t* v_ok = bars + 3 * STAGES;                       // values checked
+  uint64_t* q_full = bars + 4 * STAGES;                     // per stream: queries there, O zero
   uint64_t* s_full = q_full + 2;
   uint64_t* p_half = q_full + 4;                            // P of the tile's first 64 keys
   uint64_t* p_full = q_full + 6;
@@ -357,14 +371,15 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   uint64_t* pv_half = i_empty + ITEMS;                      // per stream: the product with the values of a tile's first 64 keys
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_half + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* s_bad = reinterpret_cast<uint32_t*>(bars + 48); // [STAGES][4] keys with values that are not finite
-  float* s_ml = reinterpret_cast<float*>(bars + 58);        // [2][128] maximum and sum of stream 1
-  Item* s_item = reinterpret_cast<Item*>(bars + 58 + 128);  // [ITEMS]
+  uint32_t* s_bad = reinterpret_cast<uint32_t*>(bars + 52); // [STAGES][4] keys with values that are not finite
+  float* s_ml = reinterpret_cast<float*>(bars + 62);        // [2][128] maximum and sum of stream 1
+  Item* s_item = reinterpret_cast<Item*>(bars + 62 + 128);  // [ITEMS]
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform: the issuer depends on it
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&r_full[i], 1);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
       mbar_init(&r_empty[i], 1);
       mbar_init(&v_ok[i], 1);
     }
@@ -415,7 +430,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   // registers per thread at launch: 168 (3 x 168 = 2 x 224 + 56)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    Ring r = {0, 0}, c = {0, 0};                           // places of tiles in the ring; of value tiles among their checks
+    Ring r = {0, 0}, c = {0, 0};                           // a stage; a tile
     bool ok = true;
     if (warp == 8) {
       const int rows = min(p.bs, BKV), per_tile = BKV / rows;              // pages (or parts of one) in a tile
@@ -466,16 +481,18 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           for (int kv = 0; kv < 2; ++kv) {
             ok = warp_wait(&r_empty[r.st], r.ph) && !*abort_flag;
             if (!ok) break;
-            if (lane == 0) mbar_expect_tx(&r_full[r.st], n * 2 * sub_bytes);
+            uint64_t* full = (kv ? v_full : k_full) + c.st;
+            if (lane == 0) mbar_expect_tx(full, n * 2 * sub_bytes);
             __syncwarp();
             if (lane < n) {
               uint8_t* dst = sR + r.st * TILE + lane * sub_bytes;
-              tma_load_2d(dst, kv ? &tmV : &tmK, &r_full[r.st], 0, row);
-              tma_load_2d(dst + ATOM, kv ? &tmV : &tmK, &r_full[r.st], 64, row);
+              tma_load_2d(dst, kv ? &tmV : &tmK, full, 0, row);
+              tma_load_2d(dst + ATOM, kv ? &tmV : &tmK, full, 64, row);
             }
             r.next();
           }
           row = next_row;
+          c.next();
         }
       }
       if (!ok && lane == 0) { atomicExch(p.status, ERR_WAIT_STAGE); *abort_flag = 1; }
@@ -490,7 +507,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       };
       const uint64_t dq0 = umma_desc_sw128(sQ), dk = umma_desc_sw128(sR), dv = desc_mn_sw128(sR, ATOM, 1024);
       uint32_t ph_q[2] = {0, 0}, ph_p[2] = {0, 0};
-      Ring k = {0, 0}, v = {1, 0};                         // places of the next key tile and the next value tile
+      Ring k = {0, 0}, v = {1, 0}, kt = {0, 0};            // stages of the next key tile and the next value tile; the next key tile
       for (;;) {
         if (ok) ok = next_item();
         if (!ok || it.n_rows == 0) break;
@@ -507,11 +524,12 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           if (dual || m) {
             umma_commit_warp(on, &r_empty[k.st]);
             k.two();
+            kt.next();
           }
         };
 #pragma unroll
         for (int m = 0; m < 2; ++m)
-          if (ok && m < steps && wait2(&q_full[m], ph_q[m], &r_full[k.st], k.ph)) {
+          if (ok && m < steps && wait2(&q_full[m], ph_q[m], &k_full[kt.st], kt.ph)) {
             ph_q[m] ^= 1;
             tc_fence_after();
             scores(m);
@@ -528,7 +546,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             for (int s = 0; s < 4; ++s) umma_bf16_ts_warp(on, tmem + 256 + m * 128, tmem + m * 128 + s * 8, b + s * 128, idesc_pv, 1u);
             umma_commit_warp(on, &pv_half[m]);
             const bool more = u + 2 < steps;
-            if (!wait2(&p_full[m], ph_p[m], more ? &r_full[k.st] : &p_full[m], more ? k.ph : ph_p[m])) break;
+            if (!wait2(&p_full[m], ph_p[m], more ? &k_full[kt.st] : &p_full[m], more ? kt.ph : ph_p[m])) break;
             ph_p[m] ^= 1;
             tc_fence_after();
 #pragma unroll
@@ -550,7 +568,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         if (!ok || it.n_rows == 0) break;
         for (int t = it.t0; ok && t < it.t1; ++t) {
           r.next();
-          ok = warp_wait(&r_full[r.st], r.ph) && !*abort_flag;
+          ok = warp_wait(&v_full[c.st], c.ph) && !*abort_flag;
           if (!ok) break;
           const int key0 = t * BKV;
           if (key0 < it.lo_max || key0 + BKV > it.hi_min) {

@@ -407,6 +407,22 @@ def shared_groups(pages, block_size: int) -> tuple[list[int], list[int]]:
     return start, shared
 
 
+def _shared_splits(rows: int, groups: int, g: int, hkv: int, tiles: int, own_keys: int) -> int:
+    """Items the shared keys are cut into.  A tile of 128 keys takes an SM about 2 us for a row tile of more than 128 (row, head) pairs and
+    half of it for a smaller one, which is cut half as often; a sequence's own keys come at 40 KB an SM and us, on the SMs
+    that are left.  Cut as finely as fills the GPU where the shared keys are most of the work (64 rows on 32768 keys: 4 / 9 / 18 / 36 items
+    121 / 93 / 108 / 128 us), and by their share of it where they are not (16 rows on 1024 keys, 2000 own ones each: 1 / 4 / 18 items
+    38 / 50 / 58 us)."""
+    if groups == 0:
+        return 1
+    per_group = max(1, rows * g // groups)
+    whole, rest = divmod(per_group, ROW_TILE)
+    halves = groups * hkv * (2 * (whole + (rest > ROW_TILE // 2)) + (0 < rest <= ROW_TILE // 2))          # row tiles, in halves of the time
+    work, own_work = halves * tiles * 1.0, rows * hkv * own_keys * (4 * D / 40e3)
+    sms = NUM_SMS if 2 * work >= own_work else max(1.0, NUM_SMS * work / (work + own_work))
+    return max(1, min(64, int(2 * sms / halves), -(-tiles // 2)))
+
+
 def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_len, gate=None, scale=None, cap: float = 0.0,
                   max_shared: int | None = None, max_kv_len: int | None = None, splits: int | None = None, out=None):
     """``decode`` (one query row per sequence) where groups of sequences hold the same leading pages, as a prefix cache hands them
@@ -427,14 +443,15 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     longest = max_kv_len if max_kv_len is not None else width * bs
     common = 0 if n == 0 else longest if max_shared is None else min(longest, max(0, int(max_shared)))
     g = hq // hkv
+    own_keys = longest - common
     if splits is None:
-        tiles = (b * g // ROW_TILE + n) * hkv
-        splits = max(1, min(64, NUM_SMS // max(1, tiles), -(-common // (2 * KEY_TILE))))
-    if not 1 <= splits <= 1024:
+        splits = _shared_splits(b, n, g, hkv, -(-common // KEY_TILE), own_keys)
+    if not 1 <= splits <= 64:
         raise ValueError(f"{splits} splits")
-    # blocks that share a sequence's own keys: while the GPU has room for more and a block has 128 keys
+    # Blocks that share a sequence's own keys: a cluster is slow to launch (32 sequences of 128 keys: 32 us alone, 39 / 53 / 108 us with 2 / 4 / 8
+    # blocks), so that it pays only where sequences and kv heads leave SMs idle (2 of 16000 keys: 331 us alone, 172 / 90 / 64 us).
     blocks, cluster = b * hkv * -(-g // 16), 1
-    while cluster < 8 and 2 * cluster * blocks <= 3 * NUM_SMS and (longest - common) > 128 * cluster:
+    while cluster < 8 and cluster * blocks <= NUM_SMS and own_keys > 256 * cluster:
         cluster *= 2
     with _on(dev):
         lib, stream = _kernels(), torch._C._cuda_getCurrentRawStream(dev)

@@ -84,7 +84,7 @@ def test_refusals_on_a_device():
     for change in ({"lo": i(3)}, {"hi": i(2).long()}, {"q_start": i(1)}, {"splits": 0}, {"splits": 5000}):
         with pytest.raises(ValueError):
             attention.prefill_spans(**dev(_args()) | spans | change)
-    for change in ({"group_start": i(1)}, {"shared_len": i(2)}, {"splits": 0}, {"block_table": i(3, 3), "kv_len": i(3)}):
+    for change in ({"group_start": i(1)}, {"shared_len": i(2)}, {"splits": 65}, {"block_table": i(3, 3), "kv_len": i(3)}):
         with pytest.raises(ValueError):
             attention.decode_shared(**dev(_args()) | shared | change)
     src, kc = c(2, 1024), c(3, 2, 64, 128)

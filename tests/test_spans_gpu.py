@@ -273,3 +273,31 @@ def test_head_counts(hq, hkv):
 @pytest.mark.parametrize("own", [15, 16, 17, 500, 2100, 9000])
 def test_long_own_contexts(own):
     run_shared([(64, [own, 1]), (0, [own])], 6, 2, 16, cap=20.0)
+
+
+def test_results_do_not_depend_on_the_memory_s_pace():
+    """Several items a block, loads that finish late and in any order (another stream keeps the memory busy): the same bits every time."""
+    from deepseek_v4_2080ti_b200.ops import _lib, attention
+    torch.manual_seed(5)
+    b, hq, hkv, bs, shared, own = 40, 40, 8, 64, 4096, 200
+    total = shared // bs + b * 4
+    kc, vc = rand(total, hkv, bs, 128), rand(total, hkv, bs, 128)
+    table = torch.zeros(b, shared // bs + 4, dtype=torch.long, device=DEV)
+    table[:, :shared // bs] = torch.arange(shared // bs, device=DEV)
+    table[:, shared // bs:] = shared // bs + torch.arange(b * 4, device=DEV).view(b, 4)
+    q, table, kv = rand(b, hq, 128), _i32(table), _i32([shared + own] * b)
+    rows = rand(1200, hq, 128)
+    side, big = torch.cuda.Stream(), torch.empty(1 << 28, dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    want = None
+    for i in range(60):
+        if i:
+            with torch.cuda.stream(side):
+                big[:1 << 27].copy_(big[1 << 27:])
+        got = (attention.decode_shared(q, kc, vc, table, kv, _i32([0, b]), _i32([shared]), max_shared=shared, max_kv_len=shared + own, splits=12),
+               attention.prefill_spans(rows, kc, vc, table[:1].contiguous(), _i32([0]), _i32([1200]), _i32([shared + own]), 1200, splits=1))
+        torch.cuda.synchronize()
+        _lib.check_status()
+        if want is None:
+            want = got
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), i
