@@ -65,7 +65,7 @@ struct Params {
   int n_groups;
   float* part_o;                  // [slots, T, Hq, 128], null: every row has one item
   float* part_ml;                 // [slots, T, Hq, 2]
-  int batch, T, max_blocks, bs, Hq, Hkv, G;
+  int batch, T, max_blocks, bs, bs_log2, Hq, Hkv, G;
   int row_tiles;                  // row tiles per sequence (prompt rows), over all groups (shared keys)
   int splits;                     // key ranges per row tile
   int n_items;
@@ -102,6 +102,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
       if (__any_sync(0xffffffffu, now - t0 > B200_WAIT_BUDGET_NS)) return false;
     }
   }
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      :
+      : "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
 }
 __device__ __forceinline__ void l2_prefetch(const void* p, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
@@ -156,41 +164,31 @@ __device__ __forceinline__ void exp2_fma(float& a, float& b) {
   b = __int_as_float(__float_as_int(y1) + (__float_as_int(r1) << 23));
 }
 
-// Scores s to tanh(k s).  On [-1, 1], where scores hardly ever leave, tanh(z) = z P(z^2) with an interpolation of tanh(z) / z at
-// Chebyshev points, off by 5e-7 at most, on the arithmetic units: two exponential units' steps per score cost as much as both
-// products.  NaN stays.
+// Scores s to tanh(k s) where |k s| <= 1, as it hardly ever is not: z P(z^2) with an interpolation of tanh(z) / z at Chebyshev points, off by
+// 5e-7 at most, on the arithmetic units - two exponential units' steps per score cost as much as both products.
 __device__ __forceinline__ void cap_scores(uint32_t (&sv)[2][32], float k) {
-  float big = 0.f;
+  constexpr float C[6] = {0.9999994039535522f, -0.3332895040512085f, 0.1328072100877762f, -0.0515859872102737f, 0.0167208556085825f, -0.0030582291074097f};
+  const uint64_t k2 = pack2(k, k);
 #pragma unroll
-  for (int i = 0; i < 64; i += 2) big = max3(big, fabsf(__uint_as_float(sv[i >> 5][i & 31])), fabsf(__uint_as_float(sv[i >> 5][(i & 31) + 1])));
-  if (__all_sync(0xffffffffu, big * k <= 1.f)) {
-    constexpr float C[6] = {0.9999994039535522f, -0.3332895040512085f, 0.1328072100877762f, -0.0515859872102737f, 0.0167208556085825f, -0.0030582291074097f};
-    const uint64_t k2 = pack2(k, k);
+  for (int i = 0; i < 64; i += 8) {                          // four chains of two
+    uint64_t z[4], u[4], y[4];
 #pragma unroll
-    for (int i = 0; i < 64; i += 8) {                        // four chains of two
-      uint64_t z[4], u[4], y[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        z[x] = mul2(pack2(__uint_as_float(sv[i >> 5][(i & 31) + 2 * x]), __uint_as_float(sv[i >> 5][(i & 31) + 2 * x + 1])), k2);
-        u[x] = mul2(z[x], z[x]);
-        y[x] = fma2(u[x], pack2(C[5], C[5]), pack2(C[4], C[4]));
-      }
-#pragma unroll
-      for (int d = 3; d >= 0; --d)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) y[x] = fma2(y[x], u[x], pack2(C[d], C[d]));
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float a, b;
-        unpack2(mul2(y[x], z[x]), a, b);
-        sv[i >> 5][(i & 31) + 2 * x] = __float_as_uint(a);
-        sv[i >> 5][(i & 31) + 2 * x + 1] = __float_as_uint(b);
-      }
+    for (int x = 0; x < 4; ++x) {
+      z[x] = mul2(pack2(__uint_as_float(sv[i >> 5][(i & 31) + 2 * x]), __uint_as_float(sv[i >> 5][(i & 31) + 2 * x + 1])), k2);
+      u[x] = mul2(z[x], z[x]);
+      y[x] = fma2(u[x], pack2(C[5], C[5]), pack2(C[4], C[4]));
     }
-  } else {
 #pragma unroll
-    for (int i = 0; i < 64; ++i)
-      sv[i >> 5][i & 31] = __float_as_uint(1.f - 2.f * __fdividef(1.f, 1.f + exp2f(__uint_as_float(sv[i >> 5][i & 31]) * k * 2.885390081777927f)));
+    for (int d = 3; d >= 0; --d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) y[x] = fma2(y[x], u[x], pack2(C[d], C[d]));
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      float a, b;
+      unpack2(mul2(y[x], z[x]), a, b);
+      sv[i >> 5][(i & 31) + 2 * x] = __float_as_uint(a);
+      sv[i >> 5][(i & 31) + 2 * x + 1] = __float_as_uint(b);
+    }
   }
 }
 
@@ -204,9 +202,9 @@ struct Item {
   int lo_max, hi_min;    // keys in [lo_max, hi_min) are seen by every row
   int k_end;             // first key that no row sees
   int kv_end;            // keys of the sequence
-  int own_lo, own_hi;    // span of rows that have no span of their own (one row per sequence)
+  int own_hi;            // shared keys: end of the rows' span
   int delta;             // position of a token minus its q row (prompt rows)
-  int pad;
+  int tok0, tok1;        // tokens of the rows
   __device__ __forceinline__ bool dual() const { return n_rows <= BQ; }
   __device__ __forceinline__ int steps() const { return dual() ? t1 - t0 : 2 * (t1 - t0); }
 };
@@ -214,7 +212,7 @@ struct Item {
 template <bool SHARED>
 __device__ __forceinline__ void span_of(const Params& p, const Item& it, int tok, int& lo, int& hi) {
   if (SHARED) {
-    lo = it.own_lo;
+    lo = 0;
     hi = min(it.own_hi, min(p.kv_len[tok], p.max_blocks * p.bs));
   } else {
     lo = p.lo ? max(0, p.lo[tok]) : 0;
@@ -265,25 +263,24 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
     const bool last = y >= whole;                          // the rest
     splits = last ? few : p.splits;
     if (last) y -= whole;
-    split = y % splits;
-    it.kvh = y / splits % p.Hkv;
-    const int tile = last ? tiles : y / (splits * p.Hkv);
+    const uint32_t z = (uint32_t)y / (uint32_t)splits, head = z / (uint32_t)p.Hkv;       // (unsigned: a third of the code)
+    split = y - (int)z * splits;
+    it.kvh = (int)(z - head * p.Hkv);
+    const int tile = last ? tiles : (int)head;
     it.slot = split;
     it.base_tok = it.trow = b0;
     it.r0 = tile * 2 * BQ;
     rows_all = rows;
-    it.own_lo = 0;
     it.own_hi = shared;
     it.kv_end = p.max_blocks * p.bs;
     it.delta = 0;
   } else {
-    split = idx % p.splits;
     splits = p.splits;
-    int x = idx / p.splits;
-    it.kvh = x % p.Hkv;
-    x /= p.Hkv;
+    const uint32_t x = (uint32_t)idx / (uint32_t)splits, y = x / (uint32_t)p.Hkv, z = y / (uint32_t)p.batch;
+    split = idx - (int)x * splits;
+    it.kvh = (int)(x - y * p.Hkv);
     it.slot = split;
-    const int b = x % p.batch, tile = p.row_tiles - 1 - x / p.batch;       // long contexts first
+    const int b = (int)(y - z * p.batch), tile = p.row_tiles - 1 - (int)z;                 // long contexts first
     const int q0 = p.q_start[b], n = p.q_len[b];
     const int len = q0 < 0 ? 0 : min(n, p.T - q0);
     rows_all = max(0, len) * p.G;
@@ -292,11 +289,13 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
     it.base_tok = q0;
     it.kv_end = max(0, min(p.kv_len[b], p.max_blocks * p.bs));
     it.delta = p.kv_len[b] - n - q0;
-    it.own_lo = it.own_hi = 0;
+    it.own_hi = 0;
   }
   it.n_rows = min(2 * BQ, rows_all - it.r0);
   if (it.n_rows <= 0) return false;
-  const int tok0 = it.base_tok + it.r0 / p.G, tok1 = it.base_tok + (it.r0 + it.n_rows - 1) / p.G;
+  const int tok0 = it.base_tok + (int)((uint32_t)it.r0 / (uint32_t)p.G), tok1 = it.base_tok + (int)((uint32_t)(it.r0 + it.n_rows - 1) / (uint32_t)p.G);
+  it.tok0 = tok0;
+  it.tok1 = tok1;
   int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = 0;
   for (int t = tok0 + lane; t <= tok1; t += 32) {
     int lo, hi;
@@ -314,7 +313,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
   it.k_end = __reduce_max_sync(0xffffffffu, hi_max);
   it.t0 = it.t1 = 0;
   if (it.k_end > lo_min) {
-    const int a = lo_min / BKV, n = (it.k_end + BKV - 1) / BKV - a, per = (n + splits - 1) / splits;
+    const int a = lo_min / BKV, n = (it.k_end + BKV - 1) / BKV - a, per = (int)((uint32_t)(n + splits - 1) / (uint32_t)splits);
     it.t0 = a + min(n, split * per);
     it.t1 = a + min(n, (split + 1) * per);
   }
@@ -433,7 +432,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
     Ring r = {0, 0}, c = {0, 0};                           // a stage; a tile
     bool ok = true;
     if (warp == 8) {
-      const int rows = min(p.bs, BKV), per_tile = BKV / rows;              // pages (or parts of one) in a tile
+      const int rows = min(p.bs, BKV), rows_log2 = 31 - __clz(rows), per_tile = BKV >> rows_log2;              // pages (or parts of one) in a tile
       const uint32_t sub_bytes = rows * 128;                               // one 64-column half of one
       if (lane == 0) {
         tma_prefetch_desc(&tmK);
@@ -459,23 +458,22 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         if (++i_at == ITEMS) { i_at = 0; i_ph ^= 1; }
         if (!more) break;
         {                                                                  // queries and gate on their way to L2
-          const int tok0 = it.base_tok + it.r0 / p.G, tok1 = it.base_tok + (it.r0 + it.n_rows - 1) / p.G;
-          for (int t = tok0 + lane; t <= tok1; t += 32) {
+          for (int t = it.tok0 + lane; t <= it.tok1; t += 32) {
             const size_t at = ((size_t)t * p.Hq + it.kvh * p.G) * D;
             l2_prefetch(p.q + at, p.G * D * 2);
             if (p.gate && !p.part_o) l2_prefetch(p.gate + at, p.G * D * 2);
           }
         }
         const int* bt = p.block_table + (size_t)it.trow * p.max_blocks;
-        const int last_page = (it.k_end - 1) / p.bs;
+        const int last_page = (it.k_end - 1) >> p.bs_log2;
         auto page_row = [&](int tile) {                                    // cache row where this lane's part of a tile begins
-          const int key = tile * BKV + lane * rows;
-          const int page = min(key / p.bs, last_page);
-          return tile < it.t1 && lane < per_tile ? (bt[page] * p.Hkv + it.kvh) * p.bs + key % p.bs : 0;
+          const int key = tile * BKV + (lane << rows_log2);
+          const int page = min(key >> p.bs_log2, last_page);
+          return tile < it.t1 && lane < per_tile ? ((bt[page] * p.Hkv + it.kvh) << p.bs_log2) + (key & (p.bs - 1)) : 0;
         };
         int row = page_row(it.t0);
         for (int t = it.t0; ok && t < it.t1; ++t) {
-          const int n = min(per_tile, (it.k_end - t * BKV + rows - 1) / rows);
+          const int n = min(per_tile, (it.k_end - t * BKV + rows - 1) >> rows_log2);
           const int next_row = page_row(t + 1);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
@@ -625,8 +623,9 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       const bool row_ok = row < it.n_rows;
       const bool warp_on = __any_sync(0xffffffffu, row_ok);
       const int rr = it.r0 + min(row, it.n_rows - 1);
-      const int tok = it.base_tok + rr / p.G;
-      const uint32_t at = (uint32_t)tok * p.Hq + it.kvh * p.G + rr % p.G;      // row of q and out
+      const uint32_t rt = (uint32_t)rr / (uint32_t)p.G;
+      const int tok = it.base_tok + (int)rt;
+      const uint32_t at = (uint32_t)tok * p.Hq + it.kvh * p.G + (rr - rt * p.G);         // row of q and out
       int lo, hi;
       span_of<SHARED>(p, it, tok, lo, hi);
       float m_run = -INFINITY, l_run = 0.f;
@@ -666,95 +665,89 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         const bool edge = key0 < it.lo_max || key0 + BKV > it.hi_min;
         if (warp_on) {
           tc_fence_after();
-          // The tile's scores in halves of 64, each a step of the online softmax: the second half is loaded and its maximum found
-          // under the exponentials of the first, and the products with the first half's values begin before the
-          // second is done.  Cycles a tile of one warp alone / two warps of a scheduler, without the products: 1977 / 2853
-          // in one piece, 1396 / 2314 in halves, 1197 / 2098 with a quarter of the exponentials on the arithmetic units.
-          uint32_t sv[2][2][32];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              tmem_ld_32x32(tS + h * 64 + c * 32, sv[h][c]);
-              if (h == 0 && c == 1) tmem_ld_wait();
-            }
+          // The tile's scores in halves of 64, each a step of the online softmax.
           const float scale = CAP ? p.cap_out : p.scale_log2;
           const uint64_t sc2 = pack2(scale, scale);
-          auto max_of = [&](const int h) {                 // independent chains
+          auto load = [&](int h, uint32_t (&sv)[2][32]) {
+            tmem_ld_32x32(tS + h * 64, sv[0]);
+            tmem_ld_32x32(tS + h * 64 + 32, sv[1]);
+          };
+          auto cap = [&](int h, uint32_t (&sv)[2][32]) {
+            float big = 0.f;                               // (NaN stays in it)
+#pragma unroll
+            for (int i = 0; i < 64; i += 2)
+              big = max3(big, fabsf(__uint_as_float(sv[i >> 5][i & 31])), fabsf(__uint_as_float(sv[i >> 5][(i & 31) + 1])));
+            if (__all_sync(0xffffffffu, big * p.cap_in <= 1.f)) {
+              cap_scores(sv, p.cap_in);
+            } else {                                       // in place in tensor memory, to keep the code short; NaN stays
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                uint32_t v[16];
+                tmem_ld_32x16(tS + h * 64 + c * 16, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  v[i] = __float_as_uint(1.f - 2.f * __fdividef(1.f, 1.f + exp2f(__uint_as_float(v[i]) * p.cap_in * 2.885390081777927f)));
+                tmem_st_32x16(tS + h * 64 + c * 16, v);
+              }
+              tmem_st_wait();
+              load(h, sv);
+              tmem_ld_wait();
+            }
+          };
+          auto max_of = [&](const uint32_t (&sv)[2][32]) { // independent chains
             float mx[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(sv[h][0][i]);
+            for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(sv[0][i]);
 #pragma unroll
             for (int i = 4; i < 60; i += 8)
 #pragma unroll
               for (int x = 0; x < 4; ++x)
-                mx[x] = max3(mx[x], __uint_as_float(sv[h][(i + 2 * x) >> 5][(i + 2 * x) & 31]), __uint_as_float(sv[h][(i + 2 * x + 1) >> 5][(i + 2 * x + 1) & 31]));
-            return scale * max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], __uint_as_float(sv[h][1][28]), __uint_as_float(sv[h][1][29])),
-                                max3(__uint_as_float(sv[h][1][29]), __uint_as_float(sv[h][1][30]), __uint_as_float(sv[h][1][31])));
+                mx[x] = max3(mx[x], __uint_as_float(sv[(i + 2 * x) >> 5][(i + 2 * x) & 31]), __uint_as_float(sv[(i + 2 * x + 1) >> 5][(i + 2 * x + 1) & 31]));
+            return max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], __uint_as_float(sv[1][28]), __uint_as_float(sv[1][29])),
+                        max3(__uint_as_float(sv[1][29]), __uint_as_float(sv[1][30]), __uint_as_float(sv[1][31])));
           };
-          float m_edge = -INFINITY;
-          if (edge) {                                      // both halves at once: their products wait for the check of the values
-            tmem_ld_wait();
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (CAP) cap_scores(sv[h], p.cap_in);
-              const int a = lo - key0 - h * 64, b = hi - key0 - h * 64;          // bits [a, b) of these 64 stay
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const int x = min(32, max(0, a - c * 32)), y = min(32, max(0, b - c * 32));
-                const uint32_t seen = (uint32_t)((1ull << y) - 1) & ~(uint32_t)((1ull << x) - 1);
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (!(seen & (1u << i))) sv[h][c][i] = 0xff800000u;            // -inf
-              }
-              const float x = max_of(h);
-              m_edge = max3(m_edge, x, x);
-            }
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float m_tile = h == 0 ? m_edge : -INFINITY;
-            if (!edge) {
-              if (h == 1) tmem_ld_wait();
-              if (CAP) cap_scores(sv[h], p.cap_in);
-              m_tile = max_of(h);
-            }
+          // The running maximum up to that of new scores, where it is far enough behind; false: the product that last added to O has not
+          // finished in time.  The tile before's has, as it was issued before the scores that arrived; `half`: the first half's may be on its way.
+          auto raise = [&](float m_tile, bool half) {
             // a score of NaN or +inf makes the whole row NaN, whatever the exponentials below give
             if (!(m_tile < INFINITY)) l_run = __int_as_float(0x7fffffff);
             const float m_new = fmaxf(m_run, m_tile);
             const bool grow = m_new > m_run + 8.f;         // (the first visible key: from -inf)
             const float m_next = grow ? m_new : m_run;
             if (__any_sync(0xffffffffu, grow && l_run != 0.f)) {
-              // The product that last added to O has to have finished: the one of the tile before has, as it was issued before the scores
-              // that arrived; the first half's may be on its way.
-              if (h == 1 && !(alive = warp_wait(&pv_half[m], ph_s ^ 1))) break;
+              if (half && !warp_wait(&pv_half[m], ph_s ^ 1)) return false;
               tc_fence_after();
               const float alpha = !grow ? 1.f : exp2f(m_run - m_next);
               l_run *= alpha;
 #pragma unroll 1
-              for (int c = 0; c < 4; ++c) {
-                uint32_t v[32];
-                tmem_ld_32x32(tO + c * 32, v);
+              for (int c = 0; c < 8; ++c) {
+                uint32_t v[16];
+                tmem_ld_32x16(tO + c * 16, v);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-                tmem_st_32x32(tO + c * 32, v);
+                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                tmem_st_32x16(tO + c * 16, v);
               }
             }
             m_run = m_next;
+            return true;
+          };
+          // The weights of half h, as packed pairs over the first half's scores.
+          auto weigh = [&](int h, const uint32_t (&sv)[2][32]) {
             const float m_use = m_run == -INFINITY ? 0.f : m_run;        // (nothing visible yet: every exponential is zero)
             const uint64_t nm2 = pack2(-m_use, -m_use);
             uint64_t sum2[4] = {0, 0, 0, 0};
             uint32_t w[32];
             float e[2][16];
 #pragma unroll
-            for (int b = 0; b < 5; ++b) {                  // 16 exponentials, then the sums and packing of the 16 before
-              if (b < 4) {
+            for (int c = 0; c < 5; ++c) {                  // 16 exponentials, then the sums and packing of the 16 before
+              if (c < 4) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                  float &x = e[b & 1][2 * i], &y = e[b & 1][2 * i + 1];
-                  unpack2(fma2(pack2(__uint_as_float(sv[h][b >> 1][(b & 1) * 16 + 2 * i]), __uint_as_float(sv[h][b >> 1][(b & 1) * 16 + 2 * i + 1])), sc2, nm2), x, y);
-                  if (i >= 8 - EMULATED) {
+                  float &x = e[c & 1][2 * i], &y = e[c & 1][2 * i + 1];
+                  unpack2(fma2(pack2(__uint_as_float(sv[c >> 1][(c & 1) * 16 + 2 * i]), __uint_as_float(sv[c >> 1][(c & 1) * 16 + 2 * i + 1])), sc2, nm2), x, y);
+                  if (i >= 8 - (CAP ? 0 : EMULATED)) {
                     exp2_fma(x, y);
                   } else {
                     x = exp2f(x);
@@ -762,26 +755,92 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                   }
                 }
               }
-              if (b > 0) {
+              if (c > 0) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                  const float x = e[(b - 1) & 1][2 * i], y = e[(b - 1) & 1][2 * i + 1];
+                  const float x = e[(c - 1) & 1][2 * i], y = e[(c - 1) & 1][2 * i + 1];
                   sum2[i & 3] = add2(sum2[i & 3], pack2(x, y));
                   const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
-                  w[(b - 1) * 8 + i] = *reinterpret_cast<const uint32_t*>(&z);
+                  w[(c - 1) * 8 + i] = *reinterpret_cast<const uint32_t*>(&z);
                 }
               }
             }
-            tmem_st_32x32(tS + h * 32, w);                 // packed pairs over the first half's scores
+            tmem_st_32x32(tS + h * 32, w);
             tmem_st_wait();
-            if (h == 0 && !edge) {                         // (values that are not finite go to O before any product does)
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_half[m]);
-            }
             float l0, l1;
             unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), l0, l1);
             l_run += l0 + l1;
+          };
+          if (!edge) {
+            // The second half is loaded and its maximum found under the exponentials of the first, and the products with the first half's
+            // values begin before the second is done.  Cycles a tile of one warp alone / two warps of a scheduler, without
+            // the products: 1977 / 2853 in one piece, 1396 / 2314 in halves, 1197 / 2098 with a quarter of the exponentials
+            // on the arithmetic units.
+            uint32_t sa[2][32], sb[2][32];
+            load(0, sa);
+            tmem_ld_wait();
+            load(1, sb);
+            if (CAP) cap(0, sa);
+            if (!(alive = raise(scale * max_of(sa), false))) break;
+            weigh(0, sa);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_half[m]);
+            tmem_ld_wait();
+            if (CAP) cap(1, sb);
+            if (!(alive = raise(scale * max_of(sb), true))) break;
+            weigh(1, sb);
+          } else {
+            // With masked keys the products wait for the check of the values, so that O must not be rescaled between the halves' weights:
+            // both halves' maximum comes first (of the scores themselves: a cap keeps their order).  Halves that no row of the warp sees cost
+            // nothing; a loop keeps the code short.
+            uint32_t sv[2][32];
+            auto sees = [&](int h, int& a, int& b) {       // keys [a, b) of the half's 64
+              a = lo - key0 - h * 64;
+              b = hi - key0 - h * 64;
+              return (bool)__any_sync(0xffffffffu, max(a, 0) < min(b, 64));
+            };
+            auto mask = [&](int a, int b) {
+              if (__all_sync(0xffffffffu, a <= 0 && b >= 64)) return;
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const int x = min(32, max(0, a - c * 32)), y = min(32, max(0, b - c * 32));
+                const uint32_t seen = (uint32_t)((1ull << y) - 1) & ~(uint32_t)((1ull << x) - 1);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!(seen & (1u << i))) sv[c][i] = 0xff800000u;         // -inf
+              }
+            };
+            float m_edge = -INFINITY;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              int a, b;
+              if (!sees(h, a, b)) continue;
+              load(h, sv);
+              tmem_ld_wait();
+              mask(a, b);
+              const float x = max_of(sv);
+              m_edge = max3(m_edge, x, x);
+            }
+            if (CAP && m_edge != -INFINITY) m_edge = 1.f - 2.f * __fdividef(1.f, 1.f + exp2f(m_edge * p.cap_in * 2.885390081777927f));
+            raise(m_edge * scale, false);
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              int a, b;
+              if (sees(h, a, b)) {
+                load(h, sv);
+                tmem_ld_wait();
+                if (CAP) cap(h, sv);
+                mask(a, b);
+                weigh(h, sv);
+              } else {
+                uint32_t z[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) z[i] = 0;
+                tmem_st_32x32(tS + h * 32, z);
+                tmem_st_wait();
+              }
+            }
           }
           if (!alive) break;
           if (edge) {
@@ -798,7 +857,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 const float pv = __uint_as_float(kx & 1 ? w & 0xFFFF0000u : w << 16);
                 if (key >= it.k_end) continue;
                 const bool seen = key >= lo && key < hi && pv != 0.f;
-                const size_t vrow = ((size_t)p.block_table[(size_t)it.trow * p.max_blocks + key / p.bs] * p.Hkv + it.kvh) * p.bs + key % p.bs;
+                const size_t vrow = ((size_t)p.block_table[(size_t)it.trow * p.max_blocks + (key >> p.bs_log2)] * p.Hkv + it.kvh) * p.bs + (key & (p.bs - 1));
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                   uint32_t o[32];
@@ -847,31 +906,29 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       }
       // ---- results of the item: O / l through the gate, or O with (m, l) for the join of several items.  A warp's rows go through
       // the shared memory that held its queries, so that whole lines are stored: as bf16 over the gate, or in fp32
-      // 64 columns at a time, four columns of a row at place (column / 4, row ^ column / 4 mod 8).
+      // 32 columns at a time, four columns of a row at place (column / 4, row ^ column / 4).
       if (!writer && !joined) continue;                    // (a stream without a part, or without rows: the others write)
       float w_own = 1.f, w_other = 0.f;
-      auto staged = [&](int tile, int c4, int r) -> float4* {
-        return reinterpret_cast<float4*>(sQ + tile * TILE + (c4 >> 3) * ATOM + (warp & 3) * 4096 + (((c4 & 7) * 32 + (r ^ (c4 & 7))) << 4));
+      auto staged = [&](int stream, int c4, int r) -> float4* {
+        return reinterpret_cast<float4*>(sQ + stream * TILE + (warp & 3) * 4096 + ((c4 * 32 + (r ^ c4)) << 4));
       };
 #pragma unroll 1
-      for (int half = 0; half < 2 && alive; ++half) {
-        uint32_t v[2][32];
+      for (int c = 0; c < 4 && alive; ++c) {               // 32 columns
+        uint32_t v[32];
         if (my_steps > 0) {
-          tmem_ld_32x32(tO + half * 64, v[0]);
-          tmem_ld_32x32(tO + half * 64 + 32, v[1]);
+          tmem_ld_32x32(tO + c * 32, v);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = 0;
+          for (int i = 0; i < 32; ++i) v[i] = 0;
         }
         auto four = [&](int i) {
-          return make_float4(__uint_as_float(v[i >> 3][4 * (i & 7)]), __uint_as_float(v[i >> 3][4 * (i & 7) + 1]), __uint_as_float(v[i >> 3][4 * (i & 7) + 2]),
-                             __uint_as_float(v[i >> 3][4 * (i & 7) + 3]));
+          return make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
         };
         if (joined && m == 1) {
           if (warp_on) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) *staged(1, i, lane) = four(i);
+            for (int i = 0; i < 8; ++i) *staged(1, i, lane) = four(i);
           }
           s_ml[lr] = m_run;
           s_ml[128 + lr] = l_run;
@@ -885,7 +942,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           alive = warp_wait(j_full, ph_j);
           ph_j ^= 1;
           if (!alive) break;
-          if (half == 0) {
+          if (c == 0) {
             const float m1 = s_ml[lr], l1 = s_ml[128 + lr], mm = fmaxf(m_run, m1);
             w_own = m_run == -INFINITY ? 0.f : exp2f(m_run - mm);
             w_other = m1 == -INFINITY ? 0.f : exp2f(m1 - mm);
@@ -893,82 +950,82 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             m_run = mm;
           }
         }
-        if (half == 0) {
+        if (c == 0) {
           if (p.part_o) {
-            if (row_ok) *reinterpret_cast<float2*>(p.part_ml + ((size_t)it.slot * p.T * p.Hq + at) * 2) = make_float2(m_run, l_run);
+            if (row_ok) *reinterpret_cast<float2*>(p.part_ml + (row0 + at) * 2) = make_float2(m_run, l_run);
           } else {
             const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
             w_own *= inv;
             w_other *= inv;
+            if (gated) {
+              if (joined) load_gate();
+              asm volatile("cp.async.wait_all;" ::: "memory");
+              __syncwarp();
+            }
           }
         }
-        if (warp_on && p.part_o) {
+        if (warp_on) {
+          if (joined || !p.part_o) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float4 o = four(i);
-            if (joined) {
-              const float4 x = *staged(1, i, lane);
-              o.x = o.x * w_own + x.x * w_other;
-              o.y = o.y * w_own + x.y * w_other;
-              o.z = o.z * w_own + x.z * w_other;
-              o.w = o.w * w_own + x.w * w_other;
-            }
-            *staged(m, i, lane) = o;
-          }
-          __syncwarp();
-          if (steps) {
-#pragma unroll 4
-            for (int i = 0; i < (rows_here + 1) / 2; ++i) {                // half a warp per row
-              const int r = 2 * i + (lane >> 4);
-              const size_t prow = row0 + __shfl_sync(0xffffffffu, at, r);
-              if (r < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + half * 64)[lane & 15] = *staged(m, lane & 15, r);
+            for (int i = 0; i < 8; ++i) {
+              float4 o = four(i);
+              o.x *= w_own; o.y *= w_own; o.z *= w_own; o.w *= w_own;
+              if (joined) {
+                const float4 x = *staged(1, i, lane);
+                o.x += x.x * w_other; o.y += x.y * w_other; o.z += x.z * w_other; o.w += x.w * w_other;
+              }
+              v[4 * i] = __float_as_uint(o.x); v[4 * i + 1] = __float_as_uint(o.y); v[4 * i + 2] = __float_as_uint(o.z); v[4 * i + 3] = __float_as_uint(o.w);
             }
           }
-        } else if (warp_on) {
-          if (half == 0 && gated) {
-            if (joined) load_gate();
-            asm volatile("cp.async.wait_all;" ::: "memory");
+          if (p.part_o) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *staged(m, i, lane) = four(i);
             __syncwarp();
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint4* place = reinterpret_cast<uint4*>(own + half * ATOM + lane * 128 + ((i ^ (lane & 7)) << 4));
-            const float4 a = four(2 * i), b = four(2 * i + 1);
-            float o[8] = {a.x * w_own, a.y * w_own, a.z * w_own, a.w * w_own, b.x * w_own, b.y * w_own, b.z * w_own, b.w * w_own};
-            if (joined) {
-              const float4 x = *staged(1, 2 * i, lane), y = *staged(1, 2 * i + 1, lane);
-              o[0] += x.x * w_other; o[1] += x.y * w_other; o[2] += x.z * w_other; o[3] += x.w * w_other;
-              o[4] += y.x * w_other; o[5] += y.y * w_other; o[6] += y.z * w_other; o[7] += y.w * w_other;
-            }
-            if (p.gate) {
-              const uint4 g = *place;
-              const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&g);
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const float2 gf = __bfloat1622float2(gh[x]);
-                o[2 * x] = __fdividef(o[2 * x], 1.f + __expf(-gf.x));
-                o[2 * x + 1] = __fdividef(o[2 * x + 1], 1.f + __expf(-gf.y));
+            if (steps) {
+#pragma unroll 2
+              for (int i = 0; i < (rows_here + 3) / 4; ++i) {              // a quarter warp per row
+                const int r = 4 * i + (lane >> 3);
+                const size_t prow = row0 + __shfl_sync(0xffffffffu, at, r);
+                if (r < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + c * 32)[lane & 7] = *staged(m, lane & 7, r);
               }
             }
-            uint4 u4;
-            __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u4);
+          } else {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) h2[x] = __floats2bfloat162_rn(o[2 * x], o[2 * x + 1]);
-            *place = u4;
-          }
-          if (half) {
-            __syncwarp();
-#pragma unroll 4
-            for (int i = 0; i < (rows_here + 1) / 2; ++i) {
-              const int r = 2 * i + (lane >> 4);
-              const uint4 u4 = *reinterpret_cast<const uint4*>(own + ((lane >> 3) & 1) * ATOM + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-              const size_t to = __shfl_sync(0xffffffffu, at, r);
-              if (r < rows_here) reinterpret_cast<uint4*>(p.out + to * D)[lane & 15] = u4;
+            for (int i = 0; i < 4; ++i) {
+              uint4* place = reinterpret_cast<uint4*>(own + (c >> 1) * ATOM + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4));
+              float o[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) o[x] = __uint_as_float(v[8 * i + x]);
+              if (p.gate) {
+                const uint4 g = *place;
+                const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&g);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float2 gf = __bfloat1622float2(gh[x]);
+                  o[2 * x] = __fdividef(o[2 * x], 1.f + __expf(-gf.x));
+                  o[2 * x + 1] = __fdividef(o[2 * x + 1], 1.f + __expf(-gf.y));
+                }
+              }
+              uint4 u4;
+              __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u4);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) h2[x] = __floats2bfloat162_rn(o[2 * x], o[2 * x + 1]);
+              *place = u4;
             }
           }
         }
         __syncwarp();
         if (joined && lane == 0) mbar_arrive(j_empty);
+      }
+      if (alive && writer && !p.part_o) {
+#pragma unroll 4
+        for (int i = 0; i < (rows_here + 1) / 2; ++i) {    // half a warp per row
+          const int r = 2 * i + (lane >> 4);
+          const uint4 u4 = *reinterpret_cast<const uint4*>(own + ((lane >> 3) & 1) * ATOM + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          const size_t to = __shfl_sync(0xffffffffu, at, r);
+          if (r < rows_here) reinterpret_cast<uint4*>(p.out + to * D)[lane & 15] = u4;
+        }
+        __syncwarp();
       }
       tc_fence_before();
     }
@@ -1066,6 +1123,7 @@ int launch(Params& p, const void* q, const void* k_cache, const void* v_cache, v
   p.block_table = block_table;
   p.kv_len = kv_len;
   p.batch = batch; p.T = T; p.max_blocks = max_blocks; p.bs = block_size;
+  while ((1 << p.bs_log2) < block_size) ++p.bs_log2;
   p.Hq = n_q_heads; p.Hkv = n_kv_heads; p.G = n_q_heads / n_kv_heads;
   const size_t rows = (size_t)T * n_q_heads;
   const bool parts = SHARED || p.splits > 1;

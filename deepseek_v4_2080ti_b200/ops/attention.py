@@ -417,10 +417,14 @@ def _shared_splits(rows: int, groups: int, g: int, hkv: int, tiles: int, own_key
         return 1
     per_group = max(1, rows * g // groups)
     whole, rest = divmod(per_group, ROW_TILE)
-    halves = groups * hkv * (2 * (whole + (rest > ROW_TILE // 2)) + (0 < rest <= ROW_TILE // 2))          # row tiles, in halves of the time
-    work, own_work = halves * tiles * 1.0, rows * hkv * own_keys * (4 * D / 40e3)
-    sms = NUM_SMS if 2 * work >= own_work else max(1.0, NUM_SMS * work / (work + own_work))
-    return max(1, min(64, int(2 * sms / halves), -(-tiles // 2)))
+    full = groups * hkv * (whole + (rest > ROW_TILE // 2))               # row tiles of the two kinds
+    half = groups * hkv * (0 < rest <= ROW_TILE // 2)
+    work, own_work = (2 * full + half) * tiles * 1.0, rows * hkv * own_keys * (4 * D / 40e3)
+    sms = NUM_SMS if 2 * work >= own_work else NUM_SMS * work / (work + own_work)
+    splits = 1
+    while splits < min(64, -(-tiles // 2)) and full * (splits + 1) + half * ((splits + 2) // 2) <= sms:
+        splits += 1
+    return splits
 
 
 def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_len, gate=None, scale=None, cap: float = 0.0,
