@@ -2,9 +2,9 @@
 // plain gamma), half-split RoPE over the first `rot` dims where pair i turns by positions[axis(i)] * inv_freq[i], split of the
 // q||gate projection layout, and the write of K/V rows into the paged cache.
 //
-// Bound by memory: every row is read and written once.  A block takes a few tokens, computes their cosines and sines once for
-// all heads (angles in 64 bits: the product of a far position loses its fraction in 32) and then walks the rows of
-// their heads, a warp per row, lane l dims [4l, 4l + 4).
+// Bound by memory: every row is read and written once.  A block takes a token, computes its cosines and sines once for all
+// heads (angles in 64 bits: the product of a far position loses its fraction in 32) and then walks the rows of its heads,
+// a warp per row, lane l dims [4l, 4l + 4), several rows of a warp on their way at a time.
 //
 // Reference behaviour: src/models/qwen4_exp/layers.py:288-326 (interleaved axes); norm, gate split and append as in rope_kv.cu.
 #include <cuda_bf16.h>
@@ -16,7 +16,6 @@ namespace {
 
 constexpr int D = 128;
 constexpr int WARPS = 8;
-constexpr int MAX_TOKENS = 4;        // of a block
 
 struct AxesParams {
   const __nv_bfloat16* q_src; int ldq, q_off, q_head_stride, gate_in_q;      // head h at q_src[t * ldq + q_off + h * q_head_stride]
@@ -30,7 +29,7 @@ struct AxesParams {
   __nv_bfloat16* q_out; __nv_bfloat16* gate_out;                             // [T, Hq, 128]
   __nv_bfloat16* k_cache; __nv_bfloat16* v_cache; int bs; unsigned n_slots;  // [nb, Hkv, bs, 128]
   int T, Hq, Hkv;
-  int block_tokens, block_rows;                                              // of a block: tokens, rows of each (grid.y blocks share a token's)
+  int block_rows;                                                            // of a block (grid.y blocks share a token's)
   unsigned char axis[D / 2];                                                 // of every pair
 };
 
@@ -47,71 +46,93 @@ __device__ __forceinline__ uint2 pack4(const float (&f)[4]) {
   return u;
 }
 
+// U: rows of a warp that are on their way from memory together.
+template <int U>
 __global__ void __launch_bounds__(WARPS * 32)
 qk_norm_rope_axes_append_kernel(const __grid_constant__ AxesParams p) {
-  __shared__ float s_cos[MAX_TOKENS][D / 2], s_sin[MAX_TOKENS][D / 2];
+  __shared__ __align__(16) float s_cos[D / 2], s_sin[D / 2];
   b200::pdl_grid_trigger();
   b200::pdl_grid_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = blockIdx.x * p.block_tokens, n_tok = min(p.block_tokens, p.T - t0);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x;
   const int half = p.rot >> 1, heads = p.Hq + 2 * p.Hkv;
-  for (int i = threadIdx.x; i < n_tok * half; i += WARPS * 32) {
-    const int t = i / half, f = i - t * half;
-    double a = (double)p.positions[(size_t)p.axis[f] * p.ld_pos + t0 + t] * (double)p.inv_freq[f];
+  const int r0 = blockIdx.y * p.block_rows, r1 = min(heads, r0 + p.block_rows);
+  auto source = [&](int hh) {
+    return hh < p.Hq           ? p.q_src + (size_t)t * p.ldq + p.q_off + (size_t)hh * p.q_head_stride
+           : hh < p.Hq + p.Hkv ? p.k_src + (size_t)t * p.ldk + p.k_off + (hh - p.Hq) * D
+                               : p.v_src + (size_t)t * p.ldv + p.v_off + (hh - p.Hq - p.Hkv) * D;
+  };
+  uint2 u[U], gate[U];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int hh = first + j * WARPS;
+      if (hh < r1) {
+        const __nv_bfloat16* src = source(hh) + lane * 4;
+        u[j] = *reinterpret_cast<const uint2*>(src);
+        if (p.gate_in_q && hh < p.Hq) gate[j] = *reinterpret_cast<const uint2*>(src + D);
+      }
+    }
+  };
+  load(r0 + warp);                                          // on their way while the angles are computed
+  const int slot = p.slots[t];
+  uint2 gq = make_uint2(0, 0), gk = make_uint2(0, 0);
+  if (p.q_gamma) gq = *reinterpret_cast<const uint2*>(p.q_gamma + lane * 4);
+  if (p.k_gamma) gk = *reinterpret_cast<const uint2*>(p.k_gamma + lane * 4);
+  if (threadIdx.x < half) {
+    const int f = threadIdx.x;
+    double a = (double)p.positions[(size_t)p.axis[f] * p.ld_pos + t] * (double)p.inv_freq[f];
     a -= 6.283185307179586 * rint(a * 0.15915494309189535);
     float sn, cs;
     __sincosf((float)a, &sn, &cs);
-    s_cos[t][f] = cs * p.mscale;
-    s_sin[t][f] = sn * p.mscale;
+    s_cos[f] = cs * p.mscale;
+    s_sin[f] = sn * p.mscale;
   }
   __syncthreads();
-  const int r0 = blockIdx.y * p.block_rows, rows = min(p.block_rows, heads - r0);
-  for (int i = warp; i < n_tok * rows; i += WARPS) {
-    const int tt = i / rows, hh = r0 + i - tt * rows, t = t0 + tt;
-    const bool is_q = hh < p.Hq, is_k = !is_q && hh < p.Hq + p.Hkv;
-    const int h = is_q ? hh : is_k ? hh - p.Hq : hh - p.Hq - p.Hkv;
-    const __nv_bfloat16* src = is_q   ? p.q_src + (size_t)t * p.ldq + p.q_off + (size_t)h * p.q_head_stride
-                               : is_k ? p.k_src + (size_t)t * p.ldk + p.k_off + h * D
-                                      : p.v_src + (size_t)t * p.ldv + p.v_off + h * D;
-    uint2 u = *reinterpret_cast<const uint2*>(src + lane * 4);
-    if (is_q && p.gate_in_q)
-      *reinterpret_cast<uint2*>(p.gate_out + ((size_t)t * p.Hq + h) * D + lane * 4) = *reinterpret_cast<const uint2*>(src + D + lane * 4);
-    if (is_q || is_k) {
-      float x[4];
-      unpack4(u, x);
-      const __nv_bfloat16* gamma = is_q ? p.q_gamma : p.k_gamma;
-      if (gamma) {
-        float ss = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
+  // a lane's four dims: the first or the second of their pairs, or none of a pair
+  const int d0 = lane * 4;
+  const bool low = d0 < half, turns = d0 < p.rot;
+  const int f = turns ? (low ? d0 : d0 - half) : 0, partner = low ? lane + (half >> 2) : lane - (half >> 2);
+  const float4 cs = *reinterpret_cast<const float4*>(s_cos + f), sn = *reinterpret_cast<const float4*>(s_sin + f);
+  const float c4[4] = {turns ? cs.x : 1.f, turns ? cs.y : 1.f, turns ? cs.z : 1.f, turns ? cs.w : 1.f};
+  const float s4[4] = {turns ? (low ? -sn.x : sn.x) : 0.f, turns ? (low ? -sn.y : sn.y) : 0.f, turns ? (low ? -sn.z : sn.z) : 0.f,
+                       turns ? (low ? -sn.w : sn.w) : 0.f};
+  const size_t slot_row = (unsigned)slot < p.n_slots ? ((size_t)(slot / p.bs) * p.Hkv * p.bs + slot % p.bs) * D + d0 : ~(size_t)0;
+  for (int first = r0 + warp; first < r1; first += WARPS * U) {
+    if (first != r0 + warp) load(first);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rsqrtf(ss * (1.f / D) + p.eps);
-        float g[4];
-        unpack4(*reinterpret_cast<const uint2*>(gamma + lane * 4), g);
+    for (int j = 0; j < U; ++j) {
+      const int hh = first + j * WARPS;
+      if (hh >= r1) break;
+      const bool is_q = hh < p.Hq, is_k = !is_q && hh < p.Hq + p.Hkv;
+      if (is_q || is_k) {
+        float x[4];
+        unpack4(u[j], x);
+        if (is_q ? p.q_gamma != nullptr : p.k_gamma != nullptr) {
+          float ss = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = x[k] * inv * (p.unit_offset ? 1.f + g[k] : g[k]);
-      }
-      // partner of dim d < half: d + half, (half / 4) lanes on
-      const int d0 = lane * 4;
-      const bool low = d0 < half;
-      float y[4];
+          for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float inv = rsqrtf(ss * (1.f / D) + p.eps);
+          float g[4];
+          unpack4(is_q ? gq : gk, g);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) y[k] = __shfl_sync(0xffffffffu, x[k], low ? lane + (half >> 2) : lane - (half >> 2));
-      if (d0 < p.rot) {
-        const int f = low ? d0 : d0 - half;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float cs = s_cos[tt][f + k], sn = s_sin[tt][f + k];
-          x[k] = low ? x[k] * cs - y[k] * sn : x[k] * cs + y[k] * sn;
+          for (int k = 0; k < 4; ++k) x[k] = x[k] * inv * (p.unit_offset ? 1.f + g[k] : g[k]);
         }
+        // partner of dim d < half: d + half, (half / 4) lanes on
+        float y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = __shfl_sync(0xffffffffu, x[k], partner);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = turns ? x[k] * c4[k] + y[k] * s4[k] : x[k];
+        u[j] = pack4(x);
       }
-      u = pack4(x);
-    }
-    if (is_q) {
-      *reinterpret_cast<uint2*>(p.q_out + ((size_t)t * p.Hq + h) * D + lane * 4) = u;
-    } else {
-      const int slot = p.slots[t];
-      if ((unsigned)slot < p.n_slots)
-        *reinterpret_cast<uint2*>((is_k ? p.k_cache : p.v_cache) + (((size_t)(slot / p.bs) * p.Hkv + h) * p.bs + slot % p.bs) * D + lane * 4) = u;
+      if (is_q) {
+        const size_t at = ((size_t)t * p.Hq + hh) * D + d0;
+        *reinterpret_cast<uint2*>(p.q_out + at) = u[j];
+        if (p.gate_in_q) *reinterpret_cast<uint2*>(p.gate_out + at) = gate[j];
+      } else if (slot_row != ~(size_t)0) {
+        const int h = hh - p.Hq - (is_k ? 0 : p.Hkv);
+        *reinterpret_cast<uint2*>((is_k ? p.k_cache : p.v_cache) + slot_row + (size_t)h * p.bs * D) = u[j];
+      }
     }
   }
 }
@@ -151,8 +172,10 @@ extern "C" int b200_qk_norm_rope_axes_append(
   p.bs = block_size; p.n_slots = (unsigned)num_blocks * block_size;
   p.T = T; p.Hq = Hq; p.Hkv = Hkv;
   const int heads = Hq + 2 * Hkv;
-  p.block_tokens = 1;
-  p.block_rows = heads;
-  const unsigned gy = (heads + p.block_rows - 1) / p.block_rows;
-  return (int)b200::launch_pdl(qk_norm_rope_axes_append_kernel, dim3((T + p.block_tokens - 1) / p.block_tokens, gy), dim3(WARPS * 32), 0, stream, p);
+  // few tokens: a row per warp, so that the SMs share a token's heads
+  const bool few = (long long)T * heads <= 148 * 2 * WARPS;
+  p.block_rows = few ? WARPS : heads;
+  const dim3 grid(T, (heads + p.block_rows - 1) / p.block_rows), block(WARPS * 32);
+  return (int)(few ? b200::launch_pdl(qk_norm_rope_axes_append_kernel<1>, grid, block, 0, stream, p)
+                   : b200::launch_pdl(qk_norm_rope_axes_append_kernel<4>, grid, block, 0, stream, p));
 }
