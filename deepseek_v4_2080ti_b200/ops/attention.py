@@ -4,8 +4,8 @@ append, tcgen05 flash prefill, split-context decode.  Cache layout:
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 import math
 
 import torch
@@ -199,6 +199,7 @@ def decode_kv8(fmt: int, q, k8, v8, k_scale, v_scale, block_table, kv_len, gate=
 
 # ---------------------------------------------------------------- several rotary axes, spans of keys, shared pages
 NUM_SMS = 148
+SCALE = 1.0 / math.sqrt(D)
 ROW_TILE, KEY_TILE = 256, 128            # (token, head) rows and keys of a tile in attn_spans.cu
 
 
@@ -207,42 +208,52 @@ def _need(ok, what: str) -> None:
         raise ValueError(what)
 
 
+_I32, _BF16, _F32 = torch.int32, torch.bfloat16, torch.float32
+
+
 def _index(t, shape, dev: int, what: str) -> None:
-    if t.dtype != torch.int32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+    if t.dtype is not _I32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{what}: contiguous int32 {list(shape)} on cuda:{dev} expected, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
-def _like(t, q, dev: int, what: str) -> None:
-    if t.dtype != torch.bfloat16 or t.shape != q.shape or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError(f"{what}: contiguous bf16 {list(q.shape)} on cuda:{dev} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+def _like(t, shape, dev: int, what: str) -> None:
+    if t.dtype is not _BF16 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous bf16 {list(shape)} on cuda:{dev} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _caches(k_cache, v_cache, dev: int):
+    """Shape of a pair of caches."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[3] != D or k_cache.dtype is not _BF16 or k_cache.get_device() != dev or not k_cache.is_contiguous():
+        raise ValueError("caches: contiguous bf16 [pages, kv heads, page size, 128] on the device of the rows expected")
+    _like(v_cache, shape, dev, "v_cache")
+    return shape
 
 
 def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
     """Checks what the calls over spans have in common; (device, rows, Hq, pages, Hkv, page size, sequences, table width, scale, out)."""
-    dev = q.get_device()
-    if dev < 0 or q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != D or not q.is_contiguous():
-        raise ValueError(f"q: contiguous bf16 [T, Hq, 128] on a GPU expected, got {q.dtype} {list(q.shape)} on {q.device}")
-    t, hq, _ = q.shape
-    if k_cache.dim() != 4 or k_cache.dtype != torch.bfloat16 or k_cache.shape[3] != D or k_cache.get_device() != dev or not k_cache.is_contiguous():
-        raise ValueError("caches: contiguous bf16 [pages, kv heads, page size, 128] on the device of q expected")
-    _like(v_cache, k_cache, dev, "v_cache")
-    nb, hkv, bs, _ = k_cache.shape
+    dev, rows = q.get_device(), q.shape
+    if dev < 0 or len(rows) != 3 or rows[2] != D or q.dtype is not _BF16 or not q.is_contiguous():
+        raise ValueError(f"q: contiguous bf16 [T, Hq, 128] on a GPU expected, got {q.dtype} {list(rows)} on {q.device}")
+    t, hq, _ = rows
+    nb, hkv, bs, _ = _caches(k_cache, v_cache, dev)
     if nb < 1 or hkv < 1 or hq < 1 or hq % hkv:
         raise ValueError(f"{hq} query heads over {hkv} key/value heads in {nb} pages")
     if bs not in (16, 32, 64, 128, 256):
         raise ValueError(f"page size {bs}: 16, 32, 64, 128 or 256 expected")
-    if block_table.dim() != 2 or block_table.shape[1] < 1:
+    table = block_table.shape
+    if len(table) != 2 or table[1] < 1:
         raise ValueError("block_table: int32 [sequences, pages] expected")
-    b, width = block_table.shape
-    _index(block_table, (b, width), dev, "block_table")
+    b, width = table
+    _index(block_table, table, dev, "block_table")
     _index(kv_len, (b,), dev, "kv_len")
     if gate is not None:
-        _like(gate, q, dev, "gate")
+        _like(gate, rows, dev, "gate")
     if out is None:
         out = torch.empty_like(q)
     else:
-        _like(out, q, dev, "out")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+        _like(out, rows, dev, "out")
+    scale = SCALE if scale is None else float(scale)
     if not 0.0 < scale < math.inf or not 0.0 <= cap < math.inf:
         raise ValueError(f"scale {scale}, cap {cap}: a positive scale and a cap that is positive, or 0 for none, expected")
     return dev, t, hq, nb, hkv, bs, b, width, scale, out
@@ -266,19 +277,28 @@ def _kernels() -> ctypes.CDLL:
     return lib
 
 
+def _rows(x, t: int, dev: int, what: str) -> int:
+    """Checks a tensor of rows; their distance."""
+    shape, (ld, one) = x.shape, x.stride() if x.dim() == 2 else (0, 0)
+    if one != 1 or shape[0] != t or ld % 4 or x.dtype is not _BF16 or x.get_device() != dev or x.data_ptr() % 8:
+        raise ValueError(f"{what}: bf16 rows [{t}, ..] on cuda:{dev}, 8-byte aligned, expected; got {x.dtype} {list(shape)} on {x.device}")
+    return ld
+
+
 def _at(t):
     return None if t is None else t.data_ptr()
 
 
-def _on(dev: int):
-    """Makes ``dev`` the current device for a launch, where it is not."""
-    return contextlib.nullcontext() if torch._C._cuda_getDevice() == dev else torch.cuda.device(dev)
+_current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def rotary_axes(sections, interleaved: bool = False) -> tuple[int, ...]:
-    """Axis of every rotary pair from the number of pairs of each axis: one block per axis, or - ``interleaved`` - the axes in
-    turn (T H W T H W ..), where pairs that no other axis claims stay on the first."""
-    sections = [int(n) for n in sections]
+def _status(dev: int) -> int:
+    t = _lib._status.get(dev)
+    return (_lib.status_word(dev) if t is None else t).data_ptr()
+
+
+@functools.lru_cache(maxsize=64)
+def _pair_axes(sections: tuple, interleaved: bool) -> tuple[int, ...]:
     _need(sections and min(sections) >= 0 and 0 < sum(sections) <= D // 2, f"sections {sections}: 1 to {D // 2} pairs in all expected")
     if not interleaved:
         return tuple(a for a, n in enumerate(sections) for _ in range(n))
@@ -289,6 +309,12 @@ def rotary_axes(sections, interleaved: bool = False) -> tuple[int, ...]:
     return tuple(axes)
 
 
+def rotary_axes(sections, interleaved: bool = False) -> tuple[int, ...]:
+    """Axis of every rotary pair from the number of pairs of each axis: one block per axis, or - ``interleaved`` - the axes in
+    turn (T H W T H W ..), where pairs that no other axis claims stay on the first."""
+    return _pair_axes(tuple(int(n) for n in sections), bool(interleaved))
+
+
 def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_off, v_src, v_off, q_gamma, k_gamma,
                              unit_offset, eps, inv_freq, axes, positions, slots, k_cache, v_cache, n_q_heads, n_kv_heads,
                              mscale: float = 1.0):
@@ -297,39 +323,44 @@ def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_of
     ``axes`` from ``rotary_axes`` (a multiple of 4 pairs); ``positions`` int32 [axes, T]; ``slots`` int32 [T], distinct; rows
     with a negative slot are not cached.  Returns (q [T, Hq, 128], gate [T, Hq, 128] or None).
     """
-    dev, t = q_src.get_device(), q_src.shape[0]
-    for x, off, last, what in ((q_src, q_off, q_off + (n_q_heads - 1) * q_head_stride + (2 * D if gate_in_q else D), "q_src"),
-                               (k_src, k_off, k_off + n_kv_heads * D, "k_src"), (v_src, v_off, v_off + n_kv_heads * D, "v_src")):
-        if (dev < 0 or x.get_device() != dev or x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[0] != t or x.stride(1) != 1 or last > x.shape[1] or
-                off < 0 or off % 4 or x.stride(0) % 4 or x.data_ptr() % 8):
-            raise ValueError(f"{what}: bf16 rows [{t}, >= {last}] on a GPU, 8-byte aligned, expected; got {x.dtype} {list(x.shape)} on {x.device} from {off}")
-    if q_head_stride < 0 or q_head_stride % 4 or n_q_heads < 1 or n_kv_heads < 1:
-        raise ValueError(f"{n_q_heads} / {n_kv_heads} heads, {q_head_stride} columns apart")
-    if (k_cache.dim() != 4 or k_cache.dtype != torch.bfloat16 or k_cache.shape[1] != n_kv_heads or k_cache.shape[3] != D or
-            k_cache.get_device() != dev or not k_cache.is_contiguous()):
-        raise ValueError("caches: contiguous bf16 [pages, kv heads, page size, 128] on the device of the rows expected")
-    _like(v_cache, k_cache, dev, "v_cache")
+    dev = q_src.get_device()
+    if dev < 0:
+        raise ValueError(f"q_src: rows on a GPU expected, got {q_src.device}")
+    if _current() != dev:
+        with torch.cuda.device(dev):
+            return qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_off, v_src, v_off, q_gamma, k_gamma, unit_offset, eps,
+                                            inv_freq, axes, positions, slots, k_cache, v_cache, n_q_heads, n_kv_heads, mscale)
+    t = q_src.shape[0]
+    ldq = _rows(q_src, t, dev, "q_src")
+    ldk = ldq if k_src is q_src else _rows(k_src, t, dev, "k_src")
+    ldv = ldq if v_src is q_src else _rows(v_src, t, dev, "v_src")
+    kv = n_kv_heads * D
+    if (q_off % 4 or k_off % 4 or v_off % 4 or q_head_stride % 4 or min(q_off, k_off, v_off, q_head_stride) < 0 or n_q_heads < 1 or n_kv_heads < 1 or
+            q_off + (n_q_heads - 1) * q_head_stride + (2 * D if gate_in_q else D) > q_src.shape[1] or k_off + kv > k_src.shape[1] or
+            v_off + kv > v_src.shape[1]):
+        raise ValueError(f"{n_q_heads} / {n_kv_heads} heads from columns {q_off} (every {q_head_stride}), {k_off}, {v_off}: multiples of 4 inside the rows expected")
+    nb, hkv, bs, _ = _caches(k_cache, v_cache, dev)
+    if hkv != n_kv_heads:
+        raise ValueError(f"caches of {hkv} heads, {n_kv_heads} in the rows")
     for g in (q_gamma, k_gamma):
-        if g is not None and (g.dtype != torch.bfloat16 or g.numel() != D or not g.is_contiguous() or g.get_device() != dev):
+        if g is not None and (g.dtype is not _BF16 or g.numel() != D or not g.is_contiguous() or g.get_device() != dev):
             raise ValueError("gammas: bf16 [128] on the device of the rows expected")
-    n = len(axes)
-    if n % 4 or not 0 < n <= D // 2 or min(axes) < 0 or positions.dim() != 2 or positions.shape[0] <= max(axes):
+    table, n, n_axes = bytes(axes), len(axes), positions.shape[0]
+    if n % 4 or not 0 < n <= D // 2 or n_axes <= max(table):
         raise ValueError(f"axes: 4, 8 .. {D // 2} pairs, each with a row of positions, expected")
-    if inv_freq.dtype != torch.float32 or inv_freq.numel() != n or not inv_freq.is_contiguous() or inv_freq.get_device() != dev:
+    if inv_freq.dtype is not _F32 or inv_freq.numel() != n or not inv_freq.is_contiguous() or inv_freq.get_device() != dev:
         raise ValueError("inv_freq: fp32, one per pair, on the device of the rows expected")
-    _index(positions, (positions.shape[0], t), dev, "positions")
+    _index(positions, (n_axes, t), dev, "positions")
     _index(slots, (t,), dev, "slots")
-    q_out = torch.empty((t, n_q_heads, D), dtype=torch.bfloat16, device=q_src.device)
+    q_out = q_src.new_empty(t, n_q_heads, D)
     gate_out = torch.empty_like(q_out) if gate_in_q else None
     if t == 0:
         return q_out, gate_out
-    with _on(dev):
-        _lib.check_indices(slots, 0, k_cache.shape[0] * k_cache.shape[2], 2, keep=-1)
-        rc = _kernels().b200_qk_norm_rope_axes_append(
-            q_src.data_ptr(), q_src.stride(0), q_off, q_head_stride, gate_in_q, k_src.data_ptr(), k_src.stride(0), k_off, v_src.data_ptr(),
-            v_src.stride(0), v_off, _at(q_gamma), _at(k_gamma), unit_offset, eps, inv_freq.data_ptr(), 2 * n, mscale, bytes(axes),
-            positions.shape[0], positions.data_ptr(), t, slots.data_ptr(), q_out.data_ptr(), _at(gate_out), k_cache.data_ptr(),
-            v_cache.data_ptr(), k_cache.shape[0], k_cache.shape[2], t, n_q_heads, n_kv_heads, torch._C._cuda_getCurrentRawStream(dev))
+    _lib.check_indices(slots, 0, nb * bs, 2, keep=-1)
+    rc = _kernels().b200_qk_norm_rope_axes_append(
+        q_src.data_ptr(), ldq, q_off, q_head_stride, gate_in_q, k_src.data_ptr(), ldk, k_off, v_src.data_ptr(), ldv, v_off, _at(q_gamma), _at(k_gamma),
+        unit_offset, eps, inv_freq.data_ptr(), 2 * n, mscale, table, n_axes, positions.data_ptr(), t, slots.data_ptr(), q_out.data_ptr(),
+        _at(gate_out), k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, t, n_q_heads, n_kv_heads, _stream(dev))
     _lib.check(rc, "qk_norm_rope_axes_append")
     return q_out, gate_out
 
@@ -364,6 +395,9 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
     sequence are not written (``out``: where to write).  ``max_kv_len`` bounds the contexts, for the choice of ``splits``.
     """
     dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
+    if _current() != dev:
+        with torch.cuda.device(dev):
+            return prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_q_len, lo, hi, gate, scale, cap, max_kv_len, splits, out)
     _index(q_start, (b,), dev, "q_start")
     _index(q_len, (b,), dev, "q_len")
     if lo is not None:
@@ -380,13 +414,11 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
         splits = max(1, min(NUM_SMS // tiles, keys // 2))
     if not 1 <= splits <= 1024:
         raise ValueError(f"{splits} splits")
-    with _on(dev):
-        ws = torch.empty(splits * t * hq * (D + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-        _lib.check_indices(block_table, 0, nb, 3)
-        rc = _kernels().b200_attn_spans(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), q_start.data_ptr(),
-            q_len.data_ptr(), kv_len.data_ptr(), _at(lo), _at(hi), b, max_q_len, t, width, nb, bs, hq, hkv, scale, cap, splits, _at(ws),
-            _lib.status_word(q.device).data_ptr(), torch._C._cuda_getCurrentRawStream(dev))
+    ws = q.new_empty(splits * t * hq * (D + 2), dtype=_F32) if splits > 1 else None
+    _lib.check_indices(block_table, 0, nb, 3)
+    rc = _kernels().b200_attn_spans(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
+        kv_len.data_ptr(), _at(lo), _at(hi), b, max_q_len, t, width, nb, bs, hq, hkv, scale, cap, splits, _at(ws), _status(dev), _stream(dev))
     _lib.check(rc, "prefill_spans", 2 if splits > 1 else 1)
     return out
 
@@ -421,10 +453,10 @@ def _shared_splits(rows: int, groups: int, g: int, hkv: int, tiles: int, own_key
     half = groups * hkv * (0 < rest <= ROW_TILE // 2)
     work, own_work = (2 * full + half) * tiles * 1.0, rows * hkv * own_keys * (4 * D / 40e3)
     sms = NUM_SMS if 2 * work >= own_work else NUM_SMS * work / (work + own_work)
-    splits = 1
-    while splits < min(64, -(-tiles // 2)) and full * (splits + 1) + half * ((splits + 2) // 2) <= sms:
-        splits += 1
-    return splits
+    splits = int(sms / (full + half / 2))
+    if full * splits + half * ((splits + 1) // 2) > sms:
+        splits -= 1
+    return max(1, min(64, splits, -(-tiles // 2)))
 
 
 def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_len, gate=None, scale=None, cap: float = 0.0,
@@ -437,6 +469,9 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     in common (keys at ``kv_len`` and beyond stay unseen); rows of no group are on their own.  ``cap`` as in ``prefill_spans``;
     ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys)."""
     dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
+    if _current() != dev:
+        with torch.cuda.device(dev):
+            return decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_len, gate, scale, cap, max_shared, max_kv_len, splits, out)
     if b != t or shared_len.dim() != 1:
         raise ValueError(f"{t} rows for {b} sequences, shared lengths {list(shared_len.shape)}: a row per sequence and a length per group expected")
     n = shared_len.shape[0]
@@ -457,18 +492,16 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     blocks, cluster = b * hkv * -(-g // 16), 1
     while cluster < 8 and cluster * blocks <= NUM_SMS and own_keys > 256 * cluster:
         cluster *= 2
-    with _on(dev):
-        lib, stream = _kernels(), torch._C._cuda_getCurrentRawStream(dev)
-        _lib.check_indices(block_table, 0, nb, 3)
-        ws = torch.empty(splits * b * hq * (D + 2), dtype=torch.float32, device=q.device) if n else None
-        if n:
-            rc = lib.b200_attn_shared(
-                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(), group_start.data_ptr(),
-                shared_len.data_ptr(), n, b, width, nb, bs, hq, hkv, scale, cap, splits, ws.data_ptr(), _lib.status_word(q.device).data_ptr(), stream)
-            _lib.check(rc, "decode_shared")
-        rc = lib.b200_attn_own_rows(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
-            group_start.data_ptr(), shared_len.data_ptr(), n, b, width, nb, bs, hq, hkv, scale, cap, splits if n else 0, _at(ws), cluster, stream)
+    lib, stream = _kernels(), _stream(dev)
+    _lib.check_indices(block_table, 0, nb, 3)
+    pq, pk, pv, pt, pl, pg, ps = (x.data_ptr() for x in (q, k_cache, v_cache, block_table, kv_len, group_start, shared_len))
+    ws = None
+    if n:
+        ws = q.new_empty(splits * b * hq * (D + 2), dtype=_F32)
+        rc = lib.b200_attn_shared(pq, pk, pv, pt, pl, pg, ps, n, b, width, nb, bs, hq, hkv, scale, cap, splits, ws.data_ptr(), _status(dev), stream)
+        _lib.check(rc, "decode_shared")
+    rc = lib.b200_attn_own_rows(pq, pk, pv, out.data_ptr(), _at(gate), pt, pl, pg, ps, n, b, width, nb, bs, hq, hkv, scale, cap, splits if n else 0,
+                                _at(ws), cluster, stream)
     _lib.check(rc, "decode_shared")
     return out
 
