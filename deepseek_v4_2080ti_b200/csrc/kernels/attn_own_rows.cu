@@ -15,7 +15,6 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 #include "launch.h"
-#include "per_device.h"
 #include "ops.h"
 
 namespace {
@@ -112,7 +111,7 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
   const int first = shared >> 4, n_blk = max(0, ((kv + 15) >> 4) - first);               // blocks of 16 keys
   const int* bt = p.block_table + (size_t)b * p.max_blocks;
 
-  // The queries stay in shared memory (rows of 320 bytes: free of bank conflicts for the reads below), so that four blocks fit an SM.
+  // The queries stay in shared memory (rows of 320 bytes: free of bank conflicts for the reads below): registers hold loads on their way.
   for (int i = threadIdx.x; i < H * 16; i += WARPS * 32) {
     const int h = i >> 4, d = i & 15;
     s_q[h][d] = h < heads ? reinterpret_cast<const uint4*>(p.q + ((size_t)b * p.Hq + kvh * p.G + h0 + h) * D)[d] : make_uint4(0, 0, 0, 0);
@@ -355,14 +354,6 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
 
 template <int NB>
 cudaError_t launch(const OwnParams& p, cudaStream_t stream) {
-  static b200::PerDeviceOnce once_;
-  bool& configured = once_.slot();
-  if (!configured) {
-    // the split of the SMs' memory that the kernel over the shared keys has: another one would wait for every block of that kernel to leave
-    const cudaError_t e = cudaFuncSetAttribute(own_rows_kernel<NB>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hkv * p.chunks * p.cluster));
   cfg.blockDim = dim3(WARPS * 32);

@@ -9,19 +9,28 @@
 //
 // Work is a list of items that as many CTAs as there are SMs walk in turn: 256 rows (token, head of one kv head) - all query
 // heads of a kv head are packed into the rows, so a tile is full however few tokens there are - times a range of key tiles of
-// 128.  A row's result comes from one item, or from several whose partial sums the second kernel joins.
+// 128.  A row's result comes from one item, or from several whose partial sums (fp32) the second kernel here, or the one over
+// the sequences' own keys, joins.
 //
 // Two streams of 128 rows keep the tensor core and the exponential units busy in turn.  An item of at most 128 rows gives both
 // streams the same rows and every other key tile, and joins them at its end.  Warp roles:
-//   warps 0-3, 4-7: softmax of stream 0 and 1 - one row per thread, online maximum / sum in the exp2 domain, P as bf16 back
-//             into the tensor memory its scores came from, lazy rescale of the stream's O (when a maximum grows by 2^8);
-//   warp 8  : TMA producer - key and value tiles gathered page by page through the block table into one ring, running ahead
-//             into the next item;
+//   warps 0-3, 4-7: softmax of stream 0 and 1 - one row per thread, online maximum / sum in the exp2 domain (fp32), P rounded to
+//             bf16 for the product (relative 2^-9 a weight; the sum adds the weights before they are rounded) into the tensor
+//             memory its scores came from, lazy rescale of the stream's O (when a maximum grows by 2^8); then the item's rows;
+//   warp 8  : items - which rows and keys are next, up to four ahead of the slowest role - and their loads: key and value tiles
+//             gathered page by page through the block table into one ring (TMA), running ahead into the next item;
 //   warp 9  : tcgen05.mma issuer - step u: P V of step u, scores of step u + 2 (steps alternate between the streams);
-//   warps 10, 11: value check of tiles with masked keys - rows that are not there (behind the last key) or not finite are
-//             set to zero, because 0 x inf in a product would reach rows that do not see them; rows that do see a key
-//             with values that are not finite add it themselves.
+//   warp 10 : value check of tiles with masked keys - rows that are not there (behind the last key) or not finite are set to
+//             zero, because 0 x inf in a product would reach rows that do not see them; rows that do see a key with values that
+//             are not finite add it themselves;
+//   warp 11 : nothing (a warpgroup gives its registers up as a whole).
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each.  All mbarrier waits are bounded and unwind through the common exit.
+//
+// What bounds it (8192 causal rows of 40 heads over 8 kv heads, gated: 619 us, 1.1 PFLOP/s): 256 rows times 128 keys cost 2048
+// cycles of the tensor core and about 2100 of each scheduler's softmax warps, and take 3500 together, because a stream's scores,
+// weights and products follow each other through tensor memory and two streams do not hide all of that; an item's start and end
+// take another 10 %.  Packed documents of 4000 rows, capped: 128 us, of which masked tiles and the items' ends are half.  Shared
+// keys, 64 rows per sequence's head over 32768 keys: 320 rows a kv head, 44 us; 32 over 8192: 15 us.
 #include <cuda_bf16.h>
 #include "per_device.h"
 #include "../ptx/sm100.cuh"
@@ -38,10 +47,7 @@ constexpr int BKV = 128;          // keys per tile
 constexpr int ATOM = 16384;       // bytes of one [128 x 64] bf16 swizzled slab
 constexpr int TILE = 2 * ATOM;
 constexpr int STAGES = 5;
-#ifndef EMU
-#define EMU 2
-#endif
-constexpr int EMULATED = EMU;       // of 8 pairs of exponentials: those on the arithmetic units
+constexpr int EMULATED = 2;       // of 8 pairs of exponentials: those on the arithmetic units (0 / 1 / 2 / 3: 641 / 639 / 624 / 626 us, see below)
 constexpr int ITEMS = 4;          // items the producer may be ahead of the slowest role
 constexpr int NTHREADS = 384;
 constexpr int SMEM_BYTES = 1024 + (2 + STAGES) * TILE + 2048;
@@ -65,7 +71,7 @@ struct Params {
   int n_groups;
   float* part_o;                  // [slots, T, Hq, 128], null: every row has one item
   float* part_ml;                 // [slots, T, Hq, 2]
-  int batch, T, max_blocks, bs, bs_log2, Hq, Hkv, G;
+  int batch, T, max_blocks, num_blocks, bs, bs_log2, Hq, Hkv, G;
   int row_tiles;                  // row tiles per sequence (prompt rows), over all groups (shared keys)
   int splits;                     // key ranges per row tile
   int n_items;
@@ -213,10 +219,10 @@ template <bool SHARED>
 __device__ __forceinline__ void span_of(const Params& p, const Item& it, int tok, int& lo, int& hi) {
   if (SHARED) {
     lo = 0;
-    hi = min(it.own_hi, min(p.kv_len[tok], p.max_blocks * p.bs));
+    hi = max(0, min(it.own_hi, min(p.kv_len[tok], p.max_blocks * p.bs)));
   } else {
     lo = p.lo ? max(0, p.lo[tok]) : 0;
-    hi = min(p.hi ? p.hi[tok] : tok + it.delta + 1, it.kv_end);
+    hi = max(0, min(p.hi ? p.hi[tok] : tok + it.delta + 1, it.kv_end));    // (differences of these fit 32 bits)
   }
 }
 
@@ -469,7 +475,10 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         auto page_row = [&](int tile) {                                    // cache row where this lane's part of a tile begins
           const int key = tile * BKV + (lane << rows_log2);
           const int page = min(key >> p.bs_log2, last_page);
-          return tile < it.t1 && lane < per_tile ? ((bt[page] * p.Hkv + it.kvh) << p.bs_log2) + (key & (p.bs - 1)) : 0;
+          if (tile >= it.t1 || lane >= per_tile) return 0;
+          // a page that is not there (an entry before the first key that is seen, or a bad one) lies behind the cache: it reads as zeros
+          const int id = min((unsigned)bt[page], (unsigned)p.num_blocks);
+          return ((id * p.Hkv + it.kvh) << p.bs_log2) + (key & (p.bs - 1));
         };
         int row = page_row(it.t0);
         for (int t = it.t0; ok && t < it.t1; ++t) {
@@ -1114,7 +1123,7 @@ int launch(Params& p, const void* q, const void* k_cache, const void* v_cache, v
   const bool pow2 = block_size >= 16 && block_size <= 256 && !(block_size & (block_size - 1));
   if (!pow2 || n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads || batch < 1 || T < 1 || max_blocks < 1 || num_blocks < 1 ||
       !(scale > 0.f) || !(cap >= 0.f) || (long long)max_blocks * block_size > 0x7fffff00ll ||
-      (long long)num_blocks * n_kv_heads * block_size > 0x7fffff00ll || ((SHARED || p.splits > 1) && !workspace))
+      ((long long)num_blocks + 1) * n_kv_heads * block_size > 0x7fffff00ll || ((SHARED || p.splits > 1) && !workspace))
     return -ERR_BAD_ARG;
   p.q = reinterpret_cast<const __nv_bfloat16*>(q);
   p.gate = reinterpret_cast<const __nv_bfloat16*>(gate);
@@ -1122,7 +1131,7 @@ int launch(Params& p, const void* q, const void* k_cache, const void* v_cache, v
   p.v_cache = reinterpret_cast<const __nv_bfloat16*>(v_cache);
   p.block_table = block_table;
   p.kv_len = kv_len;
-  p.batch = batch; p.T = T; p.max_blocks = max_blocks; p.bs = block_size;
+  p.batch = batch; p.T = T; p.max_blocks = max_blocks; p.num_blocks = num_blocks; p.bs = block_size;
   while ((1 << p.bs_log2) < block_size) ++p.bs_log2;
   p.Hq = n_q_heads; p.Hkv = n_kv_heads; p.G = n_q_heads / n_kv_heads;
   const size_t rows = (size_t)T * n_q_heads;

@@ -217,15 +217,15 @@ def _index(t, shape, dev: int, what: str) -> None:
 
 
 def _like(t, shape, dev: int, what: str) -> None:
-    if t.dtype is not _BF16 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError(f"{what}: contiguous bf16 {list(shape)} on cuda:{dev} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+    if t.dtype is not _BF16 or t.shape != shape or t.get_device() != dev or not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"{what}: contiguous bf16 {list(shape)} on cuda:{dev}, 16-byte aligned, expected; got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _caches(k_cache, v_cache, dev: int):
     """Shape of a pair of caches."""
     shape = k_cache.shape
-    if len(shape) != 4 or shape[3] != D or k_cache.dtype is not _BF16 or k_cache.get_device() != dev or not k_cache.is_contiguous():
-        raise ValueError("caches: contiguous bf16 [pages, kv heads, page size, 128] on the device of the rows expected")
+    if len(shape) != 4 or shape[3] != D or k_cache.dtype is not _BF16 or k_cache.get_device() != dev or not k_cache.is_contiguous() or k_cache.data_ptr() % 16:
+        raise ValueError("caches: contiguous bf16 [pages, kv heads, page size, 128] on the device of the rows, 16-byte aligned, expected")
     _like(v_cache, shape, dev, "v_cache")
     return shape
 
@@ -233,8 +233,8 @@ def _caches(k_cache, v_cache, dev: int):
 def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
     """Checks what the calls over spans have in common; (device, rows, Hq, pages, Hkv, page size, sequences, table width, scale, out)."""
     dev, rows = q.get_device(), q.shape
-    if dev < 0 or len(rows) != 3 or rows[2] != D or q.dtype is not _BF16 or not q.is_contiguous():
-        raise ValueError(f"q: contiguous bf16 [T, Hq, 128] on a GPU expected, got {q.dtype} {list(rows)} on {q.device}")
+    if dev < 0 or len(rows) != 3 or rows[2] != D or q.dtype is not _BF16 or not q.is_contiguous() or q.data_ptr() % 16:
+        raise ValueError(f"q: contiguous bf16 [T, Hq, 128] on a GPU, 16-byte aligned, expected; got {q.dtype} {list(rows)} on {q.device}")
     t, hq, _ = rows
     nb, hkv, bs, _ = _caches(k_cache, v_cache, dev)
     if nb < 1 or hkv < 1 or hq < 1 or hq % hkv:
@@ -343,8 +343,8 @@ def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_of
     if hkv != n_kv_heads:
         raise ValueError(f"caches of {hkv} heads, {n_kv_heads} in the rows")
     for g in (q_gamma, k_gamma):
-        if g is not None and (g.dtype is not _BF16 or g.numel() != D or not g.is_contiguous() or g.get_device() != dev):
-            raise ValueError("gammas: bf16 [128] on the device of the rows expected")
+        if g is not None and (g.dtype is not _BF16 or g.numel() != D or not g.is_contiguous() or g.get_device() != dev or g.data_ptr() % 8):
+            raise ValueError("gammas: bf16 [128] on the device of the rows, 8-byte aligned, expected")
     table, n, n_axes = bytes(axes), len(axes), positions.shape[0]
     if n % 4 or not 0 < n <= D // 2 or n_axes <= max(table):
         raise ValueError(f"axes: 4, 8 .. {D // 2} pairs, each with a row of positions, expected")
@@ -356,7 +356,7 @@ def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_of
     gate_out = torch.empty_like(q_out) if gate_in_q else None
     if t == 0:
         return q_out, gate_out
-    _lib.check_indices(slots, 0, nb * bs, 2, keep=-1)
+    _lib.check_indices(slots, -2 ** 31, nb * bs, 2)         # (a bad slot becomes a negative one)
     rc = _kernels().b200_qk_norm_rope_axes_append(
         q_src.data_ptr(), ldq, q_off, q_head_stride, gate_in_q, k_src.data_ptr(), ldk, k_off, v_src.data_ptr(), ldv, v_off, _at(q_gamma), _at(k_gamma),
         unit_offset, eps, inv_freq.data_ptr(), 2 * n, mscale, table, n_axes, positions.data_ptr(), t, slots.data_ptr(), q_out.data_ptr(),
@@ -392,7 +392,9 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
     it, whatever the cache holds there.
 
     q: [T, Hq, 128]; block_table [B, max_blocks], q_start / q_len / kv_len [B], lo / hi [T]: int32 device tensors.  Rows of no
-    sequence are not written (``out``: where to write).  ``max_kv_len`` bounds the contexts, for the choice of ``splits``.
+    sequence are not written (``out``: where to write, ``q`` itself if it is not needed any more).  Entries of ``block_table`` for
+    pages that no row sees are not followed.  ``max_q_len`` (host) is at least the longest of ``q_len``; ``max_kv_len`` bounds the
+    contexts, for the choice of ``splits`` (items a row's keys are cut into).
     """
     dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
     if _current() != dev:
@@ -467,7 +469,8 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     q: [B, Hq, 128]; group_start int32 [groups + 1], shared_len int32 [groups] (device; ``shared_groups``): the rows
     group_start[g] .. group_start[g + 1] - 1 of ``block_table`` begin with the same pages, whose first shared_len[g] keys they have
     in common (keys at ``kv_len`` and beyond stay unseen); rows of no group are on their own.  ``cap`` as in ``prefill_spans``;
-    ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys)."""
+    ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys); a sequence with ``kv_len`` 0
+    gives 0."""
     dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
     if _current() != dev:
         with torch.cuda.device(dev):
