@@ -29,7 +29,7 @@
 // What bounds it (8192 causal rows of 40 heads over 8 kv heads, gated: 619 us, 1.1 PFLOP/s): 256 rows times 128 keys cost 2048
 // cycles of the tensor core and about 2100 of each scheduler's softmax warps, and take 3500 together, because a stream's scores,
 // weights and products follow each other through tensor memory and two streams do not hide all of that; an item's start and end
-// take another 10 %.  Packed documents of 4000 rows, capped: 128 us, of which masked tiles and the items' ends are half.  Shared
+// take another 10 %.  Packed documents of 4000 rows, capped: 115 us, of which masked tiles and the items' ends are half.  Shared
 // keys, 64 rows per sequence's head over 32768 keys: 320 rows a kv head, 44 us; 32 over 8192: 15 us.
 #include <cuda_bf16.h>
 #include "per_device.h"
@@ -77,6 +77,8 @@ struct Params {
   int n_items;
   float scale_log2;               // scale * log2(e)
   float cap_in, cap_out;          // scale / cap, cap * log2(e)
+  float cap_small;                // scores to which cap_c reach: half of cap / scale, 0 where the powers of scale / cap leave 32 bits
+  float4 cap_c;                   // tanh(cap_in s) = s (c.x + c.y s^2 + c.z s^4 + c.w s^6)
   int* status;
 };
 
@@ -151,6 +153,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // 2^x of two numbers below 128 on the arithmetic units: 2^round(x) by the exponent bits, 2^f of the rest, |f| <= 1/2, by a cubic with
 // constant term 1 (fitted to the relative error, 1e-4: P is rounded to 2^-9).  From -127 down the result is exactly zero.  Not for NaN.
@@ -170,32 +177,17 @@ __device__ __forceinline__ void exp2_fma(float& a, float& b) {
   b = __int_as_float(__float_as_int(y1) + (__float_as_int(r1) << 23));
 }
 
-// Scores s to tanh(k s) where |k s| <= 1, as it hardly ever is not: z P(z^2) with an interpolation of tanh(z) / z at Chebyshev points, off by
-// 5e-7 at most, on the arithmetic units - two exponential units' steps per score cost as much as both products.
-__device__ __forceinline__ void cap_scores(uint32_t (&sv)[2][32], float k) {
-  constexpr float C[6] = {0.9999994039535522f, -0.3332895040512085f, 0.1328072100877762f, -0.0515859872102737f, 0.0167208556085825f, -0.0030582291074097f};
-  const uint64_t k2 = pack2(k, k);
-#pragma unroll
-  for (int i = 0; i < 64; i += 8) {                          // four chains of two
-    uint64_t z[4], u[4], y[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      z[x] = mul2(pack2(__uint_as_float(sv[i >> 5][(i & 31) + 2 * x]), __uint_as_float(sv[i >> 5][(i & 31) + 2 * x + 1])), k2);
-      u[x] = mul2(z[x], z[x]);
-      y[x] = fma2(u[x], pack2(C[5], C[5]), pack2(C[4], C[4]));
-    }
-#pragma unroll
-    for (int d = 3; d >= 0; --d)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) y[x] = fma2(y[x], u[x], pack2(C[d], C[d]));
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      float a, b;
-      unpack2(mul2(y[x], z[x]), a, b);
-      sv[i >> 5][(i & 31) + 2 * x] = __float_as_uint(a);
-      sv[i >> 5][(i & 31) + 2 * x + 1] = __float_as_uint(b);
-    }
-  }
+// tanh(z) = z P(z^2) on the arithmetic units - two exponential units' steps per score would cost as much as both products -, P an
+// interpolation of tanh(z) / z at Chebyshev points, off by 6e-7 of itself at most: four terms with the powers of k in them where
+// |z| = |k s| <= 1/2, as it is almost always (Params::cap_c; five steps a pair of scores, taken between the exponentials) ..
+// .. and six where |k s| <= 1.
+__device__ __forceinline__ float cap_one(float s, float k) {
+  const float z = s * k, u = z * z;
+  float y = fmaf(u, -0.0030582291074097f, 0.0167208556085825f);
+  y = fmaf(y, u, -0.0515859872102737f);
+  y = fmaf(y, u, 0.1328072100877762f);
+  y = fmaf(y, u, -0.3332895040512085f);
+  return fmaf(y, u, 0.9999994039535522f) * z;
 }
 
 // One piece of work; the same in every thread of a warp.
@@ -681,29 +673,6 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             tmem_ld_32x32(tS + h * 64, sv[0]);
             tmem_ld_32x32(tS + h * 64 + 32, sv[1]);
           };
-          auto cap = [&](int h, uint32_t (&sv)[2][32]) {
-            float big = 0.f;                               // (NaN stays in it)
-#pragma unroll
-            for (int i = 0; i < 64; i += 2)
-              big = max3(big, fabsf(__uint_as_float(sv[i >> 5][i & 31])), fabsf(__uint_as_float(sv[i >> 5][(i & 31) + 1])));
-            if (__all_sync(0xffffffffu, big * p.cap_in <= 1.f)) {
-              cap_scores(sv, p.cap_in);
-            } else {                                       // in place in tensor memory, to keep the code short; NaN stays
-#pragma unroll 1
-              for (int c = 0; c < 4; ++c) {
-                uint32_t v[16];
-                tmem_ld_32x16(tS + h * 64 + c * 16, v);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  v[i] = __float_as_uint(1.f - 2.f * __fdividef(1.f, 1.f + exp2f(__uint_as_float(v[i]) * p.cap_in * 2.885390081777927f)));
-                tmem_st_32x16(tS + h * 64 + c * 16, v);
-              }
-              tmem_st_wait();
-              load(h, sv);
-              tmem_ld_wait();
-            }
-          };
           auto max_of = [&](const uint32_t (&sv)[2][32]) { // independent chains
             float mx[4];
 #pragma unroll
@@ -716,6 +685,46 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             return max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], __uint_as_float(sv[1][28]), __uint_as_float(sv[1][29])),
                         max3(__uint_as_float(sv[1][29]), __uint_as_float(sv[1][30]), __uint_as_float(sv[1][31])));
           };
+          // A cap: tanh(k s) = s (c0 + c1 s^2 + ..) where the half's scores are small; else it is taken in place in tensor memory, to keep
+          // the code short, and the polynomial that follows is s.
+          uint64_t cap_c[4];
+          auto cap = [&](int h, uint32_t (&sv)[2][32], float top) {
+            float mn[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mn[i] = __uint_as_float(sv[0][i]);
+#pragma unroll
+            for (int i = 4; i < 64; i += 2)
+              mn[(i >> 1) & 3] = min3(mn[(i >> 1) & 3], __uint_as_float(sv[i >> 5][i & 31]), __uint_as_float(sv[i >> 5][(i & 31) + 1]));
+            const float low = min3(min3(mn[0], mn[1], mn[2]), mn[3], mn[3]);
+            cap_c[0] = pack2(p.cap_c.x, p.cap_c.x);
+            cap_c[1] = pack2(p.cap_c.y, p.cap_c.y);
+            cap_c[2] = pack2(p.cap_c.z, p.cap_c.z);
+            cap_c[3] = pack2(p.cap_c.w, p.cap_c.w);
+            if (__all_sync(0xffffffffu, top <= p.cap_small && low >= -p.cap_small)) return;        // (NaN: no)
+            const bool below_1 = __all_sync(0xffffffffu, top * p.cap_in <= 1.f && low * p.cap_in >= -1.f);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t v[16];
+              tmem_ld_32x16(tS + h * 64 + c * 16, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float x = __uint_as_float(v[i]);
+                float t = cap_one(x, p.cap_in);            // (the quotient below loses what is small against 1)
+                if (!below_1 && !(fabsf(x * p.cap_in) <= 1.f)) t = 1.f - 2.f * __fdividef(1.f, 1.f + exp2f(x * p.cap_in * 2.885390081777927f));
+                v[i] = __float_as_uint(t);
+              }
+              tmem_st_32x16(tS + h * 64 + c * 16, v);
+            }
+            tmem_st_wait();
+            load(h, sv);
+            tmem_ld_wait();
+            cap_c[0] = pack2(1.f, 1.f);
+            cap_c[1] = cap_c[2] = cap_c[3] = 0;
+          };
+          // What the weights of scores up to `top` are taken relative to.  With a cap k top, limited to 1, stands for tanh(k top): within
+          // a quarter of the cap, and NaN stays.
+          auto level = [&](float top) { return CAP ? scale * min3(max3(top * p.cap_in, -1.f, -1.f), 1.f, 1.f) : scale * top; };
           // The running maximum up to that of new scores, where it is far enough behind; false: the product that last added to O has not
           // finished in time.  The tile before's has, as it was issued before the scores that arrived; `half`: the first half's may be on its way.
           auto raise = [&](float m_tile, bool half) {
@@ -742,8 +751,8 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             m_run = m_next;
             return true;
           };
-          // The weights of half h, as packed pairs over the first half's scores.
-          auto weigh = [&](int h, const uint32_t (&sv)[2][32]) {
+          // The weights of half h, as packed pairs over the first half's scores.  seen: not 0 for the scores that count, if not all do.
+          auto weigh = [&](int h, const uint32_t (&sv)[2][32], auto masked, const uint32_t (&seen)[2]) {
             const float m_use = m_run == -INFINITY ? 0.f : m_run;        // (nothing visible yet: every exponential is zero)
             const uint64_t nm2 = pack2(-m_use, -m_use);
             uint64_t sum2[4] = {0, 0, 0, 0};
@@ -755,12 +764,21 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                   float &x = e[c & 1][2 * i], &y = e[c & 1][2 * i + 1];
-                  unpack2(fma2(pack2(__uint_as_float(sv[c >> 1][(c & 1) * 16 + 2 * i]), __uint_as_float(sv[c >> 1][(c & 1) * 16 + 2 * i + 1])), sc2, nm2), x, y);
+                  uint64_t s2 = pack2(__uint_as_float(sv[c >> 1][(c & 1) * 16 + 2 * i]), __uint_as_float(sv[c >> 1][(c & 1) * 16 + 2 * i + 1]));
+                  if (CAP) {
+                    const uint64_t u = mul2(s2, s2);
+                    s2 = mul2(fma2(fma2(fma2(u, cap_c[3], cap_c[2]), u, cap_c[1]), u, cap_c[0]), s2);
+                  }
+                  unpack2(fma2(s2, sc2, nm2), x, y);
                   if (i >= 8 - (CAP ? 0 : EMULATED)) {
                     exp2_fma(x, y);
                   } else {
                     x = exp2f(x);
                     y = exp2f(y);
+                  }
+                  if (masked.value) {
+                    if (!(seen[c >> 1] & (1u << ((c & 1) * 16 + 2 * i)))) x = 0.f;
+                    if (!(seen[c >> 1] & (2u << ((c & 1) * 16 + 2 * i)))) y = 0.f;
                   }
                 }
               }
@@ -784,21 +802,26 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             // The second half is loaded and its maximum found under the exponentials of the first, and the products with the first half's
             // values begin before the second is done.  Cycles a tile of one warp alone / two warps of a scheduler, without
             // the products: 1977 / 2853 in one piece, 1396 / 2314 in halves, 1197 / 2098 with a quarter of the exponentials
-            // on the arithmetic units.
+            // on the arithmetic units; with a cap and none there: 2448 / 4064 with the polynomial before the weights, 1711 / 2981 with
+            // its steps between their exponentials.
             uint32_t sa[2][32], sb[2][32];
             load(0, sa);
             tmem_ld_wait();
-            load(1, sb);
-            if (CAP) cap(0, sa);
-            if (!(alive = raise(scale * max_of(sa), false))) break;
-            weigh(0, sa);
+            if (!CAP) load(1, sb);                         // (with a cap the registers hold its polynomial instead)
+            const uint32_t all[2] = {};
+            const float top_a = max_of(sa);
+            if (CAP) cap(0, sa, top_a);
+            if (!(alive = raise(level(top_a), false))) break;
+            weigh(0, sa, Int<0>(), all);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_half[m]);
+            if (CAP) load(1, sb);
             tmem_ld_wait();
-            if (CAP) cap(1, sb);
-            if (!(alive = raise(scale * max_of(sb), true))) break;
-            weigh(1, sb);
+            const float top_b = max_of(sb);
+            if (CAP) cap(1, sb, top_b);
+            if (!(alive = raise(level(top_b), true))) break;
+            weigh(1, sb, Int<0>(), all);
           } else {
             // With masked keys the products wait for the check of the values, so that O must not be rescaled between the halves' weights:
             // both halves' maximum comes first (of the scores themselves: a cap keeps their order).  Halves that no row of the warp sees cost
@@ -809,16 +832,22 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
               b = hi - key0 - h * 64;
               return (bool)__any_sync(0xffffffffu, max(a, 0) < min(b, 64));
             };
-            auto mask = [&](int a, int b) {
-              if (__all_sync(0xffffffffu, a <= 0 && b >= 64)) return;
+            uint32_t seen[2];
+            auto bits = [&](int a, int b) {
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 const int x = min(32, max(0, a - c * 32)), y = min(32, max(0, b - c * 32));
-                const uint32_t seen = (uint32_t)((1ull << y) - 1) & ~(uint32_t)((1ull << x) - 1);
+                seen[c] = (uint32_t)((1ull << y) - 1) & ~(uint32_t)((1ull << x) - 1);
+              }
+            };
+            auto mask = [&](int a, int b) {
+              if (__all_sync(0xffffffffu, a <= 0 && b >= 64)) return;
+              bits(a, b);
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                  if (!(seen & (1u << i))) sv[c][i] = 0xff800000u;         // -inf
-              }
+                  if (!(seen[c] & (1u << i))) sv[c][i] = 0xff800000u;      // -inf
             };
             float m_edge = -INFINITY;
 #pragma unroll 1
@@ -831,17 +860,20 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
               const float x = max_of(sv);
               m_edge = max3(m_edge, x, x);
             }
-            if (CAP && m_edge != -INFINITY) m_edge = 1.f - 2.f * __fdividef(1.f, 1.f + exp2f(m_edge * p.cap_in * 2.885390081777927f));
-            raise(m_edge * scale, false);
+            raise(max(lo, key0) < min(hi, key0 + BKV) ? level(m_edge) : -INFINITY, false);
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
               int a, b;
               if (sees(h, a, b)) {
                 load(h, sv);
                 tmem_ld_wait();
-                if (CAP) cap(h, sv);
-                mask(a, b);
-                weigh(h, sv);
+                if (CAP) {                                 // (the weights are masked: a polynomial of -inf is not -inf)
+                  cap(h, sv, max_of(sv));
+                  bits(a, b);
+                } else {
+                  mask(a, b);
+                }
+                weigh(h, sv, Int<CAP>(), seen);
               } else {
                 uint32_t z[32];
 #pragma unroll
@@ -1141,6 +1173,12 @@ int launch(Params& p, const void* q, const void* k_cache, const void* v_cache, v
   p.scale_log2 = scale * 1.4426950408889634f;
   p.cap_in = cap > 0.f ? scale / cap : 0.f;
   p.cap_out = cap * 1.4426950408889634f;
+  if (p.cap_in > 1e-5f && p.cap_in < 1e5f) {
+    const double k = p.cap_in, k3 = k * k * k;
+    p.cap_small = (float)(0.5 / k);
+    p.cap_c = make_float4((float)(0.999999463558197 * k), (float)(-0.3332628309726715 * k3), (float)(0.1318994015455246 * k3 * k * k),
+                          (float)(-0.0443927384912968 * k3 * k3 * k));
+  }
   p.status = status;
   CUtensorMap tmK, tmV;
   const uint64_t kv_rows = (uint64_t)num_blocks * n_kv_heads * block_size;

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_spans_gpu import DEV, NAN, _i32, close, oracle, pages, rand, run_spans
+from test_spans_gpu import DEV, NAN, _i32, causal, close, oracle, pages, rand, run_spans
 
 pytestmark = pytest.mark.gpu
 HQ, HKV, BS = 10, 2, 64
@@ -226,6 +226,21 @@ def test_two_streams_at_once():
     _lib.check_status()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+@pytest.mark.parametrize("cap,q_scale", [(30.0, 1.5), (5.0, 1.5), (2.0, 0.5), (1.0, 3.0), (0.01, 1.0), (1e-6, 1.0), (1e6, 1.0), (1e9, 0.5)])
+def test_scores_on_every_side_of_a_cap(cap, q_scale):
+    """Far below the cap, around half of it, around it, beyond; caps whose powers leave 32 bits.  Whole tiles and masked ones."""
+    run_spans([(150, 700), (20, 20)], 4, 2, 64, causal, cap=cap, q_scale=q_scale, splits=1)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+def test_infinite_scores_under_a_cap(splits):
+    """Keys with an infinity give the cap or its negative, also where a row sees nothing else."""
+    def poke(seqs):
+        seqs[0][0][[0, 5, 64, 300], :, 3] = math.inf
+        seqs[1][0][:, :, 9] = -math.inf
+    run_spans([(400, 400), (30, 200)], 4, 2, 64, causal, cap=4.0, splits=splits, poke=poke)
 
 
 @pytest.mark.parametrize("splits", [1, 3])
