@@ -16,6 +16,7 @@
 #include <stdint.h>
 #include "launch.h"
 #include "ops.h"
+#include "score_cap.cuh"
 
 namespace {
 
@@ -180,10 +181,21 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
     uint32_t pt[NB][2];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
+      if (p.cap_out > 0.f) {
+        const float big = fmaxf(fmaxf(fabsf(s[i][0]), fabsf(s[i][1])), fmaxf(fabsf(s[i][2]), fabsf(s[i][3])));
+        if (__all_sync(0xffffffffu, big * p.cap_in <= 1.f)) {              // (NaN beside others: the polynomial keeps it)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) s[i][y] = p.cap_out * b200::score_cap_small(s[i][y], p.cap_in);
+        } else {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) s[i][y] = p.cap_out * b200::score_cap(s[i][y], p.cap_in);
+        }
+      } else {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) s[i][y] *= p.scale_log2;
+      }
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        if (p.cap_out > 0.f) s[i][y] = p.cap_out * (1.f - 2.f * __fdividef(1.f, 1.f + exp2f(s[i][y] * p.cap_in * 2.885390081777927f)));
-        else s[i][y] *= p.scale_log2;
         if (!((y < 2) ? ok0 : ok1)) s[i][y] = -INFINITY;
       }
       float alpha[2];

@@ -34,6 +34,7 @@
 #include <cuda_bf16.h>
 #include "per_device.h"
 #include "../ptx/sm100.cuh"
+#include "score_cap.cuh"
 #include "tma_host.h"
 #include "launch.h"
 #include "ops.h"
@@ -175,19 +176,6 @@ __device__ __forceinline__ void exp2_fma(float& a, float& b) {
   unpack2(y, y0, y1);
   a = __int_as_float(__float_as_int(y0) + (__float_as_int(r0) << 23));
   b = __int_as_float(__float_as_int(y1) + (__float_as_int(r1) << 23));
-}
-
-// tanh(z) = z P(z^2) on the arithmetic units - two exponential units' steps per score would cost as much as both products -, P an
-// interpolation of tanh(z) / z at Chebyshev points, off by 6e-7 of itself at most: four terms with the powers of k in them where
-// |z| = |k s| <= 1/2, as it is almost always (Params::cap_c; five steps a pair of scores, taken between the exponentials) ..
-// .. and six where |k s| <= 1.
-__device__ __forceinline__ float cap_one(float s, float k) {
-  const float z = s * k, u = z * z;
-  float y = fmaf(u, -0.0030582291074097f, 0.0167208556085825f);
-  y = fmaf(y, u, -0.0515859872102737f);
-  y = fmaf(y, u, 0.1328072100877762f);
-  y = fmaf(y, u, -0.3332895040512085f);
-  return fmaf(y, u, 0.9999994039535522f) * z;
 }
 
 // One piece of work; the same in every thread of a warp.
@@ -685,8 +673,10 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             return max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], __uint_as_float(sv[1][28]), __uint_as_float(sv[1][29])),
                         max3(__uint_as_float(sv[1][29]), __uint_as_float(sv[1][30]), __uint_as_float(sv[1][31])));
           };
-          // A cap: tanh(k s) = s (c0 + c1 s^2 + ..) where the half's scores are small; else it is taken in place in tensor memory, to keep
-          // the code short, and the polynomial that follows is s.
+          // A cap on the arithmetic units, as two exponential units' steps per score would cost as much as both products: where
+          // |k s| <= 1/2 for a half's scores, as almost always, tanh(k s) = s (c0 + c1 s^2 + c2 s^4 + c3 s^6), an interpolation at
+          // Chebyshev points off by 6e-7 of itself at most, five steps a pair of scores that are taken between the exponentials.  Else
+          // it is taken in place in tensor memory, to keep the code short, and the polynomial that follows is s.
           uint64_t cap_c[4];
           auto cap = [&](int h, uint32_t (&sv)[2][32], float top) {
             float mn[4];
@@ -710,9 +700,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 const float x = __uint_as_float(v[i]);
-                float t = cap_one(x, p.cap_in);            // (the quotient below loses what is small against 1)
-                if (!below_1 && !(fabsf(x * p.cap_in) <= 1.f)) t = 1.f - 2.f * __fdividef(1.f, 1.f + exp2f(x * p.cap_in * 2.885390081777927f));
-                v[i] = __float_as_uint(t);
+                v[i] = __float_as_uint(below_1 ? score_cap_small(x, p.cap_in) : score_cap(x, p.cap_in));
               }
               tmem_st_32x16(tS + h * 64 + c * 16, v);
             }

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_spans_gpu import DEV, NAN, _i32, causal, close, oracle, pages, rand, run_spans
+from test_spans_gpu import DEV, NAN, _i32, causal, close, oracle, pages, rand, run_shared, run_spans
 
 pytestmark = pytest.mark.gpu
 HQ, HKV, BS = 10, 2, 64
@@ -232,6 +232,11 @@ def test_two_streams_at_once():
 def test_scores_on_every_side_of_a_cap(cap, q_scale):
     """Far below the cap, around half of it, around it, beyond; caps whose powers leave 32 bits.  Whole tiles and masked ones."""
     run_spans([(150, 700), (20, 20)], 4, 2, 64, causal, cap=cap, q_scale=q_scale, splits=1)
+
+
+@pytest.mark.parametrize("cap", [5.0, 1.0, 0.01, 1e6, 1e9])
+def test_shared_and_own_scores_on_every_side_of_a_cap(cap):
+    run_shared([(192, [70, 5, 300]), (64, [33, 1])], 6, 2, 64, cap=cap, gate=True, alone=1)
 
 
 @pytest.mark.parametrize("splits", [1, 3])
