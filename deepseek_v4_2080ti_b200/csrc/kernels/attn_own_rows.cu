@@ -383,38 +383,38 @@ cudaError_t launch(const OwnParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-// q / out / gate [B, Hq, 128]; sequence b: the keys shared .. kv_len[b] - 1 of table row b, shared = shared_len[g] of the group with
-// group_start[g] <= b < group_start[g + 1] (0 without one).  slots > 0: partial sums over the shared keys from b200_attn_shared,
-// launched before this one.  cluster: blocks (1, 2, 4 or 8) that share a sequence's keys.
-extern "C" int b200_attn_own_rows(const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate,
-                                  const int* block_table, const int* kv_len, const int* group_start, const int* shared_len, int n_groups,
-                                  int batch, int max_blocks, int num_blocks, int block_size, int n_q_heads, int n_kv_heads, float scale,
-                                  float cap, int slots, const float* workspace, int cluster, cudaStream_t stream) {
-  const bool pow2 = block_size >= 16 && block_size <= 256 && !(block_size & (block_size - 1));
-  if (!pow2 || n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads || batch < 1 || max_blocks < 1 || num_blocks < 1 || n_groups < 0 ||
-      !(scale > 0.f) || !(cap >= 0.f) || (long long)max_blocks * block_size > 0x7fffff00ll || slots < 0 || slots > 64 || (slots > 0 && !workspace) ||
-      (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8))
+// Sequence b: the keys shared .. kv_len[b] - 1 of table row b, shared = shared_len[g] of the group with group_start[g] <= b <
+// group_start[g + 1] (0 without one).  With groups: joined with the partial sums of b200_attn_shared, launched before this one with
+// the same block.  cluster: thread blocks (1, 2, 4 or 8) that share a sequence's keys.
+extern "C" int b200_attn_own_rows(const SpansCall* call) {
+  const SpansCall& a = *call;
+  const int bs = a.block_size;
+  const bool pow2 = bs >= 16 && bs <= 256 && !(bs & (bs - 1));
+  const int slots = a.n_groups > 0 ? a.splits : 0;
+  if (a.bytes != (int)sizeof(a) || !pow2 || a.n_kv_heads < 1 || a.n_q_heads < 1 || a.n_q_heads % a.n_kv_heads || a.batch < 1 || a.max_blocks < 1 ||
+      a.num_blocks < 1 || a.n_groups < 0 || !(a.scale > 0.f) || !(a.cap >= 0.f) || (long long)a.max_blocks * bs > 0x7fffff00ll || slots < 0 ||
+      slots > 64 || (slots > 0 && !a.workspace) || (a.cluster != 1 && a.cluster != 2 && a.cluster != 4 && a.cluster != 8))
     return -6;
   OwnParams p = {};
-  p.q = reinterpret_cast<const __nv_bfloat16*>(q);
-  p.gate = reinterpret_cast<const __nv_bfloat16*>(gate);
-  p.out = reinterpret_cast<__nv_bfloat16*>(out);
-  p.k_cache = reinterpret_cast<const __nv_bfloat16*>(k_cache);
-  p.v_cache = reinterpret_cast<const __nv_bfloat16*>(v_cache);
-  p.block_table = block_table; p.kv_len = kv_len;
-  p.group_start = group_start; p.shared_len = shared_len; p.n_groups = n_groups;
-  p.part_o = workspace;
-  p.part_ml = workspace ? workspace + (size_t)slots * batch * n_q_heads * D : nullptr;
+  p.q = reinterpret_cast<const __nv_bfloat16*>(a.q);
+  p.gate = reinterpret_cast<const __nv_bfloat16*>(a.gate);
+  p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
+  p.k_cache = reinterpret_cast<const __nv_bfloat16*>(a.k_cache);
+  p.v_cache = reinterpret_cast<const __nv_bfloat16*>(a.v_cache);
+  p.block_table = a.block_table; p.kv_len = a.kv_len;
+  p.group_start = a.group_start; p.shared_len = a.shared_len; p.n_groups = a.n_groups;
+  p.part_o = a.workspace;
+  p.part_ml = a.workspace ? a.workspace + (size_t)slots * a.batch * a.n_q_heads * D : nullptr;
   p.slots = slots;
-  p.B = batch; p.max_blocks = max_blocks; p.num_blocks = num_blocks; p.bs = block_size;
-  while ((1 << p.bs_log2) < block_size) ++p.bs_log2;
-  p.Hq = n_q_heads; p.Hkv = n_kv_heads; p.G = n_q_heads / n_kv_heads;
+  p.B = a.batch; p.max_blocks = a.max_blocks; p.num_blocks = a.num_blocks; p.bs = bs;
+  while ((1 << p.bs_log2) < bs) ++p.bs_log2;
+  p.Hq = a.n_q_heads; p.Hkv = a.n_kv_heads; p.G = a.n_q_heads / a.n_kv_heads;
   const int H = p.G <= 8 ? 8 : 16;
   p.chunks = (p.G + H - 1) / H;
-  p.cluster = cluster;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.cap_in = cap > 0.f ? scale / cap : 0.f;
-  p.cap_out = cap * 1.4426950408889634f;
-  if ((long long)batch * n_kv_heads * p.chunks * cluster > 0x7fffffffll) return -6;
-  return (int)(H == 8 ? launch<1>(p, stream) : launch<2>(p, stream));
+  p.cluster = a.cluster;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.cap_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
+  p.cap_out = a.cap * 1.4426950408889634f;
+  if ((long long)a.batch * a.n_kv_heads * p.chunks * a.cluster > 0x7fffffffll) return -6;
+  return (int)(H == 8 ? launch<1>(p, a.stream) : launch<2>(p, a.stream));
 }

@@ -1137,44 +1137,44 @@ int launch_as(const CUtensorMap& tmK, const CUtensorMap& tmV, const Params& p, c
 }
 
 template <bool SHARED>
-int launch(Params& p, const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate, const int* block_table,
-           const int* kv_len, int batch, int T, int max_blocks, int num_blocks, int block_size, int n_q_heads, int n_kv_heads, float scale,
-           float cap, float* workspace, int* status, cudaStream_t stream) {
-  const bool pow2 = block_size >= 16 && block_size <= 256 && !(block_size & (block_size - 1));
-  if (!pow2 || n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads || batch < 1 || T < 1 || max_blocks < 1 || num_blocks < 1 ||
-      !(scale > 0.f) || !(cap >= 0.f) || (long long)max_blocks * block_size > 0x7fffff00ll ||
-      ((long long)num_blocks + 1) * n_kv_heads * block_size > 0x7fffff00ll || ((SHARED || p.splits > 1) && !workspace))
+int launch(Params& p, const SpansCall& a) {
+  const int bs = a.block_size;
+  const bool pow2 = bs >= 16 && bs <= 256 && !(bs & (bs - 1));
+  if (!pow2 || a.n_q_heads % a.n_kv_heads || a.batch < 1 || a.T < 1 || a.max_blocks < 1 || a.num_blocks < 1 || !(a.scale > 0.f) || !(a.cap >= 0.f) ||
+      (long long)a.max_blocks * bs > 0x7fffff00ll || ((long long)a.num_blocks + 1) * a.n_kv_heads * bs > 0x7fffff00ll ||
+      ((SHARED || a.splits > 1) && !a.workspace))
     return -ERR_BAD_ARG;
-  p.q = reinterpret_cast<const __nv_bfloat16*>(q);
-  p.gate = reinterpret_cast<const __nv_bfloat16*>(gate);
-  p.out = reinterpret_cast<__nv_bfloat16*>(out);
-  p.v_cache = reinterpret_cast<const __nv_bfloat16*>(v_cache);
-  p.block_table = block_table;
-  p.kv_len = kv_len;
-  p.batch = batch; p.T = T; p.max_blocks = max_blocks; p.num_blocks = num_blocks; p.bs = block_size;
-  while ((1 << p.bs_log2) < block_size) ++p.bs_log2;
-  p.Hq = n_q_heads; p.Hkv = n_kv_heads; p.G = n_q_heads / n_kv_heads;
-  const size_t rows = (size_t)T * n_q_heads;
+  p.q = reinterpret_cast<const __nv_bfloat16*>(a.q);
+  p.gate = SHARED ? nullptr : reinterpret_cast<const __nv_bfloat16*>(a.gate);
+  p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
+  p.v_cache = reinterpret_cast<const __nv_bfloat16*>(a.v_cache);
+  p.block_table = a.block_table;
+  p.kv_len = a.kv_len;
+  p.batch = a.batch; p.T = a.T; p.max_blocks = a.max_blocks; p.num_blocks = a.num_blocks; p.bs = bs;
+  while ((1 << p.bs_log2) < bs) ++p.bs_log2;
+  p.Hq = a.n_q_heads; p.Hkv = a.n_kv_heads; p.G = a.n_q_heads / a.n_kv_heads;
+  p.splits = a.splits;
+  const size_t rows = (size_t)a.T * a.n_q_heads;
   const bool parts = SHARED || p.splits > 1;
-  p.part_o = parts ? workspace : nullptr;
-  p.part_ml = parts ? workspace + rows * p.splits * D : nullptr;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.cap_in = cap > 0.f ? scale / cap : 0.f;
-  p.cap_out = cap * 1.4426950408889634f;
+  p.part_o = parts ? a.workspace : nullptr;
+  p.part_ml = parts ? a.workspace + rows * p.splits * D : nullptr;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.cap_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
+  p.cap_out = a.cap * 1.4426950408889634f;
   if (p.cap_in > 1e-5f && p.cap_in < 1e5f) {
     const double k = p.cap_in, k3 = k * k * k;
     p.cap_small = (float)(0.5 / k);
     p.cap_c = make_float4((float)(0.999999463558197 * k), (float)(-0.3332628309726715 * k3), (float)(0.1318994015455246 * k3 * k * k),
                           (float)(-0.0443927384912968 * k3 * k3 * k));
   }
-  p.status = status;
+  p.status = a.status;
   CUtensorMap tmK, tmV;
-  const uint64_t kv_rows = (uint64_t)num_blocks * n_kv_heads * block_size;
-  const uint32_t box = block_size < BKV ? block_size : BKV;
-  if (!make_tmap_2d(&tmK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, k_cache, kv_rows, D, D * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tmap_2d(&tmV, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, v_cache, kv_rows, D, D * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B))
+  const uint64_t kv_rows = (uint64_t)a.num_blocks * a.n_kv_heads * bs;
+  const uint32_t box = bs < BKV ? bs : BKV;
+  if (!make_tmap_2d(&tmK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.k_cache, kv_rows, D, D * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_2d(&tmV, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.v_cache, kv_rows, D, D * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B))
     return -ERR_BAD_ARG;
-  return cap > 0.f ? launch_as<SHARED, true>(tmK, tmV, p, stream) : launch_as<SHARED, false>(tmK, tmV, p, stream);
+  return a.cap > 0.f ? launch_as<SHARED, true>(tmK, tmV, p, a.stream) : launch_as<SHARED, false>(tmK, tmV, p, a.stream);
 }
 
 }  // namespace spans
@@ -1182,43 +1182,34 @@ int launch(Params& p, const void* q, const void* k_cache, const void* v_cache, v
 
 using namespace b200;
 
-// Prompt rows.  q / out / gate [T, Hq, 128] bf16; caches [num_blocks, Hkv, block_size, 128] bf16, block_size a power of two from
-// 16 to 256; sequence b: rows [q_start, q_start + q_len) and the first kv_len keys of table row b.  Row t sees the keys
+// Prompt rows.  Sequence b: rows [q_start, q_start + q_len) and the first kv_len keys of table row b.  Row t sees the keys
 // lo[t] <= j < min(hi[t], kv_len); without lo from 0, without hi up to its own position kv_len - q_len + i.  splits: items a
-// row's keys are cut into; from 2 on workspace: fp32 [splits T Hq 130].  Rows of no sequence are left as they are.
-extern "C" int b200_attn_spans(const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate,
-                               const int* block_table, const int* q_start, const int* q_len, const int* kv_len, const int* lo,
-                               const int* hi, int batch, int max_q_len, int T, int max_blocks, int num_blocks, int block_size,
-                               int n_q_heads, int n_kv_heads, float scale, float cap, int splits, float* workspace, int* status,
-                               cudaStream_t stream) {
-  if (max_q_len < 1 || max_q_len > T || splits < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads) return -ERR_BAD_ARG;
+// row's keys are cut into.  Rows of no sequence are left as they are.
+extern "C" int b200_attn_spans(const SpansCall* call) {
+  const SpansCall& a = *call;
+  if (a.bytes != (int)sizeof(a) || a.max_q_len < 1 || a.max_q_len > a.T || a.splits < 1 || a.n_kv_heads < 1 || a.n_q_heads < a.n_kv_heads)
+    return -ERR_BAD_ARG;
   spans::Params p = {};
-  p.q_start = q_start; p.q_len = q_len; p.lo = lo; p.hi = hi;
-  const long long tiles = ((long long)max_q_len * (n_q_heads / n_kv_heads) + 2 * spans::BQ - 1) / (2 * spans::BQ);
-  if (tiles * batch * n_kv_heads * splits > 0x7fffffffll) return -ERR_BAD_ARG;
+  p.q_start = a.q_start; p.q_len = a.q_len; p.lo = a.lo; p.hi = a.hi;
+  const long long tiles = ((long long)a.max_q_len * (a.n_q_heads / a.n_kv_heads) + 2 * spans::BQ - 1) / (2 * spans::BQ);
+  if (tiles * a.batch * a.n_kv_heads * a.splits > 0x7fffffffll) return -ERR_BAD_ARG;
   p.row_tiles = (int)tiles;
-  p.splits = splits;
-  p.n_items = (int)(tiles * batch * n_kv_heads * splits);
-  return spans::launch<false>(p, q, k_cache, v_cache, out, gate, block_table, kv_len, batch, T, max_blocks, num_blocks, block_size, n_q_heads,
-                              n_kv_heads, scale, cap, workspace, status, stream);
+  p.n_items = (int)(tiles * a.batch * a.n_kv_heads * a.splits);
+  return spans::launch<false>(p, a);
 }
 
-// One row per sequence: partial sums over the keys that groups of sequences share, for b200_attn_own_rows.  q [B, Hq, 128];
-// the sequences group_start[g] <= b < group_start[g + 1] hold the same first shared_len[g] keys in the same pages (those of the
-// group's first row of the table); sequence b sees kv_len[b] of them.  splits: items the keys are cut into; workspace: fp32
-// [splits B Hq 130].
-extern "C" int b200_attn_shared(const void* q, const void* k_cache, const void* v_cache, const int* block_table, const int* kv_len,
-                                const int* group_start, const int* shared_len, int n_groups, int batch, int max_blocks, int num_blocks,
-                                int block_size, int n_q_heads, int n_kv_heads, float scale, float cap, int splits, float* workspace,
-                                int* status, cudaStream_t stream) {
-  if (n_groups < 1 || splits < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || batch < 1) return -ERR_BAD_ARG;
+// One row per sequence: partial sums over the keys that groups of sequences share, for b200_attn_own_rows.  The sequences
+// group_start[g] <= b < group_start[g + 1] hold the same first shared_len[g] keys in the same pages (those of the group's first row
+// of the table); sequence b sees kv_len[b] of them.  splits: items the keys are cut into.
+extern "C" int b200_attn_shared(const SpansCall* call) {
+  const SpansCall& a = *call;
+  if (a.bytes != (int)sizeof(a) || a.n_groups < 1 || a.splits < 1 || a.n_kv_heads < 1 || a.n_q_heads < a.n_kv_heads || a.T != a.batch)
+    return -ERR_BAD_ARG;
   spans::Params p = {};
-  p.group_start = group_start; p.shared_len = shared_len; p.n_groups = n_groups;
-  const long long rows = (long long)batch * (n_q_heads / n_kv_heads), tiles = rows / (2 * spans::BQ) + n_groups;
-  if (tiles * splits * n_kv_heads > 0x7fffffffll) return -ERR_BAD_ARG;
+  p.group_start = a.group_start; p.shared_len = a.shared_len; p.n_groups = a.n_groups;
+  const long long rows = (long long)a.batch * (a.n_q_heads / a.n_kv_heads), tiles = rows / (2 * spans::BQ) + a.n_groups;
+  if (tiles * a.splits * a.n_kv_heads > 0x7fffffffll) return -ERR_BAD_ARG;
   p.row_tiles = (int)tiles;
-  p.splits = splits;
-  p.n_items = (int)(tiles * splits * n_kv_heads);
-  return spans::launch<true>(p, q, k_cache, v_cache, nullptr, nullptr, block_table, kv_len, batch, batch, max_blocks, num_blocks, block_size,
-                             n_q_heads, n_kv_heads, scale, cap, workspace, status, stream);
+  p.n_items = (int)(tiles * a.splits * a.n_kv_heads);
+  return spans::launch<true>(p, a);
 }

@@ -180,25 +180,39 @@ int b200_gqa_decode(const void* q, const void* k_cache, const void* v_cache, voi
                     const int* block_table, const int* kv_len, float* workspace, int batch, int max_blocks,
                     int block_size, int n_q_heads, int n_kv_heads, int splits, float softmax_scale, cudaStream_t stream);
 // rotary positions of several axes with the append (rope_axes_kv.cu); rows with spans of keys of their own (attn_spans.cu); one row per
-// sequence over pages that groups of sequences share: partial sums over those (attn_spans.cu), own keys and join (attn_own_rows.cu)
-int b200_qk_norm_rope_axes_append(const void* q_src, int ldq, int q_off, int q_head_stride, int gate_in_q, const void* k_src,
-                                  int ldk, int k_off, const void* v_src, int ldv, int v_off, const void* q_gamma,
-                                  const void* k_gamma, int unit_offset, float eps, const float* inv_freq, int rot, float mscale,
-                                  const unsigned char* axes, int n_axes, const int* positions, int ld_pos, const int* slots,
-                                  void* q_out, void* gate_out, void* k_cache, void* v_cache, int num_blocks, int block_size,
-                                  int T, int Hq, int Hkv, cudaStream_t stream);
-int b200_attn_spans(const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate, const int* block_table,
-                    const int* q_start, const int* q_len, const int* kv_len, const int* lo, const int* hi, int batch,
-                    int max_q_len, int T, int max_blocks, int num_blocks, int block_size, int n_q_heads, int n_kv_heads,
-                    float scale, float cap, int splits, float* workspace, int* status, cudaStream_t stream);
-int b200_attn_shared(const void* q, const void* k_cache, const void* v_cache, const int* block_table, const int* kv_len,
-                     const int* group_start, const int* shared_len, int n_groups, int batch, int max_blocks, int num_blocks,
-                     int block_size, int n_q_heads, int n_kv_heads, float scale, float cap, int splits, float* workspace,
-                     int* status, cudaStream_t stream);
-int b200_attn_own_rows(const void* q, const void* k_cache, const void* v_cache, void* out, const void* gate, const int* block_table,
-                       const int* kv_len, const int* group_start, const int* shared_len, int n_groups, int batch, int max_blocks,
-                       int num_blocks, int block_size, int n_q_heads, int n_kv_heads, float scale, float cap, int slots,
-                       const float* workspace, int cluster, cudaStream_t stream);
+// sequence over pages that groups of sequences share: partial sums over those (attn_spans.cu), own keys and join (attn_own_rows.cu).
+// Their arguments come as one block, which begins with its size: a call of 33 arguments costs the Python side 3.7 us, a block 0.6.
+struct AxesAppendCall {
+  int bytes, T;
+  const void *q_src, *k_src, *v_src;          // bf16: q head h at q_src[t ldq + q_off + h q_head_stride], k and v heads 128 apart
+  const void *q_gamma, *k_gamma;              // bf16 [128], null: no norm
+  const float* inv_freq;                      // [rot / 2]
+  const int *positions, *slots;               // [n_axes, ld_pos], [T]; negative slots are not cached
+  void *q_out, *gate_out;                     // bf16 [T, Hq, 128]
+  void *k_cache, *v_cache;                    // bf16 [num_blocks, Hkv, block_size, 128]
+  cudaStream_t stream;
+  int ldq, q_off, q_head_stride, gate_in_q, ldk, k_off, ldv, v_off, unit_offset, rot, n_axes, ld_pos, num_blocks, block_size, Hq, Hkv;
+  float eps, mscale;
+  unsigned char axis[64];                     // of every pair
+};
+struct SpansCall {
+  int bytes, batch;
+  const void *q, *k_cache, *v_cache;          // bf16 [T, Hq, 128], [num_blocks, Hkv, block_size, 128]; block_size a power of two, 16 to 256
+  void* out;                                  // bf16 [T, Hq, 128]
+  const void* gate;                           // optional, as out
+  const int *block_table, *kv_len;            // [batch, max_blocks], [batch]
+  const int *q_start, *q_len, *lo, *hi;       // prompt rows: [batch] twice, optional [T] twice
+  const int *group_start, *shared_len;        // one row per sequence (T = batch): [n_groups + 1], [n_groups]
+  float* workspace;                           // [splits T Hq 130]: partial sums of several items, or of the shared keys
+  int* status;
+  cudaStream_t stream;
+  int n_groups, max_q_len, T, max_blocks, num_blocks, block_size, n_q_heads, n_kv_heads, splits, cluster;
+  float scale, cap;
+};
+int b200_qk_norm_rope_axes_append(const AxesAppendCall* call);
+int b200_attn_spans(const SpansCall* call);
+int b200_attn_shared(const SpansCall* call);
+int b200_attn_own_rows(const SpansCall* call);
 // FlashMemory retriever (flashmemory.cu): chunk scores of one scorer layer, layer ensemble, top-k, index offset
 int b200_fm_score_layer(const float* hidden, const void* wq_a, const void* wq_b, const float* q_norm, const void* weights_proj,
                         const float* inv_freqs, const void* keys8, const float* keysf, float* q_scratch, float* qlora_scratch,

@@ -139,43 +139,39 @@ qk_norm_rope_axes_append_kernel(const __grid_constant__ AxesParams p) {
 
 }  // namespace
 
-// As b200_qk_norm_rope_append, with positions int32 [n_axes, T] (rows ld_pos apart) and `axes` (host, rot / 2 bytes): the axis of
-// every rotary pair.  rot: a multiple of 8.
-extern "C" int b200_qk_norm_rope_axes_append(
-    const void* q_src, int ldq, int q_off, int q_head_stride, int gate_in_q, const void* k_src, int ldk, int k_off,
-    const void* v_src, int ldv, int v_off, const void* q_gamma, const void* k_gamma, int unit_offset, float eps,
-    const float* inv_freq, int rot, float mscale, const unsigned char* axes, int n_axes, const int* positions, int ld_pos,
-    const int* slots, void* q_out, void* gate_out, void* k_cache, void* v_cache, int num_blocks, int block_size, int T, int Hq,
-    int Hkv, cudaStream_t stream) {
-  if (rot < 0 || rot > D || (rot & 7) || n_axes < 1 || T < 1 || Hq < 1 || Hkv < 1 || block_size < 1 || num_blocks < 1 ||
-      (long long)num_blocks * block_size > 0x7fffffffll || (ldq & 3) || (q_off & 3) || (q_head_stride & 3) || (ldk & 3) || (k_off & 3) ||
-      (ldv & 3) || (v_off & 3) || ld_pos < T || (gate_in_q && !gate_out) || (rot && (!axes || !inv_freq || !positions)))
+// As b200_qk_norm_rope_append, with a row of positions for every axis and the axis of every rotary pair.  rot: a multiple of 8.
+extern "C" int b200_qk_norm_rope_axes_append(const AxesAppendCall* call) {
+  const AxesAppendCall& a = *call;
+  if (a.bytes != (int)sizeof(a) || a.rot < 0 || a.rot > D || (a.rot & 7) || a.n_axes < 1 || a.T < 1 || a.Hq < 1 || a.Hkv < 1 || a.block_size < 1 ||
+      a.num_blocks < 1 || (long long)a.num_blocks * a.block_size > 0x7fffffffll || (a.ldq & 3) || (a.q_off & 3) || (a.q_head_stride & 3) ||
+      (a.ldk & 3) || (a.k_off & 3) || (a.ldv & 3) || (a.v_off & 3) || a.ld_pos < a.T || (a.gate_in_q && !a.gate_out) ||
+      (a.rot && (!a.inv_freq || !a.positions)))
     return -6;
   AxesParams p = {};
-  for (int i = 0; i < rot / 2; ++i) {
-    if (axes[i] >= n_axes) return -6;
-    p.axis[i] = axes[i];
+  for (int i = 0; i < a.rot / 2; ++i) {
+    if (a.axis[i] >= a.n_axes) return -6;
+    p.axis[i] = a.axis[i];
   }
-  p.q_src = reinterpret_cast<const __nv_bfloat16*>(q_src); p.ldq = ldq; p.q_off = q_off; p.q_head_stride = q_head_stride;
-  p.gate_in_q = gate_in_q;
-  p.k_src = reinterpret_cast<const __nv_bfloat16*>(k_src); p.ldk = ldk; p.k_off = k_off;
-  p.v_src = reinterpret_cast<const __nv_bfloat16*>(v_src); p.ldv = ldv; p.v_off = v_off;
-  p.q_gamma = reinterpret_cast<const __nv_bfloat16*>(q_gamma);
-  p.k_gamma = reinterpret_cast<const __nv_bfloat16*>(k_gamma);
-  p.unit_offset = unit_offset; p.eps = eps;
-  p.inv_freq = inv_freq; p.rot = rot; p.mscale = mscale;
-  p.positions = positions; p.ld_pos = ld_pos; p.slots = slots;
-  p.q_out = reinterpret_cast<__nv_bfloat16*>(q_out);
-  p.gate_out = reinterpret_cast<__nv_bfloat16*>(gate_out);
-  p.k_cache = reinterpret_cast<__nv_bfloat16*>(k_cache);
-  p.v_cache = reinterpret_cast<__nv_bfloat16*>(v_cache);
-  p.bs = block_size; p.n_slots = (unsigned)num_blocks * block_size;
-  p.T = T; p.Hq = Hq; p.Hkv = Hkv;
-  const int heads = Hq + 2 * Hkv;
-  // few tokens: a row per warp, so that the SMs share a token's heads
-  const bool few = (long long)T * heads <= 148 * 2 * WARPS;
+  p.q_src = reinterpret_cast<const __nv_bfloat16*>(a.q_src); p.ldq = a.ldq; p.q_off = a.q_off; p.q_head_stride = a.q_head_stride;
+  p.gate_in_q = a.gate_in_q;
+  p.k_src = reinterpret_cast<const __nv_bfloat16*>(a.k_src); p.ldk = a.ldk; p.k_off = a.k_off;
+  p.v_src = reinterpret_cast<const __nv_bfloat16*>(a.v_src); p.ldv = a.ldv; p.v_off = a.v_off;
+  p.q_gamma = reinterpret_cast<const __nv_bfloat16*>(a.q_gamma);
+  p.k_gamma = reinterpret_cast<const __nv_bfloat16*>(a.k_gamma);
+  p.unit_offset = a.unit_offset; p.eps = a.eps;
+  p.inv_freq = a.inv_freq; p.rot = a.rot; p.mscale = a.mscale;
+  p.positions = a.positions; p.ld_pos = a.ld_pos; p.slots = a.slots;
+  p.q_out = reinterpret_cast<__nv_bfloat16*>(a.q_out);
+  p.gate_out = reinterpret_cast<__nv_bfloat16*>(a.gate_out);
+  p.k_cache = reinterpret_cast<__nv_bfloat16*>(a.k_cache);
+  p.v_cache = reinterpret_cast<__nv_bfloat16*>(a.v_cache);
+  p.bs = a.block_size; p.n_slots = (unsigned)a.num_blocks * a.block_size;
+  p.T = a.T; p.Hq = a.Hq; p.Hkv = a.Hkv;
+  const int heads = a.Hq + 2 * a.Hkv;
+  // few tokens: a row per warp, so that the SMs share a token's heads (37 tokens of 64 rows: 2.8 us; with the other form 8.0)
+  const bool few = (long long)a.T * heads <= 148 * 2 * WARPS;
   p.block_rows = few ? WARPS : heads;
-  const dim3 grid(T, (heads + p.block_rows - 1) / p.block_rows), block(WARPS * 32);
-  return (int)(few ? b200::launch_pdl(qk_norm_rope_axes_append_kernel<1>, grid, block, 0, stream, p)
-                   : b200::launch_pdl(qk_norm_rope_axes_append_kernel<4>, grid, block, 0, stream, p));
+  const dim3 grid(a.T, (heads + p.block_rows - 1) / p.block_rows), block(WARPS * 32);
+  return (int)(few ? b200::launch_pdl(qk_norm_rope_axes_append_kernel<1>, grid, block, 0, a.stream, p)
+                   : b200::launch_pdl(qk_norm_rope_axes_append_kernel<4>, grid, block, 0, a.stream, p));
 }

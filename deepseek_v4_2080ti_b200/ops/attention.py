@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 
 import torch
 
@@ -259,20 +260,18 @@ def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
     return dev, t, hq, nb, hkv, bs, b, width, scale, out
 
 
-_P, _I = ctypes.c_void_p, ctypes.c_int
+# The kernels' arguments as one block each (AxesAppendCall and SpansCall in ops.h), packed: a third of what 33 arguments cost one by one.
+_AXES_CALL, _SPANS_CALL = struct.Struct("@ii13P16iff64s"), struct.Struct("@ii16P10iff")
 _typed = False
 
 
 def _kernels() -> ctypes.CDLL:
-    """The kernel library with the parameter types of the calls below, which take plain addresses and numbers."""
+    """The kernel library with the parameter types of the calls below, which take a block."""
     global _typed
     lib = _lib.lib()
     if not _typed:
-        lib.b200_qk_norm_rope_axes_append.argtypes = [_P, _I, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _f, _P, _I, _f, ctypes.c_char_p, _I, _P,
-                                                      _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]
-        lib.b200_attn_spans.argtypes = [_P] * 11 + [_I] * 8 + [_f, _f, _I, _P, _P, _P]
-        lib.b200_attn_shared.argtypes = [_P] * 7 + [_I] * 7 + [_f, _f, _I, _P, _P, _P]
-        lib.b200_attn_own_rows.argtypes = [_P] * 9 + [_I] * 7 + [_f, _f, _I, _P, _I, _P]
+        for f in (lib.b200_qk_norm_rope_axes_append, lib.b200_attn_spans, lib.b200_attn_shared, lib.b200_attn_own_rows):
+            f.argtypes = [ctypes.c_char_p]
         _typed = True
     return lib
 
@@ -286,7 +285,7 @@ def _rows(x, t: int, dev: int, what: str) -> int:
 
 
 def _at(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 _current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
@@ -357,10 +356,10 @@ def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_of
     if t == 0:
         return q_out, gate_out
     _lib.check_indices(slots, -2 ** 31, nb * bs, 2)         # (a bad slot becomes a negative one)
-    rc = _kernels().b200_qk_norm_rope_axes_append(
-        q_src.data_ptr(), ldq, q_off, q_head_stride, gate_in_q, k_src.data_ptr(), ldk, k_off, v_src.data_ptr(), ldv, v_off, _at(q_gamma), _at(k_gamma),
-        unit_offset, eps, inv_freq.data_ptr(), 2 * n, mscale, table, n_axes, positions.data_ptr(), t, slots.data_ptr(), q_out.data_ptr(),
-        _at(gate_out), k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, t, n_q_heads, n_kv_heads, _stream(dev))
+    rc = _kernels().b200_qk_norm_rope_axes_append(_AXES_CALL.pack(
+        _AXES_CALL.size, t, q_src.data_ptr(), k_src.data_ptr(), v_src.data_ptr(), _at(q_gamma), _at(k_gamma), inv_freq.data_ptr(), positions.data_ptr(),
+        slots.data_ptr(), q_out.data_ptr(), _at(gate_out), k_cache.data_ptr(), v_cache.data_ptr(), _stream(dev), ldq, q_off, q_head_stride, gate_in_q,
+        ldk, k_off, ldv, v_off, unit_offset, 2 * n, n_axes, t, nb, bs, n_q_heads, n_kv_heads, eps, mscale, table))
     _lib.check(rc, "qk_norm_rope_axes_append")
     return q_out, gate_out
 
@@ -418,9 +417,10 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
         raise ValueError(f"{splits} splits")
     ws = q.new_empty(splits * t * hq * (D + 2), dtype=_F32) if splits > 1 else None
     _lib.check_indices(block_table, 0, nb, 3)
-    rc = _kernels().b200_attn_spans(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
-        kv_len.data_ptr(), _at(lo), _at(hi), b, max_q_len, t, width, nb, bs, hq, hkv, scale, cap, splits, _at(ws), _status(dev), _stream(dev))
+    rc = _kernels().b200_attn_spans(_SPANS_CALL.pack(
+        _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
+        q_start.data_ptr(), q_len.data_ptr(), _at(lo), _at(hi), 0, 0, _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq, hkv,
+        splits, 1, scale, cap))
     _lib.check(rc, "prefill_spans", 2 if splits > 1 else 1)
     return out
 
@@ -495,17 +495,16 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     blocks, cluster = b * hkv * -(-g // 16), 1
     while cluster < 8 and cluster * blocks <= NUM_SMS and own_keys > 256 * cluster:
         cluster *= 2
-    lib, stream = _kernels(), _stream(dev)
+    lib = _kernels()
     _lib.check_indices(block_table, 0, nb, 3)
-    pq, pk, pv, pt, pl, pg, ps = (x.data_ptr() for x in (q, k_cache, v_cache, block_table, kv_len, group_start, shared_len))
-    ws = None
+    ws = q.new_empty(splits * b * hq * (D + 2), dtype=_F32) if n else None
+    call = _SPANS_CALL.pack(
+        _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
+        0, 0, 0, 0, group_start.data_ptr(), shared_len.data_ptr(), _at(ws), _status(dev), _stream(dev), n, 1, t, width, nb, bs, hq, hkv, splits, cluster,
+        scale, cap)
     if n:
-        ws = q.new_empty(splits * b * hq * (D + 2), dtype=_F32)
-        rc = lib.b200_attn_shared(pq, pk, pv, pt, pl, pg, ps, n, b, width, nb, bs, hq, hkv, scale, cap, splits, ws.data_ptr(), _status(dev), stream)
-        _lib.check(rc, "decode_shared")
-    rc = lib.b200_attn_own_rows(pq, pk, pv, out.data_ptr(), _at(gate), pt, pl, pg, ps, n, b, width, nb, bs, hq, hkv, scale, cap, splits if n else 0,
-                                _at(ws), cluster, stream)
-    _lib.check(rc, "decode_shared")
+        _lib.check(lib.b200_attn_shared(call), "decode_shared")
+    _lib.check(lib.b200_attn_own_rows(call), "decode_shared")
     return out
 
 
