@@ -267,14 +267,14 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
     it.kvh = (int)(x - y * p.Hkv);
     it.slot = split;
     const int b = (int)(y - z * p.batch), tile = p.row_tiles - 1 - (int)z;                 // long contexts first
-    const int q0 = p.q_start[b], n = p.q_len[b];
+    const int q0 = p.q_start[b], n = p.q_len[b], kv = p.kv_len[b];
     const int len = q0 < 0 ? 0 : min(n, p.T - q0);
     rows_all = max(0, len) * p.G;
     it.r0 = tile * 2 * BQ;
     it.trow = b;
     it.base_tok = q0;
-    it.kv_end = max(0, min(p.kv_len[b], p.max_blocks * p.bs));
-    it.delta = p.kv_len[b] - n - q0;
+    it.kv_end = max(0, min(kv, p.max_blocks * p.bs));
+    it.delta = kv - n - q0;
     it.own_hi = 0;
   }
   it.n_rows = min(2 * BQ, rows_all - it.r0);
@@ -349,9 +349,9 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   uint64_t* p_half = q_full + 4;                            // P of the tile's first 64 keys
   uint64_t* p_full = q_full + 6;
   uint64_t* o_full = q_full + 8;
-  uint64_t* j_full = q_full + 10;                           // stream 1's part lies in the scratch
-  uint64_t* j_empty = q_full + 11;                          // and has been read
-  uint64_t* i_full = q_full + 12;                           // items
+  uint64_t* j_full = q_full + 10;                           // by slot of the scratch: 32 columns of stream 1's part lie there
+  uint64_t* j_empty = q_full + 12;                          // and have been read
+  uint64_t* i_full = q_full + 14;                           // items
   uint64_t* i_empty = i_full + ITEMS;
   uint64_t* pv_half = i_empty + ITEMS;                      // per stream: the product with the values of a tile's first 64 keys
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_half + 2);
@@ -380,8 +380,10 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       mbar_init(&i_empty[i], 10);
     }
     for (int m = 0; m < 2; ++m) mbar_init(&pv_half[m], 1);
-    mbar_init(j_full, 4);
-    mbar_init(j_empty, 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&j_full[i], 4);
+      mbar_init(&j_empty[i], 4);
+    }
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -432,6 +434,17 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         more = round * gridDim.x < p.n_items;
         it.n_rows = 0;
         if (more && (idx >= p.n_items || !get_item<SHARED>(p, idx, lane, it))) continue;
+        const int* bt = p.block_table + (size_t)it.trow * p.max_blocks;
+        const int last_page = (it.k_end - 1) >> p.bs_log2;
+        auto page_row = [&](int tile) {                                    // cache row where this lane's part of a tile begins
+          const int key = tile * BKV + (lane << rows_log2);
+          const int page = min(key >> p.bs_log2, last_page);
+          if (tile >= it.t1 || lane >= per_tile) return 0;
+          // a page that is not there (an entry before the first key that is seen, or a bad one) lies behind the cache: it reads as zeros
+          const int id = min((unsigned)bt[page], (unsigned)p.num_blocks);
+          return ((id * p.Hkv + it.kvh) << p.bs_log2) + (key & (p.bs - 1));
+        };
+        int row = more ? page_row(it.t0) : 0;              // (on its way while the item is handed out)
         ok = warp_wait(&i_empty[i_at], i_ph ^ 1) && !*abort_flag;
         if (!ok) break;
         if (lane == 0) {
@@ -443,24 +456,6 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         }
         if (++i_at == ITEMS) { i_at = 0; i_ph ^= 1; }
         if (!more) break;
-        {                                                                  // queries and gate on their way to L2
-          for (int t = it.tok0 + lane; t <= it.tok1; t += 32) {
-            const size_t at = ((size_t)t * p.Hq + it.kvh * p.G) * D;
-            l2_prefetch(p.q + at, p.G * D * 2);
-            if (p.gate && !p.part_o) l2_prefetch(p.gate + at, p.G * D * 2);
-          }
-        }
-        const int* bt = p.block_table + (size_t)it.trow * p.max_blocks;
-        const int last_page = (it.k_end - 1) >> p.bs_log2;
-        auto page_row = [&](int tile) {                                    // cache row where this lane's part of a tile begins
-          const int key = tile * BKV + (lane << rows_log2);
-          const int page = min(key >> p.bs_log2, last_page);
-          if (tile >= it.t1 || lane >= per_tile) return 0;
-          // a page that is not there (an entry before the first key that is seen, or a bad one) lies behind the cache: it reads as zeros
-          const int id = min((unsigned)bt[page], (unsigned)p.num_blocks);
-          return ((id * p.Hkv + it.kvh) << p.bs_log2) + (key & (p.bs - 1));
-        };
-        int row = page_row(it.t0);
         for (int t = it.t0; ok && t < it.t1; ++t) {
           const int n = min(per_tile, (it.k_end - t * BKV + rows - 1) >> rows_log2);
           const int next_row = page_row(t + 1);
@@ -480,6 +475,13 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           }
           row = next_row;
           c.next();
+          if (t == it.t0) {                                // queries and gate of items ahead on their way to L2
+            for (int y = it.tok0 + lane; y <= it.tok1; y += 32) {
+              const size_t at = ((size_t)y * p.Hq + it.kvh * p.G) * D;
+              l2_prefetch(p.q + at, p.G * D * 2);
+              if (p.gate && !p.part_o) l2_prefetch(p.gate + at, p.G * D * 2);
+            }
+          }
         }
       }
       if (!ok && lane == 0) { atomicExch(p.status, ERR_WAIT_STAGE); *abort_flag = 1; }
@@ -600,7 +602,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
     const int lr = threadIdx.x & 127;                      // row of the stream == TMEM lane
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + m * 128 + lane_off, tO = tmem + 256 + m * 128 + lane_off;
-    uint32_t ph_s = 0, ph_o = 0, ph_j = 0;
+    uint32_t ph_s = 0, ph_o = 0;
     Ring checks = {0, 0};
     bool alive = true;
     for (;;) {
@@ -876,7 +878,9 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             Ring v = checks;
             v.skip(t);
             if (!(alive = warp_wait(&v_ok[v.st], v.ph))) break;
-            for (int part = 0; part < 4; ++part)
+            uint4 none;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(none.x), "=r"(none.y), "=r"(none.z), "=r"(none.w) : "r"(smem_u32(s_bad + v.st * 4)) : "memory");
+            for (int part = 0; part < 4 && (none.x | none.y | none.z | none.w); ++part)
               for (uint32_t bad = *(volatile uint32_t*)(s_bad + v.st * 4 + part); bad; bad &= bad - 1) {
                 // a key with values that are not finite: its row in shared memory is zero, the rows that see it add it here
                 const int kx = part * 32 + __ffs(bad) - 1, key = key0 + kx;
@@ -938,9 +942,10 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       // 32 columns at a time, four columns of a row at place (column / 4, row ^ column / 4).
       if (!writer && !joined) continue;                    // (a stream without a part, or without rows: the others write)
       float w_own = 1.f, w_other = 0.f;
-      auto staged = [&](int stream, int c4, int r) -> float4* {
-        return reinterpret_cast<float4*>(sQ + stream * TILE + (warp & 3) * 4096 + ((c4 * 32 + (r ^ c4)) << 4));
+      auto staged = [&](int stream, int slot, int c4, int r) -> float4* {
+        return reinterpret_cast<float4*>(sQ + stream * TILE + slot * ATOM + (warp & 3) * 4096 + ((c4 * 32 + (r ^ c4)) << 4));
       };
+      // Streams that are joined: 32 columns of stream 1 at a time through two slots of its half of the scratch, each filled and read twice.
 #pragma unroll 1
       for (int c = 0; c < 4 && alive; ++c) {               // 32 columns
         uint32_t v[32];
@@ -955,22 +960,21 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           return make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
         };
         if (joined && m == 1) {
+          if (c >= 2 && !(alive = warp_wait(&j_empty[c & 1], 0))) break;
           if (warp_on) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) *staged(1, i, lane) = four(i);
+            for (int i = 0; i < 8; ++i) *staged(1, c & 1, i, lane) = four(i);
           }
-          s_ml[lr] = m_run;
-          s_ml[128 + lr] = l_run;
+          if (c == 0) {
+            s_ml[lr] = m_run;
+            s_ml[128 + lr] = l_run;
+          }
           __syncwarp();
-          if (lane == 0) mbar_arrive(j_full);
-          alive = warp_wait(j_empty, ph_j);                // it has been read
-          ph_j ^= 1;
+          if (lane == 0) mbar_arrive(&j_full[c & 1]);
           continue;
         }
         if (joined) {                                      // (then both streams' score products, which read the queries here, have finished)
-          alive = warp_wait(j_full, ph_j);
-          ph_j ^= 1;
-          if (!alive) break;
+          if (!(alive = warp_wait(&j_full[c & 1], c >> 1))) break;
           if (c == 0) {
             const float m1 = s_ml[lr], l1 = s_ml[128 + lr], mm = fmaxf(m_run, m1);
             w_own = m_run == -INFINITY ? 0.f : exp2f(m_run - mm);
@@ -1000,7 +1004,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
               float4 o = four(i);
               o.x *= w_own; o.y *= w_own; o.z *= w_own; o.w *= w_own;
               if (joined) {
-                const float4 x = *staged(1, i, lane);
+                const float4 x = *staged(1, c & 1, i, lane);
                 o.x += x.x * w_other; o.y += x.y * w_other; o.z += x.z * w_other; o.w += x.w * w_other;
               }
               v[4 * i] = __float_as_uint(o.x); v[4 * i + 1] = __float_as_uint(o.y); v[4 * i + 2] = __float_as_uint(o.z); v[4 * i + 3] = __float_as_uint(o.w);
@@ -1008,14 +1012,14 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           }
           if (p.part_o) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) *staged(m, i, lane) = four(i);
+            for (int i = 0; i < 8; ++i) *staged(m, 0, i, lane) = four(i);
             __syncwarp();
             if (steps) {
-#pragma unroll 2
-              for (int i = 0; i < (rows_here + 3) / 4; ++i) {              // a quarter warp per row
+#pragma unroll 4
+              for (int i = 0; i < 8; ++i) {                // a quarter warp per row
                 const int r = 4 * i + (lane >> 3);
                 const size_t prow = row0 + __shfl_sync(0xffffffffu, at, r);
-                if (r < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + c * 32)[lane & 7] = *staged(m, lane & 7, r);
+                if (r < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + c * 32)[lane & 7] = *staged(m, 0, lane & 7, r);
               }
             }
           } else {
@@ -1044,8 +1048,9 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           }
         }
         __syncwarp();
-        if (joined && lane == 0) mbar_arrive(j_empty);
+        if (joined && lane == 0) mbar_arrive(&j_empty[c & 1]);
       }
+      if (joined && m == 1 && alive) alive = warp_wait(&j_empty[0], 1) && warp_wait(&j_empty[1], 1);     // all of it has been read
       if (alive && writer && !p.part_o) {
 #pragma unroll 4
         for (int i = 0; i < (rows_here + 1) / 2; ++i) {    // half a warp per row
