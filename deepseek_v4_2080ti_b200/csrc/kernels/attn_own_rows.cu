@@ -17,11 +17,11 @@
 #include "launch.h"
 #include "ops.h"
 #include "score_cap.cuh"
+#include "tma_host.h"
 
 namespace {
 
 constexpr int D = 128;
-constexpr int WARPS = 4;
 constexpr int LD = 132;              // floats of a row of O in shared memory: the fragments' stores then meet no bank twice
 
 struct OwnParams {
@@ -80,9 +80,9 @@ __device__ __forceinline__ float4 ld_cluster4(const float* p, uint32_t rank) {
   return v;
 }
 
-// NB: groups of 8 heads a block works on.
-template <int NB>
-__global__ void __launch_bounds__(WARPS * 32, NB == 1 ? 3 : 2)
+// NB: groups of 8 heads a block works on.  WARPS: 4, or 3 of which four blocks fit an SM instead of three.
+template <int NB, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, NB == 2 ? 2 : 12 / WARPS)
 own_rows_kernel(const __grid_constant__ OwnParams p) {
   constexpr int H = 8 * NB;
   __shared__ float s_m[WARPS][H], s_l[WARPS][H];
@@ -364,7 +364,7 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
   if (p.cluster > 1) cluster_sync();                     // the others may still read this block's sums
 }
 
-template <int NB>
+template <int NB, int WARPS>
 cudaError_t launch(const OwnParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hkv * p.chunks * p.cluster));
@@ -378,7 +378,7 @@ cudaError_t launch(const OwnParams& p, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, own_rows_kernel<NB>, p);
+  return cudaLaunchKernelEx(&cfg, own_rows_kernel<NB, WARPS>, p);
 }
 
 }  // namespace
@@ -416,5 +416,12 @@ extern "C" int b200_attn_own_rows(const SpansCall* call) {
   p.cap_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
   p.cap_out = a.cap * 1.4426950408889634f;
   if ((long long)a.batch * a.n_kv_heads * p.chunks * a.cluster > 0x7fffffffll) return -6;
-  return (int)(H == 8 ? launch<1>(p, a.stream) : launch<2>(p, a.stream));
+  if (H == 16) return (int)launch<2, 4>(p, a.stream);
+  // A block of 3 warps takes a third longer, but four of them fit an SM: taken where that saves enough rounds of blocks, of which one in
+  // twenty finds the kernel before still there.  Sequences of 500 own keys and 2048 shared ones, 8 kv heads, 4 / 3 warps: 32: 27.9 / 27.8 us,
+  // 64: 67.6 / 48.3, 74: 69.2 / 73.9, 100: 76.1 / 78.2, 128: 89.4 / 81.9, 148: 91.4 / 95.9; 64 of 3000: 179.6 / 126.0.
+  const long long blocks = (long long)a.batch * a.n_kv_heads * p.chunks * a.cluster, sms = b200::sm_count();
+  auto rounds = [&](int per_sm) { return blocks * 20 / (per_sm * sms * 19) + 1; };
+  const bool three = rounds(4) * 4 < rounds(3) * 3;
+  return (int)(three ? launch<1, 3>(p, a.stream) : launch<1, 4>(p, a.stream));
 }

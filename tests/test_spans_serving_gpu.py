@@ -239,6 +239,18 @@ def test_shared_and_own_scores_on_every_side_of_a_cap(cap):
     run_shared([(192, [70, 5, 300]), (64, [33, 1])], 6, 2, 64, cap=cap, gate=True, alone=1)
 
 
+@pytest.mark.parametrize("n,hq,hkv", [(57, 8, 8), (64, 16, 8), (128, 8, 8)])
+def test_many_sequences(n, hq, hkv):
+    """More (sequence, kv head) pairs than blocks of the larger form run at once."""
+    run_shared([(64, [1 + 13 * i % 90 for i in range(n - 9)])], hq, hkv, 32, alone=9, gate=True)
+
+
+def test_a_portion_beside_single_rows():
+    """The longest portion would leave most row tiles empty; and portions in any order, empty ones among them."""
+    run_spans([(1, 70)] * 40 + [(700, 900)] + [(1, 3), (2, 2)], 4, 1, 64, causal, gate=True)
+    run_spans([(500, 500)] + [(1, 129)] * 5 + [(300, 310)], 10, 2, 16, causal, splits=2)
+
+
 @pytest.mark.parametrize("splits", [1, 3])
 def test_infinite_scores_under_a_cap(splits):
     """Keys with an infinity give the cap or its negative, also where a row sees nothing else."""
