@@ -798,9 +798,9 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             cap_c[0] = pack2(1.f, 1.f);
             cap_c[1] = cap_c[2] = cap_c[3] = 0;
           };
-          // What the weights of scores up to `top` are taken relative to.  With a cap k top, limited to 1, stands for tanh(k top): within
-          // a quarter of the cap, and NaN stays.
-          auto level = [&](float top) { return CAP ? scale * min3(max3(top * p.cap_in, -1.f, -1.f), 1.f, 1.f) : scale * top; };
+          // What the weights of scores up to `top` are taken relative to: that score's own, so that the largest weight of a row, which
+          // often outweighs the others, is 1 and not rounded.
+          auto level = [&](float top) { return scale * (CAP ? score_cap(top, p.cap_in) : top); };
           // The running maximum up to that of new scores, where it is far enough behind; false: the product that last added to O has not
           // finished in time.  The tile before's has, as it was issued before the scores that arrived; `half`: the first half's may be on its way.
           auto raise = [&](float m_tile, bool half) {
