@@ -17,7 +17,7 @@
 // Two streams of 128 rows keep the tensor core and the exponential units busy in turn.  An item of at most 128 rows gives both
 // streams the same rows and every other key tile, and joins them at its end.  Warp roles:
 //   warps 0-3, 4-7: softmax of stream 0 and 1 - one row per thread, online maximum / sum in the exp2 domain (fp32), P rounded to
-//             bf16 for the product (relative 2^-9 a weight; the sum adds the weights before they are rounded) into the tensor
+//             bf16 for the product (2^-8 of a weight at most; the sum adds the weights before they are rounded) into the tensor
 //             memory its scores came from, lazy rescale of the stream's O (when a maximum grows by 2^8); then the item's rows;
 //   warp 8  : items - which rows and keys are next, up to four ahead of the slowest role - and their loads: key and value tiles
 //             gathered page by page through the block table into one ring (TMA), running ahead into the next item;
@@ -28,11 +28,12 @@
 //   warp 11 : nothing (a warpgroup gives its registers up as a whole).
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each.  All mbarrier waits are bounded and unwind through the common exit.
 //
-// What bounds it (8192 causal rows of 40 heads over 8 kv heads, gated: 619 us, 1.1 PFLOP/s): 256 rows times 128 keys cost 2048
+// What bounds it (8192 causal rows of 40 heads over 8 kv heads, gated: 628 us, 1.1 PFLOP/s): 256 rows times 128 keys cost 2048
 // cycles of the tensor core and about 2100 of each scheduler's softmax warps, and take 3500 together, because a stream's scores,
 // weights and products follow each other through tensor memory and two streams do not hide all of that; an item's start and end
-// take another 10 %.  Packed documents of 4000 rows, capped: 115 us, of which masked tiles and the items' ends are half.  Shared
-// keys, 64 rows per sequence's head over 32768 keys: 320 rows a kv head, 44 us; 32 over 8192: 15 us.
+// take another 10 %.  Packed documents of 4000 rows of 48 heads, capped: 118 us, half of it masked tiles (6000 cycles) and items' ends.
+// Shared keys of 40 heads over 8, in one item a block: 64 rows over 32768 keys 44 us, 32 over 8192 15 us.  The smallest call, one
+// row over 121 keys, is a chain of 9 us: the item 3, page and tiles 3, softmax 4 and product 1 thousand cycles, the row's way out 4.
 #include <cuda_bf16.h>
 #include "per_device.h"
 #include "../ptx/sm100.cuh"
@@ -50,7 +51,7 @@ constexpr int BKV = 128;          // keys per tile
 constexpr int ATOM = 16384;       // bytes of one [128 x 64] bf16 swizzled slab
 constexpr int TILE = 2 * ATOM;
 constexpr int STAGES = 5;
-constexpr int EMULATED = 2;       // of 8 pairs of exponentials: those on the arithmetic units (0 / 1 / 2 / 3: 641 / 639 / 624 / 626 us, see below)
+constexpr int EMULATED = 2;       // of 8 pairs of exponentials: those on the arithmetic units (0 / 1 / 2 / 3: 641 / 639 / 624 / 626 us for 8192 causal rows)
 constexpr int ITEMS = 4;          // items the producer may be ahead of the slowest role
 constexpr int NTHREADS = 384;
 constexpr int SMEM_BYTES = 1024 + (2 + STAGES) * TILE + 2048;
@@ -186,7 +187,7 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
 }
 
 // 2^x of two numbers below 128 on the arithmetic units: 2^round(x) by the exponent bits, 2^f of the rest, |f| <= 1/2, by a cubic with
-// constant term 1 (fitted to the relative error, 1e-4: P is rounded to 2^-9).  From -127 down the result is exactly zero.  Not for NaN.
+// constant term 1 (fitted to the relative error, 1e-4: P is rounded to 2^-8).  From -127 down the result is exactly zero.  Not for NaN.
 __device__ __forceinline__ void exp2_fma(float& a, float& b) {
   constexpr float BIG = 12582912.f;                          // 1.5 2^23: the sum's low bits are the rounded integer
   constexpr float E1 = 0.693282961845398f, E2 = 0.24221111834049225f, E3 = 0.05500898137688637f;
@@ -299,7 +300,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
         }
         const int items = (len_ * p.G + 2 * BQ - 1) / (2 * BQ) * p.Hkv * splits;
         int upto = items;
-  #pragma unroll
+#pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int before = __shfl_up_sync(0xffffffffu, upto, o);
           if (lane >= o) upto += before;
