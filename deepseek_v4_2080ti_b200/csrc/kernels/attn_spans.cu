@@ -1110,28 +1110,32 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
               }
             }
           } else {
+            auto put = [&](auto with_gate) {              // (one look at the gate, not four)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint4* place = reinterpret_cast<uint4*>(own + (c >> 1) * ATOM + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4));
-              float o[8];
+              for (int i = 0; i < 4; ++i) {
+                uint4* place = reinterpret_cast<uint4*>(own + (c >> 1) * ATOM + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4));
+                float o[8];
 #pragma unroll
-              for (int x = 0; x < 8; ++x) o[x] = __uint_as_float(v[8 * i + x]);
-              if (p.gate) {
-                const uint4 g = *place;
-                const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&g);
+                for (int x = 0; x < 8; ++x) o[x] = __uint_as_float(v[8 * i + x]);
+                if (with_gate.value) {
+                  const uint4 g = *place;
+                  const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&g);
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                  const float2 gf = __bfloat1622float2(gh[x]);
-                  o[2 * x] = __fdividef(o[2 * x], 1.f + __expf(-gf.x));
-                  o[2 * x + 1] = __fdividef(o[2 * x + 1], 1.f + __expf(-gf.y));
+                  for (int x = 0; x < 4; ++x) {
+                    const float2 gf = __bfloat1622float2(gh[x]);
+                    o[2 * x] = __fdividef(o[2 * x], 1.f + __expf(-gf.x));
+                    o[2 * x + 1] = __fdividef(o[2 * x + 1], 1.f + __expf(-gf.y));
+                  }
                 }
-              }
-              uint4 u4;
-              __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u4);
+                uint4 u4;
+                __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u4);
 #pragma unroll
-              for (int x = 0; x < 4; ++x) h2[x] = __floats2bfloat162_rn(o[2 * x], o[2 * x + 1]);
-              *place = u4;
-            }
+                for (int x = 0; x < 4; ++x) h2[x] = __floats2bfloat162_rn(o[2 * x], o[2 * x + 1]);
+                *place = u4;
+              }
+            };
+            if (p.gate) put(Int<1>());
+            else put(Int<0>());
           }
         }
         __syncwarp();
