@@ -31,7 +31,7 @@
 // What bounds it (8192 causal rows of 40 heads over 8 kv heads, gated: 628 us, 1.1 PFLOP/s): 256 rows times 128 keys cost 2048
 // cycles of the tensor core and about 2100 of each scheduler's softmax warps, and take 3500 together, because a stream's scores,
 // weights and products follow each other through tensor memory and two streams do not hide all of that; an item's start and end
-// take another 10 %.  Packed documents of 4000 rows of 48 heads, capped: 118 us, half of it masked tiles (6000 cycles) and items' ends.
+// take another 10 %.  Packed documents of 4000 rows of 48 heads, capped: 116 us, half of it masked tiles (6000 cycles) and items' ends.
 // Shared keys of 40 heads over 8, in one item a block: 64 rows over 32768 keys 44 us, 32 over 8192 15 us.  The smallest call, one
 // row over 121 keys, is a chain of 9 us: the item 3, page and tiles 3, softmax 4 and product 1 thousand cycles, the row's way out 4.
 #include <cuda_bf16.h>
