@@ -509,8 +509,9 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       int idx = blockIdx.x;
       uint32_t ph_next = 0;
       while (idx >= 0) {
-        // (a launch that has met an error ends: its other blocks do not wait as well)
-        const bool failed = *reinterpret_cast<const volatile int*>(p.status) != 0;
+        // (a launch whose waits have run out ends: its other blocks do not wait as well.  An index that the debug mode has replaced is no failure.)
+        const int status = *reinterpret_cast<const volatile int*>(p.status);
+        const bool failed = status != 0 && (status & 0xFF) != ERR_BOUNDS;
         if (get_item<SHARED>(p, idx, lane, it) && !failed) {
         const int* bt = p.block_table + (size_t)it.trow * p.max_blocks;
         const int last_page = (it.k_end - 1) >> p.bs_log2;

@@ -296,19 +296,29 @@ def _status(dev: int) -> int:
     return (_lib.status_word(dev) if t is None else t).data_ptr()
 
 
+class PairAxes(tuple):
+    """Axis of every rotary pair, with the table that the kernel takes (laid out once: 1.2 us a call for 64 pairs otherwise)."""
+
+    def __new__(cls, axes):
+        self = super().__new__(cls, axes)
+        self.table = bytes(self)                            # (axes outside 0 .. 255: ValueError)
+        self.n_axes = max(self.table, default=0) + 1
+        return self
+
+
 @functools.lru_cache(maxsize=64)
-def _pair_axes(sections: tuple, interleaved: bool) -> tuple[int, ...]:
+def _pair_axes(sections: tuple, interleaved: bool) -> PairAxes:
     _need(sections and min(sections) >= 0 and 0 < sum(sections) <= D // 2, f"sections {sections}: 1 to {D // 2} pairs in all expected")
     if not interleaved:
-        return tuple(a for a, n in enumerate(sections) for _ in range(n))
+        return PairAxes(a for a, n in enumerate(sections) for _ in range(n))
     axes = [0] * sum(sections)
     for a, n in enumerate(sections[1:], 1):
         _need(n == 0 or a + len(sections) * (n - 1) < len(axes), f"sections {sections}: axis {a} is too long to take turns")
         axes[a:a + len(sections) * n:len(sections)] = [a] * n
-    return tuple(axes)
+    return PairAxes(axes)
 
 
-def rotary_axes(sections, interleaved: bool = False) -> tuple[int, ...]:
+def rotary_axes(sections, interleaved: bool = False) -> PairAxes:
     """Axis of every rotary pair from the number of pairs of each axis: one block per axis, or - ``interleaved`` - the axes in
     turn (T H W T H W ..), where pairs that no other axis claims stay on the first."""
     return _pair_axes(tuple(int(n) for n in sections), bool(interleaved))
@@ -344,8 +354,10 @@ def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_of
     for g in (q_gamma, k_gamma):
         if g is not None and (g.dtype is not _BF16 or g.numel() != D or not g.is_contiguous() or g.get_device() != dev or g.data_ptr() % 8):
             raise ValueError("gammas: bf16 [128] on the device of the rows, 8-byte aligned, expected")
-    table, n, n_axes = bytes(axes), len(axes), positions.shape[0]
-    if n % 4 or not 0 < n <= D // 2 or n_axes <= max(table):
+    if type(axes) is not PairAxes:
+        axes = PairAxes(axes)
+    n, n_axes = len(axes), positions.shape[0]
+    if n % 4 or not 0 < n <= D // 2 or n_axes < axes.n_axes:
         raise ValueError(f"axes: 4, 8 .. {D // 2} pairs, each with a row of positions, expected")
     if inv_freq.dtype is not _F32 or inv_freq.numel() != n or not inv_freq.is_contiguous() or inv_freq.get_device() != dev:
         raise ValueError("inv_freq: fp32, one per pair, on the device of the rows expected")
@@ -359,7 +371,7 @@ def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_of
     rc = _kernels().b200_qk_norm_rope_axes_append(_AXES_CALL.pack(
         _AXES_CALL.size, t, q_src.data_ptr(), k_src.data_ptr(), v_src.data_ptr(), _at(q_gamma), _at(k_gamma), inv_freq.data_ptr(), positions.data_ptr(),
         slots.data_ptr(), q_out.data_ptr(), _at(gate_out), k_cache.data_ptr(), v_cache.data_ptr(), _stream(dev), ldq, q_off, q_head_stride, gate_in_q,
-        ldk, k_off, ldv, v_off, unit_offset, 2 * n, n_axes, t, nb, bs, n_q_heads, n_kv_heads, eps, mscale, table))
+        ldk, k_off, ldv, v_off, unit_offset, 2 * n, n_axes, t, nb, bs, n_q_heads, n_kv_heads, eps, mscale, axes.table))
     _lib.check(rc, "qk_norm_rope_axes_append")
     return q_out, gate_out
 
@@ -416,7 +428,7 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
     if not 1 <= splits <= 1024:
         raise ValueError(f"{splits} splits")
     ws = q.new_empty(splits * t * hq * (D + 2), dtype=_F32) if splits > 1 else None
-    _lib.check_indices(block_table, 0, nb, 3)
+    _lib.check_indices(block_table, 0, nb, 3, keep=-1)
     rc = _kernels().b200_attn_spans(_SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
         q_start.data_ptr(), q_len.data_ptr(), _at(lo), _at(hi), 0, 0, _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq, hkv,
@@ -496,7 +508,7 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     while cluster < 8 and cluster * blocks <= NUM_SMS and own_keys > 256 * cluster:
         cluster *= 2
     lib = _kernels()
-    _lib.check_indices(block_table, 0, nb, 3)
+    _lib.check_indices(block_table, 0, nb, 3, keep=-1)
     ws = q.new_empty(splits * b * hq * (D + 2), dtype=_F32) if n else None
     call = _SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),

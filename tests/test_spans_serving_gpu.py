@@ -293,6 +293,37 @@ def test_pages_that_no_row_sees_are_not_followed():
             close(out, *oracle(q, k, v, lo.long(), hi.long(), 1 / math.sqrt(128)))
 
 
+def test_debug_mode(monkeypatch):
+    """With index checks on: tables with -1 for pages that are not there and negative slots pass; a page beyond the cache is reported, and
+    the kernels have run on what took its place."""
+    from deepseek_v4_2080ti_b200.ops import _lib
+    monkeypatch.setenv("B200_BOUNDS_CHECK", "1")
+    a = _attention()
+    torch.manual_seed(8)
+    n, new = 400, 20
+    k, v = rand(n, HKV, 128), rand(n, HKV, 128)
+    kc, vc, table = pages([(k, v)], BS)
+    lo, hi = (x[n - new:].to(DEV) for x in a.visible_spans(n, window=100))
+    q = rand(new, HQ, 128)
+    want, bound = oracle(q, k, v, lo.long(), hi.long(), 1 / math.sqrt(128))
+    table[0, :4] = -1
+    args = _i32([0]), _i32([new]), _i32([n]), new, lo, hi
+    close(a.prefill_spans(q, kc, vc, table, *args), want, bound)
+    layer = Layer(2)
+    src, slots = _src(3), _i32([-7, 5, -1])
+    rows, _ = layer.append(src, _i32(torch.zeros(3, 3)), slots)
+    layer.check_append(src, _i32(torch.zeros(3, 3)), slots, rows)
+    assert slots.tolist() == [-7, 5, -1]
+    _lib.check_status()
+    table[0, 0] = kc.shape[0] + 3
+    close(a.prefill_spans(q, kc, vc, table, *args), want, bound)
+    with pytest.raises(_lib.KernelError, match="index out of range"):
+        _lib.check_status()
+    one = a.decode_shared(q[:1].contiguous(), kc, vc, table.clamp(min=0), _i32([n]), _i32([0, 1]), _i32([0]))
+    _lib.check_status()
+    assert one.shape == (1, HQ, 128)
+
+
 def test_in_place():
     """Rows whose results take the queries' place."""
     a = _attention()
