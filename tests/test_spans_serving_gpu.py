@@ -324,6 +324,47 @@ def test_debug_mode(monkeypatch):
     assert one.shape == (1, HQ, 128)
 
 
+def test_guard_bands(monkeypatch):
+    """Nothing is written beside caches, results and workspaces: bands around all of them stay as they are."""
+    from deepseek_v4_2080ti_b200.ops import _lib
+    from deepseek_v4_2080ti_b200.utils import canary
+    a = _attention()
+    torch.manual_seed(9)
+
+    kept = []                                              # (a buffer's bands are looked at while it lives)
+
+    def guarded(t, *shape, dtype=None):
+        kept.append(canary.empty(*shape, dtype=dtype or t.dtype, device=t.device, name="workspace"))
+        return kept[-1]
+
+    def empty_like(t):
+        return guarded(t, *t.shape)
+    with canary.enabled(True):
+        monkeypatch.setattr(torch.Tensor, "new_empty", guarded)
+        layer = Layer(1)
+        layer.kc, layer.vc = (canary.zeros(12, HKV, BS, 128, dtype=torch.bfloat16, device=DEV, name="cache") for _ in range(2))
+        for t in (1, 37, 300):
+            layer.append(_src(t), _i32(torch.randint(0, 99, (3, t))), _i32(torch.randperm(12 * BS)[:t]))
+        table = _i32(torch.arange(12).view(1, 12).repeat(40, 1))
+        for lens in ([1], [300], [7, 128, 200], [1] * 39 + [150]):
+            starts, total = [sum(lens[:b]) for b in range(len(lens))], sum(lens)
+            q = guarded(layer.kc, total, HQ, 128).normal_()
+            out = empty_like(q)
+            for splits in (1, 3):
+                a.prefill_spans(q, layer.kc, layer.vc, table[:len(lens)].contiguous(), _i32(starts), _i32(lens), _i32([12 * BS - b for b in range(len(lens))]),
+                                max(lens), gate=q, splits=splits, out=out)
+        for b in (1, 3, 40):
+            q = guarded(layer.kc, b, HQ, 128).normal_()
+            for splits in (1, 5):
+                a.decode_shared(q, layer.kc, layer.vc, table[:b].contiguous(), _i32([12 * BS - i for i in range(b)]), _i32([0, b // 2, b]), _i32([300, 512]),
+                                gate=q, splits=splits, out=empty_like(q))
+        torch.cuda.synchronize()
+        monkeypatch.undo()
+        _lib.check_status()
+        assert canary.live_buffers() >= len(kept)
+        canary.assert_clean()
+
+
 def test_in_place():
     """Rows whose results take the queries' place."""
     a = _attention()
