@@ -508,11 +508,22 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       };
       int idx = blockIdx.x;
       uint32_t ph_next = 0;
+      auto next_block = [&]() {                            // cancels a block that has not begun; idx: its number, -1 if there is none
+        idx = -1;
+        if (lane == 0) {
+          mbar_expect_tx(next_full, 16);
+          request_block(s_next, next_full);
+        }
+        __syncwarp();
+        if (!warp_wait(next_full, ph_next)) return false;
+        ph_next ^= 1;
+        idx = requested_block(s_next);
+        fence_proxy_async_smem();                          // read before the next answer is written
+        __syncwarp();
+        return true;
+      };
       while (idx >= 0) {
-        // (a launch whose waits have run out ends: its other blocks do not wait as well.  An index that the debug mode has replaced is no failure.)
-        const int status = *reinterpret_cast<const volatile int*>(p.status);
-        const bool failed = status != 0 && (status & 0xFF) != ERR_BOUNDS;
-        if (get_item<SHARED>(p, idx, lane, it) && !failed) {
+        if (get_item<SHARED>(p, idx, lane, it)) {
         const int* bt = p.block_table + (size_t)it.trow * p.max_blocks;
         const int last_page = (it.k_end - 1) >> p.bs_log2;
         auto page_row = [&](int tile) {                                    // cache row where this lane's part of a tile begins
@@ -554,25 +565,18 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         }
         }
         // the next one only now, when this one's tiles are all on their way: blocks that are ahead take more
-        idx = -1;
-        if (!ok || failed) break;
-        if (lane == 0) {
-          mbar_expect_tx(next_full, 16);
-          request_block(s_next, next_full);
-        }
-        __syncwarp();
-        ok = warp_wait(next_full, ph_next);
-        if (!ok) break;
-        ph_next ^= 1;
-        idx = requested_block(s_next);
-        fence_proxy_async_smem();                          // read before the next answer is written
-        __syncwarp();
+        if (!ok || !(ok = next_block())) break;
       }
       if (ok) {
         it.n_rows = 0;
         hand_out();
       }
-      if (!ok && lane == 0) { atomicExch(p.status, ERR_WAIT_STAGE); *abort_flag = 1; }
+      // A launch whose waits have run out ends: its blocks that have not begun are cancelled, so that they do not wait as well.  (The error
+      // word does not tell: it is the device's, and may hold what another kernel has reported.)
+      if (!ok) {
+        if (lane == 0) { atomicExch(p.status, ERR_WAIT_STAGE); *abort_flag = 1; }
+        while (idx >= 0 && next_block()) {}
+      }
     } else if (warp == 9) {
       // The whole warp walks the loop, so that addresses and descriptors stay warp-uniform, and one elected lane issues.  What a step
       // costs beside the products is as long as they are if it is not kept short: even lanes wait for one barrier while odd lanes

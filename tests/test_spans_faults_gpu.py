@@ -1,0 +1,40 @@
+"""Attention over spans and shared pages where something else went wrong: an error that another kernel has reported, pages that are not there,
+values that are not finite under weights of zero, and what the debug mode says of them.  Bounds as in ``test_spans_gpu``."""
+import math
+
+import pytest
+import torch
+
+from test_spans_gpu import DEV, NAN, _i32, close, oracle, pages, rand, run_spans
+
+pytestmark = pytest.mark.gpu
+SCALE = 1 / math.sqrt(128)
+
+
+def _modules():
+    from deepseek_v4_2080ti_b200.ops import _lib, attention
+    return _lib, attention
+
+
+@pytest.mark.parametrize("code", [4, 2])
+def test_an_error_of_another_kernel_changes_no_result(code):
+    """The error word is the device's, and stays set until the host has read it: calls meanwhile do all their work."""
+    lib, a = _modules()
+    torch.manual_seed(11)
+    n, new, hq, hkv, bs = 900, 300, 10, 2, 64
+    k, v = rand(n, hkv, 128), rand(n, hkv, 128)
+    kc, vc, table = pages([(k, v)], bs)
+    q, at = rand(new, hq, 128), torch.arange(n - new, n, device=DEV)
+    want, bound = oracle(q, k, v, torch.zeros_like(at), at + 1, SCALE)
+    lib.check_status()
+    lib.status_word(q.device).fill_(code)
+    got = [a.prefill_spans(q, kc, vc, table, _i32([0]), _i32([new]), _i32([n]), new, splits=s, out=torch.full_like(q, 7.0)) for s in (1, 4)]
+    rows = q[-5:].contiguous()
+    got.append(a.decode_shared(rows, kc, vc, table.repeat(5, 1), _i32([n - 4 + i for i in range(5)]), _i32([0, 5]), _i32([640]), splits=3))
+    torch.cuda.synchronize()
+    with pytest.raises(lib.KernelError, match=lib.ERR_NAMES[code]):
+        lib.check_status()
+    lib.check_status()
+    close(got[0], want, bound)
+    close(got[1], want, bound)
+    close(got[2], want[-5:], bound[-5:])
