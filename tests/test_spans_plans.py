@@ -1,0 +1,21 @@
+"""Plans of the calls over spans and shared pages, on the host: spans of blocks that overlap, groups of sequences, limits of scale and cap, pages
+that a row sees, and a torch without CUDA."""
+import math
+import random
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+from deepseek_v4_2080ti_b200.ops import attention
+
+
+@pytest.mark.parametrize("blocks", [[(0, 8), (2, 4)], [(1, 9), (3, 7), (4, 5)], [(0, 4), (2, 7)], [(5, 5), (2, 6), (2, 3)]])
+def test_blocks_that_overlap_see_to_the_furthest_end(blocks):
+    """In any order: a position sees up to the furthest end of the blocks that it lies in."""
+    want = [max([j + 1] + [e for f, e in blocks if f <= j < e]) for j in range(10)]
+    for order in (blocks, blocks[::-1], sorted(blocks)):
+        lo, hi = attention.visible_spans(10, blocks=order)
+        assert hi.tolist() == want and lo.tolist() == [0] * 10
