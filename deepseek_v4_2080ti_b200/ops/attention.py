@@ -379,17 +379,19 @@ def qk_norm_rope_axes_append(q_src, q_off, q_head_stride, gate_in_q, k_src, k_of
 def visible_spans(kv_len: int, documents=None, blocks=(), window: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
     """``lo``, ``hi`` int32 [kv_len] (host) of the positions of one sequence: causal within each of ``documents`` (lengths that add
     up to ``kv_len``), not further back than ``window`` keys, and inside a block ``(first, end)`` - an image, a prefix - up to
-    the block's end (the furthest of them, where blocks overlap)."""
+    the block's end (the furthest of them, where blocks overlap).  A block lies in one document."""
     pos = torch.arange(kv_len)
     lo, hi = torch.zeros_like(pos), pos + 1
     if documents is not None:
         lengths = torch.as_tensor(documents, dtype=torch.long).reshape(-1)
         _need(int(lengths.sum()) == kv_len and bool((lengths >= 0).all()), f"documents of {int(lengths.sum())} tokens in a context of {kv_len}")
+        ends = torch.repeat_interleave(lengths.cumsum(0), lengths)
         lo = torch.repeat_interleave(lengths.cumsum(0) - lengths, lengths)
     if window > 0:
         lo = torch.maximum(lo, pos + 1 - window)
     for first, end in blocks:
         _need(0 <= first <= end <= kv_len, f"block ({first}, {end}) in a context of {kv_len}")
+        _need(documents is None or first == end or end <= int(ends[first]), f"block ({first}, {end}) reaches into another document")
         hi[first:end].clamp_(min=end)
     return lo.to(torch.int32), hi.to(torch.int32)
 

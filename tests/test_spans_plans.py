@@ -19,3 +19,12 @@ def test_blocks_that_overlap_see_to_the_furthest_end(blocks):
     for order in (blocks, blocks[::-1], sorted(blocks)):
         lo, hi = attention.visible_spans(10, blocks=order)
         assert hi.tolist() == want and lo.tolist() == [0] * 10
+
+
+def test_blocks_stay_in_their_document():
+    lo, hi = attention.visible_spans(7, [3, 0, 4], blocks=[(0, 3), (4, 7), (3, 3), (7, 7)])
+    assert lo.tolist() == [0, 0, 0, 3, 3, 3, 3] and hi.tolist() == [3, 3, 3, 4, 7, 7, 7]
+    for bad in ((1, 5), (0, 7), (2, 4)):
+        with pytest.raises(ValueError, match="document"):
+            attention.visible_spans(7, [3, 0, 4], blocks=[bad])
+    assert attention.visible_spans(7, [0, 7, 0], blocks=[(1, 7)])[1].tolist() == [1, 7, 7, 7, 7, 7, 7]
