@@ -288,7 +288,13 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
-_current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# (looked up at the call: a torch without CUDA has neither, and the oracles below serve the host runtime)
+def _current() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _status(dev: int) -> int:

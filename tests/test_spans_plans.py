@@ -28,3 +28,15 @@ def test_blocks_stay_in_their_document():
         with pytest.raises(ValueError, match="document"):
             attention.visible_spans(7, [3, 0, 4], blocks=[bad])
     assert attention.visible_spans(7, [0, 7, 0], blocks=[(1, 7)])[1].tolist() == [1, 7, 7, 7, 7, 7, 7]
+
+
+def test_the_module_loads_where_torch_has_no_cuda():
+    """The host reference runtime takes its fp32 oracles from this module; a torch built without CUDA lacks these entry points."""
+    code = ("import torch\n"
+            "for name in ('_cuda_getDevice', '_cuda_getCurrentRawStream', '_cuda_setDevice', '_cuda_getDeviceCount'):\n"
+            "    if hasattr(torch._C, name): delattr(torch._C, name)\n"
+            "import deepseek_v4_2080ti_b200.models.reference_cpu.qwen_hybrid_ref\n"
+            "from deepseek_v4_2080ti_b200.ops import attention\n"
+            "assert attention.rotary_axes((2, 1, 1), True) == (0, 1, 2, 0)\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
