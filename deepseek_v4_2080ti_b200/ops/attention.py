@@ -231,6 +231,19 @@ def _caches(k_cache, v_cache, dev: int):
     return shape
 
 
+_LEAST, _MOST = 2.0 ** -100, 2.0 ** 100
+
+
+def _scores(scale, cap) -> float:
+    """Checks scale and cap; the scale.  The kernels hold both and scale / cap in 32 bits: a cap that became zero there would be none, and
+    scores times an infinite factor NaN."""
+    scale = SCALE if scale is None else float(scale)
+    if not _LEAST <= scale <= _MOST or cap and not (_LEAST <= cap <= _MOST and _LEAST <= scale / cap <= _MOST):
+        raise ValueError(f"scale {scale}, cap {cap}: a positive scale and a cap that is positive, or 0 for none, both and their ratio "
+                         f"between 2^-100 and 2^100, expected")
+    return scale
+
+
 def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
     """Checks what the calls over spans have in common; (device, rows, Hq, pages, Hkv, page size, sequences, table width, scale, out)."""
     dev, rows = q.get_device(), q.shape
@@ -254,10 +267,7 @@ def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
         out = torch.empty_like(q)
     else:
         _like(out, rows, dev, "out")
-    scale = SCALE if scale is None else float(scale)
-    if not 0.0 < scale < math.inf or not 0.0 <= cap < math.inf:
-        raise ValueError(f"scale {scale}, cap {cap}: a positive scale and a cap that is positive, or 0 for none, expected")
-    return dev, t, hq, nb, hkv, bs, b, width, scale, out
+    return dev, t, hq, nb, hkv, bs, b, width, _scores(scale, cap), out
 
 
 # The kernels' arguments as one block each (AxesAppendCall and SpansCall in ops.h), packed: a third of what 33 arguments cost one by one.

@@ -38,3 +38,15 @@ def test_an_error_of_another_kernel_changes_no_result(code):
     close(got[0], want, bound)
     close(got[1], want, bound)
     close(got[2], want[-5:], bound[-5:])
+
+
+def test_scales_and_caps_that_32_bits_do_not_hold_are_refused():
+    _, a = _modules()
+    k, v = rand(40, 2, 128), rand(40, 2, 128)
+    kc, vc, table = pages([(k, v)], 64)
+    q = rand(1, 4, 128)
+    for kw in ({"cap": 1e-50}, {"cap": 1e-40}, {"cap": 3e38}, {"cap": 1e300}, {"scale": 1e-50}, {"scale": 1e300}, {"scale": 1e25, "cap": 1e-25}):
+        with pytest.raises(ValueError):
+            a.prefill_spans(q, kc, vc, table, _i32([0]), _i32([1]), _i32([40]), 1, **kw)
+        with pytest.raises(ValueError):
+            a.decode_shared(q, kc, vc, table, _i32([40]), _i32([0, 1]), _i32([0]), **kw)

@@ -30,6 +30,16 @@ def test_blocks_stay_in_their_document():
     assert attention.visible_spans(7, [0, 7, 0], blocks=[(1, 7)])[1].tolist() == [1, 7, 7, 7, 7, 7, 7]
 
 
+def test_scales_and_caps_that_32_bits_do_not_hold():
+    """A cap that becomes zero in 32 bits would be none at all, one beyond them infinite."""
+    for scale, cap in ((None, 0.0), (0.1, 30.0), (1.0, 1e-6), (0.0884, 1e9), (2.0 ** -100, 0.0), (2.0 ** 100, 1.0), (1.0, 2.0 ** 100)):
+        assert attention._scores(scale, cap) == 1 / math.sqrt(128) if scale is None else scale
+    for scale, cap in ((None, 1e-50), (None, 1e-40), (None, 3e38), (None, 1e300), (1e-50, 0.0), (1e300, 0.0), (1e25, 1e-25), (1e-25, 1e25), (0.0, 0.0),
+                       (-1.0, 0.0), (math.nan, 0.0), (math.inf, 0.0), (None, -1.0), (None, math.inf), (None, math.nan)):
+        with pytest.raises(ValueError):
+            attention._scores(scale, cap)
+
+
 def test_the_module_loads_where_torch_has_no_cuda():
     """The host reference runtime takes its fp32 oracles from this module; a torch built without CUDA lacks these entry points."""
     code = ("import torch\n"
