@@ -981,7 +981,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 tmem_ld_wait();
                 const float pv = __uint_as_float(kx & 1 ? w & 0xFFFF0000u : w << 16);
                 if (key >= it.k_end) continue;
-                const bool seen = key >= lo && key < hi && pv != 0.f;
+                const bool seen = key >= lo && key < hi;    // (also where its weight is zero: 0 x NaN is NaN, as in the products)
                 const size_t vrow = ((size_t)p.block_table[(size_t)it.trow * p.max_blocks + (key >> p.bs_log2)] * p.Hkv + it.kvh) * p.bs + (key & (p.bs - 1));
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {

@@ -40,6 +40,43 @@ def test_an_error_of_another_kernel_changes_no_result(code):
     close(got[2], want[-5:], bound[-5:])
 
 
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("masked", [False, True])
+def test_values_that_are_not_finite_under_weights_of_zero(splits, masked):
+    """0 x NaN is NaN, in a masked tile as in a whole one: rows that see the key, and no others."""
+    def poke(seqs):
+        k, v = seqs[0]
+        k[:, :, 0] = 0                                     # scores of three keys lie 300 x 8 / sqrt(128) under what they would be: weights below 2^-250
+        k[[20, 150, 290], :, 0] = -300
+        v[20, :, 3] = NAN                                  # a whole tile of causal rows
+        v[150, :, 5] = NAN
+        v[290, 0, 7] = NAN                                 # the last tile, masked in any case
+
+    def spans(i, n, kv):
+        if not masked:
+            return None
+        lo = torch.zeros(n, dtype=torch.long)
+        lo[::3] = 140
+        lo[1::3] = 295
+        return lo, torch.arange(kv - n, kv) + 1
+
+    import test_spans_gpu
+    made = test_spans_gpu.rand
+
+    def eights(*shape, scale=1.0):                         # queries with 8 in the first place
+        x = made(*shape, scale=scale)
+        if len(shape) == 3 and shape[1] == 4:
+            x[..., 0] = 8
+        return x
+    test_spans_gpu.rand = eights
+    try:
+        run_spans([(40, 300)], 4, 2, 64, spans, splits=splits)
+        out = run_spans([(40, 300)], 4, 2, 64, spans, splits=splits, poke=poke)
+    finally:
+        test_spans_gpu.rand = made
+    assert out.isnan().any() and not out.isnan().all()
+
+
 def test_scales_and_caps_that_32_bits_do_not_hold_are_refused():
     _, a = _modules()
     k, v = rand(40, 2, 128), rand(40, 2, 128)
