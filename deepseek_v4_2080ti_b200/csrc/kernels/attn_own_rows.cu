@@ -302,10 +302,11 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
       float M = fmaxf(mw[h], fmaxf(ml[h][0].x, ml[h][1].x));
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-      // (a sum of zero weighs nothing: what lies beside it may not have been written)
-      const float fw = lw[h] == 0.f ? 0.f : exp2f(mw[h] - M);
-      ml[h][0].x = ml[h][0].y == 0.f ? 0.f : exp2f(ml[h][0].x - M);
-      ml[h][1].x = ml[h][1].y == 0.f ? 0.f : exp2f(ml[h][1].x - M);
+      // (-1 beside a sum of zero: nothing was seen, and what lies there may not have been written.  A weight that has become zero is
+      // another thing: zero times a NaN that was seen is NaN.)
+      const float fw = lw[h] == 0.f ? -1.f : exp2f(mw[h] - M);
+      ml[h][0].x = ml[h][0].y == 0.f ? -1.f : exp2f(ml[h][0].x - M);
+      ml[h][1].x = ml[h][1].y == 0.f ? -1.f : exp2f(ml[h][1].x - M);
       float L = fw * lw[h] + ml[h][0].x * ml[h][0].y + ml[h][1].x * ml[h][1].y;
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
@@ -317,7 +318,7 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
 #pragma unroll
     for (int h = 0; h < 4; ++h)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) a[h][y] = f_own[h] == 0.f ? 0.f : f_own[h] * s_o[warp][i + h][pos + 8 * y];
+      for (int y = 0; y < 4; ++y) a[h][y] = f_own[h] < 0.f ? 0.f : f_own[h] * s_o[warp][i + h][pos + 8 * y];
 #pragma unroll 2
     for (int sl = W; sl < slots; sl += n_warps) {
       float4 x[4];
@@ -327,7 +328,7 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const float f = __shfl_sync(0xffffffffu, sl < 32 ? ml[h][0].x : ml[h][1].x, sl & 31);
-        if (f == 0.f) continue;                          // (nothing seen, or no such slot: what lies there is not looked at)
+        if (f < 0.f) continue;                           // (nothing seen, or no such slot: what lies there is not looked at)
         a[h][0] += f * x[h].x; a[h][1] += f * x[h].y; a[h][2] += f * x[h].z; a[h][3] += f * x[h].w;
       }
     }

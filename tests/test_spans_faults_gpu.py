@@ -77,6 +77,31 @@ def test_values_that_are_not_finite_under_weights_of_zero(splits, masked):
     assert out.isnan().any() and not out.isnan().all()
 
 
+@pytest.mark.parametrize("where", ["shared", "own"])
+@pytest.mark.parametrize("hq,splits", [(4, 2), (4, 1), (24, 2)])
+def test_a_part_of_the_keys_that_weighs_nothing_keeps_its_nan(where, hq, splits):
+    """A sequence's parts - items of the shared keys, warps of its own - are joined by the formula also where one weighs 2^-250: 0 x NaN is NaN."""
+    lib, a = _modules()
+    torch.manual_seed(16)
+    n, common, hkv, bs = 256 + 64, 256, 2, 64
+    k, v = rand(n, hkv, 128), rand(n, hkv, 128)
+    k[..., 0] = 0
+    low, bad = (slice(0, 256), 130) if where == "shared" else (slice(256 + 16, 256 + 32), 256 + 20)
+    k[low, :, 0] = -300                                    # every key of the part
+    v[bad, :, 9] = NAN
+    kc, vc, table = pages([(k, v)], bs)
+    q = rand(3, hq, 128)
+    q[..., 0] = 8
+    lens = [n, n - 3, n - 12]
+    args = kc, vc, table.repeat(3, 1), _i32(lens), _i32([0, 3]), _i32([common])
+    out = a.decode_shared(q, *args, splits=splits)
+    torch.cuda.synchronize()
+    lib.check_status()
+    want, bound = oracle(q, k, v, _i32([0, 0, 0]), _i32(lens), SCALE)
+    assert want[..., 9].isnan().all() and want.isnan().sum() == 3 * hq
+    close(out, want, bound)
+
+
 def test_scales_and_caps_that_32_bits_do_not_hold_are_refused():
     _, a = _modules()
     k, v = rand(40, 2, 128), rand(40, 2, 128)
