@@ -132,23 +132,24 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
   for (int i = 0; i < NB; ++i) m[i][0] = m[i][1] = -INFINITY, l[i][0] = l[i][1] = 0.f;
 
   // keys of block n: rows g and g + 8; values: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9, dims 8 g and 64 + 8 g.  Rows that do not count are
-  // zero: a product of zero with what they may hold would not be.
+  // zero: a product of zero with what they may hold would not be.  A page that is not there reads as zeros, as it does in attn_spans.cu.
   const uint4 zero = make_uint4(0, 0, 0, 0);
   uint4 k[2][4], v[4][2];
   auto row_of = [&](int blk) {
     const int key = (first + blk) << 4, page = bt[key >> p.bs_log2];
     return (unsigned)page < (unsigned)p.num_blocks ? ((size_t)page * p.Hkv + kvh) * p.bs + (key & (p.bs - 1)) : ~(size_t)0;
   };
-  auto counts = [&](int blk, int i, size_t row) {
+  auto counts = [&](int blk, int i) {
     const int key = ((first + blk) << 4) + i;
-    return blk < n_blk && row != ~(size_t)0 && key >= shared && key < kv;
+    return blk < n_blk && key >= shared && key < kv;
   };
+  auto there = [&](int blk, int i, size_t row) { return row != ~(size_t)0 && counts(blk, i); };
   auto load_k = [&](int blk, size_t row) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int d = 0; d < 4; ++d)
-        k[i][d] = counts(blk, g + 8 * i, row) ? *reinterpret_cast<const uint4*>(p.k_cache + (row + g + 8 * i) * D + d * 32 + c * 8) : zero;
+        k[i][d] = there(blk, g + 8 * i, row) ? *reinterpret_cast<const uint4*>(p.k_cache + (row + g + 8 * i) * D + d * 32 + c * 8) : zero;
   };
   auto load_v = [&](int blk, size_t row) {
 #pragma unroll
@@ -156,7 +157,7 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
       const int key = 2 * c + (i & 1) + (i >> 1) * 8;
 #pragma unroll
       for (int d = 0; d < 2; ++d)
-        v[i][d] = counts(blk, key, row) ? *reinterpret_cast<const uint4*>(p.v_cache + (row + key) * D + d * 64 + g * 8) : zero;
+        v[i][d] = there(blk, key, row) ? *reinterpret_cast<const uint4*>(p.v_cache + (row + key) * D + d * 64 + g * 8) : zero;
     }
   };
   const int step = WARPS * p.cluster;
@@ -165,7 +166,7 @@ own_rows_kernel(const __grid_constant__ OwnParams p) {
   load_k(blk, row);
   load_v(blk, row);
   for (; blk < n_blk; blk += step) {
-    const bool ok0 = counts(blk, g, row), ok1 = counts(blk, g + 8, row);
+    const bool ok0 = counts(blk, g), ok1 = counts(blk, g + 8);
     float s[NB][4];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {

@@ -422,8 +422,9 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
 
     q: [T, Hq, 128]; block_table [B, max_blocks], q_start / q_len / kv_len [B], lo / hi [T]: int32 device tensors.  Rows of no
     sequence are not written (``out``: where to write, ``q`` itself if it is not needed any more).  Entries of ``block_table`` for
-    pages that no row sees are not followed.  ``max_q_len`` (host) is at least the longest of ``q_len``; ``max_kv_len`` bounds the
-    contexts, for the choice of ``splits`` (items a row's keys are cut into).
+    pages that no row sees are not followed; a page outside the cache that a row does see reads as keys and values of zero.
+    ``max_q_len`` (host) is at least the longest of ``q_len``; ``max_kv_len`` bounds the contexts, for the choice of ``splits`` (items
+    a row's keys are cut into).
     """
     dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
     if _current() != dev:
@@ -500,7 +501,7 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     group_start[g] .. group_start[g + 1] - 1 of ``block_table`` begin with the same pages, whose first shared_len[g] keys they have
     in common (keys at ``kv_len`` and beyond stay unseen); rows of no group are on their own.  ``cap`` as in ``prefill_spans``;
     ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys); a sequence with ``kv_len`` 0
-    gives 0."""
+    gives 0.  Pages outside the cache as in ``prefill_spans``."""
     dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
     if _current() != dev:
         with torch.cuda.device(dev):

@@ -40,6 +40,33 @@ def test_an_error_of_another_kernel_changes_no_result(code):
     close(got[2], want[-5:], bound[-5:])
 
 
+@pytest.mark.parametrize("bad", [-1, 1 << 20])
+@pytest.mark.parametrize("shared", [0, 192])
+@pytest.mark.parametrize("cap", [0.0, 6.0])
+def test_pages_that_are_not_there_read_as_zeros(bad, shared, cap):
+    """A page outside the cache among the keys that a row sees: keys and values of zero, in every call alike."""
+    lib, a = _modules()
+    torch.manual_seed(12)
+    n, hq, hkv, bs = 500, 6, 2, 64
+    k, v = rand(n, hkv, 128), rand(n, hkv, 128)
+    kc, vc, table = pages([(k, v)], bs)
+    for page in (1, 4, 7):                                 # one that may be shared, one of its own, the last
+        table[0, page] = bad
+        k[page * bs:(page + 1) * bs] = 0
+        v[page * bs:(page + 1) * bs] = 0
+    lens = [n, n - 1, n - 77]
+    q = rand(3, hq, 128)
+    zero = _i32([0, 0, 0])
+    want, bound = oracle(q, k, v, zero, _i32(lens), SCALE, cap)
+    out = a.decode_shared(q, kc, vc, table.repeat(3, 1), _i32(lens), _i32([0, 3]), _i32([shared]), cap=cap)
+    rows = a.prefill_spans(q, kc, vc, table, _i32([0]), _i32([3]), _i32([n]), 3, zero, _i32(lens), cap=cap)
+    alone = a.decode_shared(q, kc, vc, table.repeat(3, 1), _i32(lens), _i32([0]), _i32([]), cap=cap)
+    torch.cuda.synchronize()
+    lib.check_status()
+    for got in (rows, out, alone):
+        close(got, want, bound)
+
+
 @pytest.mark.parametrize("splits", [1, 2])
 @pytest.mark.parametrize("masked", [False, True])
 def test_values_that_are_not_finite_under_weights_of_zero(splits, masked):
