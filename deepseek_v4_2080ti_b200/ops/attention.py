@@ -412,6 +412,34 @@ def visible_spans(kv_len: int, documents=None, blocks=(), window: int = 0) -> tu
     return lo.to(torch.int32), hi.to(torch.int32)
 
 
+def _seen_pages(t, width, bs, kv_len, q_start, q_len, lo, hi):
+    """bool [B, width]: pages with a key that some row of the sequence sees (arguments as in ``prefill_spans``)."""
+    row = torch.arange(t, device=kv_len.device)
+    kv, first, n = (x.long()[:, None] for x in (kv_len, q_start, q_len))
+    begin = torch.zeros_like(row) if lo is None else lo.long().clamp(min=0)
+    end = torch.minimum(row - first + kv - n + 1 if hi is None else hi.long(), kv.clamp(max=width * bs))
+    seen = ((first >= 0) & (row >= first) & (row < first + n) & (begin < end)).long()        # [B, T]
+    edge = torch.zeros(kv.shape[0], width + 1, dtype=torch.long, device=row.device)
+    edge.scatter_add_(1, (begin // bs).clamp(max=width).expand_as(seen), seen)
+    edge.scatter_add_(1, ((end - 1) // bs + 1).clamp(0, width), -seen)
+    return edge[:, :width].cumsum(1) > 0
+
+
+def _check_pages(block_table, nb, bs, kv_len, rows=None) -> None:
+    """Debug mode: -1 stands for a page that is not there, which only keys that no row sees may lie in.  ``rows``: T, q_start, q_len, lo, hi
+    of prompt rows, else every key of a sequence is seen."""
+    if not _lib.bounds_checks_on():
+        return
+    width = block_table.shape[1]
+    if rows is None:
+        seen = torch.arange(width, device=kv_len.device) * bs < kv_len[:, None]
+    else:
+        t, q_start, q_len, lo, hi = rows
+        seen = _seen_pages(t, width, bs, kv_len, q_start, q_len, lo, hi)
+    block_table.masked_fill_(seen & (block_table == -1), -2)
+    _lib.check_indices(block_table, 0, nb, 3, keep=-1)
+
+
 def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_q_len, lo=None, hi=None, gate=None, scale=None,
                   cap: float = 0.0, max_kv_len: int | None = None, splits: int | None = None, out=None):
     """Attention of new rows against the paged cache (which already holds their keys and values), every row over a span of keys
@@ -447,7 +475,7 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
     if not 1 <= splits <= 1024:
         raise ValueError(f"{splits} splits")
     ws = q.new_empty(splits * t * hq * (D + 2), dtype=_F32) if splits > 1 else None
-    _lib.check_indices(block_table, 0, nb, 3, keep=-1)
+    _check_pages(block_table, nb, bs, kv_len, (t, q_start, q_len, lo, hi))
     rc = _kernels().b200_attn_spans(_SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
         q_start.data_ptr(), q_len.data_ptr(), _at(lo), _at(hi), 0, 0, _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq, hkv,
@@ -527,7 +555,7 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     while cluster < 8 and cluster * blocks <= NUM_SMS and own_keys > 256 * cluster:
         cluster *= 2
     lib = _kernels()
-    _lib.check_indices(block_table, 0, nb, 3, keep=-1)
+    _check_pages(block_table, nb, bs, kv_len)
     ws = q.new_empty(splits * b * hq * (D + 2), dtype=_F32) if n else None
     call = _SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),

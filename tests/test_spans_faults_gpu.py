@@ -129,6 +129,40 @@ def test_a_part_of_the_keys_that_weighs_nothing_keeps_its_nan(where, hq, splits)
     close(out, want, bound)
 
 
+def test_debug_mode_reports_missing_pages_that_a_row_sees(monkeypatch):
+    """-1 stands for a page that is not there: allowed where no row looks, reported where one does, with its place in the table."""
+    lib, a = _modules()
+    monkeypatch.setenv("B200_BOUNDS_CHECK", "1")
+    torch.manual_seed(13)
+    n, new, hq, hkv, bs = 700, 30, 4, 2, 64
+    k, v = rand(n, hkv, 128), rand(n, hkv, 128)
+    kc, vc, table = pages([(k, v)], bs, table_width=14)
+    q = rand(new, hq, 128)
+    lo, hi = (x[n - new:].to(DEV) for x in a.visible_spans(n, window=200))
+    args = _i32([0]), _i32([new]), _i32([n]), new
+    unseen = list(range((n - new - 199) // bs)) + [11, 12, 13]
+    for page in range(14):
+        odd = table.clone()
+        odd[0, page] = -1
+        a.prefill_spans(q, kc, vc, odd, *args, lo, hi)
+        if page in unseen:
+            lib.check_status()
+        else:
+            with pytest.raises(lib.KernelError, match=f"page table at element {page} "):
+                lib.check_status()
+        odd = table.repeat(2, 1)
+        odd[1, page] = -1
+        kv = [n, 5 * bs + 1]
+        got = a.decode_shared(q[:2].contiguous(), kc, vc, odd, _i32(kv), _i32([0, 2]), _i32([128]))
+        if page > 5:
+            lib.check_status()
+            close(got, *oracle(q[:2], k, v, _i32([0, 0]), _i32(kv), SCALE))
+        else:
+            with pytest.raises(lib.KernelError, match=f"page table at element {14 + page} "):
+                lib.check_status()
+    lib.check_status()
+
+
 def test_scales_and_caps_that_32_bits_do_not_hold_are_refused():
     _, a = _modules()
     k, v = rand(40, 2, 128), rand(40, 2, 128)

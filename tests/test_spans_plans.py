@@ -40,6 +40,30 @@ def test_scales_and_caps_that_32_bits_do_not_hold():
             attention._scores(scale, cap)
 
 
+def test_pages_that_a_row_sees():
+    rng = random.Random(2)
+    for trial in range(60):
+        bs, width, b = rng.choice((16, 32)), rng.randint(1, 6), rng.randint(1, 4)
+        q_len = [rng.randint(0, 9) for _ in range(b)]
+        q_start, t = [], rng.randint(0, 3)
+        for n in q_len:
+            q_start.append(t)
+            t += n + rng.randint(0, 2)
+        kv = [rng.randint(0, width * bs + 20) for _ in range(b)]
+        lo = [rng.randint(-5, width * bs + 5) for _ in range(t)] if trial % 3 else None
+        hi = [rng.choice((rng.randint(-5, width * bs + 50), 2 ** 31 - 1, -2 ** 31)) for _ in range(t)] if trial % 2 else None
+        want = [[False] * width for _ in range(b)]
+        for i in range(b):
+            for r in range(q_start[i], q_start[i] + q_len[i]):
+                first = max(0, lo[r]) if lo else 0
+                end = hi[r] if hi else kv[i] - q_len[i] + r - q_start[i] + 1
+                for j in range(first, min(end, kv[i], width * bs)):
+                    want[i][j // bs] = True
+        ints = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32)
+        got = attention._seen_pages(t, width, bs, ints(kv), ints(q_start), ints(q_len), ints(lo), ints(hi))
+        assert got.tolist() == want
+
+
 def test_the_module_loads_where_torch_has_no_cuda():
     """The host reference runtime takes its fp32 oracles from this module; a torch built without CUDA lacks these entry points."""
     code = ("import torch\n"
