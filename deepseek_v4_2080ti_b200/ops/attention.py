@@ -485,19 +485,34 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
 
 
 def shared_groups(pages, block_size: int) -> tuple[list[int], list[int]]:
-    """``group_start``, ``shared_len`` for ``decode_shared`` from the page lists of the sequences, in batch order: neighbours with the
-    same first page form a group, which shares their common leading pages (a sequence alone shares nothing)."""
-    start, shared, b = [0], [], 0
+    """``group_start``, ``shared_len`` for ``decode_shared`` from the page lists of the sequences, in batch order: runs of neighbours that
+    share their common leading pages (a sequence alone shares nothing), cut where that saves the most reads of pages - documents behind one
+    system page are groups of their own, the page alone is shared where there is no more."""
     pages = [[int(x) for x in row] for row in pages]
-    while b < len(pages):
-        e, n = b + 1, len(pages[b])
-        while e < len(pages) and n and pages[e][:1] == pages[b][:1]:
-            n = next((i for i, (x, y) in enumerate(zip(pages[b][:n], pages[e])) if x != y), min(n, len(pages[e])))
-            e += 1
-        start.append(e)
-        shared.append(n * block_size if e - b > 1 else 0)
-        b = e
-    return start, shared
+    common = [next((i for i, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b))) for a, b in zip(pages, pages[1:])]   # of neighbours
+    # Cuts to consider: where neighbours share equally much several times in a row, the first and the last of them (one in between can move to an
+    # end and lose nothing).
+    at = [0] + [b for b in range(1, len(pages)) if b in (1, len(pages) - 1) or common[b - 2] != common[b - 1] or common[b] != common[b - 1]] + [len(pages)]
+    least = [min(common[a:b - 1], default=math.inf) for a, b in zip(at, at[1:])]              # within the stretches between them
+    best = [(0, 0, 0)]                                     # of the sequences up to a cut: pages saved, the last group's cut, what it shares
+    for e in range(1, len(at)):
+        top, n = (-1, 0, 0), math.inf
+        for b in range(e - 1, -1, -1):
+            n = min(n, least[b], common[at[b + 1] - 1] if b + 1 < e else math.inf)
+            if n == 0 and top[0] >= 0:                     # nothing in common from here on
+                break
+            saved, shares = (best[b][0] + (at[e] - 1 - at[b]) * n, n) if at[e] - at[b] > 1 else (best[b][0], 0)
+            if saved >= top[0]:                            # (of equals, the fewest groups)
+                top = (saved, b, shares)
+        best.append(top)
+    start, shared, e = [len(pages)], [], len(at) - 1
+    while e > 0 and pages:
+        _, b, n = best[e]
+        firsts = [at[b]] if n else range(at[e] - 1, at[b] - 1, -1)
+        start += firsts
+        shared += [n * block_size] * len(firsts)
+        e = b
+    return start[::-1], shared[::-1]
 
 
 def _shared_splits(rows: int, groups: int, g: int, hkv: int, tiles: int, own_keys: int) -> int:

@@ -30,6 +30,56 @@ def test_blocks_stay_in_their_document():
     assert attention.visible_spans(7, [0, 7, 0], blocks=[(1, 7)])[1].tolist() == [1, 7, 7, 7, 7, 7, 7]
 
 
+def _saved(pages, start, shared, block_size):
+    """Pages that need not be read again, after a look at the plan itself."""
+    assert start[0] == 0 and start[-1] == len(pages) and len(shared) == len(start) - 1 and all(a < b for a, b in zip(start, start[1:]))
+    saved = 0
+    for a, b, n in zip(start, start[1:], shared):
+        assert n % block_size == 0 and (b - a > 1 or n == 0)
+        n //= block_size
+        assert all(row[:n] == pages[a][:n] and len(row) >= n for row in pages[a:b])
+        saved += (b - a - 1) * n
+    return saved
+
+
+def _best(pages):
+    """The most that any cut of the sequences into runs of neighbours saves: all cuts, one by one."""
+    n, best = len(pages), 0
+    for cuts in range(1 << max(0, n - 1)):
+        edges = [0] + [i + 1 for i in range(n - 1) if cuts >> i & 1] + [n]
+        total = 0
+        for a, b in zip(edges, edges[1:]):
+            common = 0
+            while all(len(row) > common and row[common] == pages[a][common] for row in pages[a:b]):
+                common += 1
+            total += (b - a - 1) * common
+        best = max(best, total)
+    return best
+
+
+def test_a_system_page_before_several_documents():
+    a, b = [9] + list(range(100, 120)), [9] + list(range(200, 220))
+    assert attention.shared_groups([a + [i] for i in range(4)] + [b + [10 + i] for i in range(4)], 64) == ([0, 4, 8], [21 * 64] * 2)
+    for at in (0, 3, 6):                                   # one that has nothing but the first page in common
+        rows = [a + [i] for i in range(6)]
+        rows.insert(at, [9, 5000])
+        start, shared = attention.shared_groups(rows, 16)
+        assert _saved(rows, start, shared, 16) == _best(rows)
+    assert attention.shared_groups([[9, i] for i in range(5)], 32) == ([0, 5], [32])         # the page alone is still shared
+    assert attention.shared_groups([[i] for i in range(4)] + [[], []], 32) == ([0, 1, 2, 3, 4, 5, 6], [0] * 6)
+
+
+def test_groups_save_the_most():
+    rng = random.Random(1)
+    for trial in range(150):
+        n = rng.randint(1, 9)
+        pages = [[rng.randint(0, 1) * 10 ** i for i in range(rng.randint(0, 7))] for _ in range(n)]
+        if trial % 2:
+            pages.sort()
+        start, shared = attention.shared_groups(pages, 16)
+        assert _saved(pages, start, shared, 16) == _best(pages), pages
+
+
 def test_scales_and_caps_that_32_bits_do_not_hold():
     """A cap that becomes zero in 32 bits would be none at all, one beyond them infinite."""
     for scale, cap in ((None, 0.0), (0.1, 30.0), (1.0, 1e-6), (0.0884, 1e9), (2.0 ** -100, 0.0), (2.0 ** 100, 1.0), (1.0, 2.0 ** 100)):
