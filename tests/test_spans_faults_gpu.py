@@ -163,6 +163,54 @@ def test_debug_mode_reports_missing_pages_that_a_row_sees(monkeypatch):
     lib.check_status()
 
 
+@pytest.mark.parametrize("kv", [1, 64, 65, 300])
+def test_debug_mode_decodes_tables_with_pages_that_are_not_there(monkeypatch, kv):
+    """Decoding rows over tables that end in -1, as a scheduler keeps them, against sums in 64 bits."""
+    lib, a = _modules()
+    monkeypatch.setenv("B200_BOUNDS_CHECK", "1")
+    torch.manual_seed(14)
+    hq, hkv, bs = 10, 2, 64
+    seqs = [(rand(n, hkv, 128), rand(n, hkv, 128)) for n in (kv, 200, 0)]
+    kc, vc, table = pages(seqs, bs, table_width=8)
+    for i, (k, _) in enumerate(seqs):
+        table[i, -(-k.shape[0] // bs):] = -1
+    before = table.clone()
+    q, gate = rand(3, hq, 128), rand(3, hq, 128)
+    for groups in ([0], [0, 2]):
+        out = a.decode_shared(q, kc, vc, table, _i32([kv, 200, 0]), _i32(groups), _i32([0] * (len(groups) - 1)), gate=gate)
+        lib.check_status()
+        assert torch.equal(table, before) and not out[2].any()
+        for i in range(2):
+            close(out[i:i + 1], *oracle(q[i:i + 1], *seqs[i], _i32([0]), _i32([seqs[i][0].shape[0]]), SCALE, gate=gate[i:i + 1]))
+
+
+@pytest.mark.parametrize("t", [1, 37, 300])
+def test_guard_bands_around_the_rows_and_gates_of_an_append(monkeypatch, t):
+    """Nothing is written beside the queries and gates that an append gives, nor beside the caches."""
+    from deepseek_v4_2080ti_b200.utils import canary
+    lib, a = _modules()
+    torch.manual_seed(15)
+    hq, hkv, bs, kept = 5, 1, 32, []
+
+    def guarded(x, *shape, **kw):
+        kept.append(canary.empty(*(shape or x.shape), dtype=x.dtype, device=x.device, name="rows"))
+        return kept[-1]
+    with canary.enabled(True):
+        monkeypatch.setattr(torch.Tensor, "new_empty", guarded)
+        monkeypatch.setattr(torch, "empty_like", guarded)
+        kc, vc = (canary.zeros(12, hkv, bs, 128, dtype=torch.bfloat16, device=DEV, name="cache") for _ in range(2))
+        src = rand(t, hq * 256 + 2 * hkv * 128)
+        q, gate = a.qk_norm_rope_axes_append(src, 0, 256, True, src, hq * 256, src, (2 * hq + hkv) * 128, None, None, True, 1e-6,
+                                             a.rope_inv_freq(32, 1e6, DEV), a.rotary_axes((6, 5, 5), True), _i32(torch.zeros(3, t)),
+                                             _i32(torch.randperm(12 * bs)[:t]), kc, vc, hq, hkv)
+        torch.cuda.synchronize()
+        monkeypatch.undo()
+        lib.check_status()
+        assert len(kept) == 2 and q is kept[0] and gate is kept[1]
+        assert torch.equal(gate, src[:, :hq * 256].view(t, hq, 256)[..., 128:])
+        canary.assert_clean()
+
+
 def test_scales_and_caps_that_32_bits_do_not_hold_are_refused():
     _, a = _modules()
     k, v = rand(40, 2, 128), rand(40, 2, 128)
