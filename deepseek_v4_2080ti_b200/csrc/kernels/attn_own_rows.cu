@@ -10,8 +10,10 @@
 //   O^T [16 dims x 8 heads] = V^T [dims x keys] P^T: a lane holds the same 8 dims of its four keys and pairs them up;
 //   P^T comes from the scores by an 8 x 8 transpose in registers.
 // Heads as the narrow side of the products keep O of a kv head in 32 registers, so that a warp has 16 KB of keys and values on their way
-// beside them.  64 sequences of 500 own keys, 8 kv heads (131 MB): 40 us behind the shared keys' kernel, 3.3 TB/s (5.9 in the loop; the rest is
-// the start of a block and the joins).  A warp takes 16 keys at a time (of one page: their
+// beside them.  64 sequences of 500 own keys, 8 kv heads (131 MB, 156 with the partial sums and what is read twice): 40 us behind the shared keys'
+// kernel, 3.3 TB/s of the needed bytes and 3.8 of those moved (5.9 in the loop; the rest is the start of a block and the joins).  Weights are
+// rounded to bf16 for the products (2^-8 of a weight at most), as they are for prompt rows; attn_gqa_decode.cu keeps them in 32 bits.
+// Sums and statistics are 32 bits wide, and the sum adds the weights before they are rounded.  A warp takes 16 keys at a time (of one page: their
 // page is looked up once), the warps of up to 8 blocks of a cluster share a sequence's keys, and the sums are joined in shared memory.
 // The first products do not wait for the kernel before (it writes only the partial sums).
 #include <cuda_bf16.h>

@@ -31,7 +31,8 @@
 // What bounds it (8192 causal rows of 40 heads over 8 kv heads, gated: 628 us, 1.1 PFLOP/s): 256 rows times 128 keys cost 2048
 // cycles of the tensor core and about 2100 of each scheduler's softmax warps, and take 3500 together, because a stream's scores,
 // weights and products follow each other through tensor memory and two streams do not hide all of that; an item's start and end
-// take another 10 %.  Packed documents of 4000 rows of 48 heads, capped: 116 us, half of it masked tiles (6000 cycles) and items' ends.
+// take another 10 %.  Packed documents of 4000 rows of 48 heads, capped: 116 us, a third of it the start and end of items, and of the
+// rest most masked tiles (6000 cycles).
 // Shared keys of 40 heads over 8, in one item a block: 64 rows over 32768 keys 44 us, 32 over 8192 15 us.  The smallest call, one
 // row over 121 keys, is a chain of 9 us: the item 3, page and tiles 3, softmax 4 and product 1 thousand cycles, the row's way out 4.
 #include <cuda_bf16.h>
@@ -804,8 +805,9 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             cap_c[0] = pack2(1.f, 1.f);
             cap_c[1] = cap_c[2] = cap_c[3] = 0;
           };
-          // What the weights of scores up to `top` are taken relative to: that score's own, so that the largest weight of a row, which
-          // often outweighs the others, is 1 and not rounded.
+          // What the weights of scores up to `top` are taken relative to: that score's own, so that its weight, which often outweighs the
+          // others, is 1 and not rounded.  (Scores that are larger by less than 2^8 do not move the maximum: their weights are up to 2^8 and
+          // rounded like the others.)
           auto level = [&](float top) { return scale * (CAP ? score_cap(top, p.cap_in) : top); };
           // The running maximum up to that of new scores, where it is far enough behind; false: the product that last added to O has not
           // finished in time.  The tile before's has, as it was issued before the scores that arrived; `half`: the first half's may be on its way.

@@ -170,7 +170,9 @@ extern "C" int b200_qk_norm_rope_axes_append(const AxesAppendCall* call) {
   p.bs = a.block_size; p.n_slots = (unsigned)a.num_blocks * a.block_size;
   p.T = a.T; p.Hq = a.Hq; p.Hkv = a.Hkv;
   const int heads = a.Hq + 2 * a.Hkv;
-  // few tokens: a row per warp, so that the SMs share a token's heads (37 tokens of 64 rows: 2.8 us; with the other form 8.0)
+  // few tokens: a row per warp, so that the SMs share a token's heads (37 tokens of 64 rows: 2.2 us, with the other form 4.7; of 36 rows 2.7 / 3.5).
+  // The two cross further out than the rule: 64 rows and 64 / 128 / 256 / 512 tokens 3.3 / 4.5 / 6.9 / 11.8 us, with the other form 4.8 / 6.4 /
+  // 8.3 / 9.2; 36 rows and 128 / 256 / 512 tokens 3.3 / 4.8 / 7.8 and 4.4 / 6.0 / 6.6.
   const bool few = (long long)a.T * heads <= 148 * 2 * WARPS;
   p.block_rows = few ? WARPS : heads;
   const dim3 grid(a.T, (heads + p.block_rows - 1) / p.block_rows), block(WARPS * 32);

@@ -543,8 +543,10 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     q: [B, Hq, 128]; group_start int32 [groups + 1], shared_len int32 [groups] (device; ``shared_groups``): the rows
     group_start[g] .. group_start[g + 1] - 1 of ``block_table`` begin with the same pages, whose first shared_len[g] keys they have
     in common (keys at ``kv_len`` and beyond stay unseen); rows of no group are on their own.  ``cap`` as in ``prefill_spans``;
-    ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys); a sequence with ``kv_len`` 0
-    gives 0.  Pages outside the cache as in ``prefill_spans``."""
+    ``max_shared`` / ``max_kv_len`` bound the lengths, for the choice of ``splits`` (of the shared keys) and of the blocks that share a
+    sequence's own keys, by their difference: own keys far beyond it (of a row in no group, or without ``max_shared``) are right, but one
+    block's work for each kv head.  A sequence with ``kv_len`` 0 gives 0.  Pages outside the cache as in ``prefill_spans``.  The weights of
+    the softmax are rounded to bf16, as in ``prefill``; ``decode`` keeps them in 32 bits."""
     dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
     if _current() != dev:
         with torch.cuda.device(dev):
