@@ -2,10 +2,11 @@
 //
 //   s_ij = scale q_i . k_j, with a cap c > 0: s = c tanh(s / c); o_i = sum_j softmax_j(s_ij) v_j over lo_i <= j < hi_i
 //
-// in two forms over one kernel: prompt rows (b200_attn_spans: packed documents, prefixes, blocks of an image that see each
-// other, windows, causal rows after a context) and one row per sequence where groups of sequences hold the same leading pages
-// (b200_attn_shared: those keys are read and multiplied once for the whole group).  A row that sees nothing is zero; a masked
-// key takes no part whatever its bits are.
+// in three forms over one kernel: prompt rows (b200_attn_spans: packed documents, prefixes, blocks of an image that see each
+// other, windows, causal rows after a context), one row per sequence where groups of sequences hold the same leading pages
+// (b200_attn_shared: those keys are read and multiplied once for the whole group) and the rows of a drafted tree (b200_attn_tree: the
+// context, and of the tree's own keys, the last of the sequence, those whose bit is set in the row's mask).  A row that sees nothing is
+// zero; a masked key takes no part whatever its bits are.
 //
 // Work is a list of items, a block of the launch each: as many as there are SMs run, and one that is ready for more cancels a block that
 // has not begun and takes its item (cluster launch control; against a fixed deal 16 ragged portions take 126 us instead of 163, 8192 causal
@@ -70,6 +71,8 @@ struct Params {
   const int* q_len;               // [B]
   const int* lo;                  // optional [T]
   const int* hi;                  // optional [T]
+  const uint32_t* tree;           // rows of a tree: [T, tree_words], bit i: node i is seen
+  int tree_words;
   // one row per sequence
   const int* group_start;         // [n_groups + 1]
   const int* shared_len;          // [n_groups]
@@ -215,31 +218,41 @@ struct Item {
   int lo_max, hi_min;    // keys in [lo_max, hi_min) are seen by every row
   int k_end;             // first key that no row sees
   int kv_end;            // keys of the sequence
-  int own_hi;            // shared keys: end of the rows' span
+  int own_hi;            // shared keys: end of the rows' span; trees: position of node 0
   int delta;             // position of a token minus its q row (prompt rows)
   int tok0, tok1;        // tokens of the rows
   __device__ __forceinline__ bool dual() const { return n_rows <= BQ; }
   __device__ __forceinline__ int steps() const { return dual() ? t1 - t0 : 2 * (t1 - t0); }
 };
 
-template <bool SHARED>
+enum Form { SPANS, SHARED_KEYS, TREE_ROWS };
+
+template <Form FORM>
 __device__ __forceinline__ void span_of(const Params& p, const Item& it, int tok, int& lo, int& hi) {
-  if (SHARED) {
+  if (FORM == SHARED_KEYS) {
     lo = 0;
     hi = max(0, min(it.own_hi, min(p.kv_len[tok], p.max_blocks * p.bs)));
   } else {
     lo = p.lo ? max(0, p.lo[tok]) : 0;
-    hi = max(0, min(p.hi ? p.hi[tok] : tok + it.delta + 1, it.kv_end));    // (differences of these fit 32 bits)
+    hi = FORM == TREE_ROWS ? it.kv_end : max(0, min(p.hi ? p.hi[tok] : tok + it.delta + 1, it.kv_end));    // (differences of these fit 32 bits)
   }
 }
 
 // Item `idx` of the list; false: there is nothing to do.  Called by whole warps.
-template <bool SHARED>
+// Which of the 32 keys from `key` on a tree's row sees by its mask, node 0 lying at position `first`: all in the context.
+__device__ __forceinline__ uint32_t tree_bits(const uint32_t* words, int n_words, int key, int first) {
+  const int at = key - first;
+  if (at <= -32) return 0xffffffffu;
+  auto word = [&](int i) { return i >= 0 && i < n_words ? words[i] : i < 0 ? 0xffffffffu : 0u; };
+  return __funnelshift_r(word(at >> 5), word((at >> 5) + 1), at & 31);
+}
+
+template <Form FORM>
 __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Item& it) {
   it.n_rows = 0;
   int split, splits;
   int rows_all;
-  if (SHARED) {
+  if (FORM == SHARED_KEYS) {
     // A group's rows are whole tiles and a rest; a rest of at most 128 rows takes half the time per key (both streams work on it), so its
     // keys are cut into half as many items.
     const int few = (p.splits + 1) / 2;
@@ -340,7 +353,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
     it.base_tok = q0;
     it.kv_end = max(0, min(kv, p.max_blocks * p.bs));
     it.delta = kv - n - q0;
-    it.own_hi = 0;
+    it.own_hi = kv - n;
   }
   it.n_rows = min(2 * BQ, rows_all - it.r0);
   if (it.n_rows <= 0) return false;
@@ -350,7 +363,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
   int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = 0;
   for (int t = tok0 + lane; t <= tok1; t += 32) {
     int lo, hi;
-    span_of<SHARED>(p, it, t, lo, hi);
+    span_of<FORM>(p, it, t, lo, hi);
     lo_max = max(lo_max, lo);
     hi_min = min(hi_min, hi);
     if (lo < hi) {
@@ -361,6 +374,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
   lo_min = __reduce_min_sync(0xffffffffu, lo_min);
   it.lo_max = __reduce_max_sync(0xffffffffu, lo_max);
   it.hi_min = __reduce_min_sync(0xffffffffu, hi_min);
+  if (FORM == TREE_ROWS) it.hi_min = min(it.hi_min, it.own_hi);            // (of the tree's keys every row sees its own)
   it.k_end = __reduce_max_sync(0xffffffffu, hi_max);
   it.t0 = it.t1 = 0;
   if (it.k_end > lo_min) {
@@ -395,7 +409,7 @@ struct Ring {
   }
 };
 
-template <bool SHARED, bool CAP>
+template <Form FORM, bool CAP>
 __global__ void __launch_bounds__(NTHREADS, 1)
 spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_base[];
@@ -524,7 +538,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         return true;
       };
       while (idx >= 0) {
-        if (get_item<SHARED>(p, idx, lane, it)) {
+        if (get_item<FORM>(p, idx, lane, it)) {
         const int* bt = p.block_table + (size_t)it.trow * p.max_blocks;
         const int last_page = (it.k_end - 1) >> p.bs_log2;
         auto page_row = [&](int tile) {                                    // cache row where this lane's part of a tile begins
@@ -711,7 +725,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       const int tok = it.base_tok + (int)rt;
       const uint32_t at = (uint32_t)tok * p.Hq + it.kvh * p.G + (rr - rt * p.G);         // row of q and out
       int lo, hi;
-      span_of<SHARED>(p, it, tok, lo, hi);
+      span_of<FORM>(p, it, tok, lo, hi);
       float m_run = -INFINITY, l_run = 0.f;
       const int my_steps = (steps - m + 1) / 2;
       if (my_steps > 0) {
@@ -743,10 +757,18 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       }
       for (int j = 0; j < my_steps; ++j) {
         const int t = dual ? 2 * j + m : j;                // tile of the item
-        if (!(alive = warp_wait(&s_full[m], ph_s) && !*abort_flag)) break;
-        ph_s ^= 1;
         const int key0 = (it.t0 + t) * BKV;
         const bool edge = key0 < it.lo_max || key0 + BKV > it.hi_min;
+        uint32_t in_tree[4];                               // keys of the tile that a tree's row sees (on their way while the scores are)
+        if (FORM == TREE_ROWS && edge)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int x = min(32, max(0, lo - key0 - c * 32)), y = min(32, max(0, hi - key0 - c * 32));
+            in_tree[c] = tree_bits(p.tree + (size_t)tok * p.tree_words, p.tree_words, key0 + c * 32, it.own_hi) & (uint32_t)((1ull << y) - 1) &
+                         ~(uint32_t)((1ull << x) - 1);
+          }
+        if (!(alive = warp_wait(&s_full[m], ph_s) && !*abort_flag)) break;
+        ph_s ^= 1;
         if (warp_on) {
           tc_fence_after();
           // The tile's scores in halves of 64, each a step of the online softmax.
@@ -914,19 +936,25 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             auto sees = [&](int h, int& a, int& b) {       // keys [a, b) of the half's 64
               a = lo - key0 - h * 64;
               b = hi - key0 - h * 64;
+              if (FORM == TREE_ROWS) return (bool)__any_sync(0xffffffffu, (h ? in_tree[2] | in_tree[3] : in_tree[0] | in_tree[1]) != 0);
               return (bool)__any_sync(0xffffffffu, max(a, 0) < min(b, 64));
             };
             uint32_t seen[2];
-            auto bits = [&](int a, int b) {
+            auto bits = [&](int h, int a, int b) {
+              if (FORM == TREE_ROWS) {
+                seen[0] = h ? in_tree[2] : in_tree[0];
+                seen[1] = h ? in_tree[3] : in_tree[1];
+                return;
+              }
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 const int x = min(32, max(0, a - c * 32)), y = min(32, max(0, b - c * 32));
                 seen[c] = (uint32_t)((1ull << y) - 1) & ~(uint32_t)((1ull << x) - 1);
               }
             };
-            auto mask = [&](int a, int b) {
-              if (__all_sync(0xffffffffu, a <= 0 && b >= 64)) return;
-              bits(a, b);
+            auto mask = [&](int h, int a, int b) {
+              if (FORM != TREE_ROWS && __all_sync(0xffffffffu, a <= 0 && b >= 64)) return;
+              bits(h, a, b);
 #pragma unroll
               for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -940,11 +968,12 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
               if (!sees(h, a, b)) continue;
               load(h, sv);
               tmem_ld_wait();
-              mask(a, b);
+              mask(h, a, b);
               const float x = max_of(sv);
               m_edge = max3(m_edge, x, x);
             }
-            raise(max(lo, key0) < min(hi, key0 + BKV) ? level(m_edge) : -INFINITY, false);
+            const bool some = FORM == TREE_ROWS ? (in_tree[0] | in_tree[1] | in_tree[2] | in_tree[3]) != 0 : max(lo, key0) < min(hi, key0 + BKV);
+            raise(some ? level(m_edge) : -INFINITY, false);
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
               int a, b;
@@ -953,9 +982,9 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 tmem_ld_wait();
                 if (CAP) {                                 // (the weights are masked: a polynomial of -inf is not -inf)
                   cap(h, sv, max_of(sv));
-                  bits(a, b);
+                  bits(h, a, b);
                 } else {
-                  mask(a, b);
+                  mask(h, a, b);
                 }
                 weigh(h, sv, Int<CAP>(), seen);
               } else {
@@ -972,6 +1001,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             Ring v = checks;
             v.skip(t);
             if (!(alive = warp_wait(&v_ok[v.st], v.ph))) break;
+            auto in_tree_word = [&](int part) { return part < 2 ? part ? in_tree[1] : in_tree[0] : part == 2 ? in_tree[2] : in_tree[3]; };
             uint4 none;
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(none.x), "=r"(none.y), "=r"(none.z), "=r"(none.w) : "r"(smem_u32(s_bad + v.st * 4)) : "memory");
             for (int part = 0; part < 4 && (none.x | none.y | none.z | none.w); ++part)
@@ -983,7 +1013,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 tmem_ld_wait();
                 const float pv = __uint_as_float(kx & 1 ? w & 0xFFFF0000u : w << 16);
                 if (key >= it.k_end) continue;
-                const bool seen = key >= lo && key < hi;    // (also where its weight is zero: 0 x NaN is NaN, as in the products)
+                const bool seen = FORM == TREE_ROWS ? in_tree_word(part) >> (kx & 31) & 1 : key >= lo && key < hi;       // (also where its weight is zero: 0 x NaN is NaN, as in the products)
                 const size_t vrow = ((size_t)p.block_table[(size_t)it.trow * p.max_blocks + (key >> p.bs_log2)] * p.Hkv + it.kvh) * p.bs + (key & (p.bs - 1));
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
@@ -1225,30 +1255,30 @@ spans_join_kernel(const __grid_constant__ Params p) {
   *reinterpret_cast<uint2*>(p.out + at * D + lane * 4) = u;
 }
 
-template <bool SHARED, bool CAP>
+template <Form FORM, bool CAP>
 int launch_as(const CUtensorMap& tmK, const CUtensorMap& tmV, const Params& p, cudaStream_t stream) {
   static PerDeviceOnce once_;
   bool& configured = once_.slot();
   if (!configured) {
-    const cudaError_t e = cudaFuncSetAttribute(spans_kernel<SHARED, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    const cudaError_t e = cudaFuncSetAttribute(spans_kernel<FORM, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
-  cudaError_t e = launch_pdl(spans_kernel<SHARED, CAP>, dim3(p.n_items), dim3(NTHREADS), SMEM_BYTES, stream, tmK, tmV, p);
-  if (e != cudaSuccess || SHARED || !p.part_o) return (int)e;
+  cudaError_t e = launch_pdl(spans_kernel<FORM, CAP>, dim3(p.n_items), dim3(NTHREADS), SMEM_BYTES, stream, tmK, tmV, p);
+  if (e != cudaSuccess || FORM == SHARED_KEYS || !p.part_o) return (int)e;
   return (int)launch_pdl(spans_join_kernel, dim3((unsigned)(((size_t)p.T * p.Hq + 7) / 8)), dim3(256), 0, stream, p);
 }
 
-template <bool SHARED>
+template <Form FORM>
 int launch(Params& p, const SpansCall& a) {
   const int bs = a.block_size;
   const bool pow2 = bs >= 16 && bs <= 256 && !(bs & (bs - 1));
   if (!pow2 || a.n_q_heads % a.n_kv_heads || a.batch < 1 || a.T < 1 || a.max_blocks < 1 || a.num_blocks < 1 || !(a.scale > 0.f) || !(a.cap >= 0.f) ||
       (long long)a.max_blocks * bs > 0x7fffff00ll || ((long long)a.num_blocks + 1) * a.n_kv_heads * bs > 0x7fffff00ll ||
-      ((SHARED || a.splits > 1) && !a.workspace))
+      ((FORM == SHARED_KEYS || a.splits > 1) && !a.workspace))
     return -ERR_BAD_ARG;
   p.q = reinterpret_cast<const __nv_bfloat16*>(a.q);
-  p.gate = SHARED ? nullptr : reinterpret_cast<const __nv_bfloat16*>(a.gate);
+  p.gate = FORM == SHARED_KEYS ? nullptr : reinterpret_cast<const __nv_bfloat16*>(a.gate);
   p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
   p.v_cache = reinterpret_cast<const __nv_bfloat16*>(a.v_cache);
   p.block_table = a.block_table;
@@ -1258,7 +1288,7 @@ int launch(Params& p, const SpansCall& a) {
   p.Hq = a.n_q_heads; p.Hkv = a.n_kv_heads; p.G = a.n_q_heads / a.n_kv_heads;
   p.splits = a.splits;
   const size_t rows = (size_t)a.T * a.n_q_heads;
-  const bool parts = SHARED || p.splits > 1;
+  const bool parts = FORM == SHARED_KEYS || p.splits > 1;
   p.part_o = parts ? a.workspace : nullptr;
   p.part_ml = parts ? a.workspace + rows * p.splits * D : nullptr;
   p.scale_log2 = a.scale * 1.4426950408889634f;
@@ -1277,7 +1307,7 @@ int launch(Params& p, const SpansCall& a) {
   if (!make_tmap_2d(&tmK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.k_cache, kv_rows, D, D * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tmap_2d(&tmV, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.v_cache, kv_rows, D, D * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B))
     return -ERR_BAD_ARG;
-  return a.cap > 0.f ? launch_as<SHARED, true>(tmK, tmV, p, a.stream) : launch_as<SHARED, false>(tmK, tmV, p, a.stream);
+  return a.cap > 0.f ? launch_as<FORM, true>(tmK, tmV, p, a.stream) : launch_as<FORM, false>(tmK, tmV, p, a.stream);
 }
 
 }  // namespace spans
@@ -1288,8 +1318,8 @@ using namespace b200;
 // Prompt rows.  Sequence b: rows [q_start, q_start + q_len) and the first kv_len keys of table row b.  Row t sees the keys
 // lo[t] <= j < min(hi[t], kv_len); without lo from 0, without hi up to its own position kv_len - q_len + i.  splits: items a
 // row's keys are cut into.  Rows of no sequence are left as they are.
-extern "C" int b200_attn_spans(const SpansCall* call) {
-  const SpansCall& a = *call;
+template <spans::Form FORM>
+static int prompt_rows(const SpansCall& a) {
   if (a.bytes != (int)sizeof(a) || a.max_q_len < 1 || a.max_q_len > a.T || a.splits < 1 || a.n_kv_heads < 1 || a.n_q_heads < a.n_kv_heads)
     return -ERR_BAD_ARG;
   spans::Params p = {};
@@ -1301,7 +1331,19 @@ extern "C" int b200_attn_spans(const SpansCall* call) {
   if (each > 0x7fffff || tiles * a.n_kv_heads * a.splits > 0x7fffffffll) return -ERR_BAD_ARG;
   p.row_tiles = (int)each;
   p.n_items = (int)(tiles * a.n_kv_heads * a.splits);
-  return spans::launch<false>(p, a);
+  if (FORM == spans::TREE_ROWS) {
+    p.tree = a.tree;
+    p.tree_words = a.tree_words;
+  }
+  return spans::launch<FORM>(p, a);
+}
+extern "C" int b200_attn_spans(const SpansCall* call) { return prompt_rows<spans::SPANS>(*call); }
+
+// Rows of drafted trees: the last q_len[b] of sequence b's kv_len[b] keys are its tree's nodes.  Row t sees the context before them from
+// lo[t] on, and the nodes whose bits are set in its tree_words words of `tree`.
+extern "C" int b200_attn_tree(const SpansCall* call) {
+  if (call->bytes != (int)sizeof(SpansCall) || !call->tree || call->tree_words < 1 || call->hi) return -ERR_BAD_ARG;
+  return prompt_rows<spans::TREE_ROWS>(*call);
 }
 
 // One row per sequence: partial sums over the keys that groups of sequences share, for b200_attn_own_rows.  The sequences
@@ -1316,5 +1358,5 @@ extern "C" int b200_attn_shared(const SpansCall* call) {
   const long long rows = (long long)a.batch * (a.n_q_heads / a.n_kv_heads), tiles = rows / (2 * spans::BQ) + a.n_groups;
   if (tiles * a.splits * a.n_kv_heads > 0x7fffffffll) return -ERR_BAD_ARG;
   p.n_items = (int)(tiles * a.splits * a.n_kv_heads);
-  return spans::launch<true>(p, a);
+  return spans::launch<spans::SHARED_KEYS>(p, a);
 }

@@ -203,15 +203,69 @@ struct SpansCall {
   const int *block_table, *kv_len;            // [batch, max_blocks], [batch]
   const int *q_start, *q_len, *lo, *hi;       // prompt rows: [batch] twice, optional [T] twice
   const int *group_start, *shared_len;        // one row per sequence (T = batch): [n_groups + 1], [n_groups]
+  const uint32_t* tree;                       // rows of trees: [T, tree_words]
   float* workspace;                           // [splits T Hq 130]: partial sums of several items, or of the shared keys
   int* status;
   cudaStream_t stream;
-  int n_groups, max_q_len, T, max_blocks, num_blocks, block_size, n_q_heads, n_kv_heads, splits, cluster;
+  int n_groups, max_q_len, T, max_blocks, num_blocks, block_size, n_q_heads, n_kv_heads, splits, cluster, tree_words;
   float scale, cap;
 };
 int b200_qk_norm_rope_axes_append(const AxesAppendCall* call);
 int b200_attn_spans(const SpansCall* call);
 int b200_attn_shared(const SpansCall* call);
+int b200_attn_tree(const SpansCall* call);
+
+// ---- drafted trees (tree.cu): positions int32 [T] and masks [T, words] of their rows; the path that the target agrees with
+int b200_tree_layout(const int* parents, const int* q_start, const int* q_len, const int* kv_len, int batch, int T, int words,
+                     int* positions, uint32_t* mask, cudaStream_t stream);
+enum { ACCEPT_CACHES = 16 };
+struct AcceptCache {
+  void* base;                                 // [layers, num_blocks, heads, block_size, row_bytes], layers layer_bytes apart
+  long long layer_bytes;
+  int layers, heads, row_bytes, vec;          // vec: 16, or 4 where addresses are not multiples of 16
+};
+struct AcceptCall {
+  int bytes, batch;
+  const int *tokens, *parents, *predicted;    // [T]
+  const int *q_start, *q_len, *kv_len;        // [batch]
+  const int* block_table;                     // [batch, max_blocks]
+  int *path, *count, *emitted;                // [batch, max_path], [batch], [batch, max_path]; -1 behind a path's end
+  cudaStream_t stream;
+  int T, max_path, max_blocks, num_blocks, block_size, n_caches;
+  struct AcceptCache caches[ACCEPT_CACHES];
+};
+int b200_tree_accept(const struct AcceptCall* call);
+
+// ---- beams (beams.cu): the best continuations over beams and vocabulary; states that follow the beams
+struct SelectCall {
+  int bytes, requests;
+  const void* logits;                         // [requests beams] rows, row_stride elements apart; fp32 or bf16
+  long long row_stride;
+  const float* scores;                        // [requests, beams]
+  const unsigned char* finished;              // optional [requests, beams]
+  void* lists;                                // [requests beams, parts, n] 64-bit
+  void* sums;                                 // [requests beams, parts] two doubles
+  float* out_scores;                          // [requests, n]
+  int *out_parents, *out_tokens;
+  cudaStream_t stream;
+  int beams, vocab, n, parts, tiles, bf16, pad_token, vectors;     // tiles: of 8192 logits in a part; vectors: rows on 16-byte boundaries
+};
+int b200_beam_select(const struct SelectCall* call);
+enum { REORDER_STATES = 16 };
+struct ReorderState {
+  void* base;                                 // slot s, outer index o at base + o outer_bytes + s slot_bytes
+  long long outer_bytes, slot_bytes, inner_bytes;
+  int outer, bulk;                            // bulk: addresses and sizes are multiples of 16 bytes
+};
+struct ReorderCall {
+  int bytes, requests;
+  const int *parents, *slots;                 // [requests, beams]; slots may be null: request * beams + beam
+  int* status;
+  cudaStream_t stream;
+  int beams, n_slots, n_states, unused;
+  struct ReorderState states[REORDER_STATES];
+};
+int b200_beam_reorder(const struct ReorderCall* call);
 int b200_attn_own_rows(const SpansCall* call);
 // FlashMemory retriever (flashmemory.cu): chunk scores of one scorer layer, layer ensemble, top-k, index offset
 int b200_fm_score_layer(const float* hidden, const void* wq_a, const void* wq_b, const float* q_norm, const void* weights_proj,

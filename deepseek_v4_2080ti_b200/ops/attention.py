@@ -202,6 +202,7 @@ def decode_kv8(fmt: int, q, k8, v8, k_scale, v_scale, block_table, kv_len, gate=
 NUM_SMS = 148
 SCALE = 1.0 / math.sqrt(D)
 ROW_TILE, KEY_TILE = 256, 128            # (token, head) rows and keys of a tile in attn_spans.cu
+MAX_TREE = 1024                          # nodes of a drafted tree
 
 
 def _need(ok, what: str) -> None:
@@ -271,7 +272,7 @@ def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
 
 
 # The kernels' arguments as one block each (AxesAppendCall and SpansCall in ops.h), packed: a third of what 33 arguments cost one by one.
-_AXES_CALL, _SPANS_CALL = struct.Struct("@ii13P16iff64s"), struct.Struct("@ii16P10iff")
+_AXES_CALL, _SPANS_CALL = struct.Struct("@ii13P16iff64s"), struct.Struct("@ii17P11iff0P")
 _typed = False
 
 
@@ -280,7 +281,7 @@ def _kernels() -> ctypes.CDLL:
     global _typed
     lib = _lib.lib()
     if not _typed:
-        for f in (lib.b200_qk_norm_rope_axes_append, lib.b200_attn_spans, lib.b200_attn_shared, lib.b200_attn_own_rows):
+        for f in (lib.b200_qk_norm_rope_axes_append, lib.b200_attn_spans, lib.b200_attn_shared, lib.b200_attn_own_rows, lib.b200_attn_tree):
             f.argtypes = [ctypes.c_char_p]
         _typed = True
     return lib
@@ -440,6 +441,12 @@ def _check_pages(block_table, nb, bs, kv_len, rows=None) -> None:
     _lib.check_indices(block_table, 0, nb, 3, keep=-1)
 
 
+def _row_splits(b: int, t: int, g: int, hkv: int, max_q_len: int, max_kv_len: int) -> int:
+    """Items that the keys of a row tile are cut into: as many as there are SMs for, of two key tiles at least."""
+    tiles = hkv * min(b * -(-max_q_len * g // ROW_TILE), t * g // ROW_TILE + b)
+    return max(1, min(NUM_SMS // tiles, -(-max_kv_len // KEY_TILE) // 2))
+
+
 def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_q_len, lo=None, hi=None, gate=None, scale=None,
                   cap: float = 0.0, max_kv_len: int | None = None, splits: int | None = None, out=None):
     """Attention of new rows against the paged cache (which already holds their keys and values), every row over a span of keys
@@ -468,19 +475,75 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
     if t == 0 or b == 0 or max_q_len <= 0:
         return out
     if splits is None:
-        g = hq // hkv
-        tiles = hkv * min(b * -(-max_q_len * g // ROW_TILE), t * g // ROW_TILE + b)
-        keys = -(-(max_kv_len if max_kv_len is not None else width * bs) // KEY_TILE)
-        splits = max(1, min(NUM_SMS // tiles, keys // 2))
+        splits = _row_splits(b, t, hq // hkv, hkv, max_q_len, max_kv_len if max_kv_len is not None else width * bs)
     if not 1 <= splits <= 1024:
         raise ValueError(f"{splits} splits")
     ws = q.new_empty(splits * t * hq * (D + 2), dtype=_F32) if splits > 1 else None
     _check_pages(block_table, nb, bs, kv_len, (t, q_start, q_len, lo, hi))
     rc = _kernels().b200_attn_spans(_SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
-        q_start.data_ptr(), q_len.data_ptr(), _at(lo), _at(hi), 0, 0, _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq, hkv,
-        splits, 1, scale, cap))
+        q_start.data_ptr(), q_len.data_ptr(), _at(lo), _at(hi), 0, 0, 0, _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq, hkv,
+        splits, 1, 0, scale, cap))
     _lib.check(rc, "prefill_spans", 2 if splits > 1 else 1)
+    return out
+
+
+def _check_tree_pages(block_table, nb, bs, kv_len, q_start, q_len, lo, mask) -> None:
+    """``_check_pages`` for a tree's rows: keys of the context that some row sees, and nodes that some row has the bit of."""
+    if not _lib.bounds_checks_on():
+        return
+    (t, words), width = mask.shape, block_table.shape[1]
+    first = kv_len - q_len
+    row = torch.arange(t, device=mask.device)
+    mine = (row >= q_start[:, None]) & (row < (q_start + q_len)[:, None])                       # [B, T]
+    context = torch.where(mine, first[:, None], 0).amax(0, keepdim=True)[0].to(torch.int32) if t else first[:0]
+    seen = _seen_pages(t, width, bs, kv_len, q_start, q_len, lo, context)
+    nodes = ((mask[..., None] >> torch.arange(32, dtype=torch.int32, device=mask.device)) & 1).reshape(t, -1)
+    key = first[:, None] + torch.arange(32 * words, device=mask.device)                         # [B, nodes]
+    bits = (mine.float() @ nodes.float() > 0) & (key >= 0) & (key < torch.minimum(kv_len, torch.tensor(width * bs, device=mask.device))[:, None])
+    seen = seen.long().scatter_add(1, (key.long() // bs).clamp(0, width - 1), bits.long()) > 0
+    block_table.masked_fill_(seen & (block_table == -1), -2)
+    _lib.check_indices(block_table, 0, nb, 3, keep=-1)
+
+
+def decode_tree(q, k_cache, v_cache, block_table, mask, q_start, q_len, kv_len, max_q_len, lo=None, gate=None, scale=None, cap: float = 0.0,
+                max_kv_len: int | None = None, splits: int | None = None, out=None):
+    """Attention of the rows of drafted trees - tokens that continue one context in several ways, verified in one pass - against the paged
+    cache, which already holds their keys and values: node i of sequence b, row ``q_start[b] + i``, is the key at ``kv_len[b] - q_len[b] + i``.
+    A row sees the context before its tree (from ``lo[t]`` on, for windows) and the nodes whose bits are set in its ``mask``: int32
+    [T, words], bit i % 32 of word i / 32 for node i - itself and the nodes that it continues, as ``tree.layout`` gives it, or any others.
+    Bits of nodes that a sequence does not have count for nothing.  A row that sees nothing is 0; a key that a row does not see has no part
+    in it, whatever the cache holds there.
+
+    The other arguments, pages and rows of no sequence as in ``prefill_spans``."""
+    dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
+    if _current() != dev:
+        with torch.cuda.device(dev):
+            return decode_tree(q, k_cache, v_cache, block_table, mask, q_start, q_len, kv_len, max_q_len, lo, gate, scale, cap, max_kv_len, splits, out)
+    _index(q_start, (b,), dev, "q_start")
+    _index(q_len, (b,), dev, "q_len")
+    if lo is not None:
+        _index(lo, (t,), dev, "lo")
+    max_q_len = min(int(max_q_len), t)
+    if mask.dim() != 2 or not 0 < mask.shape[1] <= MAX_TREE // 32:
+        raise ValueError(f"mask {list(mask.shape)}: int32 [T, words] with 1 to {MAX_TREE // 32} words expected")
+    words = mask.shape[1]
+    _index(mask, (t, words), dev, "mask")
+    if max_q_len > 32 * words:
+        raise ValueError(f"trees of {max_q_len} rows, masks of {32 * words} nodes")
+    if t == 0 or b == 0 or max_q_len <= 0:
+        return out
+    if splits is None:
+        splits = _row_splits(b, t, hq // hkv, hkv, max_q_len, max_kv_len if max_kv_len is not None else width * bs)
+    if not 1 <= splits <= 1024:
+        raise ValueError(f"{splits} splits")
+    ws = q.new_empty(splits * t * hq * (D + 2), dtype=_F32) if splits > 1 else None
+    _check_tree_pages(block_table, nb, bs, kv_len, q_start, q_len, lo, mask)
+    rc = _kernels().b200_attn_tree(_SPANS_CALL.pack(
+        _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
+        q_start.data_ptr(), q_len.data_ptr(), _at(lo), 0, 0, 0, mask.data_ptr(), _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq,
+        hkv, splits, 1, words, scale, cap))
+    _lib.check(rc, "decode_tree", 2 if splits > 1 else 1)
     return out
 
 
@@ -576,8 +639,8 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     ws = q.new_empty(splits * b * hq * (D + 2), dtype=_F32) if n else None
     call = _SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
-        0, 0, 0, 0, group_start.data_ptr(), shared_len.data_ptr(), _at(ws), _status(dev), _stream(dev), n, 1, t, width, nb, bs, hq, hkv, splits, cluster,
-        scale, cap)
+        0, 0, 0, 0, group_start.data_ptr(), shared_len.data_ptr(), 0, _at(ws), _status(dev), _stream(dev), n, 1, t, width, nb, bs, hq, hkv, splits, cluster,
+        0, scale, cap)
     if n:
         _lib.check(lib.b200_attn_shared(call), "decode_shared")
     _lib.check(lib.b200_attn_own_rows(call), "decode_shared")

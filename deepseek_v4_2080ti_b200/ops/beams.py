@@ -1,0 +1,137 @@
+"""Beam search on the device (csrc/kernels/beam_select.cu, beam_reorder.cu): which continuations of a request's beams are kept, and the beams'
+states in their new order.
+
+    scores, parents, tokens = beams.select(logits, scores)               # a step of the search, [requests, beams]
+    beams.reorder([states, tails], parents, slots)                       # recurrent states; tables; the last pages of the beams' caches
+
+The same selection grows a drafted tree (``ops.tree``): the beams are its newest nodes, the candidates the nodes that it gets next."""
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from . import _lib
+from .attention import _at, _current, _index, _status, _stream
+
+MAX_BEAMS, MAX_CANDIDATES = 128, 128
+MAX_STATES = 16                          # tensors of one launch
+TILE = 8192                              # logits that a block looks at together
+NUM_SMS = 148
+_SELECT = struct.Struct("@iiPqPPPPPPPP8i0P")
+_REORDER, _STATE, _REORDER_BYTES = struct.Struct("@iiPPPP4i"), struct.Struct("@Pqqqii"), 56 + MAX_STATES * 40
+
+
+def _parts(rows: int, vocab: int) -> tuple[int, int]:
+    """Parts that a row is read in, and tiles of each."""
+    tiles = -(-vocab // TILE)
+    per = max(1, min(tiles, rows * tiles // (3 * NUM_SMS)))
+    return -(-tiles // per), per
+
+
+def select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None, finished: torch.Tensor | None = None,
+           pad_token: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``n`` best continuations (default: as many as beams) of every request: ``scores[b, w] + log_softmax(logits[b, w])`` over all beams w and
+    tokens, best first, of equals the lowest beam and token first.  logits fp32 or bf16 [B, W, V] (tokens side by side; a whole vocabulary),
+    scores fp32 [B, W].  Returns fp32 scores, int32 parents (beams) and int32 tokens, [B, n] each.
+
+    A beam with ``finished`` (bool [B, W]) offers itself alone, with ``pad_token`` and its score as it is.  Tokens with a logit of -inf and beams with a
+    score of -inf are not offered, nor are beams whose score or logits hold NaN or +inf; where fewer than n are left the rest is -inf, -1, -1.
+    Sums of exponentials are kept to 2^-30 and totals compared in 64 bits."""
+    dev, shape = logits.get_device(), logits.shape
+    if dev < 0 or len(shape) != 3 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"logits: fp32 or bf16 [requests, beams, vocabulary] on a GPU expected, got {logits.dtype} {list(shape)} on {logits.device}")
+    if _current() != dev:
+        with torch.cuda.device(dev):
+            return select(logits, scores, n, finished, pad_token)
+    b, w, v = shape
+    n = w if n is None else int(n)
+    if not 0 < w <= MAX_BEAMS or not 0 < n <= MAX_CANDIDATES or not 0 < v <= 0x7fff0000:
+        raise ValueError(f"{n} of {w} beams and {v} tokens: 1 to {MAX_BEAMS} beams, 1 to {MAX_CANDIDATES} candidates expected")
+    if not 0 <= pad_token < v:
+        raise ValueError(f"pad_token {pad_token} of a vocabulary of {v}")
+    sb, row, one = logits.stride()
+    if w == 1:
+        row = sb
+    if v > 1 and one != 1 or b > 1 and sb != w * row or b * w > 1 and row < v:
+        raise ValueError(f"logits: tokens side by side, rows one distance apart, expected; got strides {list(logits.stride())} of {list(shape)}")
+    if scores.dtype is not torch.float32 or scores.shape != (b, w) or scores.get_device() != dev or not scores.is_contiguous():
+        raise ValueError(f"scores: contiguous fp32 [{b}, {w}] on cuda:{dev} expected, got {scores.dtype} {list(scores.shape)} on {scores.device}")
+    if finished is not None and (finished.dtype is not torch.bool or finished.shape != (b, w) or finished.get_device() != dev or not finished.is_contiguous()):
+        raise ValueError(f"finished: contiguous bool [{b}, {w}] on cuda:{dev} expected, got {finished.dtype} {list(finished.shape)} on {finished.device}")
+    if b * w > 65535:
+        raise ValueError(f"{b} requests of {w} beams: 65535 rows at most")
+    out_scores = scores.new_empty(b, n)
+    parents, tokens = (torch.empty(b, n, dtype=torch.int32, device=logits.device) for _ in range(2))
+    if b == 0:
+        return out_scores, parents, tokens
+    parts, tiles = _parts(b * w, v)
+    size = logits.element_size()
+    vectors = logits.data_ptr() % 16 == 0 and row * size % 16 == 0 and v * size % 16 == 0
+    lists = torch.empty(b * w * parts * (n + 2), dtype=torch.int64, device=logits.device)      # and two doubles a part
+    rc = _lib.lib().b200_beam_select(_SELECT.pack(
+        _SELECT.size, b, logits.data_ptr(), row, scores.data_ptr(), _at(finished), lists.data_ptr() + 16 * b * w * parts, lists.data_ptr(),
+        out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _stream(dev), w, v, n, parts, tiles, size == 2, pad_token, vectors))
+    _lib.check(rc, "beam_select", 2)
+    return out_scores, parents, tokens
+
+
+def _state(x, dim: int, dev: int) -> tuple[int, bytes]:
+    """Checks a tensor of states; its number of slots, and what the kernel takes."""
+    shape, stride, size = x.shape, x.stride(), x.element_size()
+    if x.get_device() != dev or not 0 <= dim < len(shape) or x.numel() == 0:
+        raise ValueError(f"states: tensors on cuda:{dev} with slots along axis {dim} expected, got {list(shape)} on {x.device}")
+    inner = 1
+    for d in range(len(shape) - 1, dim, -1):
+        if shape[d] != 1 and stride[d] != inner:
+            raise ValueError(f"states: contiguous behind axis {dim} expected, got strides {list(stride)} of {list(shape)}")
+        inner *= shape[d]
+    outer, step = 1, 0
+    for d in range(dim - 1, -1, -1):
+        if shape[d] != 1:
+            if outer > 1 and stride[d] != outer * step:
+                raise ValueError(f"states: one distance between all parts before axis {dim} expected, got strides {list(stride)} of {list(shape)}")
+            step = step if outer > 1 else stride[d]
+            outer *= shape[d]
+    slots = shape[dim]
+    if slots > 1 and stride[dim] < inner or outer > 1 and step < inner:
+        raise ValueError(f"states: slots that lie apart expected, got strides {list(stride)} of {list(shape)}")
+    at, step, slot, inner = x.data_ptr(), step * size, stride[dim] * size, inner * size
+    return slots, _STATE.pack(at, step, slot, inner, outer, (at | step | slot | inner) % 16 == 0)
+
+
+def reorder(states, parents: torch.Tensor, slots: torch.Tensor | None = None, dim: int = 0) -> None:
+    """In place, for all beams of a request at once: the state of beam w becomes that of beam ``parents[b, w]``.
+
+    ``states``: a tensor or several of any type, their slots along axis ``dim``, everything behind it contiguous ([slots, layers, ..] with dim 0, caches
+    [layers, pages, ..] with dim 1).  parents int32 [B, W], as ``select`` returns them; a beam whose parent is itself, or none (-1), stays as it
+    is.  ``slots`` int32 [B, W]: where the beams' states are, all of them different (default: slot b W + w); a beam whose slot is not there is
+    neither read nor written.  Other slots stay as they are."""
+    dev = parents.get_device()
+    if dev < 0 or parents.dim() != 2:
+        raise ValueError(f"parents: int32 [requests, beams] on a GPU expected, got {list(parents.shape)} on {parents.device}")
+    if _current() != dev:
+        with torch.cuda.device(dev):
+            return reorder(states, parents, slots, dim)
+    b, w = parents.shape
+    _index(parents, (b, w), dev, "parents")
+    if slots is not None:
+        _index(slots, (b, w), dev, "slots")
+    if not 0 < w <= MAX_BEAMS:
+        raise ValueError(f"{w} beams: 1 to {MAX_BEAMS} expected")
+    states = [states] if isinstance(states, torch.Tensor) else list(states)
+    found = [_state(x, dim, dev) for x in states]
+    if not found or any(n != found[0][0] for n, _ in found):
+        raise ValueError(f"states: tensors of one number of slots expected, got {[n for n, _ in found]}")
+    if len({x.data_ptr() for x in states}) < len(states):
+        raise ValueError("states: a tensor that is there twice would move twice")
+    n_slots = found[0][0]
+    if slots is None and b * w > n_slots:
+        raise ValueError(f"{b} requests of {w} beams in {n_slots} slots")
+    if b == 0:
+        return
+    _lib.check_indices(slots, 0, n_slots, 4)
+    for i in range(0, len(found), MAX_STATES):
+        some = found[i:i + MAX_STATES]
+        call = _REORDER.pack(_REORDER_BYTES, b, parents.data_ptr(), _at(slots), _status(dev), _stream(dev), w, n_slots, len(some), 0)
+        _lib.check(_lib.lib().b200_beam_reorder((call + b"".join(s for _, s in some)).ljust(_REORDER_BYTES, b"\0")), "beam_reorder")
