@@ -55,6 +55,7 @@ constexpr int TILE = 2 * ATOM;
 constexpr int STAGES = 5;
 constexpr int EMULATED = 2;       // of 8 pairs of exponentials: those on the arithmetic units (0 / 1 / 2 / 3: 641 / 639 / 624 / 626 us for 8192 causal rows)
 constexpr int ITEMS = 4;          // items the producer may be ahead of the slowest role
+constexpr int TO_L2 = 4;           // rows of a tree: key tiles on their way to L2 ahead of the ring
 constexpr int NTHREADS = 384;
 constexpr int SMEM_BYTES = 1024 + (2 + STAGES) * TILE + 2048;
 static_assert(SMEM_BYTES <= 232448, "shared memory of a block");
@@ -63,7 +64,7 @@ struct Params {
   const __nv_bfloat16* q;         // [T, Hq, 128]
   const __nv_bfloat16* gate;      // optional [T, Hq, 128]
   __nv_bfloat16* out;             // [T, Hq, 128]
-  const __nv_bfloat16* v_cache;
+  const __nv_bfloat16 *k_cache, *v_cache;
   const int* block_table;         // [B, max_blocks]
   const int* kv_len;              // [B]
   // prompt rows
@@ -87,6 +88,7 @@ struct Params {
   // half of the places would be empty.
   int by_sequence;
   int splits;                     // key ranges per row tile
+  int per_item;                   // rows of a tree: key tiles of a range, so that the items of short contexts are fewer, not shorter
   int n_items;
   float scale_log2;               // scale * log2(e)
   float cap_in, cap_out;          // scale / cap, cap * log2(e)
@@ -337,7 +339,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
       const uint32_t x = (uint32_t)idx / (uint32_t)(splits * p.Hkv), z = x / (uint32_t)p.batch;
       b = (int)(x - z * p.batch);
       y = idx - (int)x * splits * p.Hkv;
-      tile = p.row_tiles - 1 - (int)z;                                     // long contexts first
+      tile = FORM == TREE_ROWS ? (int)z : p.row_tiles - 1 - (int)z;        // long contexts first; of a tree's rows, which all see the context, full tiles
       q0 = p.q_start[b];
       n = p.q_len[b];
       kv = p.kv_len[b];
@@ -348,7 +350,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
     split = y - (int)x * splits;
     it.kvh = (int)(x - z * p.Hkv);
     it.slot = split;
-    it.r0 = (p.by_sequence ? (rows_all + 2 * BQ - 1) / (2 * BQ) - 1 - (int)z : tile) * 2 * BQ;
+    it.r0 = (!p.by_sequence ? tile : FORM == TREE_ROWS ? (int)z : (rows_all + 2 * BQ - 1) / (2 * BQ) - 1 - (int)z) * 2 * BQ;
     it.trow = b;
     it.base_tok = q0;
     it.kv_end = max(0, min(kv, p.max_blocks * p.bs));
@@ -378,9 +380,9 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
   it.k_end = __reduce_max_sync(0xffffffffu, hi_max);
   it.t0 = it.t1 = 0;
   if (it.k_end > lo_min) {
-    const int a = lo_min / BKV, n = (it.k_end + BKV - 1) / BKV - a, per = (int)((uint32_t)(n + splits - 1) / (uint32_t)splits);
+    const int a = lo_min / BKV, n = (it.k_end + BKV - 1) / BKV - a, per = FORM == TREE_ROWS ? p.per_item : (int)((uint32_t)(n + splits - 1) / (uint32_t)splits);
     it.t0 = a + min(n, split * per);
-    it.t1 = a + min(n, (split + 1) * per);
+    it.t1 = a + (FORM == TREE_ROWS && split + 1 == splits ? n : min(n, (split + 1) * per));
   }
   return true;
 }
@@ -550,8 +552,18 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           return ((id * p.Hkv + it.kvh) << p.bs_log2) + (key & (p.bs - 1));
         };
         int row = page_row(it.t0);                         // (on its way while the item is handed out)
+        auto to_l2 = [&](int tile) {
+          const int ahead = page_row(tile);
+          if (tile < it.t1 && lane < per_tile && ahead < p.num_blocks * p.Hkv * p.bs) {
+            l2_prefetch(p.k_cache + (size_t)ahead * D, rows * D * 2);
+            l2_prefetch(p.v_cache + (size_t)ahead * D, rows * D * 2);
+          }
+        };
+        if (FORM == TREE_ROWS)
+          for (int t = 1; t < TO_L2; ++t) to_l2(it.t0 + t);
         hand_out();
         for (int t = it.t0; ok && t < it.t1; ++t) {
+          if (FORM == TREE_ROWS) to_l2(t + TO_L2);
           const int n = min(per_tile, (it.k_end - t * BKV + rows - 1) >> rows_log2);
           const int next_row = page_row(t + 1);
 #pragma unroll
@@ -1227,13 +1239,25 @@ spans_join_kernel(const __grid_constant__ Params p) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + at) * 2);
-    if (ml.y == 0.f) continue;                             // (nothing seen: the item may not have written its sums)
-    const float w = exp2f(ml.x - M);
-    const float4 x = *reinterpret_cast<const float4*>(p.part_o + (s * rows + at) * D + lane * 4);
-    L += w * ml.y;
-    o[0] += w * x.x; o[1] += w * x.y; o[2] += w * x.z; o[3] += w * x.w;
+  for (int s0 = 0; s0 < p.splits; s0 += 32) {              // a slot's maximum and sum per lane, then its part, eight on their way at a time
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (s0 + lane < p.splits) ml = *reinterpret_cast<const float2*>(p.part_ml + ((s0 + lane) * rows + at) * 2);
+    const float w_all = ml.y == 0.f ? -1.f : exp2f(ml.x - M);              // (below 0: nothing seen, the item may not have written its sums)
+    for (int s1 = 0; s1 < min(32, p.splits - s0); s1 += 8) {
+      float4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __shfl_sync(0xffffffffu, w_all, s1 + i);
+        if (!(w < 0.f)) x[i] = *reinterpret_cast<const float4*>(p.part_o + ((s0 + s1 + i) * rows + at) * D + lane * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __shfl_sync(0xffffffffu, w_all, s1 + i), l = __shfl_sync(0xffffffffu, ml.y, s1 + i);
+        if (w < 0.f) continue;
+        L += w * l;
+        o[0] += w * x[i].x; o[1] += w * x[i].y; o[2] += w * x[i].z; o[3] += w * x[i].w;
+      }
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
@@ -1280,6 +1304,7 @@ int launch(Params& p, const SpansCall& a) {
   p.q = reinterpret_cast<const __nv_bfloat16*>(a.q);
   p.gate = FORM == SHARED_KEYS ? nullptr : reinterpret_cast<const __nv_bfloat16*>(a.gate);
   p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
+  p.k_cache = reinterpret_cast<const __nv_bfloat16*>(a.k_cache);
   p.v_cache = reinterpret_cast<const __nv_bfloat16*>(a.v_cache);
   p.block_table = a.block_table;
   p.kv_len = a.kv_len;
@@ -1334,15 +1359,17 @@ static int prompt_rows(const SpansCall& a) {
   if (FORM == spans::TREE_ROWS) {
     p.tree = a.tree;
     p.tree_words = a.tree_words;
+    p.per_item = a.per_item;
   }
   return spans::launch<FORM>(p, a);
 }
 extern "C" int b200_attn_spans(const SpansCall* call) { return prompt_rows<spans::SPANS>(*call); }
 
 // Rows of drafted trees: the last q_len[b] of sequence b's kv_len[b] keys are its tree's nodes.  Row t sees the context before them from
-// lo[t] on, and the nodes whose bits are set in its tree_words words of `tree`.
+// lo[t] on, and the nodes whose bits are set in its tree_words words of `tree`.  per_item: key tiles of an item; what
+// lies behind splits of them goes with the last.
 extern "C" int b200_attn_tree(const SpansCall* call) {
-  if (call->bytes != (int)sizeof(SpansCall) || !call->tree || call->tree_words < 1 || call->hi) return -ERR_BAD_ARG;
+  if (call->bytes != (int)sizeof(SpansCall) || !call->tree || call->tree_words < 1 || call->per_item < 1 || call->hi) return -ERR_BAD_ARG;
   return prompt_rows<spans::TREE_ROWS>(*call);
 }
 

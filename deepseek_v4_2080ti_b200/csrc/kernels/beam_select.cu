@@ -2,21 +2,25 @@
 //
 //   total[w, v] = score[w] + x[w, v] - log sum_u exp x[w, u];  the n largest of a request, ties to the lowest (w, v)
 //
-// Candidates of different beams lie closer together than 32 bits tell apart (of 16 out of 8 beams a pair in 10^5 is nearer than 10^-6), and a
-// swapped pair swaps two beams, so the sums are kept to 2^-30 and totals compared in 64 bits.  Within a beam the order is that of the logits.
-//
 // select_parts_kernel reads the logits once: a block takes `tiles` tiles of 8192 logits of one row, 32 a thread in registers, adds
 // their exponentials and keeps its n largest logits, in order, beside the sum.  select_join_kernel, a block per request, adds up the sums of
 // every beam and joins the lists.
 //
-// The exponentials: x = (32 k + j) ln 2 / 32 + r with |r| <= 0.011, exp x = 2^k 2^(j/32) (1 + p), p = r + r^2 / 2 + r^3 / 6 in fp32
-// (off by 2^-30.7 at most), 2^(j/32) from a table as a double, whose exponent takes k; T and T p are summed in 64 bits.  exp from the
-// exponential unit is off by 2^-22, and its error is much the same in every term.
+// Candidates of different beams may lie closer together than sums in 32 bits tell apart (of the 16 best of 8 beams a neighbouring pair in
+// 10^5 is nearer than 10^-6), and a swapped pair swaps two beams.  So the sums carry a bound (off_of), and where two neighbours of different
+// beams are nearer than their bounds the beams' rows are read again and summed to 2^-30 before their order is taken as certain; totals are
+// compared in 64 bits.  Within a beam the order is that of the logits.
 //
-// The n largest: the k largest thread maxima of each of 8 warps, k = n / 8 rounded up, are 8 k >= n logits, so the least of them
-// bounds the n-th largest from below; what reaches it - little more than n of 8192 - goes to shared memory, where each counts those before it.
-// Where more than CAP reach it (ties) the n-th largest is found bit by bit instead.  Further tiles add what exceeds the list's last.
+// The sums of the second pass: x = (32 k + j) ln 2 / 32 + r with |r| <= 0.011, exp x = 2^k 2^(j/32) (1 + p), p = r + r^2 / 2 + r^3 / 6 in fp32 (off by 2^-30.7), 2^(j/32) from a table as a double, whose
+// exponent takes k; T and T p are summed in 64 bits.
+//
+// The n largest: every warp keeps a list of its own, in no order until it is full, and needs no other warp for it.  What is below a bound of
+// the block's n-th largest does not get into it: the least of the warps' k-th largest, k = n / 8 rounded up, is one (8 k >= n logits reach
+// it), first by lane maxima, then by what a warp found when it put its list in order.  So little more than n of 8192 get in, and a warp
+// whose largest logit is below the bound is done with one look.  Where more get in than a list takes (ties) a warp finds its n-th largest bit
+// by bit.
 #include <cuda_bf16.h>
+#include <limits.h>
 #include "../ptx/sm100.cuh"
 #include "launch.h"
 #include "ops.h"
@@ -25,11 +29,16 @@ namespace b200 {
 namespace select {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
+static_assert(THREADS == 256, "a thread's number in eight bits");
 constexpr int PER = 32;                    // logits of a thread
 constexpr int TILE = THREADS * PER;
 constexpr int MAX_N = 128, MAX_BEAMS = 128;
+constexpr int WARP_TILE = 32 * PER;
+constexpr int AHEAD = 2;                   // tiles on their way to L2
+constexpr int LIST = 256;                  // candidates of a warp: n and as many new ones
 constexpr int CAP = 1024;                  // candidates that are ordered by counting
 constexpr float LOWEST = -80.f;            // exp of this beside 1 is below 2^-115: smaller ones count as this
+constexpr float LOG2E = 1.44269504f;
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;
@@ -70,22 +79,61 @@ __device__ __forceinline__ uint64_t order_of(double x) {
   return u >> 63 ? ~u : u | 1ull << 63;
 }
 
-// A sum of exponentials, sum * exp(ref).
+// A sum of exponentials, sum * exp(k ln 2 + far); far is 0 for logits of at most 2^15 in size.  Those of the first pass count in powers of
+// e^(1 / LOG2E), so that what LOG2E is off by counts for the distance from the largest logit and not for the logits themselves.
+template <bool EXACT>
 struct Sum {
-  double ref, sum;
+  double sum;
+  int k;
+  float far;
+  __device__ __forceinline__ double ref() const { return (double)k * (EXACT ? 0.6931471805599453 : 1.0 / (double)LOG2E) + (double)far; }
   __device__ __forceinline__ void add(const Sum& o) {
     if (!(o.sum != 0.0)) return;                           // nothing (a NaN is something)
     if (!(sum != 0.0)) {
       *this = o;
-      return;
+    } else if (far == o.far) {                             // powers of two, no rounding
+      const int top = max(k, o.k);
+      sum = sum * power(k - top) + o.sum * power(o.k - top);
+      k = top;
+    } else {
+      const double a = ref(), b = o.ref();
+      const Sum& top = a > b ? *this : o;
+      const double t = a > b ? a : b;
+      sum = sum * (a == t ? 1.0 : exp(a - t)) + o.sum * (b == t ? 1.0 : exp(b - t));
+      k = top.k;
+      far = top.far;
     }
-    const double top = ref > o.ref ? ref : o.ref;
-    // (equal references, as those of infinities: no difference to take)
-    sum = sum * (ref == top ? 1.0 : exp(ref - top)) + o.sum * (o.ref == top ? 1.0 : exp(o.ref - top));
-    ref = top;
   }
-  __device__ __forceinline__ Sum shuffled(int o) const { return {__shfl_xor_sync(0xffffffffu, ref, o), __shfl_xor_sync(0xffffffffu, sum, o)}; }
+  static __device__ __forceinline__ double power(int e) { return __hiloint2double((1023 + max(e, -1022)) << 20, 0); }
 };
+// The sum of a warp's lanes, in every lane.
+template <bool EXACT>
+__device__ __forceinline__ void warp_sum(Sum<EXACT>& s) {
+  if (!__any_sync(0xffffffffu, s.sum != 0.0 && s.far != 0.f)) {            // as almost always
+    const int top = __reduce_max_sync(0xffffffffu, s.sum != 0.0 ? s.k : INT_MIN);
+    if (s.sum != 0.0) s.sum *= s.power(s.k - top);
+    s.k = top;
+    s.far = 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, o);
+  } else {
+    for (int o = 16; o > 0; o >>= 1)
+      s.add({__shfl_xor_sync(0xffffffffu, s.sum, o), __shfl_xor_sync(0xffffffffu, s.k, o), __shfl_xor_sync(0xffffffffu, s.far, o)});
+  }
+}
+// The sum of a block's threads, in warp 0.
+template <bool EXACT>
+__device__ __forceinline__ void block_sum(Sum<EXACT>& s, Sum<EXACT>* sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  warp_sum(s);
+  if (lane == 0) sums[warp] = s;
+  __syncthreads();
+  if (warp == 0) {
+    if (lane < WARPS) s = sums[lane];
+    else s.sum = 0.0;
+    warp_sum(s);
+  }
+}
 
 // The 32 powers of two as the halves of doubles.
 struct Table {
@@ -113,67 +161,155 @@ __device__ __forceinline__ void add_exp2(uint64_t x, const Table& t, int N, doub
   }
 }
 
-// Sum of a thread's numbers, of which m, finite, is the largest.
-__device__ __forceinline__ Sum sum_exp(const float (&v)[PER], float m, const Table& t) {
+// Numbers beyond 2^15 are taken relative to the largest: differences of such are exact where they count.
+struct Scale {
+  float far, low;                          // what is subtracted first; the least number that counts
+  int k;                                   // the largest is about k ln 2 + far
+  __device__ __forceinline__ explicit Scale(float m) {
+    const bool is_far = !(fabsf(m) <= 32768.f);
+    far = is_far ? m : 0.f;
+    low = is_far ? LOWEST : m + LOWEST;
+    k = is_far ? 0 : __float2int_rn(m * 1.44269504f);
+  }
+};
+
+// Sum of a thread's numbers, of which m, finite, is the largest, to 2^-30.
+__device__ __forceinline__ Sum<true> sum_exactly(const float (&v)[PER], float m, const Table& t) {
   constexpr int BIG_BITS = 0x4b400000;
   double a[2] = {0, 0}, b[2] = {0, 0};
-  Sum s;
-  // Numbers beyond 2^15 relative to the largest: differences of such are exact where they count.
-  const bool far = !(fabsf(m) <= 32768.f);
-  const float top = far ? 0.f : m, low = m + LOWEST;
-  const int k = __float2int_rn(top * 1.44269504f);
-  const int N = ((BIG_BITS >> 5) << 20) + (k << 20);       // (wraps: bits of the exponent)
-  if (!far) {
+  const Scale s(m);
+  const int N = ((BIG_BITS >> 5) << 20) + (s.k << 20);     // (wraps: bits of the exponent)
 #pragma unroll
-    for (int i = 0; i < PER; i += 4) {
-      add_exp2(pack2(fmaxf(v[i], low), fmaxf(v[i + 1], low)), t, N, a[0], b[0]);
-      add_exp2(pack2(fmaxf(v[i + 2], low), fmaxf(v[i + 3], low)), t, N, a[1], b[1]);
+  for (int i = 0; i < PER; i += 4) {
+    add_exp2(pack2(fmaxf(v[i] - s.far, s.low), fmaxf(v[i + 1] - s.far, s.low)), t, N, a[0], b[0]);
+    add_exp2(pack2(fmaxf(v[i + 2] - s.far, s.low), fmaxf(v[i + 3] - s.far, s.low)), t, N, a[1], b[1]);
+  }
+  return {(a[0] + a[1]) + (b[0] + b[1]), s.k, s.far};
+}
+
+// The same for the first pass, in two operations and an exponential a logit: 2^t with t = x log2 e - k.
+__device__ __forceinline__ Sum<false> sum_quickly(const float (&v)[PER], float m) {
+  const Scale s(m);
+  const float far = s.far;
+  const uint64_t far2 = pack2(-far, -far), k2 = pack2(-(float)s.k, -(float)s.k), log2e = pack2(LOG2E, LOG2E);
+  uint64_t a[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < PER; i += 2) {
+    uint64_t x = pack2(v[i], v[i + 1]);
+    if (far != 0.f) x = add2(x, far2);
+    float e[2];
+    unpack2(fma2(x, log2e, k2), e[0], e[1]);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[0]));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[1]));
+    a[i / 2 & 3] = add2(a[i / 2 & 3], pack2(e[0], e[1]));
+  }
+  double sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x, y;
+    unpack2(a[i], x, y);
+    sum += (double)x + (double)y;
+  }
+  return {sum, s.k, far};
+}
+// How far a logarithm of such a sum over v logits may be off.  t is off by 2^-24 of itself and by what LOG2E is (2^-26); weighted with the
+// exponentials |t| is log2 v + 1 at most (their entropy).  The exponentials are off by 2^-22, four terms added in 32 bits by 3 2^-24.
+__device__ __forceinline__ double off_of(int v) { return 5.1e-8 * (33 - __clz(v)) + 4.5e-7; }
+
+struct Shared {
+  unsigned long long list[WARPS][2][LIST]; // in turn
+  Sum<false> sum[WARPS];
+  uint32_t least[WARPS];
+  unsigned long long joined[WARPS * MAX_N];
+  int n_list[WARPS], count;
+};
+
+// Place of a lane's j-th logit in its warp's tile.
+template <bool BF16, bool VEC>
+__device__ __forceinline__ int place(int j) {
+  const int lane = threadIdx.x & 31;
+  if (!VEC) return j * 32 + lane;
+  return BF16 ? (j >> 3) * 256 + lane * 8 + (j & 7) : (j >> 2) * 128 + lane * 4 + (j & 3);
+}
+
+template <bool BF16, bool VEC, bool FULL>
+__device__ __forceinline__ void load_logits(const char* base, int left, float (&v)[PER]) {
+  if (VEC && BF16) {
+#pragma unroll
+    for (int i = 0; i < PER / 8; ++i) {
+      const int at = place<BF16, VEC>(i * 8);
+      uint4 x = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+      if (FULL || at < left) x = __ldcs(reinterpret_cast<const uint4*>(base + (size_t)at * 2));
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        v[i * 8 + 2 * c] = __uint_as_float(w[c] << 16);
+        v[i * 8 + 2 * c + 1] = __uint_as_float(w[c] & 0xffff0000u);
+      }
+    }
+  } else if (VEC) {
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) {
+      const int at = place<BF16, VEC>(i * 4);
+      float4 x = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (FULL || at < left) x = __ldcs(reinterpret_cast<const float4*>(base + (size_t)at * 4));
+      v[i * 4] = x.x;
+      v[i * 4 + 1] = x.y;
+      v[i * 4 + 2] = x.z;
+      v[i * 4 + 3] = x.w;
     }
   } else {
-#pragma unroll 1
-    for (int i = 0; i < PER; ++i) {
-      float x = v[0];
 #pragma unroll
-      for (int j = 1; j < PER; ++j)
-        if (i == j) x = v[j];
-      const float d = x - m;
-      double none = 0, more = 0;
-      add_exp2(pack2(fmaxf(d, LOWEST), LOWEST), t, N, none, more);
-      if (d >= LOWEST) {
-        a[0] += none;
-        b[0] += more;
+    for (int i = 0; i < PER; ++i) {
+      const int at = place<BF16, VEC>(i);
+      v[i] = -INFINITY;
+      if (FULL || at < left) {
+        if (BF16) v[i] = __uint_as_float((uint32_t)__ldcs(reinterpret_cast<const unsigned short*>(base + (size_t)at * 2)) << 16);
+        else v[i] = __ldcs(reinterpret_cast<const float*>(base + (size_t)at * 4));
       }
     }
   }
-  s.sum = (a[0] + a[1]) + (b[0] + b[1]);
-  s.ref = (double)k * 0.6931471805599453 + (far ? (double)m : 0.0);
-  return s;
 }
-
-struct Shared {
-  unsigned long long list[2][CAP];
-  uint32_t hi[32], lo[32];
-  double ref[WARPS], sum[WARPS];
-  uint32_t least[WARPS];
-  int count, votes[2][WARPS];
-};
-
-// Block-wide sum of a count per thread; `turn` alternates between calls.
-__device__ __forceinline__ int block_count(Shared& s, int mine, int& turn) {
-  const int w = __reduce_add_sync(0xffffffffu, mine);
-  if ((threadIdx.x & 31) == 0) s.votes[turn][threadIdx.x >> 5] = w;
-  __syncthreads();
-  int all = 0;
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i) all += s.votes[turn][i];
-  turn ^= 1;
-  return all;
-}
-
+// A lane's logits of the warp's tile that begins at `first`, of which `left` are there; -inf behind them.
 template <bool BF16, bool VEC>
-__device__ __forceinline__ int place(int j) {              // of a thread's j-th logit in its tile
-  if (!VEC) return j * THREADS + threadIdx.x;
-  return BF16 ? (j >> 3) * (8 * THREADS) + threadIdx.x * 8 + (j & 7) : (j >> 2) * (4 * THREADS) + threadIdx.x * 4 + (j & 3);
+__device__ __forceinline__ void load_tile(const char* base, int first, int left, float (&v)[PER]) {
+  const char* tile = base + (size_t)first * (BF16 ? 2 : 4);
+  if (left >= WARP_TILE) load_logits<BF16, VEC, true>(tile, left, v);
+  else load_logits<BF16, VEC, false>(tile, left, v);
+}
+__device__ __forceinline__ float largest(const float (&v)[PER]) {          // NaN if there is one
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i + 1 < PER; i += 2) m = max3_nan(m, v[i], v[i + 1]);
+  return max3_nan(m, v[PER - 1], v[PER - 1]);
+}
+
+// The warp's tile's n largest, when more than a list takes reach the bound: all above `cut`, and of its equals those at places up to `end`.
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void cut_tile(const float (&v)[PER], int n, uint32_t& cut, int& end) {
+  cut = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t c = cut | 1u << bit;
+    int more = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) more += order_of(v[j]) >= c;
+    if (__reduce_add_sync(0xffffffffu, more) >= n) cut = c;
+  }
+  cut = max(cut, ORDER_NONE + 1);
+  int above = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) above += order_of(v[j]) > cut;
+  const int wanted = n - __reduce_add_sync(0xffffffffu, above);
+  end = 0;                                                 // places below this hold fewer than `wanted` of the cut's equals
+#pragma unroll 1
+  for (int bit = WARP_TILE / 2; bit > 0; bit >>= 1) {
+    const int c = end + bit;
+    int earlier = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) earlier += order_of(v[j]) == cut && place<BF16, VEC>(j) < c;
+    if (__reduce_add_sync(0xffffffffu, earlier) < wanted) end = c;
+  }
 }
 
 template <bool BF16, bool VEC>
@@ -183,345 +319,393 @@ select_parts_kernel(const __grid_constant__ SelectCall p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int part = blockIdx.x;
   const size_t row = blockIdx.y;
-  if (tid < 32) {
-    const double T = exp2(tid / 32.0);
-    s.hi[tid] = (uint32_t)__double2hiint(T);
-    s.lo[tid] = (uint32_t)__double2loint(T);
-  }
   if (tid == 0) s.count = 0;
   pdl_wait();
   pdl_launch_dependents();
   // beams that are at their end, or that have come to nothing, offer nothing of their row
   const float score = p.scores[row];
   if (p.finished && p.finished[row] || !(fabsf(score) < INFINITY)) return;
-  __syncthreads();
-  const Table table = {s.hi, s.lo};
   const int n = p.n, k = (n + WARPS - 1) / WARPS;
-  Sum sum = {-INFINITY, 0.0};
-  int have = 0, cur = 0, turn = 0;
   const char* base = reinterpret_cast<const char*>(p.logits) + row * (size_t)p.row_stride * (BF16 ? 2 : 4);
-#pragma unroll 1
-  for (int t = 0; t < p.tiles; ++t) {
-    const int first = (part * p.tiles + t) * TILE;
-    if (first >= p.vocab) break;
-    const int left = p.vocab - first;
-    float v[PER];
-    if (VEC && BF16) {
-#pragma unroll
-      for (int i = 0; i < PER / 8; ++i) {
-        const int at = i * (8 * THREADS) + tid * 8;
-        uint4 x = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
-        if (at < left) x = __ldcs(reinterpret_cast<const uint4*>(base + (size_t)(first + at) * 2));
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          v[i * 8 + 2 * c] = __uint_as_float(w[c] << 16);
-          v[i * 8 + 2 * c + 1] = __uint_as_float(w[c] & 0xffff0000u);
-        }
-      }
-    } else if (VEC) {
-#pragma unroll
-      for (int i = 0; i < PER / 4; ++i) {
-        const int at = i * (4 * THREADS) + tid * 4;
-        float4 x = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (at < left) x = __ldcs(reinterpret_cast<const float4*>(base + (size_t)(first + at) * 4));
-        v[i * 4] = x.x;
-        v[i * 4 + 1] = x.y;
-        v[i * 4 + 2] = x.z;
-        v[i * 4 + 3] = x.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int at = i * THREADS + tid;
-        v[i] = -INFINITY;
-        if (at < left) {
-          if (BF16) v[i] = __uint_as_float((uint32_t)__ldcs(reinterpret_cast<const unsigned short*>(base + (size_t)(first + at) * 2)) << 16);
-          else v[i] = __ldcs(reinterpret_cast<const float*>(base + (size_t)(first + at) * 4));
-        }
-      }
-    }
-    float m = v[0];
-#pragma unroll
-    for (int i = 1; i + 1 < PER; i += 2) m = max3_nan(m, v[i], v[i + 1]);
-    m = max3_nan(m, v[PER - 1], v[PER - 1]);
-
-    if (fabsf(m) < INFINITY) sum.add(sum_exp(v, m, table));
-    else if (!(m == -INFINITY)) sum = {INFINITY, __longlong_as_double(0x7ff8000000000000ll)};       // NaN or +inf: the row counts for nothing
-
-    // ---- what exceeds the list's last, or reaches a bound of the n-th largest
-    uint32_t bound;
-    const uint32_t mine = order_of(m);
-    if (have == n) {
-      bound = (uint32_t)(s.list[cur][n - 1] >> 32) + 1;    // (of equals the earlier ones stay)
-    } else {
-      uint32_t x = mine, top = 0;
-      for (int i = 0; i < k; ++i) {
-        top = __reduce_max_sync(0xffffffffu, x);
-        if (x == top) x = 0;
-      }
-      if (lane == 0) s.least[warp] = top;
-      __syncthreads();
-      bound = s.least[0];
-#pragma unroll
-      for (int w = 1; w < WARPS; ++w) bound = min(bound, s.least[w]);
-      bound = max(bound, ORDER_NONE + 1);
-    }
-    unsigned long long* list = s.list[cur];
-    auto key = [&](uint32_t order, int j) {
-      return (unsigned long long)order << 32 | (uint32_t)~(first + place<BF16, VEC>(j));
-    };
-    if (mine >= bound) {
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const uint32_t o = order_of(v[j]);
-        if (o >= bound) {
-          const int at = have + atomicAdd(&s.count, 1);
-          if (at < CAP) list[at] = key(o, j);
-        }
-      }
-    }
-    __syncthreads();
-    int count = have + s.count;
-    if (count == have) continue;
-    __syncthreads();
-    if (tid == 0) s.count = 0;
-    if (count > CAP) {
-      // the tile's n-th largest bit by bit, and the last of its equals that counts
-      uint32_t cut = 0;
-#pragma unroll 1
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = cut | 1u << bit;
-        int more = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) more += order_of(v[j]) >= c;
-        if (block_count(s, more, turn) >= n) cut = c;
-      }
-      cut = max(cut, ORDER_NONE + 1);
-      int above = 0;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) above += order_of(v[j]) > cut;
-      const int wanted = n - block_count(s, above, turn);  // of those equal to the cut
-      int end = 0;                                         // places below this hold fewer than `wanted` of them
-#pragma unroll 1
-      for (int bit = TILE / 2; bit > 0; bit >>= 1) {
-        const int c = end + bit;
-        int before = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) before += order_of(v[j]) == cut && place<BF16, VEC>(j) < c;
-        if (block_count(s, before, turn) < wanted) end = c;
-      }
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const uint32_t o = order_of(v[j]);
-        if (o > cut || o == cut && place<BF16, VEC>(j) <= end) {
-          const int at = have + atomicAdd(&s.count, 1);
-          if (at < CAP) list[at] = key(o, j);
-        }
-      }
-      __syncthreads();
-      count = min(CAP, have + s.count);
-      __syncthreads();
-      if (tid == 0) s.count = 0;
-    }
-    for (int i = tid; i < count; i += THREADS) {
+  Sum<false> sum = {0.0, 0, 0.f};
+  unsigned long long* list = s.list[warp][0];
+  unsigned long long* other = s.list[warp][1];
+  int count = 0;                                           // of the list
+  uint32_t own = ORDER_NONE + 1;                           // what a logit has to reach for this warp's list
+  volatile uint32_t* least = s.least;
+  // The list in order, n of it at most; the warp's share in the bound.
+  auto put_in_order = [&]() {
+    __syncwarp();
+    for (int i = lane; i < count; i += 32) {
       const unsigned long long x = list[i];
       int before = 0;
       for (int j = 0; j < count; ++j) before += list[j] > x;
-      if (before < n) s.list[cur ^ 1][before] = x;
+      if (before < n) other[before] = x;
     }
-    have = min(n, count);
-    cur ^= 1;
-    __syncthreads();
-  }
-  unsigned long long* out = reinterpret_cast<unsigned long long*>(p.lists) + (row * p.parts + part) * n;
-  for (int i = tid; i < n; i += THREADS) out[i] = i < have ? s.list[cur][i] : 0ull;
+    __syncwarp();
+    unsigned long long* t = list;
+    list = other;
+    other = t;
+    count = min(count, n);
+    if (count == n) own = max(own, (uint32_t)(list[n - 1] >> 32) + 1);     // (of equals the earlier ones stay, and this warp's earlier ones come first)
+    if (count >= k && lane == 0) least[warp] = (uint32_t)(list[k - 1] >> 32);
+  };
+#pragma unroll 1
+  for (int t = 0; t < p.tiles; ++t) {
+    const int first = (part * p.tiles + t) * TILE + warp * WARP_TILE, left = p.vocab - first;
+    if (t > 0 && left <= 0) break;
+    if (t + AHEAD < p.tiles && lane < WARP_TILE * (BF16 ? 2 : 4) / 128 && left > AHEAD * TILE + lane * (128 / (BF16 ? 2 : 4)))
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(base + ((size_t)first + AHEAD * TILE) * (BF16 ? 2 : 4) + lane * 128));
+    float v[PER];
+    load_tile<BF16, VEC>(base, first, left, v);
+    const float m = largest(v);
+    const uint32_t mine = order_of(m);
+    if (t == 0) {
+      // the k-th largest of the lane maxima; where warps have nothing (short rows), for this warp alone the n-th, if there are as many lanes
+      const bool alone = n <= 32 && p.vocab - part * p.tiles * TILE < TILE;
+      uint32_t x = mine, top = 0, share = 0;
+      for (int i = 0; i < (alone ? n : k); ++i) {
+        top = __reduce_max_sync(0xffffffffu, x);
+        if (x == top) x = 0;
+        if (i == k - 1) share = top;
+      }
+      if (alone) own = max(own, top);
+      if (lane == 0) least[warp] = share;
+      __syncthreads();
+    }
+    if (fabsf(m) < INFINITY) sum.add(sum_quickly(v, m));
+    else if (!(m == -INFINITY)) sum = {__longlong_as_double(0x7ff8000000000000ll), 0, 0.f};          // NaN or +inf: the row counts for nothing
+    uint32_t bound = least[0];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum.add(sum.shuffled(o));
-  if (lane == 0) {
-    s.ref[warp] = sum.ref;
-    s.sum[warp] = sum.sum;
+    for (int w = 1; w < WARPS; ++w) bound = min(bound, least[w]);
+    bound = max(bound, own);
+    if (!__any_sync(0xffffffffu, mine >= bound)) continue;
+    auto key = [&](int j) { return (unsigned long long)order_of(v[j]) << 32 | (uint32_t)~(first + place<BF16, VEC>(j)); };
+    int all = count;
+    auto collect = [&]() {                                 // what reaches the bound behind the list; how many there are then
+      if (lane == 0) s.n_list[warp] = count;
+      __syncwarp();
+      if (mine >= bound) {
+        const float least_of_all = from_order(bound);
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (v[j] >= least_of_all) {
+            const int at = atomicAdd(&s.n_list[warp], 1);
+            if (at < LIST) list[at] = key(j);
+          }
+      }
+      __syncwarp();
+      all = *(volatile int*)&s.n_list[warp];
+    };
+    collect();
+    if (all > LIST) {                                      // more than there is room for: first only the n best of those before, then of these
+      put_in_order();
+      bound = max(bound, own);
+      collect();
+      if (all > LIST) {
+        uint32_t cut;
+        int end;
+        cut_tile<BF16, VEC>(v, n, cut, end);
+        if (lane == 0) s.n_list[warp] = count;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const uint32_t o = order_of(v[j]);
+          if (o > cut || o == cut && place<BF16, VEC>(j) <= end) list[atomicAdd(&s.n_list[warp], 1)] = key(j);           // (n at most; LIST >= 2 n)
+        }
+        __syncwarp();
+        all = *(volatile int*)&s.n_list[warp];
+      }
+    }
+    count = all;
+    if (count > n + (n > 32 ? n / 2 : 0)) put_in_order();  // (at once where that is one look of every lane: a bound that is behind lets more in)
+  }
+  if (count > n) put_in_order();
+  __syncthreads();
+  uint32_t bound = s.least[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) bound = min(bound, s.least[w]);
+  unsigned long long* found = s.joined;
+  for (int i = lane; i < count; i += 32) {
+    const unsigned long long x = list[i];
+    if ((uint32_t)(x >> 32) >= bound) found[atomicAdd(&s.count, 1)] = x;
   }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < WARPS; ++w) sum.add({s.ref[w], s.sum[w]});
-    reinterpret_cast<double2*>(p.sums)[row * p.parts + part] = make_double2(sum.ref, sum.sum);
+  const int have = s.count;
+  unsigned long long* out = reinterpret_cast<unsigned long long*>(p.lists) + (row * p.parts + part) * n;
+  for (int i = tid; i < have; i += THREADS) {
+    const unsigned long long x = found[i];
+    int before = 0;
+    for (int j = 0; j < have; ++j) before += found[j] > x;
+    if (before < n) out[before] = x;
   }
+  for (int i = have + tid; i < n; i += THREADS) out[i] = 0ull;
+  block_sum(sum, s.sum);
+  if (tid == 0) reinterpret_cast<Sum<false>*>(p.sums)[row * p.parts + part] = sum;
 }
 
+// total = (x - ref) + base, so that large logits lose nothing; base: score - log of the sum, -inf where the beam offers nothing of its row.
+struct Beam {
+  double ref, base, off;                   // off: how far totals may be off
+};
 struct Candidate {
   double total;
-  long long flat;                          // beam * vocabulary + token
+  long long place;                         // beam << 32 | token
+  float x;                                 // logit; score of a beam at its end
+  __device__ __forceinline__ int beam() const { return (int)(place >> 32); }
+  __device__ __forceinline__ bool before(const Candidate& o) const { return total > o.total || total == o.total && place < o.place; }
 };
-__device__ __forceinline__ bool before(double a, long long fa, double b, long long fb) { return a > b || a == b && fa < fb; }
 
+struct Join {
+  Beam beam[MAX_BEAMS];
+  unsigned char again[MAX_BEAMS];            // beams whose order is not certain
+  unsigned char has_lists[MAX_BEAMS];        // beams that offer tokens
+  Candidate cand[CAP];                       // any order
+  ulonglong2 key[CAP];                       // their totals as numbers, and places
+  unsigned short order[CAP];                 // best first
+  alignas(16) uint32_t sample[THREADS];
+  float bound;
+  Sum<true> sum[WARPS], share;
+  uint32_t hi[32], lo[32];
+  Candidate best[WARPS];
+  int from[WARPS], list[MAX_BEAMS];
+  int count, n_again;
+};
+
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ Sum<true> of_rank(const Sum<true>* p, uint32_t rank) {
+  uint32_t a;
+  Sum<true> s;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(s.sum) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.b32 %0, [%1 + 8];" : "=r"(s.k) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1 + 12];" : "=f"(s.far) : "r"(a) : "memory");
+  return s;
+}
+
+template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 select_join_kernel(const __grid_constant__ SelectCall p) {
-  // total = (x - ref) + base, so that large logits lose nothing; base: score - log of the sum, -inf where the beam offers nothing of its row
-  __shared__ double s_ref[MAX_BEAMS], s_base[MAX_BEAMS];
-  __shared__ int s_active[MAX_BEAMS];        // beams that offer
-  __shared__ Candidate s_cand[CAP];
-  __shared__ unsigned long long s_least[WARPS];
-  __shared__ int s_count, s_n_active;
+  __shared__ Join s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x, W = p.beams, n = p.n;
+  // the blocks of a cluster do the same work, apart from the rows that are summed again; the first writes the results
+  const int b = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster, W = p.beams, n = p.n;
   pdl_wait();
   pdl_launch_dependents();
   const size_t row0 = (size_t)b * W;
+  auto offers = [&](int w) { return fabsf(p.scores[row0 + w]) < INFINITY; };
+  auto finished = [&](int w) { return p.finished && p.finished[row0 + w]; };
+  const double off = off_of(p.vocab);
+  auto settle = [&](int w, float score, double ref, double sum, double off) {
+    const double base = (double)score - log(sum);
+    const bool ok = base > -INFINITY && base < INFINITY && ref < INFINITY;             // (not a row with NaN or +inf, or of nothing but -inf)
+    s.beam[w] = {ok ? ref : 0.0, ok ? base : -INFINITY, off};
+    s.has_lists[w] = ok;
+  };
   for (int w = warp; w < W; w += WARPS) {                  // a warp per beam
     const float score = p.scores[row0 + w];
-    double base = -INFINITY, ref = 0.0;
-    if (!(p.finished && p.finished[row0 + w]) && fabsf(score) < INFINITY) {
-      Sum sum = {-INFINITY, 0.0};
-      for (int i = lane; i < p.parts; i += 32) {
-        const double2 x = reinterpret_cast<const double2*>(p.sums)[(row0 + w) * p.parts + i];
-        sum.add({x.x, x.y});
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum.add(sum.shuffled(o));
-      base = (double)score - log(sum.sum);
-      ref = sum.ref;
-      if (!(base > -INFINITY && base < INFINITY && ref < INFINITY)) base = -INFINITY;        // a row with NaN or +inf, or of nothing but -inf
-    }
-    if (lane == 0) {
-      s_base[w] = base;
-      s_ref[w] = ref;
-    }
+    const bool ended = finished(w);
+    Sum<false> sum = {0.0, 0, 0.f};                        // (of a beam that offers nothing: what lies there, and does not count)
+    for (int i = lane; i < p.parts; i += 32) sum.add(reinterpret_cast<const Sum<false>*>(p.sums)[(row0 + w) * p.parts + i]);
+    warp_sum(sum);
+    if (lane == 0) settle(w, score, sum.ref(), ended || !(fabsf(score) < INFINITY) ? 0.0 : sum.sum, off);
   }
-  if (tid == 0) s_count = 0;
+  for (int w = tid; w < W; w += THREADS) s.again[w] = 0;
+  if (tid == 0) s.count = s.n_again = 0;
   __syncthreads();
-  if (warp == 0) {
-    int active = 0;
-    for (int w0 = 0; w0 < W; w0 += 32) {
-      const bool on = w0 + lane < W && s_base[w0 + lane] > -INFINITY;
-      const uint32_t go = __ballot_sync(0xffffffffu, on);
-      if (on) s_active[active + __popc(go & ((1u << lane) - 1))] = w0 + lane;
-      active += __popc(go);
-    }
-    if (lane == 0) s_n_active = active;
-  }
-  __syncthreads();
-  const int lists = s_n_active * p.parts;
-  auto entry = [&](int list, int i, long long& flat) {     // total of the i-th of a list, -inf where there is none
-    const int w = s_active[list / p.parts];
-    const unsigned long long x = reinterpret_cast<const unsigned long long*>(p.lists)[((row0 + w) * p.parts + list % p.parts) * n + i];
-    flat = (long long)w * p.vocab + (uint32_t)~(uint32_t)x;
-    return x == 0 ? -INFINITY : ((double)from_order((uint32_t)(x >> 32)) - s_ref[w]) + s_base[w];
+  const int lists = W * p.parts;
+  auto of_beam = [&](int w, float x) { return ((double)x - s.beam[w].ref) + s.beam[w].base; };
+  auto entry = [&](int list, int i) -> Candidate {         // the i-th of a list, a total of -inf where there is none
+    const int w = (int)((uint32_t)list / (uint32_t)p.parts);
+    if (!s.has_lists[w]) return {-INFINITY, 0, 0.f};       // (nothing has been written there)
+    const unsigned long long y = reinterpret_cast<const unsigned long long*>(p.lists)[(row0 * p.parts + list) * n + i];
+    const float x = from_order((uint32_t)(y >> 32));
+    return {y == 0 ? -INFINITY : of_beam(w, x), (long long)w << 32 | (uint32_t)~(uint32_t)y, x};
   };
-  // a bound from below of the n-th largest, as in the rows: from the first d entries of the lists
-  const int k = (n + WARPS - 1) / WARPS;
-  unsigned long long bound = 0;
-  if (lists > 0) {
-    const int d = min(n, (WARPS * k + lists - 1) / lists);
-    double top = -INFINITY;
-    for (int q = warp + WARPS * lane; q < lists * d; q += THREADS) {
-      long long flat;
-      const double x = entry(q / d, q % d, flat);
-      top = x > top ? x : top;
-    }
-    unsigned long long x = order_of(top), most = 0;
-    for (int i = 0; i < k; ++i) {
-      const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32));
-      const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32) == hi ? (uint32_t)x : 0u);
-      most = (unsigned long long)hi << 32 | lo;
-      if (x == most) x = 0;
-    }
-    if (lane == 0) s_least[warp] = most;
-    __syncthreads();
-    bound = s_least[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) bound = min(bound, s_least[w]);
-  }
-  auto finished = [&](int w) { return p.finished && p.finished[row0 + w] && fabsf(p.scores[row0 + w]) < INFINITY; };
-  auto push = [&](double total, long long flat) {
-    const int at = atomicAdd(&s_count, 1);
-    if (at < CAP) s_cand[at] = {total, flat};
+  auto push = [&](const Candidate& c) {
+    const int at = atomicAdd(&s.count, 1);
+    if (at < CAP) s.cand[at] = c;
   };
-  for (int list = warp; list < lists; list += WARPS)       // a warp per list, as far as it reaches the bound
-    for (int i = 0; i < n; i += 32) {
-      long long flat = 0;
-      const double x = i + lane < n ? entry(list, i + lane, flat) : -INFINITY;
-      const bool in = x > -INFINITY && order_of(x) >= bound;
-      if (in) push(x, flat);
-      if (!__all_sync(0xffffffffu, in)) break;
-    }
-  if (p.finished)
-    for (int w = tid; w < W; w += THREADS)
-      if (finished(w)) push((double)p.scores[row0 + w], (long long)w * p.vocab + p.pad_token);
-  __syncthreads();
-  int count = s_count;
-  auto put = [&](int rank, double total, long long flat) {
-    const size_t at = (size_t)b * n + rank;
-    p.out_scores[at] = (float)total;
-    p.out_parents[at] = (int)(flat / p.vocab);
-    p.out_tokens[at] = (int)(flat % p.vocab);
-  };
-  if (count <= CAP) {
-    for (int i = tid; i < count; i += THREADS) {
-      const Candidate x = s_cand[i];
-      int rank = 0;
-      for (int j = 0; j < count; ++j) rank += before(s_cand[j].total, s_cand[j].flat, x.total, x.flat);
-      if (rank < n) put(rank, x.total, x.flat);
+  if (lists * n <= THREADS) {                              // all there are
+    if (tid < lists * n) {
+      const Candidate c = entry((uint32_t)tid / (uint32_t)n, (uint32_t)tid % (uint32_t)n);
+      if (c.total > -INFINITY) push(c);
     }
   } else {
-    // more candidates tie with the n-th than are ordered by counting: the best head of all lists, n times
-    __shared__ Candidate s_best[WARPS];
-    __shared__ int s_from[WARPS];
-    // a thread's lists are its own, so that their places need no other: list l belongs to thread l % THREADS; 16 bits for each in s_cand's room
-    unsigned short* at = reinterpret_cast<unsigned short*>(s_cand);
-    const int all = lists + W;                             // (behind the lists: beams at their end)
+    // A bound from below of the n-th largest: that of THREADS of them, the first d of every list or the best of several lists' first.  As
+    // numbers of 32 bits, rounded down, the last eight the thread's, so that no two are equal; lower by how far two totals may be off.
+    const int d = lists < THREADS ? THREADS / lists : 1;
+    double mine = -INFINITY;
+    if (d > 1) {
+      if (tid < lists * d) mine = entry((uint32_t)tid / (uint32_t)d, (uint32_t)tid % (uint32_t)d).total;
+    } else {
+      for (int list = tid; list < lists; list += THREADS) mine = fmax(mine, entry(list, 0).total);
+    }
+    const uint32_t key = order_of(__double2float_rd(mine - 2 * off)) & ~255u | (uint32_t)(255 - tid);
+    s.sample[tid] = key;
+    if (tid == 0) s.bound = -INFINITY;
     __syncthreads();
-    for (int l = tid; l < all; l += THREADS) at[l] = l < lists || finished(l - lists) ? 0 : 1;
-    count = 0;
+    int above = 0;
+#pragma unroll 8
+    for (int i = 0; i < THREADS / 4; ++i) {
+      const uint4 x = reinterpret_cast<const uint4*>(s.sample)[i];
+      above += (int)(x.x > key) + (int)(x.y > key) + (int)(x.z > key) + (int)(x.w > key);
+    }
+    if (above == n - 1 && key > (ORDER_NONE | 255u)) s.bound = from_order(key & ~255u);
+    __syncthreads();
+    const double bound = s.bound;
+    auto reaches = [&](const Candidate& c) { return c.total > -INFINITY && c.total >= bound; };
+    for (int list = tid; list < lists; list += THREADS)    // a thread per list, whose entries are in order, four on their way at a time
+      for (int i = 0; i < n; i += 4) {
+        Candidate c[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) c[x] = i + x < n ? entry(list, i + x) : Candidate{-INFINITY, 0, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (reaches(c[x])) push(c[x]);
+        if (!reaches(c[3])) break;
+      }
+  }
+  for (int w = tid; w < W; w += THREADS)
+    if (finished(w) && offers(w)) {
+      s.beam[w] = {0.0, 0.0, 0.0};                         // offers its score, which is what it is
+      push({(double)p.scores[row0 + w], (long long)w << 32 | p.pad_token, p.scores[row0 + w]});
+    }
+  __syncthreads();
+  const int count = s.count;
+  const bool ties = count > CAP;                           // more candidates about the n-th than are ordered by counting
+  auto put = [&](int r, const Candidate& c) {
+    if (rank > 0) return;
+    const size_t at = (size_t)b * n + r;
+    p.out_scores[at] = (float)c.total;
+    p.out_parents[at] = c.beam();
+    p.out_tokens[at] = (int)(uint32_t)c.place;
+  };
+  for (;;) {
+    if (ties) {
+      for (int w = tid; w < W; w += THREADS) s.again[w] = W > 1 && s.beam[w].base > -INFINITY && s.beam[w].off > 0.0;
+    } else {
+      for (int i = tid; i < count; i += THREADS) s.key[i] = make_ulonglong2(order_of(s.cand[i].total), (unsigned long long)s.cand[i].place);
+      __syncthreads();
+      for (int i = tid; i < count; i += THREADS) {
+        const ulonglong2 x = s.key[i];
+        int better = 0;
+#pragma unroll 4
+        for (int j = 0; j < count; ++j) {
+          const ulonglong2 y = s.key[j];
+          better += (int)(y.x > x.x) | ((int)(y.x == x.x) & (int)(y.y < x.y));         // (no branches)
+        }
+        s.order[better] = (unsigned short)i;
+      }
+      __syncthreads();
+      for (int r = tid; r < n && r + 1 < count; r += THREADS) {            // (the last one's neighbour is the first that is left out)
+        const Candidate &x = s.cand[s.order[r]], &y = s.cand[s.order[r + 1]];
+        const int v = x.beam(), w = y.beam();
+        if (v != w && x.total - y.total <= s.beam[v].off + s.beam[w].off) s.again[v] = s.again[w] = 1;
+      }
+    }
+    __syncthreads();
+    if (warp == 0) {
+      int found = 0;
+      for (int w0 = 0; w0 < W; w0 += 32) {
+        const bool on = w0 + lane < W && s.again[w0 + lane] && s.beam[w0 + lane].off > 0.0;
+        const uint32_t go = __ballot_sync(0xffffffffu, on);
+        if (on) s.list[found + __popc(go & ((1u << lane) - 1))] = w0 + lane;
+        found += __popc(go);
+      }
+      if (lane == 0) s.n_again = found;
+      if (found) {
+        const double T = exp2(lane / 32.0);
+        s.hi[lane] = (uint32_t)__double2hiint(T);
+        s.lo[lane] = (uint32_t)__double2loint(T);
+      }
+    }
+    __syncthreads();
+    if (s.n_again == 0) break;
+    const Table table = {s.hi, s.lo};
+    for (int a = 0; a < s.n_again; ++a) {                  // (every beam once at most: its `off` is 0 afterwards)
+      const int w = s.list[a];
+      const char* base = reinterpret_cast<const char*>(p.logits) + (row0 + w) * (size_t)p.row_stride * (BF16 ? 2 : 4);
+      Sum<true> sum = {0.0, 0, 0.f};
+#pragma unroll 1
+      for (int first = (rank * WARPS + warp) * WARP_TILE; first < p.vocab; first += p.cluster * TILE) {
+        float v[PER];
+        load_tile<BF16, VEC>(base, first, p.vocab - first, v);
+        const float m = largest(v);
+        if (fabsf(m) < INFINITY) sum.add(sum_exactly(v, m, table));        // (others than -inf are not among a beam's that offers)
+      }
+      block_sum(sum, s.sum);
+      if (p.cluster > 1) {                                 // (all blocks of a cluster come here for the same beams)
+        if (tid == 0) s.share = sum;
+        cluster_sync();
+        if (warp == 0) {
+          sum = of_rank(&s.share, lane < p.cluster ? lane : 0);
+          if (lane >= p.cluster) sum.sum = 0.0;
+          warp_sum(sum);
+        }
+        cluster_sync();                                    // read before the next beam's, or the block's end
+      }
+      if (tid == 0) settle(w, p.scores[row0 + w], sum.ref(), sum.sum, 0.0);
+      __syncthreads();
+    }
+    if (!ties)
+      for (int i = tid; i < count; i += THREADS) {
+        Candidate& c = s.cand[i];
+        c.total = of_beam(c.beam(), c.x);
+      }
+    __syncthreads();
+  }
+  int done = min(count, n);
+  if (!ties) {
+    for (int r = tid; r < done; r += THREADS) put(r, s.cand[s.order[r]]);
+  } else {
+    // the best head of all lists, n times: a thread's lists are its own, list l thread l % THREADS's, their places 16 bits each in s.cand's room
+    unsigned short* at = reinterpret_cast<unsigned short*>(s.cand);
+    const int all = lists + W;                             // (behind the lists: beams at their end)
+    for (int l = tid; l < all; l += THREADS) at[l] = l < lists || finished(l - lists) && offers(l - lists) ? 0 : 1;
+    done = 0;
     for (int r = 0; r < n; ++r) {
-      double best = -INFINITY;
-      long long where = 0x7fffffffffffffffll;
+      Candidate best = {-INFINITY, 0x7fffffffffffffffll, 0.f};
       int from = -1;
       for (int l = tid; l < all; l += THREADS) {
-        double x = -INFINITY;
-        long long flat = 0;
+        Candidate c = {-INFINITY, 0, 0.f};
         if (l < lists) {
-          if (at[l] < n) x = entry(l, at[l], flat);
+          if (at[l] < n) c = entry(l, at[l]);
         } else if (at[l] == 0) {
-          x = (double)p.scores[row0 + l - lists];
-          flat = (long long)(l - lists) * p.vocab + p.pad_token;
+          c = {(double)p.scores[row0 + l - lists], (long long)(l - lists) << 32 | p.pad_token, 0.f};
         }
-        if (x > -INFINITY && before(x, flat, best, where)) {
-          best = x;
-          where = flat;
+        if (c.total > -INFINITY && c.before(best)) {
+          best = c;
           from = l;
         }
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
-        const double x = __shfl_xor_sync(0xffffffffu, best, o);
-        const long long f = __shfl_xor_sync(0xffffffffu, where, o);
+        const Candidate c = {__shfl_xor_sync(0xffffffffu, best.total, o), __shfl_xor_sync(0xffffffffu, best.place, o), 0.f};
         const int l = __shfl_xor_sync(0xffffffffu, from, o);
-        if (before(x, f, best, where)) {
-          best = x;
-          where = f;
+        if (c.before(best)) {
+          best = c;
           from = l;
         }
       }
       __syncthreads();
       if (lane == 0) {
-        s_best[warp] = {best, where};
-        s_from[warp] = from;
+        s.best[warp] = best;
+        s.from[warp] = from;
       }
       __syncthreads();
       for (int w = 0; w < WARPS; ++w)
-        if (before(s_best[w].total, s_best[w].flat, best, where)) {
-          best = s_best[w].total;
-          where = s_best[w].flat;
-          from = s_from[w];
+        if (s.best[w].before(best)) {
+          best = s.best[w];
+          from = s.from[w];
         }
       if (from < 0) break;
       if (from % THREADS == tid) ++at[from];
-      if (tid == 0) put(r, best, where);
-      ++count;
+      if (tid == 0) put(r, best);
+      ++done;
     }
   }
-  for (int r = count + tid; r < n; r += THREADS) {
+  for (int r = done + tid; r < n && rank == 0; r += THREADS) {
     const size_t at = (size_t)b * n + r;
     p.out_scores[at] = -INFINITY;
     p.out_parents[at] = p.out_tokens[at] = -1;
@@ -541,10 +725,27 @@ extern "C" int b200_beam_select(const SelectCall* call) {
       a.pad_token < 0 || a.pad_token >= a.vocab)
     return -ERR_BAD_ARG;
   const dim3 grid(a.parts, a.requests * a.beams), block(select::THREADS);
-  cudaError_t e = a.bf16 ? (a.vectors ? launch_pdl(select::select_parts_kernel<true, true>, grid, block, 0, a.stream, a)
-                                      : launch_pdl(select::select_parts_kernel<true, false>, grid, block, 0, a.stream, a))
-                         : (a.vectors ? launch_pdl(select::select_parts_kernel<false, true>, grid, block, 0, a.stream, a)
-                                      : launch_pdl(select::select_parts_kernel<false, false>, grid, block, 0, a.stream, a));
-  if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(select::select_join_kernel, dim3(a.requests), block, 0, a.stream, a);
+  SelectCall c = a;
+  c.cluster = 8;
+  while (c.cluster > 1 && c.cluster * c.requests > 148 * 3) c.cluster /= 2;
+  auto both = [&](auto parts, auto joined) {
+    cudaError_t e = launch_pdl(parts, grid, block, 0, c.stream, c);
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c.requests * c.cluster);
+    cfg.blockDim = block;
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = c.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = c.cluster > 1 ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, joined, c);
+  };
+  using namespace select;
+  if (a.bf16) return a.vectors ? both(select_parts_kernel<true, true>, select_join_kernel<true, true>) : both(select_parts_kernel<true, false>, select_join_kernel<true, false>);
+  return a.vectors ? both(select_parts_kernel<false, true>, select_join_kernel<false, true>) : both(select_parts_kernel<false, false>, select_join_kernel<false, false>);
 }

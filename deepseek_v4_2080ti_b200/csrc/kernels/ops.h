@@ -207,7 +207,7 @@ struct SpansCall {
   float* workspace;                           // [splits T Hq 130]: partial sums of several items, or of the shared keys
   int* status;
   cudaStream_t stream;
-  int n_groups, max_q_len, T, max_blocks, num_blocks, block_size, n_q_heads, n_kv_heads, splits, cluster, tree_words;
+  int n_groups, max_q_len, T, max_blocks, num_blocks, block_size, n_q_heads, n_kv_heads, splits, cluster, tree_words, per_item;
   float scale, cap;
 };
 int b200_qk_norm_rope_axes_append(const AxesAppendCall* call);
@@ -216,8 +216,15 @@ int b200_attn_shared(const SpansCall* call);
 int b200_attn_tree(const SpansCall* call);
 
 // ---- drafted trees (tree.cu): positions int32 [T] and masks [T, words] of their rows; the path that the target agrees with
-int b200_tree_layout(const int* parents, const int* q_start, const int* q_len, const int* kv_len, int batch, int T, int words,
-                     int* positions, uint32_t* mask, cudaStream_t stream);
+struct TreeLayoutCall {
+  int bytes, batch;
+  const int *parents, *q_start, *q_len, *kv_len;
+  int* positions;
+  uint32_t* mask;
+  cudaStream_t stream;
+  int T, words;
+};
+int b200_tree_layout(const struct TreeLayoutCall* call);
 enum { ACCEPT_CACHES = 16 };
 struct AcceptCache {
   void* base;                                 // [layers, num_blocks, heads, block_size, row_bytes], layers layer_bytes apart
@@ -249,6 +256,7 @@ struct SelectCall {
   int *out_parents, *out_tokens;
   cudaStream_t stream;
   int beams, vocab, n, parts, tiles, bf16, pad_token, vectors;     // tiles: of 8192 logits in a part; vectors: rows on 16-byte boundaries
+  int cluster, unused;                        // (set here)
 };
 int b200_beam_select(const struct SelectCall* call);
 enum { REORDER_STATES = 16 };

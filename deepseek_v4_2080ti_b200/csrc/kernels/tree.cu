@@ -172,11 +172,11 @@ tree_accept_kernel(const __grid_constant__ AcceptCall p) {
 
 using namespace b200;
 
-extern "C" int b200_tree_layout(const int* parents, const int* q_start, const int* q_len, const int* kv_len, int batch, int T, int words,
-                                int* positions, uint32_t* mask, cudaStream_t stream) {
-  if (T < 1 || batch < 0 || words < 1 || words > tree::MAX_NODES / 32) return -ERR_BAD_ARG;
-  return (int)launch_pdl(tree::tree_layout_kernel, dim3((T + 7) / 8), dim3(256), 0, stream, parents, q_start, q_len, kv_len, batch, T, words,
-                         positions, mask);
+extern "C" int b200_tree_layout(const TreeLayoutCall* call) {
+  const TreeLayoutCall& a = *call;
+  if (a.bytes != (int)sizeof(a) || a.T < 1 || a.batch < 0 || a.words < 1 || a.words > tree::MAX_NODES / 32) return -ERR_BAD_ARG;
+  return (int)launch_pdl(tree::tree_layout_kernel, dim3((a.T + 7) / 8), dim3(256), 0, a.stream, a.parents, a.q_start, a.q_len, a.kv_len, a.batch, a.T,
+                         a.words, a.positions, a.mask);
 }
 
 extern "C" int b200_tree_accept(const AcceptCall* call) {

@@ -272,7 +272,7 @@ def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
 
 
 # The kernels' arguments as one block each (AxesAppendCall and SpansCall in ops.h), packed: a third of what 33 arguments cost one by one.
-_AXES_CALL, _SPANS_CALL = struct.Struct("@ii13P16iff64s"), struct.Struct("@ii17P11iff0P")
+_AXES_CALL, _SPANS_CALL = struct.Struct("@ii13P16iff64s"), struct.Struct("@ii17P12iff0P")
 _typed = False
 
 
@@ -483,7 +483,7 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
     rc = _kernels().b200_attn_spans(_SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
         q_start.data_ptr(), q_len.data_ptr(), _at(lo), _at(hi), 0, 0, 0, _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq, hkv,
-        splits, 1, 0, scale, cap))
+        splits, 1, 0, 0, scale, cap))
     _lib.check(rc, "prefill_spans", 2 if splits > 1 else 1)
     return out
 
@@ -533,8 +533,9 @@ def decode_tree(q, k_cache, v_cache, block_table, mask, q_start, q_len, kv_len, 
         raise ValueError(f"trees of {max_q_len} rows, masks of {32 * words} nodes")
     if t == 0 or b == 0 or max_q_len <= 0:
         return out
+    longest = max_kv_len if max_kv_len is not None else width * bs
     if splits is None:
-        splits = _row_splits(b, t, hq // hkv, hkv, max_q_len, max_kv_len if max_kv_len is not None else width * bs)
+        splits = _row_splits(b, t, hq // hkv, hkv, max_q_len, longest)
     if not 1 <= splits <= 1024:
         raise ValueError(f"{splits} splits")
     ws = q.new_empty(splits * t * hq * (D + 2), dtype=_F32) if splits > 1 else None
@@ -542,7 +543,7 @@ def decode_tree(q, k_cache, v_cache, block_table, mask, q_start, q_len, kv_len, 
     rc = _kernels().b200_attn_tree(_SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
         q_start.data_ptr(), q_len.data_ptr(), _at(lo), 0, 0, 0, mask.data_ptr(), _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq,
-        hkv, splits, 1, words, scale, cap))
+        hkv, splits, 1, words, max(1, -(-longest // (KEY_TILE * splits))), scale, cap))
     _lib.check(rc, "decode_tree", 2 if splits > 1 else 1)
     return out
 
@@ -640,7 +641,7 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     call = _SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
         0, 0, 0, 0, group_start.data_ptr(), shared_len.data_ptr(), 0, _at(ws), _status(dev), _stream(dev), n, 1, t, width, nb, bs, hq, hkv, splits, cluster,
-        0, scale, cap)
+        0, 0, scale, cap)
     if n:
         _lib.check(lib.b200_attn_shared(call), "decode_shared")
     _lib.check(lib.b200_attn_own_rows(call), "decode_shared")

@@ -7,6 +7,8 @@ states in their new order.
 The same selection grows a drafted tree (``ops.tree``): the beams are its newest nodes, the candidates the nodes that it gets next."""
 from __future__ import annotations
 
+import ctypes
+import functools
 import struct
 
 import torch
@@ -18,8 +20,22 @@ MAX_BEAMS, MAX_CANDIDATES = 128, 128
 MAX_STATES = 16                          # tensors of one launch
 TILE = 8192                              # logits that a block looks at together
 NUM_SMS = 148
-_SELECT = struct.Struct("@iiPqPPPPPPPP8i0P")
-_REORDER, _STATE, _REORDER_BYTES = struct.Struct("@iiPPPP4i"), struct.Struct("@Pqqqii"), 56 + MAX_STATES * 40
+# SelectCall, ReorderCall and ReorderState in ops.h, packed
+_SELECT = struct.Struct("@iiPqPPPPPPPP10i0P")
+_REORDER, _STATE = struct.Struct("@iiPPPP4i"), struct.Struct("@Pqqqii")
+_REORDER_BYTES = _REORDER.size + MAX_STATES * _STATE.size
+_REST = [b"\0" * ((MAX_STATES - i) * _STATE.size) for i in range(MAX_STATES + 1)]
+_typed = False
+
+
+def _kernels() -> ctypes.CDLL:
+    global _typed
+    lib = _lib.lib()
+    if not _typed:
+        for f in (lib.b200_beam_select, lib.b200_beam_reorder):
+            f.argtypes = [ctypes.c_char_p]
+        _typed = True
+    return lib
 
 
 def _parts(rows: int, vocab: int) -> tuple[int, int]:
@@ -62,25 +78,27 @@ def select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None, fin
     if b * w > 65535:
         raise ValueError(f"{b} requests of {w} beams: 65535 rows at most")
     out_scores = scores.new_empty(b, n)
-    parents, tokens = (torch.empty(b, n, dtype=torch.int32, device=logits.device) for _ in range(2))
+    parents = torch.empty(b, n, dtype=torch.int32, device=logits.device)
+    tokens = torch.empty_like(parents)
     if b == 0:
         return out_scores, parents, tokens
     parts, tiles = _parts(b * w, v)
     size = logits.element_size()
     vectors = logits.data_ptr() % 16 == 0 and row * size % 16 == 0 and v * size % 16 == 0
     lists = torch.empty(b * w * parts * (n + 2), dtype=torch.int64, device=logits.device)      # and two doubles a part
-    rc = _lib.lib().b200_beam_select(_SELECT.pack(
+    rc = _kernels().b200_beam_select(_SELECT.pack(
         _SELECT.size, b, logits.data_ptr(), row, scores.data_ptr(), _at(finished), lists.data_ptr() + 16 * b * w * parts, lists.data_ptr(),
-        out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _stream(dev), w, v, n, parts, tiles, size == 2, pad_token, vectors))
+        out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _stream(dev), w, v, n, parts, tiles, size == 2, pad_token, vectors, 0, 0))
     _lib.check(rc, "beam_select", 2)
     return out_scores, parents, tokens
 
 
-def _state(x, dim: int, dev: int) -> tuple[int, bytes]:
-    """Checks a tensor of states; its number of slots, and what the kernel takes."""
-    shape, stride, size = x.shape, x.stride(), x.element_size()
-    if x.get_device() != dev or not 0 <= dim < len(shape) or x.numel() == 0:
-        raise ValueError(f"states: tensors on cuda:{dev} with slots along axis {dim} expected, got {list(shape)} on {x.device}")
+@functools.lru_cache(maxsize=256)
+def _state(shape: tuple, stride: tuple, size: int, dim: int) -> tuple[int, tuple[int, int, int, int], int]:
+    """Checks the sizes of a tensor of states (elements of ``size`` bytes); its slots, bytes from part to part before the axis, from slot to slot and
+    of a slot, number of such parts, and the low bits of all three."""
+    if not 0 <= dim < len(shape) or min(shape) < 1:
+        raise ValueError(f"states: slots along axis {dim} expected, got {list(shape)}")
     inner = 1
     for d in range(len(shape) - 1, dim, -1):
         if shape[d] != 1 and stride[d] != inner:
@@ -96,8 +114,8 @@ def _state(x, dim: int, dev: int) -> tuple[int, bytes]:
     slots = shape[dim]
     if slots > 1 and stride[dim] < inner or outer > 1 and step < inner:
         raise ValueError(f"states: slots that lie apart expected, got strides {list(stride)} of {list(shape)}")
-    at, step, slot, inner = x.data_ptr(), step * size, stride[dim] * size, inner * size
-    return slots, _STATE.pack(at, step, slot, inner, outer, (at | step | slot | inner) % 16 == 0)
+    step, slot, inner = step * size, stride[dim] * size if slots > 1 else 0, inner * size
+    return slots, (step, slot, inner, outer), (step | slot | inner) & 15
 
 
 def reorder(states, parents: torch.Tensor, slots: torch.Tensor | None = None, dim: int = 0) -> None:
@@ -119,19 +137,24 @@ def reorder(states, parents: torch.Tensor, slots: torch.Tensor | None = None, di
         _index(slots, (b, w), dev, "slots")
     if not 0 < w <= MAX_BEAMS:
         raise ValueError(f"{w} beams: 1 to {MAX_BEAMS} expected")
-    states = [states] if isinstance(states, torch.Tensor) else list(states)
-    found = [_state(x, dim, dev) for x in states]
-    if not found or any(n != found[0][0] for n, _ in found):
-        raise ValueError(f"states: tensors of one number of slots expected, got {[n for n, _ in found]}")
-    if len({x.data_ptr() for x in states}) < len(states):
-        raise ValueError("states: a tensor that is there twice would move twice")
-    n_slots = found[0][0]
+    states = [states] if isinstance(states, torch.Tensor) else states
+    packed, n_slots = {}, None
+    for x in states:
+        n, sizes, low = _state(x.shape, x.stride(), x.element_size(), dim)
+        at = x.data_ptr()
+        if x.get_device() != dev or n_slots is not None and n != n_slots or at in packed:
+            raise ValueError(f"states: different tensors of one number of slots on cuda:{dev} expected, got {list(x.shape)} on {x.device}")
+        n_slots = n
+        packed[at] = _STATE.pack(at, *sizes, (at | low) & 15 == 0)
+    if n_slots is None:
+        raise ValueError("states: a tensor or several expected")
     if slots is None and b * w > n_slots:
         raise ValueError(f"{b} requests of {w} beams in {n_slots} slots")
     if b == 0:
         return
     _lib.check_indices(slots, 0, n_slots, 4)
-    for i in range(0, len(found), MAX_STATES):
-        some = found[i:i + MAX_STATES]
+    packed = list(packed.values())
+    for i in range(0, len(packed), MAX_STATES):
+        some = packed[i:i + MAX_STATES]
         call = _REORDER.pack(_REORDER_BYTES, b, parents.data_ptr(), _at(slots), _status(dev), _stream(dev), w, n_slots, len(some), 0)
-        _lib.check(_lib.lib().b200_beam_reorder((call + b"".join(s for _, s in some)).ljust(_REORDER_BYTES, b"\0")), "beam_reorder")
+        _lib.check(_kernels().b200_beam_reorder(call + b"".join(some) + _REST[len(some)]), "beam_reorder")

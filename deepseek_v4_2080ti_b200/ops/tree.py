@@ -11,6 +11,8 @@ last, then the drafts.  ``parents[t]`` is the node of its own tree that row t co
 come out are distributed as without drafts.  The context grows by ``count``: kv_len - q_len + count keys are valid after it."""
 from __future__ import annotations
 
+import ctypes
+import functools
 import struct
 
 import torch
@@ -20,7 +22,21 @@ from .attention import MAX_TREE, _at, _current, _index, _stream
 
 MAX_PATH = 256                           # longest path that is kept
 MAX_CACHES = 16
-_CALL, _CACHE, _CALL_BYTES = struct.Struct("@ii10PP6i"), struct.Struct("@Pqiiii"), 120 + MAX_CACHES * 32
+# TreeLayoutCall, AcceptCall and AcceptCache in ops.h, packed
+_LAYOUT, _CALL, _CACHE = struct.Struct("@ii7Pii"), struct.Struct("@ii10PP6i"), struct.Struct("@Pqiiii")
+_CALL_BYTES = _CALL.size + MAX_CACHES * _CACHE.size
+_REST = [b"\0" * ((MAX_CACHES - i) * _CACHE.size) for i in range(MAX_CACHES + 1)]
+_typed = False
+
+
+def _kernels() -> ctypes.CDLL:
+    global _typed
+    lib = _lib.lib()
+    if not _typed:
+        for f in (lib.b200_tree_layout, lib.b200_tree_accept):
+            f.argtypes = [ctypes.c_char_p]
+        _typed = True
+    return lib
 
 
 def layout(parents: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, kv_len: torch.Tensor, max_nodes: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -36,17 +52,36 @@ def layout(parents: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, kv
             return layout(parents, q_start, q_len, kv_len, max_nodes)
     t, b = parents.shape[0], q_len.shape[0] if q_len.dim() == 1 else -1
     _index(parents, (t,), dev, "parents")
-    for x, what in ((q_start, "q_start"), (q_len, "q_len"), (kv_len, "kv_len")):
-        _index(x, (b,), dev, what)
+    _index(q_start, (b,), dev, "q_start")
+    _index(q_len, (b,), dev, "q_len")
+    _index(kv_len, (b,), dev, "kv_len")
     if not 1 <= max_nodes <= MAX_TREE:
         raise ValueError(f"trees of {max_nodes} nodes: 1 to {MAX_TREE} expected")
     words = (int(max_nodes) + 31) // 32
     positions, mask = parents.new_empty(t), parents.new_empty(t, words)
     if t:
-        rc = _lib.lib().b200_tree_layout(_lib.ptr(parents), _lib.ptr(q_start), _lib.ptr(q_len), _lib.ptr(kv_len), b, t, words, _lib.ptr(positions),
-                                         _lib.ptr(mask), _lib.stream())
+        rc = _kernels().b200_tree_layout(_LAYOUT.pack(
+            _LAYOUT.size, b, parents.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), mask.data_ptr(), _stream(dev),
+            t, words))
         _lib.check(rc, "tree_layout")
     return positions, mask
+
+
+@functools.lru_cache(maxsize=256)
+def _cache(shape: tuple, stride: tuple, size: int) -> tuple[int, int, int, int, int, int, int]:
+    """Checks a cache's sizes (elements of ``size`` bytes); layers, pages, heads, page size, bytes of a row, of a layer, and the low bits of both."""
+    if len(shape) < 4 or min(shape, default=0) < 1:
+        raise ValueError(f"caches: [layers, pages, heads, page size, ..] expected, got {list(shape)}")
+    layers, nb, heads, bs = shape[:4]
+    inner = 1
+    for d in range(len(shape) - 1, 0, -1):
+        if stride[d] != inner and shape[d] != 1:
+            raise ValueError(f"caches: contiguous layers expected, got strides {list(stride)} of {list(shape)}")
+        inner *= shape[d]
+    if layers > 1 and stride[0] < inner:
+        raise ValueError(f"caches: layers that lie apart expected, got strides {list(stride)} of {list(shape)}")
+    row, step = inner // (nb * heads * bs) * size, stride[0] * size if layers > 1 else 0
+    return layers, nb, heads, bs, row, step, (row | step) & 15
 
 
 def _caches(caches, dev: int):
@@ -55,27 +90,19 @@ def _caches(caches, dev: int):
         raise ValueError(f"{len(caches)} caches: 1 to {MAX_CACHES} expected")
     if len({c.data_ptr() for c in caches}) < len(caches):
         raise ValueError("caches: a tensor that is there twice would move twice")
-    pages = size = None
-    packed = b""
+    pages = None
+    packed = []
     for c in caches:
-        shape, stride = c.shape, c.stride()
-        if c.get_device() != dev or len(shape) < 4:
-            raise ValueError(f"caches: [layers, pages, heads, page size, ..] on cuda:{dev} expected, got {list(shape)} on {c.device}")
-        layers, nb, heads, bs = shape[:4]
-        pages, size = (nb, bs) if pages is None else (pages, size)
-        inner = 1
-        for d in range(len(shape) - 1, 0, -1):
-            if stride[d] != inner and shape[d] != 1:
-                raise ValueError(f"caches: contiguous layers expected, got strides {list(stride)} of {list(shape)}")
-            inner *= shape[d]
-        row = inner // max(1, nb * heads * bs) * c.element_size()
-        step = stride[0] * c.element_size() if layers > 1 else 0
-        if inner == 0 or layers == 0 or (nb, bs) != (pages, size) or layers > 1 and stride[0] < inner:
-            raise ValueError(f"caches: of {pages} pages of {size} rows each, layers apart, expected; got {list(shape)}, strides {list(stride)}")
-        if row % 4 or c.data_ptr() % 4 or step % 4:
+        layers, nb, heads, bs, row, step, low = _cache(c.shape, c.stride(), c.element_size())
+        at = c.data_ptr()
+        if c.get_device() != dev or pages is not None and pages != (nb, bs):
+            raise ValueError(f"caches: on cuda:{dev}, of as many pages and rows of them each, expected; got {list(c.shape)} on {c.device}")
+        pages = nb, bs
+        low |= at & 15
+        if low & 3:
             raise ValueError(f"caches: rows of a multiple of 4 bytes on 4-byte boundaries expected, got {row} bytes")
-        packed += _CACHE.pack(c.data_ptr(), step, layers, heads, row, 4 if row % 16 or c.data_ptr() % 16 or step % 16 else 16)
-    return pages, size, packed
+        packed.append(_CACHE.pack(at, step, layers, heads, row, 4 if low else 16))
+    return nb, bs, b"".join(packed)
 
 
 def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=None, block_table=None, caches=()):
@@ -96,10 +123,11 @@ def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=Non
         with torch.cuda.device(dev):
             return accept(tokens, parents, predicted, q_start, q_len, max_path, kv_len, block_table, caches)
     t, b = tokens.shape[0], q_len.shape[0] if q_len.dim() == 1 else -1
-    for x, what in ((tokens, "tokens"), (parents, "parents"), (predicted, "predicted")):
-        _index(x, (t,), dev, what)
-    for x, what in ((q_start, "q_start"), (q_len, "q_len")):
-        _index(x, (b,), dev, what)
+    _index(tokens, (t,), dev, "tokens")
+    _index(parents, (t,), dev, "parents")
+    _index(predicted, (t,), dev, "predicted")
+    _index(q_start, (b,), dev, "q_start")
+    _index(q_len, (b,), dev, "q_len")
     if not 1 <= max_path <= MAX_PATH:
         raise ValueError(f"paths of {max_path} nodes: 1 to {MAX_PATH} expected")
     caches = list(caches)
@@ -115,5 +143,5 @@ def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=Non
     if b:
         call = _CALL.pack(_CALL_BYTES, b, tokens.data_ptr(), parents.data_ptr(), predicted.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), _at(kv_len),
                           _at(block_table), path.data_ptr(), count.data_ptr(), emitted.data_ptr(), _stream(dev), t, int(max_path), width, nb, bs, len(caches))
-        _lib.check(_lib.lib().b200_tree_accept((call + packed).ljust(_CALL_BYTES, b"\0")), "tree_accept")
+        _lib.check(_kernels().b200_tree_accept(call + packed + _REST[len(caches)]), "tree_accept")
     return path, count, emitted
