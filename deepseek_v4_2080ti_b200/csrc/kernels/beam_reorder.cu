@@ -6,8 +6,8 @@
 // it has been read, whatever cycles the parents make, and there is no copy of the state anywhere else.  Beams that continue themselves move
 // nothing.
 //
-// What bounds it is memory: warp 0 keeps bulk copies of items on their way both in and out, STAGES items in shared memory; it only
-// issues them.  Warps 1 to 3 do the tensors whose rows are no multiples of 16 bytes (tables, tails) by plain loads, at the same time.
+// What bounds it is memory (16 beams of 12 to 100 MB: 6.0 to 6.2 TB/s of copies in and out): warp 0 keeps bulk copies of items on their way
+// both in and out, STAGES items in shared memory; it only issues them.  Warps 1 to 3 do the tensors whose rows are no multiples of 16 bytes (tables, tails) by plain loads, at the same time.
 #include "../ptx/sm100.cuh"
 #include "launch.h"
 #include "ops.h"
@@ -17,8 +17,8 @@ namespace b200 {
 namespace reorder {
 
 constexpr int MAX_BEAMS = 128;
-constexpr int STAGES = 4, AHEAD = 2;       // an item's stage is loaded AHEAD items before it is stored, and stored AHEAD before it is loaded again
-constexpr int STAGE_BYTES = 49152;
+constexpr int STAGES = 3, AHEAD = 2;       // an item is loaded AHEAD items before it is stored
+constexpr int STAGE_BYTES = 65536;
 constexpr int PLAIN_BYTES = 16384;
 constexpr int THREADS = 128;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + PLAIN_BYTES + 128;
@@ -29,6 +29,7 @@ struct Params {
   int chunk, plain_chunk;                  // bytes of a state that an item takes of every beam
   int bulk_items, plain_items;             // of all tensors
   int items[REORDER_STATES];               // of each
+  uint32_t chunks[REORDER_STATES];         // items that a state of each is cut into
 };
 
 struct Item {
@@ -46,7 +47,7 @@ __device__ __forceinline__ Item item_of(const Params& p, int at, int bulk, int c
     ++i;
   }
   const ReorderState& s = p.c.states[i];
-  const uint32_t chunks = (uint32_t)((s.inner_bytes + chunk - 1) / chunk);
+  const uint32_t chunks = p.chunks[i];
   const uint32_t x = (uint32_t)at / chunks, col = (uint32_t)at - x * chunks, outer = x / (uint32_t)p.c.requests;
   Item it;
   it.request = (int)(x - outer * p.c.requests);
@@ -99,7 +100,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 reorder_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[STAGES];
-  __shared__ uint8_t wanted[MAX_BEAMS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const ReorderCall& c = p.c;
   if (threadIdx.x == 0) {
@@ -111,61 +111,68 @@ reorder_kernel(const __grid_constant__ Params p) {
   pdl_launch_dependents();
   if (warp == 0) {
     const int step = gridDim.x, mine = p.bulk_items <= (int)blockIdx.x ? 0 : (p.bulk_items - (int)blockIdx.x + step - 1) / step;
-    bool loaded[STAGES];                                   // whether the item of a stage moves anything
+    // Beams of a request in turn, 32 at a time: with (w, its slot, its parent, whether it moves) of a lane.
+    const auto beams = [&](int request, auto with) {
+      const int* parents = c.parents + (size_t)request * c.beams;
+      const int* slots = c.slots + (size_t)request * c.beams;
+      for (int w = lane; w - lane < c.beams; w += 32) {
+        int parent = -1, slot = -1;
+        if (w < c.beams) {
+          parent = parents[w];
+          slot = c.slots ? slots[w] : request * c.beams + w;
+        }
+        bool moves = (unsigned)parent < (unsigned)c.beams && parent != w && (unsigned)slot < (unsigned)c.n_slots;
+        if (moves) {
+          const int from = c.slots ? slots[parent] : request * c.beams + parent;
+          moves = (unsigned)from < (unsigned)c.n_slots && from != slot;
+        }
+        with(w, slot, parent, moves);
+      }
+    };
+    uint32_t loaded = 0, phases = 0;                       // a bit per stage: its item moves something; parity of its next load
     auto load = [&](int i) {                               // of this block
       const Item it = item_of(p, blockIdx.x + i * step, 1, p.chunk);
-      for (int w = lane; w < c.beams; w += 32) wanted[w] = 0;
-      __syncwarp();
-      for (int w = lane; w < c.beams; w += 32) {
-        int parent, from, to;
-        if (move_of(c, it.request, w, parent, from, to)) wanted[parent] = 1;
-      }
-      __syncwarp();
+      const int st = i % STAGES;
+      uint8_t* stage = smem + st * STAGE_BYTES;
+      // parents that are wanted: a bit each, 32 to a lane's word
+      uint32_t want[MAX_BEAMS / 32] = {};
+      beams(it.request, [&](int, int, int parent, bool moves) {
+#pragma unroll
+        for (int x = 0; x < MAX_BEAMS / 32; ++x)
+          if (32 * x < c.beams) want[x] |= __reduce_or_sync(0xffffffffu, moves && parent >> 5 == x ? 1u << (parent & 31) : 0u);
+      });
       int n = 0;
-      for (int w = lane; w < c.beams; w += 32) n += wanted[w];
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (n == 0) return false;
-      uint64_t* bar = &full[i % STAGES];
-      if (lane == 0) mbar_expect_tx(bar, n * it.bytes);
+#pragma unroll
+      for (int x = 0; x < MAX_BEAMS / 32; ++x) n += __popc(want[x]);
+      loaded = loaded & ~(1u << st) | (n > 0 ? 1u << st : 0u);
+      if (n == 0) return;
+      if (lane == 0) mbar_expect_tx(&full[st], n * it.bytes);
       __syncwarp();
-      for (int w = lane; w < c.beams; w += 32)
-        if (wanted[w]) {
-          const int from = c.slots ? c.slots[(size_t)it.request * c.beams + w] : it.request * c.beams + w;
-          bulk_load(smem + (i % STAGES) * STAGE_BYTES + w * p.chunk, it.base + from * it.slot_bytes, it.bytes, bar);
+#pragma unroll
+      for (int x = 0; x < MAX_BEAMS / 32; ++x)
+        if (want[x] >> lane & 1) {
+          const int w = 32 * x + lane, from = c.slots ? c.slots[(size_t)it.request * c.beams + w] : it.request * c.beams + w;
+          bulk_load(stage + w * p.chunk, it.base + from * it.slot_bytes, it.bytes, &full[st]);
         }
       __syncwarp();
-      return true;
     };
-    uint32_t phases = 0;                                   // a bit per stage: completed loads
-#pragma unroll
-    for (int i = 0; i < STAGES; ++i) loaded[i] = false;
     bool ok = true;
     for (int i = -AHEAD; i < mine && ok; ++i) {
-      const int next = i + AHEAD;
-      if (next < mine) {
-        bulk_wait_read<AHEAD - 1>();                       // what was stored from that stage, STAGES items before, has been read
+      if (i + AHEAD < mine) {
+        bulk_wait_read<STAGES - AHEAD - 1>();              // what was stored from that stage, STAGES items before, has been read
         __syncwarp();
-        const bool on = load(next);
-#pragma unroll
-        for (int s = 0; s < STAGES; ++s)
-          if (s == next % STAGES) loaded[s] = on;
+        load(i + AHEAD);
       }
-      if (i >= 0) {
-        bool on = false;
-#pragma unroll
-        for (int s = 0; s < STAGES; ++s)
-          if (s == i % STAGES) on = loaded[s];
-        if (on) {
-          const Item it = item_of(p, blockIdx.x + i * step, 1, p.chunk);
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[i % STAGES], phases >> (i % STAGES) & 1));
-          if (!ok) break;
-          phases ^= 1u << (i % STAGES);
-          for (int w = lane; w < c.beams; w += 32) {
-            int parent, from, to;
-            if (move_of(c, it.request, w, parent, from, to))
-              bulk_store(it.base + to * it.slot_bytes, smem + (i % STAGES) * STAGE_BYTES + parent * p.chunk, it.bytes);
-          }
-        }
+      const int st = i % STAGES;
+      if (i >= 0 && loaded >> st & 1) {
+        const Item it = item_of(p, blockIdx.x + i * step, 1, p.chunk);
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phases >> st & 1));
+        if (!ok) break;
+        phases ^= 1u << st;
+        beams(it.request, [&](int, int slot, int parent, bool moves) {
+          if (moves) bulk_store(it.base + slot * it.slot_bytes, smem + st * STAGE_BYTES + parent * p.chunk, it.bytes);
+        });
+        __syncwarp();
       }
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");            // (one per item, also of items that store nothing)
     }
@@ -207,8 +214,10 @@ extern "C" int b200_beam_reorder(const ReorderCall* call) {
     if (s.outer < 1 || s.inner_bytes < 1 || (s.bulk && ((uintptr_t)s.base | s.outer_bytes | s.slot_bytes | s.inner_bytes) % 16)) return -ERR_BAD_ARG;
     if (s.bulk) bulk += s.inner_bytes * s.outer * a.requests;
   }
-  // Items as large as a stage holds, or smaller ones of at least 1 KB a beam where that gives every SM eight.
-  const long long most = STAGE_BYTES / a.beams / 128 * 128, even = bulk / (148 * 8) / 128 * 128;
+  // Items as large as a stage holds: an item costs its warp 0.5 us however small it is, and stages of 32 / 48 / 64 KB take 179 / 122 / 111 us
+  // for 16 beams of 48 MB.  Smaller ones, of 1 KB a beam at least, where every SM would not have two otherwise (8 / 4 / 2 a SM: 15.7 / 10.1 /
+  // 7.3 us for the last pages of 4 beams in 16 layers).
+  const long long most = STAGE_BYTES / a.beams / 128 * 128, even = bulk / (148 * 2) / 128 * 128;
   p.chunk = (int)(even < 1024 ? (most < 1024 ? most : 1024) : even < most ? even : most);
   p.plain_chunk = PLAIN_BYTES / a.beams / 16 * 16;
   for (int i = 0; i < a.n_states; ++i) {
@@ -218,6 +227,7 @@ extern "C" int b200_beam_reorder(const ReorderCall* call) {
     all[s.bulk != 0] += n;
     if (all[s.bulk != 0] > 0x7fffffffll) return -ERR_BAD_ARG;
     p.c.states[i].bulk = s.bulk != 0;
+    p.chunks[i] = (uint32_t)((s.inner_bytes + chunk - 1) / chunk);
     p.items[i] = (int)n;
   }
   p.bulk_items = (int)all[1];
