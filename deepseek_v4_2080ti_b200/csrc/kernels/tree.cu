@@ -12,6 +12,7 @@ namespace b200 {
 namespace tree {
 
 constexpr int MAX_NODES = 1024, MAX_PATH = 256;
+constexpr int PAGES = 64;
 constexpr int THREADS = 128;
 constexpr int RESIDENT = 148 * 16;         // blocks of THREADS threads that run at once
 
@@ -71,7 +72,8 @@ __device__ __forceinline__ void move_rows(char* at, const long long* src, const 
 // Block (x, b): every block of a sequence walks its path, the first writes it down, each moves a share of the rows' bytes.
 __global__ void __launch_bounds__(THREADS)
 tree_accept_kernel(const __grid_constant__ AcceptCall p) {
-  __shared__ int s_child[MAX_NODES];
+  __shared__ int s_child[MAX_NODES], s_predicted[MAX_NODES];
+  __shared__ int s_pages[PAGES];                           // of the tree's first keys
   __shared__ int s_path[MAX_PATH];
   __shared__ long long s_src[MAX_PATH], s_dst[MAX_PATH];
   __shared__ int s_count, s_moves;
@@ -80,15 +82,27 @@ tree_accept_kernel(const __grid_constant__ AcceptCall p) {
   pdl_launch_dependents();
   const int q0 = p.q_start[b], len = p.q_len[b];
   const int n = q0 < 0 ? 0 : max(0, min(min(len, p.T - q0), MAX_NODES));
-  for (int i = tid; i < n; i += THREADS) s_child[i] = MAX_NODES;
+  // What has to be read before the rows comes in two waits, the pages of the keys with the nodes.
+  const int first = p.n_caches ? p.kv_len[b] - len : 0, page0 = p.n_caches ? max(0, first) / p.block_size : 0;
+  const int* pages = p.block_table + (size_t)b * p.max_blocks;
+  for (int i = tid; i < PAGES && page0 + i < p.max_blocks; i += THREADS) s_pages[i] = pages[page0 + i];
+  int up[MAX_NODES / THREADS], token[MAX_NODES / THREADS];
+#pragma unroll
+  for (int x = 0; x < MAX_NODES / THREADS; ++x) {
+    const int i = x * THREADS + tid;
+    if (i < n) {
+      up[x] = p.parents[q0 + i];
+      token[x] = p.tokens[q0 + i];
+      s_predicted[i] = p.predicted[q0 + i];
+      s_child[i] = MAX_NODES;
+    }
+  }
   if (tid == 0) s_moves = 0;
   __syncthreads();
-  for (int i = tid; i < n; i += THREADS) {
-    const int up = p.parents[q0 + i];
-    if (up >= 0 && up < i) {
-      const int token = p.tokens[q0 + i];
-      if (token >= 0 && token == p.predicted[q0 + up]) atomicMin(&s_child[up], i);
-    }
+#pragma unroll
+  for (int x = 0; x < MAX_NODES / THREADS; ++x) {
+    const int i = x * THREADS + tid;
+    if (i < n && up[x] >= 0 && up[x] < i && token[x] >= 0 && token[x] == s_predicted[up[x]]) atomicMin(&s_child[up[x]], i);
   }
   __syncthreads();
   if (tid == 0) {
@@ -105,13 +119,16 @@ tree_accept_kernel(const __grid_constant__ AcceptCall p) {
     for (int i = tid; i < p.max_path; i += THREADS) {
       const int node = i < count ? s_path[i] : -1;
       p.path[(size_t)b * p.max_path + i] = node;
-      p.emitted[(size_t)b * p.max_path + i] = node < 0 ? -1 : p.predicted[q0 + node];
+      p.emitted[(size_t)b * p.max_path + i] = node < 0 ? -1 : s_predicted[node];
     }
     if (tid == 0) p.count[b] = count;
   }
   if (p.n_caches == 0 || count <= 1) return;
   // Places of the rows that move, in the path's order, as (page, row of it).
-  const int first = p.kv_len[b] - len;
+  const auto page_of = [&](int key) {
+    const int page = key / p.block_size;
+    return page - page0 < PAGES ? s_pages[page - page0] : pages[page];
+  };
   if (tid < 32) {
     int moves = 0;
     for (int base = 0; base < count; base += 32) {
@@ -119,8 +136,7 @@ tree_accept_kernel(const __grid_constant__ AcceptCall p) {
       long long src = 0, dst = 0;
       bool ok = from != i && first >= 0 && (long long)first + from < (long long)p.max_blocks * p.block_size;
       if (ok) {
-        const int* pages = p.block_table + (size_t)b * p.max_blocks;
-        const int ps = pages[(first + from) / p.block_size], pd = pages[(first + i) / p.block_size];
+        const int ps = page_of(first + from), pd = page_of(first + i);
         ok = (unsigned)ps < (unsigned)p.num_blocks && (unsigned)pd < (unsigned)p.num_blocks;
         src = (long long)ps << 32 | (first + from) % p.block_size;
         dst = (long long)pd << 32 | (first + i) % p.block_size;
