@@ -55,7 +55,6 @@ constexpr int TILE = 2 * ATOM;
 constexpr int STAGES = 5;
 constexpr int EMULATED = 2;       // of 8 pairs of exponentials: those on the arithmetic units (0 / 1 / 2 / 3: 641 / 639 / 624 / 626 us for 8192 causal rows)
 constexpr int ITEMS = 4;          // items the producer may be ahead of the slowest role
-constexpr int TO_L2 = 4;           // rows of a tree: key tiles on their way to L2 ahead of the ring
 constexpr int NTHREADS = 384;
 constexpr int SMEM_BYTES = 1024 + (2 + STAGES) * TILE + 2048;
 static_assert(SMEM_BYTES <= 232448, "shared memory of a block");
@@ -64,7 +63,7 @@ struct Params {
   const __nv_bfloat16* q;         // [T, Hq, 128]
   const __nv_bfloat16* gate;      // optional [T, Hq, 128]
   __nv_bfloat16* out;             // [T, Hq, 128]
-  const __nv_bfloat16 *k_cache, *v_cache;
+  const __nv_bfloat16* v_cache;
   const int* block_table;         // [B, max_blocks]
   const int* kv_len;              // [B]
   // prompt rows
@@ -552,18 +551,8 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           return ((id * p.Hkv + it.kvh) << p.bs_log2) + (key & (p.bs - 1));
         };
         int row = page_row(it.t0);                         // (on its way while the item is handed out)
-        auto to_l2 = [&](int tile) {
-          const int ahead = page_row(tile);
-          if (tile < it.t1 && lane < per_tile && ahead < p.num_blocks * p.Hkv * p.bs) {
-            l2_prefetch(p.k_cache + (size_t)ahead * D, rows * D * 2);
-            l2_prefetch(p.v_cache + (size_t)ahead * D, rows * D * 2);
-          }
-        };
-        if (FORM == TREE_ROWS)
-          for (int t = 1; t < TO_L2; ++t) to_l2(it.t0 + t);
         hand_out();
         for (int t = it.t0; ok && t < it.t1; ++t) {
-          if (FORM == TREE_ROWS) to_l2(t + TO_L2);
           const int n = min(per_tile, (it.k_end - t * BKV + rows - 1) >> rows_log2);
           const int next_row = page_row(t + 1);
 #pragma unroll
@@ -1304,7 +1293,6 @@ int launch(Params& p, const SpansCall& a) {
   p.q = reinterpret_cast<const __nv_bfloat16*>(a.q);
   p.gate = FORM == SHARED_KEYS ? nullptr : reinterpret_cast<const __nv_bfloat16*>(a.gate);
   p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
-  p.k_cache = reinterpret_cast<const __nv_bfloat16*>(a.k_cache);
   p.v_cache = reinterpret_cast<const __nv_bfloat16*>(a.v_cache);
   p.block_table = a.block_table;
   p.kv_len = a.kv_len;
