@@ -720,7 +720,7 @@ using namespace b200;
 extern "C" int b200_beam_select(const SelectCall* call) {
   const SelectCall& a = *call;
   if (a.bytes != (int)sizeof(a) || a.requests < 1 || a.beams < 1 || a.beams > select::MAX_BEAMS || a.vocab < 1 || a.n < 1 || a.n > select::MAX_N ||
-      a.tiles < 1 || a.parts < 1 || (long long)a.parts * a.beams + a.beams > select::CAP * 8 || a.vocab > 0x7fff0000 ||
+      a.tiles < 1 || a.parts < 1 || (long long)a.parts * a.beams + a.beams > select::CAP * 8 || a.vocab > 1 << 29 ||
       ((long long)a.vocab + select::TILE - 1) / select::TILE > (long long)a.parts * a.tiles || (long long)a.requests * a.beams > 65535 ||
       a.pad_token < 0 || a.pad_token >= a.vocab)
     return -ERR_BAD_ARG;

@@ -16,7 +16,7 @@ import torch
 from . import _lib
 from .attention import _at, _current, _index, _status, _stream
 
-MAX_BEAMS, MAX_CANDIDATES = 128, 128
+MAX_BEAMS, MAX_CANDIDATES, MAX_VOCAB = 128, 128, 1 << 29          # (places of a row's tiles fit 32 bits)
 MAX_STATES = 16                          # tensors of one launch
 TILE = 8192                              # logits that a block looks at together
 NUM_SMS = 148
@@ -62,8 +62,8 @@ def select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None, fin
             return select(logits, scores, n, finished, pad_token)
     b, w, v = shape
     n = w if n is None else int(n)
-    if not 0 < w <= MAX_BEAMS or not 0 < n <= MAX_CANDIDATES or not 0 < v <= 0x7fff0000:
-        raise ValueError(f"{n} of {w} beams and {v} tokens: 1 to {MAX_BEAMS} beams, 1 to {MAX_CANDIDATES} candidates expected")
+    if not 0 < w <= MAX_BEAMS or not 0 < n <= MAX_CANDIDATES or not 0 < v <= MAX_VOCAB:
+        raise ValueError(f"{n} of {w} beams and {v} tokens: 1 to {MAX_BEAMS} beams, 1 to {MAX_CANDIDATES} candidates and 1 to {MAX_VOCAB} tokens expected")
     if not 0 <= pad_token < v:
         raise ValueError(f"pad_token {pad_token} of a vocabulary of {v}")
     sb, row, one = logits.stride()
@@ -122,7 +122,7 @@ def reorder(states, parents: torch.Tensor, slots: torch.Tensor | None = None, di
     """In place, for all beams of a request at once: the state of beam w becomes that of beam ``parents[b, w]``.
 
     ``states``: a tensor or several of any type, their slots along axis ``dim``, everything behind it contiguous ([slots, layers, ..] with dim 0, caches
-    [layers, pages, ..] with dim 1).  parents int32 [B, W], as ``select`` returns them; a beam whose parent is itself, or none (-1), stays as it
+    [layers, pages, ..] with dim 1), none of them part of another.  parents int32 [B, W], as ``select`` returns them; a beam whose parent is itself, or none (-1), stays as it
     is.  ``slots`` int32 [B, W]: where the beams' states are, all of them different (default: slot b W + w); a beam whose slot is not there is
     neither read nor written.  Other slots stay as they are."""
     dev = parents.get_device()
@@ -152,7 +152,7 @@ def reorder(states, parents: torch.Tensor, slots: torch.Tensor | None = None, di
         raise ValueError(f"{b} requests of {w} beams in {n_slots} slots")
     if b == 0:
         return
-    _lib.check_indices(slots, 0, n_slots, 4)
+    _lib.check_indices(slots, -2 ** 31, n_slots, 4)         # (a bad slot becomes a negative one)
     packed = list(packed.values())
     for i in range(0, len(packed), MAX_STATES):
         some = packed[i:i + MAX_STATES]

@@ -115,7 +115,8 @@ def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=Non
 
     ``caches``: tensors [layers, pages, heads, page size, ..] of any type, layers contiguous (a single layer: ``cache[None]``; keys, values,
     scales of quantised rows); with them kv_len [B] and block_table int32 [B, pages], as in ``attention.decode_tree``.  The path's rows move
-    in place from kv_len - q_len + path[i] to kv_len - q_len + i; rows in pages outside the cache stay where they are."""
+    in place from kv_len - q_len + path[i] to kv_len - q_len + i; rows in pages outside the cache stay where they are.  No cache is part of
+    another, and no two sequences have the page of a row that moves."""
     dev = tokens.get_device()
     if dev < 0 or tokens.dim() != 1:
         raise ValueError(f"tokens: int32 [T] on a GPU expected, got {list(tokens.shape)} on {tokens.device}")
@@ -128,8 +129,8 @@ def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=Non
     _index(predicted, (t,), dev, "predicted")
     _index(q_start, (b,), dev, "q_start")
     _index(q_len, (b,), dev, "q_len")
-    if not 1 <= max_path <= MAX_PATH:
-        raise ValueError(f"paths of {max_path} nodes: 1 to {MAX_PATH} expected")
+    if not 1 <= max_path <= MAX_PATH or b > 65535:
+        raise ValueError(f"{b} paths of {max_path} nodes: 65535 at most, of 1 to {MAX_PATH} nodes")
     caches = list(caches)
     nb, bs, width, packed = 0, 0, 0, b""
     if caches:

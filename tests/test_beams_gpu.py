@@ -156,6 +156,24 @@ def test_candidates_closer_than_32_bits():
     check(shuffled, scores, 100)
 
 
+def test_a_long_row():
+    """More tiles than parts, offsets beyond 32 bits of bytes."""
+    from deepseek_v4_2080ti_b200.ops import beams
+    v = (1 << 29) + (1 << 28)
+    big = torch.full((2, v), -8.0, dtype=torch.bfloat16, device=DEV)
+    at = [5, 8191, 8192, 1 << 28, (1 << 29) - 1]
+    for i, t in enumerate(at):
+        big[1, t] = 10 - i
+    row = big[1:2, :1 << 29][None]
+    score, parents, tokens = beams.select(row, torch.zeros(1, 1, device=DEV), 7)
+    others = [t for t in range(7) if t not in at][:2]
+    assert tokens.tolist() == [at + others] and parents.tolist() == [[0] * 7]
+    z = math.log(sum(math.exp(10 - i) for i in range(5)) + ((1 << 29) - 5) * math.exp(-8))
+    assert all(abs(x - (l - z)) < 1e-5 * abs(l - z) + 1e-6 for x, l in zip(score[0].tolist(), [10, 9, 8, 7, 6, -8, -8]))
+    with pytest.raises(ValueError):
+        beams.select(big[None], torch.zeros(1, 2, device=DEV))
+
+
 def test_strides():
     """Rows of a longer buffer, a slice of the vocabulary off 16 bytes, one beam of several."""
     base, scores = random_logits(3, 4, 5000)
@@ -255,6 +273,41 @@ def test_slots_that_are_not_there():
     check_reorder([filled(6, 100), filled(6, 3, dtype=torch.uint8)], parents, _i32([[0, 9, 2, 3]]))
     check_reorder([filled(6, 100), filled(6, 3, dtype=torch.uint8)], parents, _i32([[-1, 4, 2, 2 ** 31 - 1]]))
     check_reorder([filled(6, 100)], _i32([[7, -5, 0, 2 ** 31 - 1]]), _i32([[5, 4, 3, 2]]))
+
+
+def test_debug_mode_leaves_slots_that_are_not_there_alone(monkeypatch):
+    from deepseek_v4_2080ti_b200.ops import _lib, beams
+    monkeypatch.setenv("B200_BOUNDS_CHECK", "1")
+    check_reorder([filled(6, 100)], _i32([[1, 2, 0, 1]]), _i32([[0, -1, 2, 3]]))              # idle ones are no error
+    x = filled(6, 100)
+    want = moved(x, _i32([[1, 0, 0, 2]]), _i32([[0, 6, 2, 3]]), 0)
+    beams.reorder(x, _i32([[1, 0, 0, 2]]), _i32([[0, 6, 2, 3]]))
+    with pytest.raises(_lib.KernelError):
+        _lib.check_status()
+    assert torch.equal(x, want)
+
+
+def test_nothing_beside_the_states_is_touched():
+    """Slots within a larger buffer: what lies before, between and behind them stays, for copies of 16 bytes and of one."""
+    parents = _i32([[3, 0, 1, 1, 4, 2]])
+    for width, dtype in ((4096, torch.float32), (70000, torch.uint8), (333, torch.bfloat16)):
+        room = filled(3, 10, width + 64, dtype=dtype)
+        for a, b in ((0, width), (16, width + 16), (64, width + 64)):
+            was = room.clone()
+            check_reorder([room[:, 2:8, a:b]], parents, dim=1)
+            was[:, 2:8, a:b] = room[:, 2:8, a:b]
+            assert torch.equal(room, was)
+
+
+@pytest.mark.parametrize("n", [1, 5, 128])
+def test_many_steps_of_one_search(n):
+    """The same inputs give the same answer every time, whatever ran before and beside it."""
+    from deepseek_v4_2080ti_b200.ops import beams
+    x, y = random_logits(5, 7, 20011, torch.bfloat16)
+    first = beams.select(x, y, n)
+    for i in range(30):
+        beams.select(*random_logits(1 + i % 3, 4, 9000, seed=i), 3 + i)
+        assert all(torch.equal(a, b) for a, b in zip(first, beams.select(x, y, n)))
 
 
 def test_large_states():

@@ -25,11 +25,12 @@ def test_host_tensors_are_refused():
 
 def test_parts_of_a_row():
     """Every logit in a part, and no more parts than the kernel that joins them takes."""
-    for v in (1, 8192, 8193, 51001, 248320, 0x7fff0000):
+    for v in (1, 8192, 8193, 51001, 248320, beams.MAX_VOCAB):
         for rows in (1, 4, 128, 512, 65535):
             parts, tiles = beams._parts(rows, v)
             assert parts * tiles * beams.TILE >= v > (parts - 1) * tiles * beams.TILE
             assert parts * min(rows, beams.MAX_BEAMS) + beams.MAX_BEAMS <= 8192
+            assert parts * tiles * beams.TILE < 2 ** 31             # places are numbers of 32 bits
 
 
 @pytest.mark.gpu

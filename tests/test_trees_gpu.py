@@ -154,6 +154,24 @@ def test_scores_far_apart():
     run_tree([(60, 900)], 2, 1, q_scale=6.0, poke=poke, cap=50.0)
 
 
+def test_in_place_and_beside_the_rows():
+    """Results over the queries, within a larger buffer; gates and a cap; nothing else is written."""
+    lib, attention, tree = _modules()
+    torch.manual_seed(9)
+    k, v = rand(700, 2, 128), rand(700, 2, 128)
+    kc, vc, table = pages([(k, v)], 32)
+    parents = random_tree(45, 3, random.Random(1))
+    args = (kc, vc, table, tree.layout(_i32(parents), _i32([0]), _i32([45]), _i32([700]), 45)[1], _i32([0]), _i32([45]), _i32([700]), 45)
+    for splits in (1, 4):
+        room = rand(60, 6, 128)
+        gate, was = rand(45, 6, 128), room.clone()
+        want = attention.decode_tree(room[7:52].clone(), *args, gate=gate, cap=9.0, splits=splits)
+        q = room[7:52]
+        assert attention.decode_tree(q, *args, gate=gate, cap=9.0, splits=splits, out=q) is q
+        assert torch.equal(q, want) and torch.equal(room[:7], was[:7]) and torch.equal(room[52:], was[52:])
+    lib.check_status()
+
+
 def test_rows_of_no_sequence_stay_and_pages_that_are_not_there(monkeypatch):
     lib, attention, _ = _modules()
     torch.manual_seed(3)
@@ -257,7 +275,9 @@ def test_accept(sizes, width, most, bs, layers, heads):
     scale = torch.randn(layers, nb, heads, bs, device=DEV)
     codes = torch.randint(0, 255, (2 * layers, nb, 2 * heads, bs, 64), device=DEV, dtype=torch.uint8)[::2]     # layers apart, other heads
     odd = torch.randint(0, 255, (1, nb, 1, bs, 20), device=DEV, dtype=torch.uint8)
-    caches = [k, k.flip(0).contiguous(), scale, codes, odd]
+    room = torch.randn(layers + 2, nb, heads, bs, 128, device=DEV).bfloat16()                                # layers of a larger cache
+    caches = [k, k.flip(0).contiguous(), scale, codes, odd, room[1:-1]]
+    beside = [(codes._base[1::2], codes._base[1::2].clone()), (room[0], room[0].clone()), (room[-1], room[-1].clone())]
     wanted = [c.clone() for c in caches]
     paths = [accept_oracle(tokens[i], trees[i], predicted[i], most) for i in range(len(sizes))]
     for b, path in enumerate(paths):
@@ -271,7 +291,7 @@ def test_accept(sizes, width, most, bs, layers, heads):
     assert count.tolist() == [len(p) for p in paths]
     assert path.tolist() == [p + [-1] * (most - len(p)) for p in paths]
     assert emitted.tolist() == [[predicted[b][x] for x in p] + [-1] * (most - len(p)) for b, p in enumerate(paths)]
-    for c, w in zip(caches, wanted):
+    for c, w in [*zip(caches, wanted), *beside]:
         assert torch.equal(c, w)
     alone = tree.accept(flat(tokens), flat(trees), flat(predicted), _i32(starts), _i32(sizes), most)
     assert all(torch.equal(x, y) for x, y in zip(alone, (path, count, emitted)))
