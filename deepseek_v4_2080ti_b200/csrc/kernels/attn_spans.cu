@@ -1220,17 +1220,21 @@ spans_join_kernel(const __grid_constant__ Params p) {
   if (at >= rows) return;
   pdl_wait();
   const int tok = (int)(at / p.Hq);
+  // the first 32 slots' maxima and sums and the gate are on their way while the row's sequence is looked for
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < p.splits) ml = *reinterpret_cast<const float2*>(p.part_ml + (lane * rows + at) * 2);
+  uint2 gate = make_uint2(0, 0);
+  if (p.gate) gate = *reinterpret_cast<const uint2*>(p.gate + at * D + lane * 4);
   int mine = 0;                                            // rows of no sequence stay as they are
   for (int b = lane; b < p.batch; b += 32) mine |= p.q_start[b] >= 0 && tok >= p.q_start[b] && tok - p.q_start[b] < p.q_len[b];
   if (!__any_sync(0xffffffffu, mine)) return;
-  float M = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, p.part_ml[(s * rows + at) * 2]);
+  float M = ml.x;
+  for (int s = lane + 32; s < p.splits; s += 32) M = fmaxf(M, p.part_ml[(s * rows + at) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < p.splits; s0 += 32) {              // a slot's maximum and sum per lane, then its part, eight on their way at a time
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (s0 + lane < p.splits) ml = *reinterpret_cast<const float2*>(p.part_ml + ((s0 + lane) * rows + at) * 2);
+    if (s0 > 0) ml = s0 + lane < p.splits ? *reinterpret_cast<const float2*>(p.part_ml + ((s0 + lane) * rows + at) * 2) : make_float2(-INFINITY, 0.f);
     const float w_all = ml.y == 0.f ? -1.f : exp2f(ml.x - M);              // (below 0: nothing seen, the item may not have written its sums)
     for (int s1 = 0; s1 < min(32, p.splits - s0); s1 += 8) {
       float4 x[8];
@@ -1252,8 +1256,7 @@ spans_join_kernel(const __grid_constant__ Params p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] *= inv;
   if (p.gate) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p.gate + at * D + lane * 4);
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&gate);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float2 f = __bfloat1622float2(h[i]);
