@@ -109,6 +109,12 @@ __device__ __forceinline__ uint64_t desc_mn_sw128(const void* p, uint32_t lbo, u
 constexpr uint32_t idesc_qk = umma_idesc_bf16(128, 128);
 constexpr uint32_t idesc_pv = umma_idesc_bf16(128, 128) | (1u << 16);   // B is MN-major
 
+__device__ __forceinline__ void tmem_ld_32x2(uint32_t taddr, uint32_t& v, uint32_t& w) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(v), "=r"(w) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x2(uint32_t taddr, uint32_t v, uint32_t w) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(v), "r"(w) : "memory");
+}
 __device__ __forceinline__ void tmem_ld_32x1(uint32_t taddr, uint32_t& v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr) : "memory");
 }
@@ -415,7 +421,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_base[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_base) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                                       // [2 streams] tiles; scratch of the join of the streams
+  uint8_t* sQ = smem;                                       // [2 streams] tiles; then gates and results
   uint8_t* sR = smem + 2 * TILE;                            // ring of key and value tiles
   uint64_t* bars = reinterpret_cast<uint64_t*>(sR + STAGES * TILE);
   // Stages are given back by place in the ring, but filled by tile: a stage holds keys and values in turn, loads finish in any order, and
@@ -429,8 +435,8 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   uint64_t* p_half = q_full + 4;                            // P of the tile's first 64 keys
   uint64_t* p_full = q_full + 6;
   uint64_t* o_full = q_full + 8;
-  uint64_t* j_full = q_full + 10;                           // by slot of the scratch: 32 columns of stream 1's part lie there
-  uint64_t* j_empty = q_full + 12;                          // and have been read
+  uint64_t* j_full = q_full + 10;                           // per stream, where both have a part of every row: its part is ready,
+  uint64_t* j_empty = q_full + 12;                          // and it has read the other's
   uint64_t* i_full = q_full + 14;                           // items
   uint64_t* i_empty = i_full + ITEMS;
   uint64_t* pv_half = i_empty + ITEMS;                      // per stream: the product with the values of a tile's first 64 keys
@@ -439,8 +445,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
   uint4* s_next = reinterpret_cast<uint4*>(bars + 48);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint32_t* s_bad = reinterpret_cast<uint32_t*>(bars + 52); // [STAGES][4] keys with values that are not finite
-  float* s_ml = reinterpret_cast<float*>(bars + 62);        // [2][128] maximum and sum of stream 1
-  Item* s_item = reinterpret_cast<Item*>(bars + 62 + 128);  // [ITEMS]
+  Item* s_item = reinterpret_cast<Item*>(bars + 62);        // [ITEMS]
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform: the issuer depends on it
   if (threadIdx.x == 0) {
@@ -710,7 +715,7 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
     const int lr = threadIdx.x & 127;                      // row of the stream == TMEM lane
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + m * 128 + lane_off, tO = tmem + 256 + m * 128 + lane_off;
-    uint32_t ph_s = 0, ph_o = 0;
+    uint32_t ph_s = 0, ph_o = 0, ph_j = 0;
     Ring checks = {0, 0};
     bool alive = true;
     for (;;) {
@@ -942,15 +947,10 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             };
             uint32_t seen[2];
             auto bits = [&](int h, int a, int b) {
-              if (FORM == TREE_ROWS) {
-                seen[0] = h ? in_tree[2] : in_tree[0];
-                seen[1] = h ? in_tree[3] : in_tree[1];
-                return;
-              }
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 const int x = min(32, max(0, a - c * 32)), y = min(32, max(0, b - c * 32));
-                seen[c] = (uint32_t)((1ull << y) - 1) & ~(uint32_t)((1ull << x) - 1);
+                seen[c] = FORM == TREE_ROWS ? h ? in_tree[2 + c] : in_tree[c] : (uint32_t)((1ull << y) - 1) & ~(uint32_t)((1ull << x) - 1);
               }
             };
             auto mask = [&](int h, int a, int b) {
@@ -1054,9 +1054,124 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
       const bool gated = p.gate && !p.part_o && writer;
-      // (this stream's score products have all finished: the scores of its last tile have arrived.  Stream 1's of a joined item
-      // read the same queries and may not have.)
-      if (gated && !joined) load_gate();
+      // ---- a joined item's results: each stream reads both streams' parts where they are - rows lie in the same lanes - and takes half of the
+      // columns, through the half of the shared memory that is its own; maxima and sums pass through the scores' columns, which are free.  (One
+      // stream alone, with the other's part handed over through shared memory, took 9400 cycles of an item, XXX)
+      if (joined) {
+        uint8_t* half = sQ + m * TILE + (warp & 3) * 4096;                 // this warp's 32 rows of 64 columns
+        const bool with_gate = p.gate && !p.part_o && warp_on;
+        uint4 g[8];                                        // (on their way; the other stream's products may still read the queries that lie in the half)
+        if (with_gate) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)                      // a quarter warp per row
+            g[i] = reinterpret_cast<const uint4*>(p.gate + (size_t)__shfl_sync(0xffffffffu, at, 4 * i + (lane >> 3)) * D + m * 64)[lane & 7];
+        }
+        if (!(alive = warp_wait(&o_full[m], ph_o))) break;
+        ph_o ^= 1;
+        tc_fence_after();
+        if (warp_on) {
+          tmem_st_32x2(tS, __float_as_uint(m_run), __float_as_uint(l_run));
+          tmem_st_wait();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&j_full[m]);
+        if (!(alive = warp_wait(&j_full[m ^ 1], ph_j))) break;
+        tc_fence_after();
+        if (warp_on) {
+          uint32_t other_m, other_l;
+          tmem_ld_32x2(tmem + (m ^ 1) * 128 + lane_off, other_m, other_l);
+          tmem_ld_wait();
+          const float m0 = m ? __uint_as_float(other_m) : m_run, m1 = m ? m_run : __uint_as_float(other_m);
+          const float l0 = m ? __uint_as_float(other_l) : l_run, l1 = m ? l_run : __uint_as_float(other_l), mm = fmaxf(m0, m1);
+          float w0 = m0 == -INFINITY ? 0.f : exp2f(m0 - mm), w1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mm);
+          const float l = (l0 == 0.f ? 0.f : l0 * w0) + (l1 == 0.f ? 0.f : l1 * w1);
+          if (p.part_o) {
+            if (row_ok && m == 0) *reinterpret_cast<float2*>(p.part_ml + (row0 + at) * 2) = make_float2(mm, l);
+          } else {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            w0 *= inv;
+            w1 *= inv;
+          }
+          if (with_gate) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + (lane >> 3);
+              *reinterpret_cast<uint4*>(half + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = g[i];
+            }
+            __syncwarp();
+          }
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {                    // 32 columns
+            uint32_t v[32], x[32];
+            tmem_ld_32x32(tmem + 256 + lane_off + m * 64 + c * 32, v);
+            tmem_ld_32x32(tmem + 384 + lane_off + m * 64 + c * 32, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float o = __uint_as_float(v[i]) * w0;
+              v[i] = __float_as_uint(fmaf(__uint_as_float(x[i]), w1, o));
+            }
+            if (p.part_o) {
+              float4* room = reinterpret_cast<float4*>(half);              // four columns of a row at place (column / 4, row ^ column / 4)
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                room[i * 32 + (lane ^ i)] =
+                    make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {                // a quarter warp per row
+                const int r = 4 * i + (lane >> 3);
+                const size_t prow = row0 + __shfl_sync(0xffffffffu, at, r);
+                if (r < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + m * 64 + c * 32)[lane & 7] = room[(lane & 7) * 32 + (r ^ (lane & 7))];
+              }
+              __syncwarp();
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint4* place = reinterpret_cast<uint4*>(half + lane * 128 + (((c * 4 + i) ^ (lane & 7)) << 4));
+                float o[8];
+#pragma unroll
+                for (int y = 0; y < 8; ++y) o[y] = __uint_as_float(v[8 * i + y]);
+                if (with_gate) {
+                  const uint4 here = *place;
+                  const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&here);
+#pragma unroll
+                  for (int y = 0; y < 4; ++y) {
+                    const float2 gf = __bfloat1622float2(gh[y]);
+                    o[2 * y] = __fdividef(o[2 * y], 1.f + __expf(-gf.x));
+                    o[2 * y + 1] = __fdividef(o[2 * y + 1], 1.f + __expf(-gf.y));
+                  }
+                }
+                uint4 u4;
+                __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u4);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) h2[y] = __floats2bfloat162_rn(o[2 * y], o[2 * y + 1]);
+                *place = u4;
+              }
+            }
+          }
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&j_empty[m]);           // this stream has read the other's part
+        if (warp_on && !p.part_o) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {                    // a quarter warp per row
+            const int r = 4 * i + (lane >> 3);
+            const uint4 u4 = *reinterpret_cast<const uint4*>(half + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            const size_t to = __shfl_sync(0xffffffffu, at, r);
+            if (r < rows_here) reinterpret_cast<uint4*>(p.out + to * D + m * 64)[lane & 7] = u4;
+          }
+          __syncwarp();
+        }
+        if (!(alive = warp_wait(&j_empty[m ^ 1], ph_j))) break;
+        tc_fence_after();
+        ph_j ^= 1;
+        continue;
+      }
+      // (this stream's score products have all finished: the scores of its last tile have arrived)
+      if (gated) load_gate();
       if (my_steps > 0) {
         if (!(alive = warp_wait(&o_full[m], ph_o))) break;
         ph_o ^= 1;
@@ -1065,14 +1180,13 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       // ---- results of the item: O / l through the gate, or O with (m, l) for the join of several items.  A warp's rows go through
       // the shared memory that held its queries, so that whole lines are stored: as bf16 over the gate, or in fp32
       // 32 columns at a time, four columns of a row at place (column / 4, row ^ column / 4).
-      if (!writer && !joined) continue;                    // (a stream without a part, or without rows: the others write)
-      float w_own = 1.f, w_other = 0.f;
+      if (!writer) continue;                               // (a stream without a part, or without rows: the others write)
+      float w_own = 1.f;
       auto staged = [&](int stream, int slot, int c4, int r) -> float4* {
         return reinterpret_cast<float4*>(sQ + stream * TILE + slot * ATOM + (warp & 3) * 4096 + ((c4 * 32 + (r ^ c4)) << 4));
       };
-      // Streams that are joined: 32 columns of stream 1 at a time through two slots of its half of the scratch, each filled and read twice.
 #pragma unroll 1
-      for (int c = 0; c < 4 && alive; ++c) {               // 32 columns
+      for (int c = 0; c < 4; ++c) {                        // 32 columns
         uint32_t v[32];
         if (my_steps > 0) {
           tmem_ld_32x32(tO + c * 32, v);
@@ -1084,103 +1198,63 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         auto four = [&](int i) {
           return make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
         };
-        if (joined && m == 1) {
-          if (c >= 2 && !(alive = warp_wait(&j_empty[c & 1], 0))) break;
-          if (warp_on) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) *staged(1, c & 1, i, lane) = four(i);
-          }
-          if (c == 0) {
-            s_ml[lr] = m_run;
-            s_ml[128 + lr] = l_run;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&j_full[c & 1]);
-          continue;
-        }
-        if (joined) {                                      // (then both streams' score products, which read the queries here, have finished)
-          if (!(alive = warp_wait(&j_full[c & 1], c >> 1))) break;
-          if (c == 0) {
-            const float m1 = s_ml[lr], l1 = s_ml[128 + lr], mm = fmaxf(m_run, m1);
-            w_own = m_run == -INFINITY ? 0.f : exp2f(m_run - mm);
-            w_other = m1 == -INFINITY ? 0.f : exp2f(m1 - mm);
-            l_run = (l_run == 0.f ? 0.f : l_run * w_own) + (l1 == 0.f ? 0.f : l1 * w_other);
-            m_run = mm;
-          }
-        }
         if (c == 0) {
           if (p.part_o) {
             if (row_ok) *reinterpret_cast<float2*>(p.part_ml + (row0 + at) * 2) = make_float2(m_run, l_run);
           } else {
-            const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-            w_own *= inv;
-            w_other *= inv;
+            w_own = l_run == 0.f ? 0.f : 1.f / l_run;
             if (gated) {
-              if (joined) load_gate();
               asm volatile("cp.async.wait_all;" ::: "memory");
               __syncwarp();
             }
           }
         }
-        if (warp_on) {
-          if (joined || !p.part_o) {
+        if (!p.part_o)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float4 o = four(i);
-              o.x *= w_own; o.y *= w_own; o.z *= w_own; o.w *= w_own;
-              if (joined) {
-                const float4 x = *staged(1, c & 1, i, lane);
-                o.x += x.x * w_other; o.y += x.y * w_other; o.z += x.z * w_other; o.w += x.w * w_other;
-              }
-              v[4 * i] = __float_as_uint(o.x); v[4 * i + 1] = __float_as_uint(o.y); v[4 * i + 2] = __float_as_uint(o.z); v[4 * i + 3] = __float_as_uint(o.w);
-            }
-          }
-          if (p.part_o) {
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * w_own);
+        if (p.part_o) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) *staged(m, 0, i, lane) = four(i);
-            __syncwarp();
-            if (steps) {
+          for (int i = 0; i < 8; ++i) *staged(m, 0, i, lane) = four(i);
+          __syncwarp();
+          if (steps) {
 #pragma unroll 4
-              for (int i = 0; i < 8; ++i) {                // a quarter warp per row
-                const int r = 4 * i + (lane >> 3);
-                const size_t prow = row0 + __shfl_sync(0xffffffffu, at, r);
-                if (r < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + c * 32)[lane & 7] = *staged(m, 0, lane & 7, r);
-              }
+            for (int i = 0; i < 8; ++i) {                // a quarter warp per row
+              const int r = 4 * i + (lane >> 3);
+              const size_t prow = row0 + __shfl_sync(0xffffffffu, at, r);
+              if (r < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + c * 32)[lane & 7] = *staged(m, 0, lane & 7, r);
             }
-          } else {
-            auto put = [&](auto with_gate) {              // (one look at the gate, not four)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint4* place = reinterpret_cast<uint4*>(own + (c >> 1) * ATOM + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4));
-                float o[8];
-#pragma unroll
-                for (int x = 0; x < 8; ++x) o[x] = __uint_as_float(v[8 * i + x]);
-                if (with_gate.value) {
-                  const uint4 g = *place;
-                  const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&g);
-#pragma unroll
-                  for (int x = 0; x < 4; ++x) {
-                    const float2 gf = __bfloat1622float2(gh[x]);
-                    o[2 * x] = __fdividef(o[2 * x], 1.f + __expf(-gf.x));
-                    o[2 * x + 1] = __fdividef(o[2 * x + 1], 1.f + __expf(-gf.y));
-                  }
-                }
-                uint4 u4;
-                __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u4);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) h2[x] = __floats2bfloat162_rn(o[2 * x], o[2 * x + 1]);
-                *place = u4;
-              }
-            };
-            if (p.gate) put(Int<1>());
-            else put(Int<0>());
           }
+        } else {
+          auto put = [&](auto with_gate) {              // (one look at the gate, not four)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4* place = reinterpret_cast<uint4*>(own + (c >> 1) * ATOM + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4));
+              float o[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) o[x] = __uint_as_float(v[8 * i + x]);
+              if (with_gate.value) {
+                const uint4 g = *place;
+                const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&g);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float2 gf = __bfloat1622float2(gh[x]);
+                  o[2 * x] = __fdividef(o[2 * x], 1.f + __expf(-gf.x));
+                  o[2 * x + 1] = __fdividef(o[2 * x + 1], 1.f + __expf(-gf.y));
+                }
+              }
+              uint4 u4;
+              __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u4);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) h2[x] = __floats2bfloat162_rn(o[2 * x], o[2 * x + 1]);
+              *place = u4;
+            }
+          };
+          if (p.gate) put(Int<1>());
+          else put(Int<0>());
         }
         __syncwarp();
-        if (joined && lane == 0) mbar_arrive(&j_empty[c & 1]);
       }
-      if (joined && m == 1 && alive) alive = warp_wait(&j_empty[0], 1) && warp_wait(&j_empty[1], 1);     // all of it has been read
-      if (alive && writer && !p.part_o) {
+      if (!p.part_o) {
 #pragma unroll 4
         for (int i = 0; i < (rows_here + 1) / 2; ++i) {    // half a warp per row
           const int r = 2 * i + (lane >> 4);
