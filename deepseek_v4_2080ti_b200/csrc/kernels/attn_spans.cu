@@ -32,10 +32,13 @@
 // What bounds it (8192 causal rows of 40 heads over 8 kv heads, gated: 628 us, 1.1 PFLOP/s): 256 rows times 128 keys cost 2048
 // cycles of the tensor core and about 2100 of each scheduler's softmax warps, and take 3500 together, because a stream's scores,
 // weights and products follow each other through tensor memory and two streams do not hide all of that; an item's start and end
-// take another 10 %.  Packed documents of 4000 rows of 48 heads, capped: 116 us, a third of it the start and end of items, and of the
+// take another 10 %.  Packed documents of 4000 rows of 48 heads, capped: 110 us, a third of it the start and end of items, and of the
 // rest most masked tiles (6000 cycles).
-// Shared keys of 40 heads over 8, in one item a block: 64 rows over 32768 keys 44 us, 32 over 8192 15 us.  The smallest call, one
-// row over 121 keys, is a chain of 9 us: the item 3, page and tiles 3, softmax 4 and product 1 thousand cycles, the row's way out 4.
+// Shared keys of 40 heads over 8, in one item a block: 64 rows over 32768 keys 44 us, 32 over 8192 15 us.
+// Trees of 40 heads over 8: 32 of 64 nodes over 8192 keys 475 to 570 us, where the second row tile of 64 rows reads the keys from DRAM
+// once more (2.2 GB; begun beside the first it gains nothing) and 512 items are 3.5 rounds of blocks; 32 of 25 nodes 204 us, 5.2 TB/s; one of
+// 16 over 32768 keys 38 us, 20 of them the keys.  The smallest, 7 nodes over 350 keys, is a chain of 18 thousand cycles: the item 2.8,
+// queries 1.5, first scores 1, three tiles 7.5 (the last one masked), the rows' way out 5.2.
 #include <cuda_bf16.h>
 #include "per_device.h"
 #include "../ptx/sm100.cuh"
@@ -1056,7 +1059,8 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
       const bool gated = p.gate && !p.part_o && writer;
       // ---- a joined item's results: each stream reads both streams' parts where they are - rows lie in the same lanes - and takes half of the
       // columns, through the half of the shared memory that is its own; maxima and sums pass through the scores' columns, which are free.  (One
-      // stream alone, with the other's part handed over through shared memory, took 9400 cycles of an item, XXX)
+      // stream alone, with the other's part handed to it through shared memory, took 9200 cycles for 35 rows instead of 5200: 7 nodes over
+      // 350 keys 14.3 us instead of 11.9.)
       if (joined) {
         uint8_t* half = sQ + m * TILE + (warp & 3) * 4096;                 // this warp's 32 rows of 64 columns
         const bool with_gate = p.gate && !p.part_o && warp_on;
@@ -1217,11 +1221,13 @@ spans_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
           for (int i = 0; i < 8; ++i) *staged(m, 0, i, lane) = four(i);
           __syncwarp();
           if (steps) {
-#pragma unroll 4
-            for (int i = 0; i < 8; ++i) {                // a quarter warp per row
-              const int r = 4 * i + (lane >> 3);
-              const size_t prow = row0 + __shfl_sync(0xffffffffu, at, r);
-              if (r < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + c * 32)[lane & 7] = *staged(m, 0, lane & 7, r);
+            float4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = *staged(m, 0, lane & 7, 4 * i + (lane >> 3));               // a quarter warp per row
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const size_t prow = row0 + __shfl_sync(0xffffffffu, at, 4 * i + (lane >> 3));
+              if (4 * i + (lane >> 3) < rows_here) reinterpret_cast<float4*>(p.part_o + prow * D + c * 32)[lane & 7] = x[i];
             }
           }
         } else {

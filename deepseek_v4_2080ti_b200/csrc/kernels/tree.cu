@@ -4,6 +4,10 @@
 // token that the target has chosen already).  b200_attn_tree (attn_spans.cu) attends with what tree_layout_kernel gives; tree_accept_kernel
 // walks from node 0 to the lowest child that holds the token predicted at its parent, for as long as there is one, and moves the
 // path's rows of every layer's caches up behind the context.
+//
+// What bounds them: a small launch's latency (one tree of 7 nodes 2.3 us, and 2.6 with its rows in 16 layers); 64 trees of 61 nodes, whose
+// walks are nine steps through L1, 4.5 us; their accepted rows, 25 MB in and out in pieces of 256 bytes, 13 to 17 us, of which the walk, the
+// pages and the first reads are a chain of 5 (16.5 instead of 13 with the nodes, the predictions and the pages in four waits and not two).
 #include "../ptx/sm100.cuh"
 #include "launch.h"
 #include "ops.h"
