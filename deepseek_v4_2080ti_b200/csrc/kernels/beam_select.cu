@@ -602,8 +602,11 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
         s.order[better] = (unsigned short)i;
       }
       __syncthreads();
-      for (int r = tid; r < n && r + 1 < count; r += THREADS) {            // (the last one's neighbour is the first that is left out)
+      // Neighbours among the n best and as many behind them as may belong before the last.  (That is enough: where two of
+      // different beams are nearer than their bounds and others lie between them, so are two neighbours of different beams on the way.)
+      for (int r = tid; r + 1 < count; r += THREADS) {
         const Candidate &x = s.cand[s.order[r]], &y = s.cand[s.order[r + 1]];
+        if (r >= n && s.cand[s.order[n - 1]].total - y.total > 2 * off) break;
         const int v = x.beam(), w = y.beam();
         if (v != w && x.total - y.total <= s.beam[v].off + s.beam[w].off) s.again[v] = s.again[w] = 1;
       }

@@ -321,6 +321,22 @@ def test_large_states():
     assert all(bool((x[i] == want[i]).all()) for i in range(10))
 
 
+def test_the_last_place_between_more_candidates_of_one_beam():
+    """Behind beam 1's best lie the two best of beam 0, 2^-29 apart, and beam 1's second, 2^-28 above both: whether sums in 32 bits see it above,
+    between or below them, it is the second (sums to 2^-30 do see it)."""
+    g = torch.Generator(device=DEV).manual_seed(31)
+    b, v = 512, 200
+    logits = -torch.rand(b, 2, v, generator=g, device=DEV)
+    logits[:, :, 40] = 0.02
+    logits[:, 0, 50] = torch.nextafter(torch.tensor(0.02), torch.tensor(0.0)).item()
+    logits[:, 1, 90] = 1.0
+    best = torch.log_softmax(logits.double(), -1)[:, :, 40]
+    scores = torch.stack([torch.zeros(b, device=DEV), (best[:, 0] - best[:, 1] + 2.0 ** -28).float()], 1)
+    for n in (2, 3, 4):
+        parents, tokens = check(logits, scores, n)[1:]
+        assert bool((parents[:, :2] == 1).all() and (tokens[:, 1] == 40).all())
+
+
 # ---------------------------------------------------------------- together
 def test_beam_search_finds_what_an_exhaustive_search_of_the_beams_finds():
     """Three steps of a search whose model is a recurrent state: the states follow the beams, so that the scores are those of whole sequences."""
