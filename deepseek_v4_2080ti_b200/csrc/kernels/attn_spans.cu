@@ -248,7 +248,6 @@ __device__ __forceinline__ void span_of(const Params& p, const Item& it, int tok
   }
 }
 
-// Item `idx` of the list; false: there is nothing to do.  Called by whole warps.
 // Which of the 32 keys from `key` on a tree's row sees by its mask, node 0 lying at position `first`: all in the context.
 __device__ __forceinline__ uint32_t tree_bits(const uint32_t* words, int n_words, int key, int first) {
   const int at = key - first;
@@ -257,6 +256,7 @@ __device__ __forceinline__ uint32_t tree_bits(const uint32_t* words, int n_words
   return __funnelshift_r(word(at >> 5), word((at >> 5) + 1), at & 31);
 }
 
+// Item `idx` of the list; false: there is nothing to do.  Called by whole warps.
 template <Form FORM>
 __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Item& it) {
   it.n_rows = 0;

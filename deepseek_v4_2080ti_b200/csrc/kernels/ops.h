@@ -243,7 +243,7 @@ struct AcceptCall {
 };
 int b200_tree_accept(const struct AcceptCall* call);
 
-// ---- beams (beams.cu): the best continuations over beams and vocabulary; states that follow the beams
+// ---- beams (beam_select.cu, beam_reorder.cu): the best continuations over beams and vocabulary; states that follow the beams
 struct SelectCall {
   int bytes, requests;
   const void* logits;                         // [requests beams] rows, row_stride elements apart; fp32 or bf16

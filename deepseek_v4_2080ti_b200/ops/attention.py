@@ -500,7 +500,7 @@ def _check_tree_pages(block_table, nb, bs, kv_len, q_start, q_len, lo, mask) -> 
     seen = _seen_pages(t, width, bs, kv_len, q_start, q_len, lo, context)
     nodes = ((mask[..., None] >> torch.arange(32, dtype=torch.int32, device=mask.device)) & 1).reshape(t, -1)
     key = first[:, None] + torch.arange(32 * words, device=mask.device)                         # [B, nodes]
-    bits = (mine.float() @ nodes.float() > 0) & (key >= 0) & (key < torch.minimum(kv_len, torch.tensor(width * bs, device=mask.device))[:, None])
+    bits = (mine.float() @ nodes.float() > 0) & (key >= 0) & (key < kv_len.clamp(max=width * bs)[:, None])
     seen = seen.long().scatter_add(1, (key.long() // bs).clamp(0, width - 1), bits.long()) > 0
     block_table.masked_fill_(seen & (block_table == -1), -2)
     _lib.check_indices(block_table, 0, nb, 3, keep=-1)
@@ -510,8 +510,8 @@ def decode_tree(q, k_cache, v_cache, block_table, mask, q_start, q_len, kv_len, 
                 max_kv_len: int | None = None, splits: int | None = None, out=None):
     """Attention of the rows of drafted trees - tokens that continue one context in several ways, verified in one pass - against the paged
     cache, which already holds their keys and values: node i of sequence b, row ``q_start[b] + i``, is the key at ``kv_len[b] - q_len[b] + i``.
-    A row sees the context before its tree (from ``lo[t]`` on, for windows) and the nodes whose bits are set in its ``mask``: int32
-    [T, words], bit i % 32 of word i / 32 for node i - itself and the nodes that it continues, as ``tree.layout`` gives it, or any others.
+    A row sees the context before its tree and the nodes whose bits are set in its ``mask``: int32 [T, words], bit i % 32 of word i / 32 for
+    node i - itself and the nodes that it continues, as ``tree.layout`` gives it, or any others; with ``lo`` only keys from ``lo[t]`` on.
     Bits of nodes that a sequence does not have count for nothing.  A row that sees nothing is 0; a key that a row does not see has no part
     in it, whatever the cache holds there.
 

@@ -108,7 +108,7 @@ def _caches(caches, dev: int):
 def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=None, block_table=None, caches=()):
     """The path that the target agrees with: from node 0 to the child whose token is the one predicted at its parent (of several the first),
     as long as there is one, ``max_path`` nodes at most.  tokens / parents / predicted int32 [T], q_start / q_len int32 [B]; negative tokens and
-    predictions agree with nothing.
+    predictions agree with nothing, nor do nodes behind the first 1024.
 
     Returns ``path`` int32 [B, max_path] (nodes, node 0 first), ``count`` int32 [B] and ``emitted`` int32 [B, max_path]: the tokens that the target puts
     behind the path's nodes - the drafts it agrees with, then one of its own; -1 behind ``count``.  A sequence of no rows has a count of 0.

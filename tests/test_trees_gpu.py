@@ -206,6 +206,25 @@ def test_rows_of_no_sequence_stay_and_pages_that_are_not_there(monkeypatch):
         lib.check_status()
 
 
+def test_a_captured_call_in_the_debug_mode(monkeypatch):
+    lib, attention, _ = _modules()
+    monkeypatch.setenv("B200_BOUNDS_CHECK", "1")
+    torch.manual_seed(5)
+    k, v = rand(300, 2, 128), rand(300, 2, 128)
+    kc, vc, table = pages([(k, v)], 64)
+    args = (rand(20, 4, 128), kc, vc, table, _i32([[1 << i] for i in range(20)]), _i32([0]), _i32([20]), _i32([300]), 20)
+    want = attention.decode_tree(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = attention.decode_tree(*args)
+    got.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    lib.check_status()
+    assert torch.equal(got, want)
+
+
 # ---------------------------------------------------------------- positions and masks
 @pytest.mark.parametrize("sizes,width", [([1], 0), ([7], 2), ([61] * 40, 8), ([1, 0, 250, 33], 1), ([1024, 5], 0), ([64, 300, 2], 1000)])
 def test_layout(sizes, width):
