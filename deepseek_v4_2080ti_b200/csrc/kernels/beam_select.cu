@@ -191,6 +191,14 @@ __device__ __forceinline__ Sum<true> sum_exactly(const float (&v)[PER], float m,
   return {(a[0] + a[1]) + (b[0] + b[1]), s.k, s.far};
 }
 
+// The same of one number.
+__device__ __forceinline__ Sum<true> sum_of_one(float m, const Table& t) {
+  double a = 0, b = 0;
+  const Scale s(m);
+  add_exp2(pack2(m - s.far, s.low), t, ((0x4b400000 >> 5) << 20) + (s.k << 20), a, b);     // (the other one, 2^-115 of it, is lost in the rounding)
+  return {a + b, s.k, s.far};
+}
+
 // The same for the first pass, in two operations and an exponential a logit: 2^t with t = x log2 e - k.
 __device__ __forceinline__ Sum<false> sum_quickly(const float (&v)[PER], float m) {
   const Scale s(m);
@@ -500,8 +508,7 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
   auto offers = [&](int w) { return fabsf(p.scores[row0 + w]) < INFINITY; };
   auto finished = [&](int w) { return p.finished && p.finished[row0 + w]; };
   const double off = off_of(p.vocab);
-  auto settle = [&](int w, float score, double ref, double sum, double off) {
-    const double base = (double)score - log(sum);
+  auto settle = [&](int w, double ref, double base, double off) {
     const bool ok = base > -INFINITY && base < INFINITY && ref < INFINITY;             // (not a row with NaN or +inf, or of nothing but -inf)
     s.beam[w] = {ok ? ref : 0.0, ok ? base : -INFINITY, off};
     s.has_lists[w] = ok;
@@ -512,7 +519,7 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
     Sum<false> sum = {0.0, 0, 0.f};                        // (of a beam that offers nothing: what lies there, and does not count)
     for (int i = lane; i < p.parts; i += 32) sum.add(reinterpret_cast<const Sum<false>*>(p.sums)[(row0 + w) * p.parts + i]);
     warp_sum(sum);
-    if (lane == 0) settle(w, score, sum.ref(), ended || !(fabsf(score) < INFINITY) ? 0.0 : sum.sum, off);
+    if (lane == 0) settle(w, sum.ref(), (double)score - log(ended || !(fabsf(score) < INFINITY) ? 0.0 : sum.sum), off);
   }
   for (int w = tid; w < W; w += THREADS) s.again[w] = 0;
   if (tid == 0) s.count = s.n_again = 0;
@@ -652,7 +659,19 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
         }
         cluster_sync();                                    // read before the next beam's, or the block's end
       }
-      if (tid == 0) settle(w, p.scores[row0 + w], sum.ref(), sum.sum, 0.0);
+      // The logarithm relative to the row's largest logit m, which is taken out of the sum as it went in: log sum = m + log1p(the others / exp m),
+      // so that the total of a token that is the only one is the score itself and beams that are equal by that stay equal.
+      if (warp == 0) {
+        uint32_t top = 0;
+        for (int i = lane; i < p.parts; i += 32)
+          top = max(top, (uint32_t)(reinterpret_cast<const unsigned long long*>(p.lists)[((row0 + w) * p.parts + i) * n] >> 32));
+        const float m = from_order(__reduce_max_sync(0xffffffffu, top));
+        if (lane == 0) {
+          const Sum<true> own = sum_of_one(m, table);
+          const double all = sum.k == own.k && sum.far == own.far ? sum.sum : sum.sum * exp(sum.ref() - own.ref());
+          settle(w, (double)m, (double)p.scores[row0 + w] - log1p(fmax(all - own.sum, 0.0) / exp((double)m - own.ref())), 0.0);
+        }
+      }
       __syncthreads();
     }
     if (!ties)

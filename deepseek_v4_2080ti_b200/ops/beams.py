@@ -53,7 +53,8 @@ def select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None, fin
 
     A beam with ``finished`` (bool [B, W]) offers itself alone, with ``pad_token`` and its score as it is.  Tokens with a logit of -inf and beams with a
     score of -inf are not offered, nor are beams whose score or logits hold NaN or +inf; where fewer than n are left the rest is -inf, -1, -1.
-    Sums of exponentials are kept to 2^-30 and totals compared in 64 bits."""
+    Scores are good to 32 bits (their rounding, and 10^-6); where candidates of different beams lie closer together than that their order is taken
+    from sums to 2^-30, in 64 bits."""
     dev, shape = logits.get_device(), logits.shape
     if dev < 0 or len(shape) != 3 or logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"logits: fp32 or bf16 [requests, beams, vocabulary] on a GPU expected, got {logits.dtype} {list(shape)} on {logits.device}")

@@ -321,6 +321,22 @@ def test_large_states():
     assert all(bool((x[i] == want[i]).all()) for i in range(10))
 
 
+@pytest.mark.parametrize("v", [1, 2, 33, 9000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_forced_tokens_of_beams_with_equal_scores(v, dtype):
+    """One token allowed: a beam's total is its score, whatever the logit, so that beams of equal scores - ended ones among them - are equal."""
+    g = torch.Generator(device=DEV).manual_seed(v)
+    logits, _ = random_logits(40, 6, v, dtype)
+    keep = torch.randint(0, v, (40, 6, 1), generator=g, device=DEV)
+    logits = torch.full_like(logits, -math.inf).scatter_(2, keep, logits.gather(2, keep))
+    logits[30:] *= 20000.0
+    scores = -torch.randint(0, 3, (40, 6), generator=g, device=DEV).float() / 3
+    finished = torch.rand(40, 6, generator=g, device=DEV) < 0.3
+    for n in (1, 4, 9):
+        check(logits, scores, n)
+        check(logits, scores, n, finished, v // 2)
+
+
 def test_the_last_place_between_more_candidates_of_one_beam():
     """Behind beam 1's best lie the two best of beam 0, 2^-29 apart, and beam 1's second, 2^-28 above both: whether sums in 32 bits see it above,
     between or below them, it is the second (sums to 2^-30 do see it)."""
