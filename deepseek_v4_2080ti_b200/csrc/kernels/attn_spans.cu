@@ -90,7 +90,6 @@ struct Params {
   // half of the places would be empty.
   int by_sequence;
   int splits;                     // key ranges per row tile
-  int per_item;                   // rows of a tree: key tiles of a range, so that the items of short contexts are fewer, not shorter
   int n_items;
   float scale_log2;               // scale * log2(e)
   float cap_in, cap_out;          // scale / cap, cap * log2(e)
@@ -388,9 +387,13 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
   it.k_end = __reduce_max_sync(0xffffffffu, hi_max);
   it.t0 = it.t1 = 0;
   if (it.k_end > lo_min) {
-    const int a = lo_min / BKV, n = (it.k_end + BKV - 1) / BKV - a, per = FORM == TREE_ROWS ? p.per_item : (int)((uint32_t)(n + splits - 1) / (uint32_t)splits);
+    // Ranges by the keys that are there, not by what the host knows of them: a captured step's bound, or the table's width, is often far above its
+    // contexts, and a window leaves few keys of them.  (16 nodes over 4000 keys with a bound of 4016 / 32768 / 131072: 16.8 / 17.8 / 17.8 us, with ranges
+    // of a length that follows from the bound 16.1 / 25.3 / 42.6; over 32768 keys in a window of 4096: 16.7, and 26.6.  Ranges of at least 2, 3 or 4
+    // tiles gain nothing.)
+    const int a = lo_min / BKV, n = (it.k_end + BKV - 1) / BKV - a, per = (int)((uint32_t)(n + splits - 1) / (uint32_t)splits);
     it.t0 = a + min(n, split * per);
-    it.t1 = a + (FORM == TREE_ROWS && split + 1 == splits ? n : min(n, (split + 1) * per));
+    it.t1 = a + min(n, (split + 1) * per);
   }
   return true;
 }
@@ -1430,17 +1433,16 @@ static int prompt_rows(const SpansCall& a) {
   if (FORM == spans::TREE_ROWS) {
     p.tree = a.tree;
     p.tree_words = a.tree_words;
-    p.per_item = a.per_item;
   }
   return spans::launch<FORM>(p, a);
 }
 extern "C" int b200_attn_spans(const SpansCall* call) { return prompt_rows<spans::SPANS>(*call); }
 
 // Rows of drafted trees: the last q_len[b] of sequence b's kv_len[b] keys are its tree's nodes.  Row t sees the context before them from
-// lo[t] on, and the nodes whose bits are set in its tree_words words of `tree`.  per_item: key tiles of an item; what
-// lies behind splits of them goes with the last.
+// lo[t] on, and the nodes whose bits are set in its tree_words words of `tree`.  splits: items that the keys a row tile sees are
+// cut into at most.
 extern "C" int b200_attn_tree(const SpansCall* call) {
-  if (call->bytes != (int)sizeof(SpansCall) || !call->tree || call->tree_words < 1 || call->per_item < 1 || call->hi) return -ERR_BAD_ARG;
+  if (call->bytes != (int)sizeof(SpansCall) || !call->tree || call->tree_words < 1 || call->hi) return -ERR_BAD_ARG;
   return prompt_rows<spans::TREE_ROWS>(*call);
 }
 

@@ -207,7 +207,7 @@ struct SpansCall {
   float* workspace;                           // [splits T Hq 130]: partial sums of several items, or of the shared keys
   int* status;
   cudaStream_t stream;
-  int n_groups, max_q_len, T, max_blocks, num_blocks, block_size, n_q_heads, n_kv_heads, splits, cluster, tree_words, per_item;
+  int n_groups, max_q_len, T, max_blocks, num_blocks, block_size, n_q_heads, n_kv_heads, splits, cluster, tree_words;
   float scale, cap;
 };
 int b200_qk_norm_rope_axes_append(const AxesAppendCall* call);

@@ -272,7 +272,7 @@ def _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap):
 
 
 # The kernels' arguments as one block each (AxesAppendCall and SpansCall in ops.h), packed: a third of what 33 arguments cost one by one.
-_AXES_CALL, _SPANS_CALL = struct.Struct("@ii13P16iff64s"), struct.Struct("@ii17P12iff0P")
+_AXES_CALL, _SPANS_CALL = struct.Struct("@ii13P16iff64s"), struct.Struct("@ii17P11iff0P")
 _typed = False
 
 
@@ -483,7 +483,7 @@ def prefill_spans(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, max_
     rc = _kernels().b200_attn_spans(_SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
         q_start.data_ptr(), q_len.data_ptr(), _at(lo), _at(hi), 0, 0, 0, _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq, hkv,
-        splits, 1, 0, 0, scale, cap))
+        splits, 1, 0, scale, cap))
     _lib.check(rc, "prefill_spans", 2 if splits > 1 else 1)
     return out
 
@@ -515,7 +515,9 @@ def decode_tree(q, k_cache, v_cache, block_table, mask, q_start, q_len, kv_len, 
     Bits of nodes that a sequence does not have count for nothing.  A row that sees nothing is 0; a key that a row does not see has no part
     in it, whatever the cache holds there.
 
-    The other arguments, pages and rows of no sequence as in ``prefill_spans``."""
+    The other arguments, pages and rows of no sequence as in ``prefill_spans``.  The keys that a row tile sees are cut
+    into ``splits`` items by how many there are; ``max_kv_len`` only bounds their number, so that a bound far above the contexts costs no more
+    than the items' join."""
     dev, t, hq, nb, hkv, bs, b, width, scale, out = _paged(q, k_cache, v_cache, block_table, kv_len, gate, out, scale, cap)
     if _current() != dev:
         with torch.cuda.device(dev):
@@ -533,9 +535,8 @@ def decode_tree(q, k_cache, v_cache, block_table, mask, q_start, q_len, kv_len, 
         raise ValueError(f"trees of {max_q_len} rows, masks of {32 * words} nodes")
     if t == 0 or b == 0 or max_q_len <= 0:
         return out
-    longest = max_kv_len if max_kv_len is not None else width * bs
     if splits is None:
-        splits = _row_splits(b, t, hq // hkv, hkv, max_q_len, longest)
+        splits = _row_splits(b, t, hq // hkv, hkv, max_q_len, max_kv_len if max_kv_len is not None else width * bs)
     if not 1 <= splits <= 1024:
         raise ValueError(f"{splits} splits")
     ws = q.new_empty(splits * t * hq * (D + 2), dtype=_F32) if splits > 1 else None
@@ -543,7 +544,7 @@ def decode_tree(q, k_cache, v_cache, block_table, mask, q_start, q_len, kv_len, 
     rc = _kernels().b200_attn_tree(_SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
         q_start.data_ptr(), q_len.data_ptr(), _at(lo), 0, 0, 0, mask.data_ptr(), _at(ws), _status(dev), _stream(dev), 0, max_q_len, t, width, nb, bs, hq,
-        hkv, splits, 1, words, max(1, -(-longest // (KEY_TILE * splits))), scale, cap))
+        hkv, splits, 1, words, scale, cap))
     _lib.check(rc, "decode_tree", 2 if splits > 1 else 1)
     return out
 
@@ -641,7 +642,7 @@ def decode_shared(q, k_cache, v_cache, block_table, kv_len, group_start, shared_
     call = _SPANS_CALL.pack(
         _SPANS_CALL.size, b, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _at(gate), block_table.data_ptr(), kv_len.data_ptr(),
         0, 0, 0, 0, group_start.data_ptr(), shared_len.data_ptr(), 0, _at(ws), _status(dev), _stream(dev), n, 1, t, width, nb, bs, hq, hkv, splits, cluster,
-        0, 0, scale, cap)
+        0, scale, cap)
     if n:
         _lib.check(lib.b200_attn_shared(call), "decode_shared")
     _lib.check(lib.b200_attn_own_rows(call), "decode_shared")

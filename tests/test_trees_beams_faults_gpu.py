@@ -1,0 +1,76 @@
+"""Faults of the calls over drafted trees and beams that were found after they had run, each with the test that shows it."""
+import random
+
+import pytest
+import torch
+
+from test_spans_gpu import DEV, _i32, close, pages, rand
+from test_trees_gpu import bits, chain_of, oracle, random_tree
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- key ranges of tree attention
+def tree_inputs(lens, hq, hkv, bs=64, wide=None, window=0, seed=0):
+    """``lens``: [(nodes, context)].  (arguments of ``decode_tree`` up to max_q_len, lo, (sequences, rows' sets of keys))."""
+    torch.manual_seed(seed + sum(n + c for n, c in lens))
+    rng = random.Random(seed)
+    seqs = [(rand(n + c, hkv, 128), rand(n + c, hkv, 128)) for n, c in lens]
+    kc, vc, table = pages(seqs, bs, table_width=wide)
+    total, most = sum(n for n, _ in lens), max(n for n, _ in lens)
+    starts = [sum(n for n, _ in lens[:i]) for i in range(len(lens))]
+    mask, lo, seen = [], [], []
+    for n, c in lens:
+        parents = random_tree(n, 3, rng)
+        see = torch.zeros(n, n + c, dtype=torch.bool)
+        see[:, :c] = True
+        for x in range(n):
+            chain = chain_of(parents, x)
+            mask.append(bits(chain, (most + 31) // 32))
+            lo.append(max(0, c + len(chain) - window) if window else 0)
+            see[x, [c + y for y in chain]] = True
+            see[x, :lo[-1]] = False
+        seen.append(see.to(DEV))
+    q = rand(total, hq, 128, scale=1.5)
+    args = (q, kc, vc, table, _i32(mask), _i32(starts), _i32([n for n, _ in lens]), _i32([n + c for n, c in lens]), most)
+    return args, _i32(lo) if window else None, (seqs, seen, starts)
+
+
+@pytest.mark.parametrize("lens,window", [([(16, 4000)], 0), ([(9, 700), (30, 2500), (4, 60)], 0), ([(16, 9000)], 1000), ([(12, 5000), (7, 3)], 300)])
+def test_key_ranges_follow_the_keys_and_not_the_bound(lens, window):
+    """A row tile's keys are cut into ``splits`` items by how many there are, so that a bound that is far above them - a captured step's, the
+    table's - leaves the work where it is: the same bits as with the longest context itself."""
+    from deepseek_v4_2080ti_b200.ops import _lib, attention
+    args, lo, (seqs, seen, starts) = tree_inputs(lens, 10, 2, wide=512, window=window)
+    most = max(n + c for n, c in lens)
+    for splits in (2, 6, 18):
+        outs = [attention.decode_tree(*args, lo=lo, splits=splits, max_kv_len=bound) for bound in (most, 4 * most, 131072, None)]
+        assert all(torch.equal(x, outs[0]) for x in outs[1:])
+        for i, (n, _) in enumerate(lens):
+            r = slice(starts[i], starts[i] + n)
+            close(outs[0][r], *oracle(args[0][r], *seqs[i], seen[i]))
+    outs = [attention.decode_tree(*args, lo=lo, max_kv_len=bound) for bound in (131072, None)]      # and as many items as either bound gives
+    for i, (n, _) in enumerate(lens):
+        r = slice(starts[i], starts[i] + n)
+        for x in outs:
+            close(x[r], *oracle(args[0][r], *seqs[i], seen[i]))
+    _lib.check_status()
+
+
+def test_a_captured_step_is_cut_as_the_contexts_that_it_meets():
+    """One graph for contexts of 40 to 7000 keys: at every replay the bits of a call that knows the longest of them."""
+    from deepseek_v4_2080ti_b200.ops import attention
+    args, _, _ = tree_inputs([(16, 7000), (16, 5000)], 10, 2)
+    kv = args[7].clone()
+    call = lambda bound: attention.decode_tree(*args[:7], kv, 16, splits=9, max_kv_len=bound)
+    call(7016)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call(None)
+    for lens in ([7016, 5016], [1500, 40], [56, 3000], [16, 16]):
+        kv.copy_(_i32(lens))
+        graph.replay()
+        want = call(max(lens))
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
