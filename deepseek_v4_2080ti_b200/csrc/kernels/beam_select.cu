@@ -41,6 +41,7 @@ constexpr int WARP_TILE = 32 * PER;
 constexpr int AHEAD = 2;                   // tiles on their way to L2
 constexpr int LIST = 256;                  // candidates of a warp: n and as many new ones
 constexpr int CAP = 1024;                  // candidates that are ordered by counting
+constexpr int FEW = 128;                   // candidates that are ordered with no look first at which may be among the best (64: 8.7 us, 9.5 with it; 256: 14.0, 10.9 with it)
 constexpr float LOWEST = -80.f;            // exp of this beside 1 is below 2^-115: smaller ones count as this
 constexpr float LOG2E = 1.44269504f;
 
@@ -471,7 +472,8 @@ struct Candidate {
 struct Join {
   Beam beam[MAX_BEAMS];
   unsigned char again[MAX_BEAMS];            // beams whose order is not certain
-  unsigned char has_lists[MAX_BEAMS];        // beams that offer tokens
+  unsigned char has_lists[MAX_BEAMS];        // beams that offer tokens,
+  unsigned char live[MAX_BEAMS];             // and which they are
   Candidate cand[CAP];                       // any order
   ulonglong2 key[CAP];                       // their totals as numbers, and places
   unsigned short order[CAP];                 // best first
@@ -481,7 +483,7 @@ struct Join {
   uint32_t hi[32], lo[32];
   Candidate best[WARPS];
   int from[WARPS], list[MAX_BEAMS];
-  int count, n_again;
+  int count, n_again, n_live;
 };
 
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
@@ -524,12 +526,25 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
   for (int w = tid; w < W; w += THREADS) s.again[w] = 0;
   if (tid == 0) s.count = s.n_again = 0;
   __syncthreads();
-  const int lists = W * p.parts;
+  // Lists of the beams that offer tokens alone: of the others nothing has been written, and samples of theirs would stand for nothing below (a
+  // search's first step, one beam of 8 and 64 candidates over 248320 tokens: 29 us, and 108 with them, as 1984 entries came in and were taken for ties).
+  if (warp == 0) {
+    int found = 0;
+    for (int w0 = 0; w0 < W; w0 += 32) {
+      const bool on = w0 + lane < W && s.has_lists[w0 + lane];
+      const uint32_t go = __ballot_sync(0xffffffffu, on);
+      if (on) s.live[found + __popc(go & ((1u << lane) - 1))] = (unsigned char)(w0 + lane);
+      found += __popc(go);
+    }
+    if (lane == 0) s.n_live = found;
+  }
+  __syncthreads();
+  const int lists = s.n_live * p.parts;
   auto of_beam = [&](int w, float x) { return ((double)x - s.beam[w].ref) + s.beam[w].base; };
   auto entry = [&](int list, int i) -> Candidate {         // the i-th of a list, a total of -inf where there is none
-    const int w = (int)((uint32_t)list / (uint32_t)p.parts);
-    if (!s.has_lists[w]) return {-INFINITY, 0, 0.f};       // (nothing has been written there)
-    const unsigned long long y = reinterpret_cast<const unsigned long long*>(p.lists)[(row0 * p.parts + list) * n + i];
+    const uint32_t at = (uint32_t)list / (uint32_t)p.parts;
+    const int w = s.live[at];
+    const unsigned long long y = reinterpret_cast<const unsigned long long*>(p.lists)[((row0 + w) * p.parts + ((uint32_t)list - at * p.parts)) * n + i];
     const float x = from_order((uint32_t)(y >> 32));
     return {y == 0 ? -INFINITY : of_beam(w, x), (long long)w << 32 | (uint32_t)~(uint32_t)y, x};
   };
@@ -537,24 +552,20 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
     const int at = atomicAdd(&s.count, 1);
     if (at < CAP) s.cand[at] = c;
   };
-  if (lists * n <= THREADS) {                              // all there are
-    if (tid < lists * n) {
-      const Candidate c = entry((uint32_t)tid / (uint32_t)n, (uint32_t)tid % (uint32_t)n);
-      if (c.total > -INFINITY) push(c);
-    }
+  // A bound from below of the n-th largest: that of THREADS of them, the first d of every list or the best of several lists' first.  As
+  // numbers of 32 bits, rounded down, the last eight the thread's, so that no two are equal; lower by how far two totals may be off.
+  const int d = lists < THREADS ? min(n, THREADS / max(1, lists)) : 1;
+  Candidate mine = {-INFINITY, 0, 0.f};
+  if (d > 1 || lists <= THREADS) {
+    if (tid < lists * d) mine = entry((uint32_t)tid / (uint32_t)d, (uint32_t)tid % (uint32_t)d);
   } else {
-    // A bound from below of the n-th largest: that of THREADS of them, the first d of every list or the best of several lists' first.  As
-    // numbers of 32 bits, rounded down, the last eight the thread's, so that no two are equal; lower by how far two totals may be off.
-    const int d = lists < THREADS ? THREADS / lists : 1;
-    double mine = -INFINITY;
-    if (d > 1) {
-      if (tid < lists * d) mine = entry((uint32_t)tid / (uint32_t)d, (uint32_t)tid % (uint32_t)d).total;
-    } else {
-      for (int list = tid; list < lists; list += THREADS) mine = fmax(mine, entry(list, 0).total);
-    }
-    const uint32_t key = order_of(__double2float_rd(mine - 2 * off)) & ~255u | (uint32_t)(255 - tid);
+    for (int list = tid; list < lists; list += THREADS) mine.total = fmax(mine.total, entry(list, 0).total);
+  }
+  if (tid == 0) s.bound = -INFINITY;
+  const bool all = lists * n <= THREADS;                   // every thread holds one, and there are no others
+  if (lists * n > FEW) {
+    const uint32_t key = order_of(__double2float_rd(mine.total - 2 * off)) & ~255u | (uint32_t)(255 - tid);
     s.sample[tid] = key;
-    if (tid == 0) s.bound = -INFINITY;
     __syncthreads();
     int above = 0;
 #pragma unroll 8
@@ -563,9 +574,13 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
       above += (int)(x.x > key) + (int)(x.y > key) + (int)(x.z > key) + (int)(x.w > key);
     }
     if (above == n - 1 && key > (ORDER_NONE | 255u)) s.bound = from_order(key & ~255u);
-    __syncthreads();
-    const double bound = s.bound;
-    auto reaches = [&](const Candidate& c) { return c.total > -INFINITY && c.total >= bound; };
+  }
+  __syncthreads();
+  const double bound = s.bound;
+  auto reaches = [&](const Candidate& c) { return c.total > -INFINITY && c.total >= bound; };
+  if (all) {
+    if (reaches(mine)) push(mine);
+  } else {
     for (int list = tid; list < lists; list += THREADS)    // a thread per list, whose entries are in order, four on their way at a time
       for (int i = 0; i < n; i += 4) {
         Candidate c[4];

@@ -1,9 +1,11 @@
 """Faults of the calls over drafted trees and beams that were found after they had run, each with the test that shows it."""
+import math
 import random
 
 import pytest
 import torch
 
+from test_beams_gpu import check, random_logits
 from test_spans_gpu import DEV, _i32, close, pages, rand
 from test_trees_gpu import bits, chain_of, oracle, random_tree
 
@@ -74,3 +76,24 @@ def test_a_captured_step_is_cut_as_the_contexts_that_it_meets():
         want = call(max(lens))
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------- what lets candidates into the join of beam selection
+def alone(logits, scores, w, n):
+    """The selection over one beam of every request: the scores that sums of the first pass give."""
+    from deepseek_v4_2080ti_b200.ops import beams
+    return beams.select(logits[:, w:w + 1], scores[:, w:w + 1].contiguous(), n)
+
+
+@pytest.mark.parametrize("w,n", [(8, 64), (20, 40), (4, 128), (13, 33)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_first_step_of_a_search(w, n, dtype):
+    """One beam of several offers tokens, as at a search's first step: its candidates are picked from its own lists, and none of them is so near to
+    another beam's that its row would be summed again - the bits of the same beam alone."""
+    for live in range(0, w, 3):
+        logits, scores = random_logits(1, w, 248320, dtype, seed=live)
+        scores[:, :live] = scores[:, live + 1:] = -math.inf
+        scores[:, live] = 0
+        got = check(logits, scores, n)
+        one = alone(logits, scores, live, n)
+        assert torch.equal(got[0], one[0]) and torch.equal(got[2], one[2]) and bool((got[1] == live).all())
