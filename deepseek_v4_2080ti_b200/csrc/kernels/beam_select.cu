@@ -497,6 +497,67 @@ __device__ __forceinline__ Sum<true> of_rank(const Sum<true>* p, uint32_t rank) 
   return s;
 }
 
+// The i-th of a list of a beam that offers tokens, a total of -inf where there is none; lists in those beams' order.
+__device__ __forceinline__ Candidate entry_of(const Join& s, const SelectCall& p, size_t row0, int list, int i) {
+  const uint32_t at = (uint32_t)list / (uint32_t)p.parts;
+  const int w = s.live[at];
+  const unsigned long long y = reinterpret_cast<const unsigned long long*>(p.lists)[((row0 + w) * p.parts + ((uint32_t)list - at * p.parts)) * p.n + i];
+  const float x = from_order((uint32_t)(y >> 32));
+  return {y == 0 ? -INFINITY : ((double)x - s.beam[w].ref) + s.beam[w].base, (long long)w << 32 | (uint32_t)~(uint32_t)y, x};
+}
+// A sample's total as a number of 32 bits, rounded down, the last eight the thread's, so that no two are equal; lower by how far two totals may be off.
+// Of all threads' samples the r-th largest becomes the bound, if it is nearer.
+__device__ __forceinline__ void raise_bound(Join& s, double total, double off, int r) {
+  const uint32_t key = order_of(__double2float_rd(total - 2 * off)) & ~255u | (uint32_t)(255 - threadIdx.x);
+  s.sample[threadIdx.x] = key;
+  __syncthreads();
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < THREADS / 4; ++i) {
+    const uint4 x = reinterpret_cast<const uint4*>(s.sample)[i];
+    above += (int)(x.x > key) + (int)(x.y > key) + (int)(x.z > key) + (int)(x.w > key);
+  }
+  if (above == r - 1 && key > (ORDER_NONE | 255u)) s.bound = fmaxf(s.bound, from_order(key & ~255u));
+  __syncthreads();
+}
+__device__ __forceinline__ void push(Join& s, const Candidate& c) {
+  const int at = atomicAdd(&s.count, 1);
+  if (at < CAP) s.cand[at] = c;
+}
+// Beams at their end offer their score, which is what it is.
+__device__ __forceinline__ void push_ended(Join& s, const SelectCall& p, size_t row0) {
+  for (int w = threadIdx.x; w < p.beams; w += THREADS) {
+    const float score = p.scores[row0 + w];
+    if (p.finished && p.finished[row0 + w] && fabsf(score) < INFINITY) {
+      s.beam[w] = {0.0, 0.0, 0.0};
+      push(s, {(double)score, (long long)w << 32 | p.pad_token, score});
+    }
+  }
+}
+// More have come in than are ordered by counting, as the first entries of the lists hold too few of a beam's that is far ahead of the others: a second
+// bound, from entries further back.  One at place step - 1 stands for `step` that reach it, so that the n / step-th largest of such is a bound;
+// lists of n let in more than CAP only where CAP / n lists or more reach far enough, of which n / step are asked for.  One of 8 beams ahead, 64
+// candidates over 248320 tokens: 53 us, and 192 where all were taken for ties.  (Not in line: small calls, which do without it, take 0.3 to 0.4 us of 10 more.)
+__device__ __noinline__ void look_further(Join& s, const SelectCall& p, size_t row0, int lists, double off) {
+  const int step = max(2, (p.n * p.n + CAP - 1) / CAP);
+  const float bound = s.bound;
+  double best = -INFINITY;
+  for (int list = threadIdx.x; list < lists && step <= p.n; list += THREADS) best = fmax(best, entry_of(s, p, row0, list, step - 1).total);
+  raise_bound(s, best, off, (p.n + step - 1) / step);
+  const float nearer = s.bound;
+  if (!(nearer > bound)) return;                           // ties
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+  for (int list = threadIdx.x; list < lists; list += THREADS)
+    for (int i = 0; i < p.n; ++i) {
+      const Candidate c = entry_of(s, p, row0, list, i);
+      if (!(c.total > -INFINITY && c.total >= nearer)) break;
+      push(s, c);
+    }
+  push_ended(s, p, row0);
+  __syncthreads();
+}
+
 template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 select_join_kernel(const __grid_constant__ SelectCall p) {
@@ -541,45 +602,23 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
   __syncthreads();
   const int lists = s.n_live * p.parts;
   auto of_beam = [&](int w, float x) { return ((double)x - s.beam[w].ref) + s.beam[w].base; };
-  auto entry = [&](int list, int i) -> Candidate {         // the i-th of a list, a total of -inf where there is none
-    const uint32_t at = (uint32_t)list / (uint32_t)p.parts;
-    const int w = s.live[at];
-    const unsigned long long y = reinterpret_cast<const unsigned long long*>(p.lists)[((row0 + w) * p.parts + ((uint32_t)list - at * p.parts)) * n + i];
-    const float x = from_order((uint32_t)(y >> 32));
-    return {y == 0 ? -INFINITY : of_beam(w, x), (long long)w << 32 | (uint32_t)~(uint32_t)y, x};
-  };
-  auto push = [&](const Candidate& c) {
-    const int at = atomicAdd(&s.count, 1);
-    if (at < CAP) s.cand[at] = c;
-  };
-  // A bound from below of the n-th largest: that of THREADS of them, the first d of every list or the best of several lists' first.  As
-  // numbers of 32 bits, rounded down, the last eight the thread's, so that no two are equal; lower by how far two totals may be off.
+  auto entry = [&](int list, int i) { return entry_of(s, p, row0, list, i); };
+  // A bound from below of the n-th largest: that of THREADS of them, the first d of every list or the best of several lists' first.
   const int d = lists < THREADS ? min(n, THREADS / max(1, lists)) : 1;
   Candidate mine = {-INFINITY, 0, 0.f};
-  if (d > 1 || lists <= THREADS) {
+  if (lists <= THREADS) {
     if (tid < lists * d) mine = entry((uint32_t)tid / (uint32_t)d, (uint32_t)tid % (uint32_t)d);
   } else {
     for (int list = tid; list < lists; list += THREADS) mine.total = fmax(mine.total, entry(list, 0).total);
   }
   if (tid == 0) s.bound = -INFINITY;
   const bool all = lists * n <= THREADS;                   // every thread holds one, and there are no others
-  if (lists * n > FEW) {
-    const uint32_t key = order_of(__double2float_rd(mine.total - 2 * off)) & ~255u | (uint32_t)(255 - tid);
-    s.sample[tid] = key;
-    __syncthreads();
-    int above = 0;
-#pragma unroll 8
-    for (int i = 0; i < THREADS / 4; ++i) {
-      const uint4 x = reinterpret_cast<const uint4*>(s.sample)[i];
-      above += (int)(x.x > key) + (int)(x.y > key) + (int)(x.z > key) + (int)(x.w > key);
-    }
-    if (above == n - 1 && key > (ORDER_NONE | 255u)) s.bound = from_order(key & ~255u);
-  }
-  __syncthreads();
+  if (lists * n > FEW) raise_bound(s, mine.total, off, n);
+  else __syncthreads();
   const double bound = s.bound;
   auto reaches = [&](const Candidate& c) { return c.total > -INFINITY && c.total >= bound; };
   if (all) {
-    if (reaches(mine)) push(mine);
+    if (reaches(mine)) push(s, mine);
   } else {
     for (int list = tid; list < lists; list += THREADS)    // a thread per list, whose entries are in order, four on their way at a time
       for (int i = 0; i < n; i += 4) {
@@ -588,16 +627,13 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
         for (int x = 0; x < 4; ++x) c[x] = i + x < n ? entry(list, i + x) : Candidate{-INFINITY, 0, 0.f};
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          if (reaches(c[x])) push(c[x]);
+          if (reaches(c[x])) push(s, c[x]);
         if (!reaches(c[3])) break;
       }
   }
-  for (int w = tid; w < W; w += THREADS)
-    if (finished(w) && offers(w)) {
-      s.beam[w] = {0.0, 0.0, 0.0};                         // offers its score, which is what it is
-      push({(double)p.scores[row0 + w], (long long)w << 32 | p.pad_token, p.scores[row0 + w]});
-    }
+  push_ended(s, p, row0);
   __syncthreads();
+  if (s.count > CAP) look_further(s, p, row0, lists, off);
   const int count = s.count;
   const bool ties = count > CAP;                           // more candidates about the n-th than are ordered by counting
   auto put = [&](int r, const Candidate& c) {

@@ -97,3 +97,29 @@ def test_the_first_step_of_a_search(w, n, dtype):
         got = check(logits, scores, n)
         one = alone(logits, scores, live, n)
         assert torch.equal(got[0], one[0]) and torch.equal(got[2], one[2]) and bool((got[1] == live).all())
+
+
+@pytest.mark.parametrize("w,n", [(8, 64), (20, 40), (4, 128), (3, 100)])
+def test_a_beam_far_ahead_of_the_others(w, n):
+    """All candidates come from one beam, more of them above what a sample of all lists gives as a bound than are ordered at once: the bits of that
+    beam alone."""
+    for ahead in range(0, w, 3):
+        logits, scores = random_logits(1, w, 248320, seed=ahead)
+        scores[:] = -1000 - torch.arange(w, device=DEV)
+        scores[:, ahead] = 0
+        got = check(logits, scores, n)
+        one = alone(logits, scores, ahead, n)
+        assert torch.equal(got[0], one[0]) and torch.equal(got[2], one[2]) and bool((got[1] == ahead).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_some_beams_far_ahead(dtype):
+    """Two or three beams share all places, beams at their end among them; equal logits by the thousand; several requests."""
+    for b, w, n in ((1, 16, 128), (2, 10, 128), (3, 6, 100), (1, 40, 64)):
+        logits, scores = random_logits(b, w, 248320, dtype, seed=n)
+        scores[:, 3:] -= 1000
+        finished = torch.zeros(b, w, dtype=torch.bool, device=DEV)
+        finished[:, -1] = finished[-1, 1] = True
+        scores[0, -1] = -3.0
+        check(logits, scores, n, finished, 17)
+        check((logits.float() * 0.5).round().to(dtype), scores.round(), n, finished, 17)
