@@ -1,6 +1,6 @@
 // Beam search's selection over the beams of a request and the vocabulary, sm_100a.
 //
-//   total[w, v] = score[w] + x[w, v] - log sum_u exp x[w, u];  the n largest of a request, ties to the lowest (w, v)
+//   total[w, v] = score[w] + x[w, v] - log sum_u exp x[w, u];  the n largest of a request, ties to the lowest w, the largest x, the lowest v
 //
 // select_parts_kernel reads the logits once: a block takes `tiles` tiles of 8192 logits of one row, 32 a thread in registers, adds
 // their exponentials and keeps its n largest logits, in order, beside the sum.  select_join_kernel, a block per request, adds up the sums of
@@ -461,12 +461,16 @@ select_parts_kernel(const __grid_constant__ SelectCall p) {
 struct Beam {
   double ref, base, off;                   // off: how far totals may be off
 };
+// Of one beam the larger logit is first, also where 64 bits do not tell the totals apart (logits of 1e-30 beside 0, scores of -1e30), so that fewer
+// candidates are the first of more.
 struct Candidate {
   double total;
   long long place;                         // beam << 32 | token
   float x;                                 // logit; score of a beam at its end
   __device__ __forceinline__ int beam() const { return (int)(place >> 32); }
-  __device__ __forceinline__ bool before(const Candidate& o) const { return total > o.total || total == o.total && place < o.place; }
+  __device__ __forceinline__ bool before(const Candidate& o) const {
+    return total > o.total || total == o.total && (x == o.x || beam() != o.beam() ? place < o.place : x > o.x);
+  }
 };
 
 struct Join {
@@ -484,6 +488,7 @@ struct Join {
   Candidate best[WARPS];
   int from[WARPS], list[MAX_BEAMS];
   int count, n_again, n_live;
+  int mixed;                                 // equal totals of one beam whose logits are not
 };
 
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
@@ -558,6 +563,63 @@ __device__ __noinline__ void look_further(Join& s, const SelectCall& p, size_t r
   __syncthreads();
 }
 
+__device__ __forceinline__ void put(const SelectCall& p, int b, int r, const Candidate& c) {
+  const size_t at = (size_t)b * p.n + r;
+  p.out_scores[at] = (float)c.total;
+  p.out_parents[at] = c.beam();
+  p.out_tokens[at] = (int)(uint32_t)c.place;
+}
+// Where counting does not give the order - more candidates about the n-th than it takes, or equal totals of one beam whose logits are not -: the best
+// head of all lists, n times.  A thread's lists are its own, list l thread l % THREADS's, their places 16 bits each in s.cand's room.  How many
+// there were.  (With the logits in every comparison of the counting, selections took 4 to 40 % longer.)
+__device__ __noinline__ int pick_in_turn(Join& s, const SelectCall& p, size_t row0, int b, int rank, int lists) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.n;
+  unsigned short* at = reinterpret_cast<unsigned short*>(s.cand);
+  const int all = lists + p.beams;                         // (behind the lists: beams at their end)
+  for (int l = tid; l < all; l += THREADS) at[l] = l < lists || p.finished && p.finished[row0 + l - lists] && fabsf(p.scores[row0 + l - lists]) < INFINITY ? 0 : 1;
+  for (int r = 0; r < n; ++r) {
+    Candidate best = {-INFINITY, 0x7fffffffffffffffll, 0.f};
+    int from = -1;
+    for (int l = tid; l < all; l += THREADS) {
+      Candidate c = {-INFINITY, 0, 0.f};
+      if (l < lists) {
+        if (at[l] < n) c = entry_of(s, p, row0, l, at[l]);
+      } else if (at[l] == 0) {
+        const float score = p.scores[row0 + l - lists];
+        c = {(double)score, (long long)(l - lists) << 32 | p.pad_token, score};
+      }
+      if (c.total > -INFINITY && c.before(best)) {
+        best = c;
+        from = l;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Candidate c = {__shfl_xor_sync(0xffffffffu, best.total, o), __shfl_xor_sync(0xffffffffu, best.place, o), __shfl_xor_sync(0xffffffffu, best.x, o)};
+      const int l = __shfl_xor_sync(0xffffffffu, from, o);
+      if (c.before(best)) {
+        best = c;
+        from = l;
+      }
+    }
+    __syncthreads();
+    if (lane == 0) {
+      s.best[warp] = best;
+      s.from[warp] = from;
+    }
+    __syncthreads();
+    for (int w = 0; w < WARPS; ++w)
+      if (s.best[w].before(best)) {
+        best = s.best[w];
+        from = s.from[w];
+      }
+    if (from < 0) return r;
+    if (from % THREADS == tid) ++at[from];
+    if (tid == 0 && rank == 0) put(p, b, r, best);
+  }
+  return n;
+}
+
 template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 select_join_kernel(const __grid_constant__ SelectCall p) {
@@ -585,7 +647,7 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
     if (lane == 0) settle(w, sum.ref(), (double)score - log(ended || !(fabsf(score) < INFINITY) ? 0.0 : sum.sum), off);
   }
   for (int w = tid; w < W; w += THREADS) s.again[w] = 0;
-  if (tid == 0) s.count = s.n_again = 0;
+  if (tid == 0) s.count = s.n_again = s.mixed = 0;
   __syncthreads();
   // Lists of the beams that offer tokens alone: of the others nothing has been written, and samples of theirs would stand for nothing below (a
   // search's first step, one beam of 8 and 64 candidates over 248320 tokens: 29 us, and 108 with them, as 1984 entries came in and were taken for ties).
@@ -636,13 +698,6 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
   if (s.count > CAP) look_further(s, p, row0, lists, off);
   const int count = s.count;
   const bool ties = count > CAP;                           // more candidates about the n-th than are ordered by counting
-  auto put = [&](int r, const Candidate& c) {
-    if (rank > 0) return;
-    const size_t at = (size_t)b * n + r;
-    p.out_scores[at] = (float)c.total;
-    p.out_parents[at] = c.beam();
-    p.out_tokens[at] = (int)(uint32_t)c.place;
-  };
   for (;;) {
     if (ties) {
       for (int w = tid; w < W; w += THREADS) s.again[w] = W > 1 && s.beam[w].base > -INFINITY && s.beam[w].off > 0.0;
@@ -667,6 +722,7 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
         if (r >= n && s.cand[s.order[n - 1]].total - y.total > 2 * off) break;
         const int v = x.beam(), w = y.beam();
         if (v != w && x.total - y.total <= s.beam[v].off + s.beam[w].off) s.again[v] = s.again[w] = 1;
+        if (x.total == y.total && v == w && x.x < y.x) s.mixed = 1;
       }
     }
     __syncthreads();
@@ -733,54 +789,10 @@ select_join_kernel(const __grid_constant__ SelectCall p) {
     __syncthreads();
   }
   int done = min(count, n);
-  if (!ties) {
-    for (int r = tid; r < done; r += THREADS) put(r, s.cand[s.order[r]]);
+  if (!ties && !s.mixed) {
+    for (int r = tid; r < done && rank == 0; r += THREADS) put(p, b, r, s.cand[s.order[r]]);
   } else {
-    // the best head of all lists, n times: a thread's lists are its own, list l thread l % THREADS's, their places 16 bits each in s.cand's room
-    unsigned short* at = reinterpret_cast<unsigned short*>(s.cand);
-    const int all = lists + W;                             // (behind the lists: beams at their end)
-    for (int l = tid; l < all; l += THREADS) at[l] = l < lists || finished(l - lists) && offers(l - lists) ? 0 : 1;
-    done = 0;
-    for (int r = 0; r < n; ++r) {
-      Candidate best = {-INFINITY, 0x7fffffffffffffffll, 0.f};
-      int from = -1;
-      for (int l = tid; l < all; l += THREADS) {
-        Candidate c = {-INFINITY, 0, 0.f};
-        if (l < lists) {
-          if (at[l] < n) c = entry(l, at[l]);
-        } else if (at[l] == 0) {
-          c = {(double)p.scores[row0 + l - lists], (long long)(l - lists) << 32 | p.pad_token, 0.f};
-        }
-        if (c.total > -INFINITY && c.before(best)) {
-          best = c;
-          from = l;
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const Candidate c = {__shfl_xor_sync(0xffffffffu, best.total, o), __shfl_xor_sync(0xffffffffu, best.place, o), 0.f};
-        const int l = __shfl_xor_sync(0xffffffffu, from, o);
-        if (c.before(best)) {
-          best = c;
-          from = l;
-        }
-      }
-      __syncthreads();
-      if (lane == 0) {
-        s.best[warp] = best;
-        s.from[warp] = from;
-      }
-      __syncthreads();
-      for (int w = 0; w < WARPS; ++w)
-        if (s.best[w].before(best)) {
-          best = s.best[w];
-          from = s.from[w];
-        }
-      if (from < 0) break;
-      if (from % THREADS == tid) ++at[from];
-      if (tid == 0) put(r, best);
-      ++done;
-    }
+    done = pick_in_turn(s, p, row0, b, rank, lists);
   }
   for (int r = done + tid; r < n && rank == 0; r += THREADS) {
     const size_t at = (size_t)b * n + r;

@@ -48,7 +48,7 @@ def _parts(rows: int, vocab: int) -> tuple[int, int]:
 def select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None, finished: torch.Tensor | None = None,
            pad_token: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``n`` best continuations (default: as many as beams) of every request: ``scores[b, w] + log_softmax(logits[b, w])`` over all beams w and
-    tokens, best first, of equals the lowest beam and token first.  logits fp32 or bf16 [B, W, V] (tokens side by side; a whole vocabulary),
+    tokens, best first, of equals the lowest beam and token first (of one beam by the logits, also where 64 bits do not tell the sums apart).  logits fp32 or bf16 [B, W, V] (tokens side by side; a whole vocabulary),
     scores fp32 [B, W].  Returns fp32 scores, int32 parents (beams) and int32 tokens, [B, n] each.
 
     A beam with ``finished`` (bool [B, W]) offers itself alone, with ``pad_token`` and its score as it is.  Tokens with a logit of -inf and beams with a

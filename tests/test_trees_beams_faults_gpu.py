@@ -123,3 +123,32 @@ def test_some_beams_far_ahead(dtype):
         scores[0, -1] = -3.0
         check(logits, scores, n, finished, 17)
         check((logits.float() * 0.5).round().to(dtype), scores.round(), n, finished, 17)
+
+
+# ---------------------------------------------------------------- order within a beam
+@pytest.mark.parametrize("w", [1, 3])
+def test_logits_that_sums_in_64_bits_do_not_tell_apart(w):
+    """Of one beam the larger logit is first, also where both totals are the same number: fewer candidates are the first of more."""
+    from deepseek_v4_2080ti_b200.ops import beams
+    logits = -1 - torch.rand(4, w, 300, generator=torch.Generator(device=DEV).manual_seed(w), device=DEV)
+    logits[:, 0, [3, 50, 7, 200]] = torch.tensor([0.0, 1e-30, -1e-30, 2e-20], device=DEV)
+    scores = torch.zeros(4, w, device=DEV)
+    scores[:, 1:] = -50
+    for n in (1, 2, 3, 4):
+        assert beams.select(logits, scores, n)[2].tolist() == [[200, 50, 3, 7][:n]] * 4
+    equal = logits[:, :1].expand(4, 3, 300).contiguous()
+    got = beams.select(equal, torch.zeros(4, 3, device=DEV), 12)
+    assert got[1].tolist() == [[0] * 4 + [1] * 4 + [2] * 4] * 4 and got[2].tolist() == [[200, 50, 3, 7] * 3] * 4
+
+
+@pytest.mark.parametrize("w,v,n", [(1, 9000, 8), (3, 5000, 20), (20, 9000, 128), (4, 248320, 128)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("score", [torch.finfo(torch.float32).min, -1e30])
+def test_scores_that_outweigh_the_logits(w, v, n, dtype, score):
+    """Beams at the type's lowest value, whose totals are all one number: of equals the lowest beam, and of its tokens the best."""
+    from deepseek_v4_2080ti_b200.ops import beams
+    logits, scores = random_logits(2, w, v, dtype)
+    scores[:] = score
+    best = logits[:, 0].float().sort(descending=True, stable=True).indices[:, :n].int()
+    got = beams.select(logits, scores, n)
+    assert bool((got[0] == score).all() and (got[1] == 0).all()) and torch.equal(got[2], best)
