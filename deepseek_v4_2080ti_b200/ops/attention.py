@@ -493,15 +493,15 @@ def _check_tree_pages(block_table, nb, bs, kv_len, q_start, q_len, lo, mask) -> 
     if not _lib.bounds_checks_on():
         return
     (t, words), width = mask.shape, block_table.shape[1]
-    first = kv_len - q_len
-    row = torch.arange(t, device=mask.device)
-    mine = (row >= q_start[:, None]) & (row < (q_start + q_len)[:, None])                       # [B, T]
-    context = torch.where(mine, first[:, None], 0).amax(0, keepdim=True)[0].to(torch.int32) if t else first[:0]
+    kv, start, n = (x.long()[:, None] for x in (kv_len, q_start, q_len))
+    row, first = torch.arange(t, device=mask.device), kv - n
+    mine = (start >= 0) & (row >= start) & (row < start + n)                                    # [B, T]: a negative q_start is no sequence
+    context = torch.where(mine, first, 0).sum(0)                                                # (a row is one sequence's at most)
     seen = _seen_pages(t, width, bs, kv_len, q_start, q_len, lo, context)
     nodes = ((mask[..., None] >> torch.arange(32, dtype=torch.int32, device=mask.device)) & 1).reshape(t, -1)
-    key = first[:, None] + torch.arange(32 * words, device=mask.device)                         # [B, nodes]
-    bits = (mine.float() @ nodes.float() > 0) & (key >= 0) & (key < kv_len.clamp(max=width * bs)[:, None])
-    seen = seen.long().scatter_add(1, (key.long() // bs).clamp(0, width - 1), bits.long()) > 0
+    key = first + torch.arange(32 * words, device=mask.device)                                  # [B, nodes]
+    bits = (mine.float() @ nodes.float() > 0) & (key >= 0) & (key < kv.clamp(max=width * bs))
+    seen = seen.long().scatter_add(1, (key // bs).clamp(0, width - 1), bits.long()) > 0
     block_table.masked_fill_(seen & (block_table == -1), -2)
     _lib.check_indices(block_table, 0, nb, 3, keep=-1)
 

@@ -33,6 +33,29 @@ def test_parts_of_a_row():
             assert parts * tiles * beams.TILE < 2 ** 31             # places are numbers of 32 bits
 
 
+def seen_and_missing(monkeypatch, table, mask, q_start, q_len, kv_len, lo=None, bs=16):
+    """The table after the debug mode's look at it, without the scan that reports (-2) and replaces what it has marked."""
+    from deepseek_v4_2080ti_b200.ops import _lib
+    monkeypatch.setattr(_lib, "bounds_checks_on", lambda: True)
+    monkeypatch.setattr(_lib, "check_indices", lambda *a, **k: None)
+    i = lambda x: torch.tensor(x, dtype=I32)
+    table = i(table)
+    attention._check_tree_pages(table, 8, bs, i(kv_len), i(q_start), i(q_len), None if lo is None else i(lo), i(mask))
+    return table.tolist()
+
+
+def test_idle_sequences_claim_no_rows_in_the_debug_mode(monkeypatch):
+    """A negative q_start is no sequence, whatever its lengths: its table is not looked at, and rows of others see their own context."""
+    mask = [[1], [3], [5]]
+    for table in ([[0, 1, -1], [-1, -1, -1]], [[0, -1, -1], [-1, -1, -1]]):
+        found = seen_and_missing(monkeypatch, table, mask, [0, -1], [3, 5], [20, 200])
+        assert found == [[x if x >= 0 or i > 1 else -2 for i, x in enumerate(table[0])], [-1, -1, -1]]
+    # an idle one before and after, and one that begins behind the rows
+    assert seen_and_missing(monkeypatch, [[-1] * 3, [4, 5, -1], [-1] * 3, [-1] * 3], mask, [-3, 0, -1, 3], [4, 3, 3, 4], [40, 32, 48, 40]) == [[-1] * 3, [4, 5, -1], [-1] * 3, [-1] * 3]
+    # two sequences, each row with the context of its own
+    assert seen_and_missing(monkeypatch, [[0, -1, -1], [1, 2, -1]], [[1], [3], [1]], [0, 2], [2, 1], [10, 40]) == [[0, -1, -1], [1, 2, -2]]
+
+
 @pytest.mark.gpu
 def test_refusals_on_a_device():
     i = lambda *s: Z(*s, dtype=I32, device="cuda")

@@ -152,3 +152,21 @@ def test_scores_that_outweigh_the_logits(w, v, n, dtype, score):
     best = logits[:, 0].float().sort(descending=True, stable=True).indices[:, :n].int()
     got = beams.select(logits, scores, n)
     assert bool((got[0] == score).all() and (got[1] == 0).all()) and torch.equal(got[2], best)
+
+
+# ---------------------------------------------------------------- what the debug mode says of pages
+def test_idle_sequences_in_the_debug_mode(monkeypatch):
+    """A sequence whose q_start is negative is none: its empty table is no error and stays as it is, whatever its lengths are."""
+    from deepseek_v4_2080ti_b200.ops import _lib, attention
+    args, _, (seqs, seen, _) = tree_inputs([(20, 300)], 4, 2, wide=9)
+    q, kc, vc, table, mask = args[:5]
+    table = torch.cat([torch.full_like(table, -1), table, torch.full_like(table, -1)])
+    table[1, 5:] = -1
+    kept = table.clone()
+    for debug in "01":
+        monkeypatch.setenv("B200_BOUNDS_CHECK", debug)
+        for splits in (1, 3):
+            out = attention.decode_tree(q, kc, vc, table, mask, _i32([-3, 0, -1]), _i32([30, 20, 5]), _i32([900, 320, 40]), 20, splits=splits)
+            _lib.check_status()
+            assert torch.equal(table, kept)
+            close(out, *oracle(q, *seqs[0], seen[0]))
