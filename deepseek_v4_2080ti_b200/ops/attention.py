@@ -499,7 +499,10 @@ def _check_tree_pages(block_table, nb, bs, kv_len, q_start, q_len, lo, mask) -> 
     context = torch.where(mine, first, 0).sum(0)                                                # (a row is one sequence's at most)
     seen = _seen_pages(t, width, bs, kv_len, q_start, q_len, lo, context)
     nodes = ((mask[..., None] >> torch.arange(32, dtype=torch.int32, device=mask.device)) & 1).reshape(t, -1)
-    key = first + torch.arange(32 * words, device=mask.device)                                  # [B, nodes]
+    node = torch.arange(32 * words, device=mask.device)
+    if lo is not None:
+        nodes = nodes * (context[:, None] + node >= lo[:, None])
+    key = first + node                                                                          # [B, nodes]
     bits = (mine.float() @ nodes.float() > 0) & (key >= 0) & (key < kv.clamp(max=width * bs))
     seen = seen.long().scatter_add(1, (key // bs).clamp(0, width - 1), bits.long()) > 0
     block_table.masked_fill_(seen & (block_table == -1), -2)

@@ -56,6 +56,16 @@ def test_idle_sequences_claim_no_rows_in_the_debug_mode(monkeypatch):
     assert seen_and_missing(monkeypatch, [[0, -1, -1], [1, 2, -1]], [[1], [3], [1]], [0, 2], [2, 1], [10, 40]) == [[0, -1, -1], [1, 2, -2]]
 
 
+def test_nodes_below_lo_are_not_seen_in_the_debug_mode(monkeypatch):
+    """A node's key counts only for rows that have its bit and whose span reaches back to it."""
+    mask, args = [[1], [3], [7], [15]], ([0], [4], [18])               # nodes at the keys 14 to 17
+    assert seen_and_missing(monkeypatch, [[-1, 3, -1]], mask, *args, lo=[16, 16, 16, 16]) == [[-1, 3, -1]]
+    assert seen_and_missing(monkeypatch, [[-1, 3, -1]], mask, *args, lo=[16, 15, 16, 16]) == [[-2, 3, -1]]
+    assert seen_and_missing(monkeypatch, [[-1, -1, -1]], [[1], [2], [4], [3]], *args, lo=[18, 16, 16, 16]) == [[-1, -2, -1]]
+    assert seen_and_missing(monkeypatch, [[-1, -1, -1]], [[1], [2], [3], [3]], *args, lo=[18, 16, 16, 16]) == [[-1, -1, -1]]
+    assert seen_and_missing(monkeypatch, [[-1, -1, -1]], mask, *args) == [[-2, -2, -1]]
+
+
 @pytest.mark.gpu
 def test_refusals_on_a_device():
     i = lambda *s: Z(*s, dtype=I32, device="cuda")

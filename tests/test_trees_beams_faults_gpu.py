@@ -170,3 +170,22 @@ def test_idle_sequences_in_the_debug_mode(monkeypatch):
             _lib.check_status()
             assert torch.equal(table, kept)
             close(out, *oracle(q, *seqs[0], seen[0]))
+
+
+def test_nodes_below_lo_in_the_debug_mode(monkeypatch):
+    """A page of nodes that no row's span reaches back to may be missing; where one does it is reported."""
+    from deepseek_v4_2080ti_b200.ops import _lib, attention
+    args, _, (seqs, seen, _) = tree_inputs([(20, 60)], 4, 2, wide=3)       # nodes at the keys 60 to 79, pages of 64
+    table, lo = args[3], _i32([64] * 20)
+    table[0, 0] = table[0, 2] = -1
+    kept = table.clone()
+    seen[0][:, :64] = False
+    monkeypatch.setenv("B200_BOUNDS_CHECK", "1")
+    out = attention.decode_tree(*args, lo=lo)
+    _lib.check_status()
+    assert torch.equal(table, kept)
+    close(out, *oracle(args[0], *seqs[0], seen[0]))
+    lo[3] = 60
+    attention.decode_tree(*args, lo=lo)
+    with pytest.raises(_lib.KernelError):
+        _lib.check_status()
