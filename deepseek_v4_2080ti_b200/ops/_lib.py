@@ -30,7 +30,9 @@ ERR_NAMES = {
 
 # sites of the debug index checks (B200_BOUNDS_CHECK=1), as recorded in the second byte of the error word
 BOUNDS_SITES = {1: "token ids", 2: "kv cache element offsets", 3: "page table", 4: "state slots", 5: "selected key rows",
-                6: "expert ids", 7: "logit rows"}
+                6: "expert ids", 7: "logit rows", 8: "pages of accepted paths"}
+# what became of such an index, where it was not replaced
+BOUNDS_OUTCOMES = {8: "the rows in that page stayed where they are"}
 
 
 class KernelError(RuntimeError):
@@ -102,8 +104,8 @@ def check_status(device=None) -> None:
         t.zero_()
         if code & 0xFF == 7:
             site, pos = (code >> 8) & 0xFF, (code >> 16) & 0xFFFF
-            raise KernelError(f"index out of range in {BOUNDS_SITES.get(site, f'site {site}')} at element "
-                              f"{pos}{'+' if pos == 0xFFFF else ''} (the index was replaced by a valid one before the kernel ran)")
+            raise KernelError(f"index out of range in {BOUNDS_SITES.get(site, f'site {site}')} at element {pos}{'+' if pos == 0xFFFF else ''} "
+                              f"({BOUNDS_OUTCOMES.get(site, 'the index was replaced by a valid one before the kernel ran')})")
         raise KernelError(f"device kernel reported error {code}: {ERR_NAMES.get(code, 'unknown')}")
 
 

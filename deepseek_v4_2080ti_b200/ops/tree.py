@@ -105,6 +105,20 @@ def _caches(caches, dev: int):
     return nb, bs, b"".join(packed)
 
 
+def _check_pages(path, q_len, kv_len, block_table, nb: int, bs: int) -> None:
+    """Debug mode: reports pages that are not there, or keys behind the table, where a row of a path lies or would go.  Nothing is replaced."""
+    if not _lib.bounds_checks_on():
+        return
+    b, most = path.shape
+    to = torch.arange(most, device=path.device)
+    first = (kv_len.long() - q_len)[:, None]
+    moves = (path > to) & (first >= 0)
+    keys = torch.stack([first + path, first + to.expand(b, most)], -1)         # [B, max_path, from and to]
+    pages = block_table.long().gather(1, (keys // bs).clamp(0, block_table.shape[1] - 1).view(b, -1)).view(keys.shape)
+    pages = torch.where(keys < block_table.shape[1] * bs, pages, -1)
+    _lib.check_indices(torch.where(moves[..., None], pages, 0).to(torch.int32), 0, nb, 8)
+
+
 def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=None, block_table=None, caches=()):
     """The path that the target agrees with: from node 0 to the child whose token is the one predicted at its parent (of several the first),
     as long as there is one, ``max_path`` nodes at most.  tokens / parents / predicted int32 [T], q_start / q_len int32 [B]; negative tokens and
@@ -115,8 +129,8 @@ def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=Non
 
     ``caches``: tensors [layers, pages, heads, page size, ..] of any type, layers contiguous (a single layer: ``cache[None]``; keys, values,
     scales of quantised rows); with them kv_len [B] and block_table int32 [B, pages], as in ``attention.decode_tree``.  The path's rows move
-    in place from kv_len - q_len + path[i] to kv_len - q_len + i; rows in pages outside the cache stay where they are.  No cache is part of
-    another, and no two sequences have the page of a row that moves."""
+    in place from kv_len - q_len + path[i] to kv_len - q_len + i; rows in pages outside the cache stay where they are, which the debug mode
+    reports.  No cache is part of another, and no two sequences have the page of a row that moves."""
     dev = tokens.get_device()
     if dev < 0 or tokens.dim() != 1:
         raise ValueError(f"tokens: int32 [T] on a GPU expected, got {list(tokens.shape)} on {tokens.device}")
@@ -145,4 +159,6 @@ def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=Non
         call = _CALL.pack(_CALL_BYTES, b, tokens.data_ptr(), parents.data_ptr(), predicted.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), _at(kv_len),
                           _at(block_table), path.data_ptr(), count.data_ptr(), emitted.data_ptr(), _stream(dev), t, int(max_path), width, nb, bs, len(caches))
         _lib.check(_kernels().b200_tree_accept(call + packed + _REST[len(caches)]), "tree_accept")
+        if caches:
+            _check_pages(path, q_len, kv_len, block_table, nb, bs)
     return path, count, emitted

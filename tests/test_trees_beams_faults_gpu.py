@@ -189,3 +189,53 @@ def test_nodes_below_lo_in_the_debug_mode(monkeypatch):
     attention.decode_tree(*args, lo=lo)
     with pytest.raises(_lib.KernelError):
         _lib.check_status()
+
+
+# ---------------------------------------------------------------- accepted paths in the debug mode
+def accept_inputs():
+    """Three sequences of one cache: a path of rows that move, an idle one, one whose path is its first node."""
+    tokens, parents, predicted = _i32([9, 1, 2, 3, 2, 5, 6]), _i32([-1, 0, 0, 0, 3, -1, 0]), _i32([3, 0, 0, 2, 8, 4, 4])
+    cache = torch.arange(8 * 16, device=DEV, dtype=torch.float32).view(1, 8, 1, 16).clone()
+    return (tokens, parents, predicted, _i32([0, -1, 5]), _i32([5, 3, 2]), 4, _i32([37, 20, 40])), cache
+
+
+def test_pages_that_are_not_there_are_reported_by_accept(monkeypatch):
+    """Rows of the path that lie in pages outside the cache stay where they are; the debug mode says so, whichever page it is, and says nothing
+    of pages that no row of a path lies in.  The table is left as it is."""
+    from deepseek_v4_2080ti_b200.ops import _lib, tree
+    monkeypatch.setenv("B200_BOUNDS_CHECK", "1")
+    args, cache = accept_inputs()                          # sequence 0: keys 32 .. 36 are the tree, 35 -> 33 and 36 -> 34
+    for row, bad in (([0, 1, 2], False), ([-1, 99, 2], False), ([0, 1, -1], True), ([0, 1, 8], True), ([0, 1, -2 ** 31], True), ([0, 1, 2 ** 31 - 1], True)):
+        table = _i32([row, [-1, -1, -1], [-1, -1, -1]])
+        was, kept = cache.clone(), table.clone()
+        got = tree.accept(*args, table, [cache])
+        assert got[0].tolist() == [[0, 3, 4, -1], [-1] * 4, [0] + [-1] * 3]
+        if bad:
+            with pytest.raises(_lib.KernelError):
+                _lib.check_status()
+            assert torch.equal(cache, was)
+        else:
+            _lib.check_status()
+            was[0, 2, 0, 1], was[0, 2, 0, 2] = was[0, 2, 0, 3].clone(), was[0, 2, 0, 4].clone()
+            assert torch.equal(cache, was)
+        assert torch.equal(table, kept)
+
+
+def test_a_captured_accept_in_the_debug_mode(monkeypatch):
+    from deepseek_v4_2080ti_b200.ops import _lib, tree
+    monkeypatch.setenv("B200_BOUNDS_CHECK", "1")
+    args, cache = accept_inputs()
+    table = _i32([[0, 1, 2], [-1] * 3, [-1] * 3])
+    tree.accept(*args, table, [cache.clone()])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = tree.accept(*args, table, [cache])
+    graph.replay()
+    torch.cuda.synchronize()
+    _lib.check_status()
+    assert got[1].tolist() == [3, 0, 1]
+    table[0, 2] = 70
+    graph.replay()
+    with pytest.raises(_lib.KernelError):
+        _lib.check_status()
