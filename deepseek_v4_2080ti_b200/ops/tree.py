@@ -127,8 +127,8 @@ def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=Non
     Returns ``path`` int32 [B, max_path] (nodes, node 0 first), ``count`` int32 [B] and ``emitted`` int32 [B, max_path]: the tokens that the target puts
     behind the path's nodes - the drafts it agrees with, then one of its own; -1 behind ``count``.  A sequence of no rows has a count of 0.
 
-    ``caches``: tensors [layers, pages, heads, page size, ..] of any type, layers contiguous (a single layer: ``cache[None]``; keys, values,
-    scales of quantised rows); with them kv_len [B] and block_table int32 [B, pages], as in ``attention.decode_tree``.  The path's rows move
+    ``caches``: a list of tensors [layers, pages, heads, page size, ..] of any type, rows of a multiple of 4 bytes, layers contiguous (a single layer:
+    ``cache[None]``; keys, values, scales of quantised rows); with them kv_len [B] and block_table int32 [B, pages], as in ``attention.decode_tree``.  The path's rows move
     in place from kv_len - q_len + path[i] to kv_len - q_len + i; rows in pages outside the cache stay where they are, which the debug mode
     reports.  No cache is part of another, and no two sequences have the page of a row that moves."""
     dev = tokens.get_device()
@@ -145,6 +145,8 @@ def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=Non
     _index(q_len, (b,), dev, "q_len")
     if not 1 <= max_path <= MAX_PATH or b > 65535:
         raise ValueError(f"{b} paths of {max_path} nodes: 65535 at most, of 1 to {MAX_PATH} nodes")
+    if isinstance(caches, torch.Tensor):                     # (its layers would be taken for caches, their pages for layers)
+        raise ValueError(f"caches: a list of tensors expected, got one of {list(caches.shape)}")
     caches = list(caches)
     nb, bs, width, packed = 0, 0, 0, b""
     if caches:

@@ -239,3 +239,16 @@ def test_a_captured_accept_in_the_debug_mode(monkeypatch):
     graph.replay()
     with pytest.raises(_lib.KernelError):
         _lib.check_status()
+
+
+def test_a_tensor_in_the_place_of_a_list_of_caches_is_refused():
+    """Its layers would be taken for caches, and their pages for layers: rows of other keys would move."""
+    from deepseek_v4_2080ti_b200.ops import tree
+    args, _ = accept_inputs()
+    cache = torch.arange(2 * 3 * 2 * 16 * 4, device=DEV, dtype=torch.float32).view(2, 3, 2, 16, 4)
+    was, table = cache.clone(), _i32([[0, 1, 2], [-1] * 3, [-1] * 3])
+    with pytest.raises(ValueError):
+        tree.accept(*args, table, cache)
+    assert torch.equal(cache, was)
+    tree.accept(*args, table, (cache,))
+    assert not torch.equal(cache, was)
