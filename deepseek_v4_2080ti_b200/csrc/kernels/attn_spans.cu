@@ -35,9 +35,9 @@
 // take another 10 %.  Packed documents of 4000 rows of 48 heads, capped: 110 us, a third of it the start and end of items, and of the
 // rest most masked tiles (6000 cycles).
 // Shared keys of 40 heads over 8, in one item a block: 64 rows over 32768 keys 44 us, 32 over 8192 15 us.
-// Trees of 40 heads over 8: 32 of 64 nodes over 8192 keys 475 to 570 us, where the second row tile of 64 rows reads the keys from DRAM
-// once more (2.2 GB; begun beside the first it gains nothing) and 512 items are 3.5 rounds of blocks; 32 of 25 nodes 204 us, 5.2 TB/s; one of
-// 16 over 32768 keys 38 us, 20 of them the keys.  The smallest, 7 nodes over 350 keys, is a chain of 18 thousand cycles: the item 2.8,
+// Trees of 40 heads over 8: 32 of 64 nodes over 8192 keys 475 to 571 us, where the second row tile of 64 rows reads the keys from DRAM
+// once more (2.2 GB; begun beside the first it gains nothing) and 512 items are 3.5 rounds of blocks; 32 of 25 nodes 193 to 199 us, 5.4 to 5.6
+// TB/s; one of 16 over 32768 keys 37 us, 20 of them the keys.  The smallest, 7 nodes over 350 keys, is a chain of 18 thousand cycles: the item 2.8,
 // queries 1.5, first scores 1, three tiles 7.5 (the last one masked), the rows' way out 5.2.
 #include <cuda_bf16.h>
 #include "per_device.h"
@@ -388,8 +388,8 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, int lane, Ite
   it.t0 = it.t1 = 0;
   if (it.k_end > lo_min) {
     // Ranges by the keys that are there, not by what the host knows of them: a captured step's bound, or the table's width, is often far above its
-    // contexts, and a window leaves few keys of them.  (16 nodes over 4000 keys with a bound of 4016 / 32768 / 131072: 16.8 / 17.8 / 17.8 us, with ranges
-    // of a length that follows from the bound 16.1 / 25.3 / 42.6; over 32768 keys in a window of 4096: 16.7, and 26.6.  Ranges of at least 2, 3 or 4
+    // contexts, and a window leaves few keys of them.  (16 nodes over 4000 keys with a bound of 4016 / 32768 / 131072: 16.2 / 17.1 / 17.0 us, with ranges
+    // of a length that follows from the bound 16.1 / 25.3 / 42.6; over 32768 keys in a window of 4096: 16.6, and 26.6.  Ranges of at least 2, 3 or 4
     // tiles gain nothing.)
     const int a = lo_min / BKV, n = (it.k_end + BKV - 1) / BKV - a, per = (int)((uint32_t)(n + splits - 1) / (uint32_t)splits);
     it.t0 = a + min(n, split * per);

@@ -6,7 +6,8 @@
 // it has been read, whatever cycles the parents make, and there is no copy of the state anywhere else.  Beams that continue themselves move
 // nothing.
 //
-// What bounds it is memory (16 beams of 12 to 100 MB: 6.0 to 6.2 TB/s of copies in and out): warp 0 keeps bulk copies of items on their way
+// What bounds it is memory (16 beams of 13 to 103 MB, copies in and out: 6.0 to 6.5 TB/s where 14 or 16 of them move, 5.2 to 5.5 where 10 of 16 do,
+// whose items are less full): warp 0 keeps bulk copies of items on their way
 // both in and out, STAGES items in shared memory; it only issues them.  Warps 1 to 3 do the tensors whose rows are no multiples of 16 bytes (tables, tails) by plain loads, at the same time.
 #include "../ptx/sm100.cuh"
 #include "launch.h"
@@ -214,9 +215,9 @@ extern "C" int b200_beam_reorder(const ReorderCall* call) {
     if (s.outer < 1 || s.inner_bytes < 1 || (s.bulk && ((uintptr_t)s.base | s.outer_bytes | s.slot_bytes | s.inner_bytes) % 16)) return -ERR_BAD_ARG;
     if (s.bulk) bulk += s.inner_bytes * s.outer * a.requests;
   }
-  // Items as large as a stage holds: an item costs its warp 0.5 us however small it is, and stages of 32 / 48 / 64 KB take 179 / 122 / 111 us
-  // for 16 beams of 48 MB.  Smaller ones, of 1 KB a beam at least, where every SM would not have two otherwise (8 / 4 / 2 a SM: 15.7 / 10.1 /
-  // 7.3 us for the last pages of 4 beams in 16 layers).
+  // Items as large as a stage holds: with stages of 32 / 48 / 64 KB 16 beams of 49 MB of one request, all of which move and 11 are wanted (1.33 GB in
+  // and out), take 340 / 246 / 206 us, of 4 requests (14 and 12, 1.28 GB) 276 / 216 / 211.  Smaller ones, of 1 KB a beam at least, where every SM
+  // would not have two otherwise (8 / 4 / 2 a SM: 15.0 / 9.6 / 6.6 us for the last pages of 4 beams in 16 layers, 25 MB).
   const long long most = STAGE_BYTES / a.beams / 128 * 128, even = bulk / (148 * 2) / 128 * 128;
   p.chunk = (int)(even < 1024 ? (most < 1024 ? most : 1024) : even < most ? even : most);
   p.plain_chunk = PLAIN_BYTES / a.beams / 16 * 16;

@@ -22,7 +22,8 @@
 //
 // What it takes: 64 requests of 8 beams (a fifth of them at their end) over 248320 tokens, 16 candidates, 86 us, 76 of them the first kernel
 // at 5.4 TB/s: reading and maxima alone take 65 (at the rate of a copy 62), lists and what lets them in 10; the join is a chain of 10.
-// With sums to 2^-30 in the first pass it was 150 us.  One request of 4 beams is 12 us: two dependent kernels' latency, 6 each.
+// With sums to 2^-30 in the first pass it was 150 us.  One request of 4 beams is 12 us: two dependent kernels' latency, 6 each.  Which entries of the
+// parts' lists the join orders: see raise_bound and look_further.
 #include <cuda_bf16.h>
 #include <limits.h>
 #include "../ptx/sm100.cuh"

@@ -48,13 +48,13 @@ def _parts(rows: int, vocab: int) -> tuple[int, int]:
 def select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None, finished: torch.Tensor | None = None,
            pad_token: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``n`` best continuations (default: as many as beams) of every request: ``scores[b, w] + log_softmax(logits[b, w])`` over all beams w and
-    tokens, best first, of equals the lowest beam and token first (of one beam by the logits, also where 64 bits do not tell the sums apart).  logits fp32 or bf16 [B, W, V] (tokens side by side; a whole vocabulary),
-    scores fp32 [B, W].  Returns fp32 scores, int32 parents (beams) and int32 tokens, [B, n] each.
+    tokens, best first, of equals the lowest beam and token first (of one beam by the logits, also where 64 bits do not tell the sums apart).
+    logits fp32 or bf16 [B, W, V] (tokens side by side; a whole vocabulary), scores fp32 [B, W].  Returns fp32 scores, int32 parents (beams) and int32 tokens, [B, n] each.
 
     A beam with ``finished`` (bool [B, W]) offers itself alone, with ``pad_token`` and its score as it is.  Tokens with a logit of -inf and beams with a
     score of -inf are not offered, nor are beams whose score or logits hold NaN or +inf; where fewer than n are left the rest is -inf, -1, -1.
-    Scores are good to 32 bits (their rounding, and 10^-6); where candidates of different beams lie closer together than that their order is taken
-    from sums to 2^-30, in 64 bits."""
+    Scores are off by their rounding to 32 bits and 4.5e-7 + 5.1e-8 (log2 V + 2) at most (1.4e-6 at 248320 tokens); where candidates of different
+    beams lie closer together than that their order is taken from sums to 2^-30, in 64 bits."""
     dev, shape = logits.get_device(), logits.shape
     if dev < 0 or len(shape) != 3 or logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"logits: fp32 or bf16 [requests, beams, vocabulary] on a GPU expected, got {logits.dtype} {list(shape)} on {logits.device}")
