@@ -129,8 +129,8 @@ def accept(tokens, parents, predicted, q_start, q_len, max_path: int, kv_len=Non
 
     ``caches``: a list of tensors [layers, pages, heads, page size, ..] of any type, rows of a multiple of 4 bytes, layers contiguous (a single layer:
     ``cache[None]``; keys, values, scales of quantised rows); with them kv_len [B] and block_table int32 [B, pages], as in
-    ``attention.decode_tree``.  The path's rows move in place from kv_len - q_len + path[i] to kv_len - q_len + i; rows in pages outside the cache stay where they are, which the debug mode
-    reports.  No cache is part of another, and no two sequences have the page of a row that moves."""
+    ``attention.decode_tree``.  The path's rows move in place from kv_len - q_len + path[i] to kv_len - q_len + i; rows in pages outside the
+    cache stay where they are, which the debug mode reports.  No cache is part of another, and no two sequences have the page of a row that moves."""
     dev = tokens.get_device()
     if dev < 0 or tokens.dim() != 1:
         raise ValueError(f"tokens: int32 [T] on a GPU expected, got {list(tokens.shape)} on {tokens.device}")
