@@ -110,7 +110,7 @@ def check_status(device=None) -> None:
 
 
 def bounds_checks_on() -> bool:
-    return os.environ.get("B200_BOUNDS_CHECK", "0") == "1"
+    return "B200_BOUNDS_CHECK" in os.environ and os.environ["B200_BOUNDS_CHECK"] == "1"      # (``get`` takes twice as long where it is not set)
 
 
 def check_indices(idx: torch.Tensor | None, lo: int, hi: int, site: int, keep: int | None = None) -> None:
